@@ -33,7 +33,7 @@
 extern "C" {
 #endif
 
-#define NEST_ABI_VERSION 18
+#define NEST_ABI_VERSION 19
 
 #define NEST_OK 0
 #define NEST_ERR_INVALID_ARGUMENT (-1)
@@ -566,6 +566,77 @@ typedef struct nest_rvq_attr {
   float *raw_out;       /* or NULL */
 } nest_rvq_attr;
 int nest_rvq_decode_batch(int32_t n, const nest_rvq_attr *attrs, void *stream);
+
+/* ---- Operators of a trained decoder block (no reference counterpart) ----
+ * x + dropout(ffn(layer_norm(x))) between the composited feature map and the
+ * colour head, forward and backward.  dtype is that of x, y and their
+ * gradients (F32, F16 or BF16); rows are contiguous and row-major, with any
+ * row length and any alignment of the element type.  Sums are float32, each
+ * result is rounded once. */
+
+/* y = (x - mean) rstd w + b over each row of x [rows, cols], rstd =
+ * 1/sqrt(var + eps) with the variance about the mean, divided by cols.
+ * weight [cols] and bias [cols] (or NULL) are of param_dtype: F32 or dtype.
+ * mean and rstd [rows] float32 receive the statistics the backward needs
+ * (either may be NULL). */
+int nest_layer_norm(int64_t rows, int32_t cols, int32_t dtype, int32_t param_dtype, const void *x,
+                    const void *weight, const void *bias, float eps, void *y, float *mean, float *rstd,
+                    void *stream);
+
+/* Gradients of nest_layer_norm from dy: dx, dweight and dbias (or NULL) are
+ * overwritten; with no rows dweight and dbias are zero.  The workspace holds
+ * partial column sums, joined in a fixed order: results repeat bit for bit. */
+size_t nest_layer_norm_backward_workspace_size(int64_t rows, int32_t cols, int32_t dtype);
+int nest_layer_norm_backward(int64_t rows, int32_t cols, int32_t dtype, int32_t param_dtype, const void *dy,
+                             const void *x, const void *weight, const float *mean, const float *rstd, void *dx,
+                             void *dweight, void *dbias, void *ws, size_t ws_bytes, void *stream);
+
+/* y[i] = keep(i) ? x[i] * scale : 0, plus residual[i] unless it is NULL.
+ * keep(i) holds where a 16-bit random number is at least t =
+ * floor(65536 p + 1/2); scale = 65536 / (65536 - t), and 0 for t = 65536.
+ * Element i's number is half i%2 (low first) of word (i/2)%4 of the Philox
+ * 4x32-10 block at the counter (i/8 as two words, offset as two words) under
+ * the key seed.  The mask is not stored: the gradient of x is this call on
+ * dy with the same p, seed and offset.  y may be x or residual itself. */
+int nest_dropout(int64_t n, int32_t dtype, const void *x, const void *residual, double p, uint64_t seed,
+                 uint64_t offset, void *y, void *stream);
+
+#define NEST_ACT_RELU 0
+#define NEST_ACT_SILU 1
+#define NEST_ACT_GELU 2 /* x Phi(x), by erf */
+
+/* y = (act(x Wg^T) * (x Wu^T)) Wd^T: x [rows, in_features], w_gate and w_up
+ * [hidden, in_features], w_down [out_features, hidden], y [rows,
+ * out_features], all of dtype. */
+typedef struct nest_gated_ffn {
+  uint32_t struct_size;
+  int32_t dtype;
+  int32_t activation;
+  int32_t in_features;
+  int32_t hidden;
+  int32_t out_features;
+  int64_t rows;
+  const void *x;
+  const void *w_gate;
+  const void *w_up;
+  const void *w_down;
+} nest_gated_ffn;
+
+/* Bytes the calls below need, each may be 0 and each pointer may be NULL:
+ * kept, what a training forward leaves for the backward; the workspaces of a
+ * forward, of a backward that is given kept, and of one that is not and
+ * computes the pre-activations again.  Host only. */
+int nest_gated_ffn_sizes(const nest_gated_ffn *f, size_t *kept, size_t *forward_ws, size_t *backward_ws,
+                         size_t *backward_ws_alone);
+
+/* kept: NULL, or the array of that size a training step hands on. */
+int nest_gated_ffn_forward(const nest_gated_ffn *f, void *y, void *kept, void *ws, size_t ws_bytes, void *stream);
+
+/* dx [rows, in_features] and dw_gate, dw_up, dw_down (each NULL where it is
+ * not wanted) are overwritten; with no rows the weights' gradients are zero.
+ * Sums run in a fixed order: results repeat bit for bit. */
+int nest_gated_ffn_backward(const nest_gated_ffn *f, const void *dy, const void *kept, void *dx, void *dw_gate,
+                            void *dw_up, void *dw_down, void *ws, size_t ws_bytes, void *stream);
 
 #ifdef __cplusplus
 }

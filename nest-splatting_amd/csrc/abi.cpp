@@ -19,6 +19,7 @@
 #include <string>
 
 #include "../../include/nest_splat.h"
+#include "blocks_internal.h"
 #include "nest_internal.h"
 
 using namespace nest;
@@ -1381,6 +1382,188 @@ int nest_rvq_decode_batch(int32_t n, const nest_rvq_attr* attrs, void* stream) {
   }
   hipError_t e = launch_rvq_batch(b, static_cast<hipStream_t>(stream));
   return e == hipSuccess ? NEST_OK : hip_fail(e, "rvq_decode_batch");
+}
+
+// ---- operators of the decoder block ----
+
+namespace {
+
+constexpr int32_t kMaxFeatures = 1 << 20;   // row lengths: byte offsets inside a tile stay below 2^31
+constexpr int64_t kMaxRows = (int64_t)1 << 31;
+
+bool element_type(int32_t dt) { return dt == NEST_DTYPE_F32 || dt == NEST_DTYPE_F16 || dt == NEST_DTYPE_BF16; }
+
+int check_norm(int64_t rows, int32_t cols, int32_t dtype, int32_t param_dtype) {
+  if (rows < 0 || rows >= kMaxRows) return fail(NEST_ERR_INVALID_ARGUMENT, "rows must be in [0, 2^31) (got %lld)", (long long)rows);
+  if (cols < 1 || cols > kMaxFeatures) return fail(NEST_ERR_INVALID_ARGUMENT, "cols must be in [1, %d] (got %d)", kMaxFeatures, cols);
+  if (!element_type(dtype)) return fail(NEST_ERR_UNSUPPORTED, "dtype must be float32, float16 or bfloat16");
+  if (param_dtype != NEST_DTYPE_F32 && param_dtype != dtype)
+    return fail(NEST_ERR_UNSUPPORTED, "weight and bias must be float32 or of the rows' own type");
+  return NEST_OK;
+}
+
+struct GatedPlan {
+  size_t kept, h, dg, du, own_kept;   // bytes
+  size_t forward() const { return align_up(h); }
+  size_t backward(bool alone) const { return align_up(h) + align_up(dg) + align_up(du) + (alone ? align_up(own_kept) : 0); }
+};
+
+int check_gated(const nest_gated_ffn* f, GatedPlan& plan) {
+  if (!f || f->struct_size != sizeof(nest_gated_ffn)) return fail(NEST_ERR_INVALID_ARGUMENT, "nest_gated_ffn missing or struct_size mismatch");
+  if (f->rows < 0 || f->rows >= kMaxRows) return fail(NEST_ERR_INVALID_ARGUMENT, "rows must be in [0, 2^31) (got %lld)", (long long)f->rows);
+  const int32_t sides[3] = {f->in_features, f->hidden, f->out_features};
+  for (int32_t v : sides)
+    if (v < 1 || v > kMaxFeatures) return fail(NEST_ERR_INVALID_ARGUMENT, "in_features, hidden and out_features must be in [1, %d] (got %d)", kMaxFeatures, v);
+  if (!element_type(f->dtype)) return fail(NEST_ERR_UNSUPPORTED, "dtype must be float32, float16 or bfloat16");
+  if (f->activation != NEST_ACT_RELU && f->activation != NEST_ACT_SILU && f->activation != NEST_ACT_GELU)
+    return fail(NEST_ERR_UNSUPPORTED, "activation must be relu, silu or gelu");
+  const size_t es = f->dtype == NEST_DTYPE_F32 ? 4 : 2;
+  const size_t n = (size_t)f->rows * (size_t)f->hidden;
+  plan.kept = plan.own_kept = n * 2 * sizeof(float);
+  plan.h = plan.dg = plan.du = n * es;
+  return NEST_OK;
+}
+
+GatedParams gated_params(const nest_gated_ffn* f) {
+  GatedParams p{};
+  p.rows = f->rows;
+  p.in = f->in_features;
+  p.hidden = f->hidden;
+  p.out = f->out_features;
+  p.dtype = f->dtype;
+  p.activation = f->activation;
+  p.x = f->x;
+  p.w_gate = f->w_gate;
+  p.w_up = f->w_up;
+  p.w_down = f->w_down;
+  return p;
+}
+
+}  // namespace
+
+int nest_layer_norm(int64_t rows, int32_t cols, int32_t dtype, int32_t param_dtype, const void* x, const void* weight,
+                    const void* bias, float eps, void* y, float* mean, float* rstd, void* stream) {
+  if (int rc = check_norm(rows, cols, dtype, param_dtype); rc != NEST_OK) return rc;
+  if (!(eps >= 0.0f)) return fail(NEST_ERR_INVALID_ARGUMENT, "eps must not be negative");
+  if (rows == 0) return NEST_OK;
+  if (!x || !weight || !y) return fail(NEST_ERR_INVALID_ARGUMENT, "NULL tensor pointer");
+  LayerNormParams p{};
+  p.rows = rows;
+  p.cols = cols;
+  p.dtype = dtype;
+  p.param_dtype = param_dtype;
+  p.eps = eps;
+  p.x = x;
+  p.weight = weight;
+  p.bias = bias;
+  p.y = y;
+  p.mean = mean;
+  p.rstd = rstd;
+  hipError_t e = launch_layer_norm(p, static_cast<hipStream_t>(stream));
+  return e == hipSuccess ? NEST_OK : hip_fail(e, "layer norm");
+}
+
+size_t nest_layer_norm_backward_workspace_size(int64_t rows, int32_t cols, int32_t dtype) {
+  if (check_norm(rows, cols, dtype, dtype) != NEST_OK) return 0;
+  return (size_t)layer_norm_partials(rows, cols, dtype) * 2 * (size_t)cols * sizeof(float);
+}
+
+int nest_layer_norm_backward(int64_t rows, int32_t cols, int32_t dtype, int32_t param_dtype, const void* dy,
+                             const void* x, const void* weight, const float* mean, const float* rstd, void* dx,
+                             void* dweight, void* dbias, void* ws, size_t ws_bytes, void* stream) {
+  if (int rc = check_norm(rows, cols, dtype, param_dtype); rc != NEST_OK) return rc;
+  const size_t need = nest_layer_norm_backward_workspace_size(rows, cols, dtype);
+  if (ws_bytes < need) return fail(NEST_ERR_WORKSPACE, "layer norm workspace too small: %zu < %zu bytes", ws_bytes, need);
+  if (!dweight || (rows > 0 && (!dy || !x || !weight || !mean || !rstd || !dx || !ws)))
+    return fail(NEST_ERR_INVALID_ARGUMENT, "NULL tensor pointer");
+  LayerNormParams p{};
+  p.rows = rows;
+  p.cols = cols;
+  p.dtype = dtype;
+  p.param_dtype = param_dtype;
+  p.dy = dy;
+  p.x = x;
+  p.weight = weight;
+  p.mean = const_cast<float*>(mean);
+  p.rstd = const_cast<float*>(rstd);
+  p.dx = dx;
+  p.dweight = dweight;
+  p.dbias = dbias;
+  p.part = static_cast<float*>(ws);
+  hipError_t e = launch_layer_norm_backward(p, static_cast<hipStream_t>(stream));
+  return e == hipSuccess ? NEST_OK : hip_fail(e, "layer norm backward");
+}
+
+int nest_dropout(int64_t n, int32_t dtype, const void* x, const void* residual, double p, uint64_t seed,
+                 uint64_t offset, void* y, void* stream) {
+  if (n < 0) return fail(NEST_ERR_INVALID_ARGUMENT, "n must be >= 0");
+  if (!element_type(dtype)) return fail(NEST_ERR_UNSUPPORTED, "dtype must be float32, float16 or bfloat16");
+  if (!(p >= 0.0 && p <= 1.0)) return fail(NEST_ERR_INVALID_ARGUMENT, "p must be in [0, 1] (got %g)", p);
+  if (n == 0) return NEST_OK;
+  if (!x || !y) return fail(NEST_ERR_INVALID_ARGUMENT, "NULL tensor pointer");
+  DropoutParams d{};
+  d.n = n;
+  d.dtype = dtype;
+  d.x = x;
+  d.residual = residual;
+  d.y = y;
+  d.threshold = (uint32_t)std::floor(p * 65536.0 + 0.5);
+  d.scale = d.threshold < 65536u ? (float)(65536.0 / (65536.0 - d.threshold)) : 0.0f;
+  d.seed = seed;
+  d.offset = offset;
+  hipError_t e = launch_dropout(d, static_cast<hipStream_t>(stream));
+  return e == hipSuccess ? NEST_OK : hip_fail(e, "dropout");
+}
+
+int nest_gated_ffn_sizes(const nest_gated_ffn* f, size_t* kept, size_t* forward_ws, size_t* backward_ws,
+                         size_t* backward_ws_alone) {
+  GatedPlan plan;
+  if (int rc = check_gated(f, plan); rc != NEST_OK) return rc;
+  if (kept) *kept = plan.kept;
+  if (forward_ws) *forward_ws = plan.forward();
+  if (backward_ws) *backward_ws = plan.backward(false);
+  if (backward_ws_alone) *backward_ws_alone = plan.backward(true);
+  return NEST_OK;
+}
+
+int nest_gated_ffn_forward(const nest_gated_ffn* f, void* y, void* kept, void* ws, size_t ws_bytes, void* stream) {
+  GatedPlan plan;
+  if (int rc = check_gated(f, plan); rc != NEST_OK) return rc;
+  if (f->rows == 0) return NEST_OK;
+  if (!f->x || !f->w_gate || !f->w_up || !f->w_down || !y) return fail(NEST_ERR_INVALID_ARGUMENT, "NULL tensor pointer");
+  if (ws_bytes < plan.forward() || !ws) return fail(NEST_ERR_WORKSPACE, "gated ffn workspace too small: %zu < %zu bytes", ws_bytes, plan.forward());
+  GatedParams p = gated_params(f);
+  p.y = y;
+  p.kept = static_cast<float*>(kept);
+  p.h = ws;
+  hipError_t e = launch_gated_ffn(p, static_cast<hipStream_t>(stream), false);
+  return e == hipSuccess ? NEST_OK : hip_fail(e, "gated ffn");
+}
+
+int nest_gated_ffn_backward(const nest_gated_ffn* f, const void* dy, const void* kept, void* dx, void* dw_gate,
+                            void* dw_up, void* dw_down, void* ws, size_t ws_bytes, void* stream) {
+  GatedPlan plan;
+  if (int rc = check_gated(f, plan); rc != NEST_OK) return rc;
+  const size_t need = plan.backward(kept == nullptr);
+  if (f->rows > 0) {
+    if (!f->x || !f->w_gate || !f->w_up || !f->w_down || !dy) return fail(NEST_ERR_INVALID_ARGUMENT, "NULL tensor pointer");
+    if (ws_bytes < need || !ws) return fail(NEST_ERR_WORKSPACE, "gated ffn workspace too small: %zu < %zu bytes", ws_bytes, need);
+  }
+  GatedParams p = gated_params(f);
+  p.dy = dy;
+  p.dx = dx;
+  p.dw_gate = dw_gate;
+  p.dw_up = dw_up;
+  p.dw_down = dw_down;
+  uint8_t* w = static_cast<uint8_t*>(ws);
+  p.h = w;
+  p.dg = w + align_up(plan.h);
+  p.du = w + align_up(plan.h) + align_up(plan.dg);
+  p.kept_here = kept == nullptr;
+  p.kept = p.kept_here ? reinterpret_cast<float*>(w + align_up(plan.h) + align_up(plan.dg) + align_up(plan.du))
+                       : static_cast<float*>(const_cast<void*>(kept));
+  hipError_t e = launch_gated_ffn(p, static_cast<hipStream_t>(stream), true);
+  return e == hipSuccess ? NEST_OK : hip_fail(e, "gated ffn backward");
 }
 
 }  // extern "C"

@@ -1,0 +1,68 @@
+// Launch parameters of the decoder block's operators (layer_norm.hip,
+// dropout.hip, gated_ffn.hip), shared with the C ABI (abi.cpp).
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stddef.h>
+#include <stdint.h>
+
+#include "../../include/nest_splat.h"
+
+namespace nest {
+
+struct LayerNormParams {
+  int64_t rows;
+  int cols;
+  int dtype, param_dtype;
+  float eps;
+  const void* x;
+  const void* weight;
+  const void* bias;    // may be null
+  void* y;             // forward
+  float* mean;         // [rows]; the forward's may be null
+  float* rstd;
+  const void* dy;      // backward
+  void* dx;
+  void* dweight;
+  void* dbias;         // may be null
+  float* part;         // [layer_norm_partials][2][cols]
+};
+int layer_norm_partials(int64_t rows, int cols, int dtype);
+hipError_t launch_layer_norm(const LayerNormParams& p, hipStream_t s);
+hipError_t launch_layer_norm_backward(const LayerNormParams& p, hipStream_t s);
+
+struct DropoutParams {
+  int64_t n;
+  int dtype;
+  const void* x;
+  const void* residual;   // may be null
+  void* y;
+  uint32_t threshold;     // a 16-bit random number below it drops the element
+  float scale;
+  uint64_t seed, offset;
+};
+hipError_t launch_dropout(const DropoutParams& p, hipStream_t s);
+
+struct GatedParams {
+  int64_t rows;
+  int in, hidden, out;
+  int dtype, activation;
+  const void* x;
+  const void* w_gate;
+  const void* w_up;
+  const void* w_down;
+  void* y;             // forward
+  const void* dy;      // backward
+  void* dx;            // each gradient may be null
+  void* dw_gate;
+  void* dw_up;
+  void* dw_down;
+  float* kept;         // [rows][2 hidden] pre-activations, or null
+  int kept_here;       // the backward computes them itself, into its workspace
+  void* h;             // workspace
+  void* dg;
+  void* du;
+};
+hipError_t launch_gated_ffn(const GatedParams& p, hipStream_t s, bool backward);
+
+}  // namespace nest

@@ -27,7 +27,7 @@ MAX_LEVELS = 32
 MAX_CHANNELS = 128
 OTHERS_CHANNELS = 14
 
-ABI_VERSION = 18
+ABI_VERSION = 19
 SCAN_NOALLOC_MAX = 268431360
 (GEOM_DEPTH, GEOM_XY, GEOM_TILES, GEOM_OFFSETS, GEOM_RECORDS, GEOM_RADII, GEOM_SCAN_TMP, GEOM_DEPTH_ORDER,
  GEOM_ORDER_OFFSETS, GEOM_ORDER_TMP, GEOM_RGB, GEOM_CLAMPED, GEOM_RECT, GEOM_ORDER_RECT) = range(14)
@@ -135,6 +135,16 @@ class RvqAttr(ct.Structure):
 
 RVQ_BATCH_MAX = 4
 
+ACT_RELU, ACT_SILU, ACT_GELU = 0, 1, 2
+
+
+class GatedFfn(ct.Structure):
+    _fields_ = [("struct_size", ct.c_uint32), ("dtype", ct.c_int32), ("activation", ct.c_int32),
+                ("in_features", ct.c_int32), ("hidden", ct.c_int32), ("out_features", ct.c_int32),
+                ("rows", ct.c_int64), ("x", ct.c_void_p), ("w_gate", ct.c_void_p), ("w_up", ct.c_void_p),
+                ("w_down", ct.c_void_p)]
+
+
 EXPORTS = {
     "nest_abi_version": (ct.c_int, []),
     "nest_last_error": (ct.c_char_p, []),
@@ -181,6 +191,20 @@ EXPORTS = {
     "nest_rvq_decode": (ct.c_int, [ct.c_int64, ct.c_int32, ct.c_int32, ct.c_int32, ct.c_void_p, ct.c_void_p,
                                    ct.POINTER(ct.c_float), ct.c_int32, ct.c_void_p, ct.c_void_p, ct.c_void_p]),
     "nest_rvq_decode_batch": (ct.c_int, [ct.c_int32, ct.POINTER(RvqAttr), ct.c_void_p]),
+    "nest_layer_norm": (ct.c_int, [ct.c_int64, ct.c_int32, ct.c_int32, ct.c_int32, ct.c_void_p, ct.c_void_p,
+                                   ct.c_void_p, ct.c_float, ct.c_void_p, ct.c_void_p, ct.c_void_p, ct.c_void_p]),
+    "nest_layer_norm_backward_workspace_size": (ct.c_size_t, [ct.c_int64, ct.c_int32, ct.c_int32]),
+    "nest_layer_norm_backward": (ct.c_int, [ct.c_int64, ct.c_int32, ct.c_int32, ct.c_int32, ct.c_void_p, ct.c_void_p,
+                                            ct.c_void_p, ct.c_void_p, ct.c_void_p, ct.c_void_p, ct.c_void_p,
+                                            ct.c_void_p, ct.c_void_p, ct.c_size_t, ct.c_void_p]),
+    "nest_dropout": (ct.c_int, [ct.c_int64, ct.c_int32, ct.c_void_p, ct.c_void_p, ct.c_double, ct.c_uint64,
+                                ct.c_uint64, ct.c_void_p, ct.c_void_p]),
+    "nest_gated_ffn_sizes": (ct.c_int, [ct.POINTER(GatedFfn), ct.POINTER(ct.c_size_t), ct.POINTER(ct.c_size_t),
+                                        ct.POINTER(ct.c_size_t), ct.POINTER(ct.c_size_t)]),
+    "nest_gated_ffn_forward": (ct.c_int, [ct.POINTER(GatedFfn), ct.c_void_p, ct.c_void_p, ct.c_void_p, ct.c_size_t,
+                                          ct.c_void_p]),
+    "nest_gated_ffn_backward": (ct.c_int, [ct.POINTER(GatedFfn), ct.c_void_p, ct.c_void_p, ct.c_void_p, ct.c_void_p,
+                                           ct.c_void_p, ct.c_void_p, ct.c_void_p, ct.c_size_t, ct.c_void_p]),
 }
 
 _lib = None
