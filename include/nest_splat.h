@@ -572,7 +572,8 @@ int nest_rvq_decode_batch(int32_t n, const nest_rvq_attr *attrs, void *stream);
  * colour head, forward and backward.  dtype is that of x, y and their
  * gradients (F32, F16 or BF16); rows are contiguous and row-major, with any
  * row length and any alignment of the element type.  Sums are float32, each
- * result is rounded once. */
+ * result is rounded once.  The pointers of nest_gated_ffn_* are multiples of
+ * 16 bytes. */
 
 /* y = (x - mean) rstd w + b over each row of x [rows, cols], rstd =
  * 1/sqrt(var + eps) with the variance about the mean, divided by cols.

@@ -24,7 +24,8 @@ OUT = os.path.join(HERE, "nest_splat", "libnest_splat.so")
 INCLUDE = os.path.join(os.path.dirname(HERE), "include")
 
 SOURCES = ["abi.cpp", "preprocess.hip", "binning.hip", "render.hip", "backward.hip", "grid_encode.hip", "mlp.hip",
-           "rvq.hip", "surface.hip", "layer_norm.hip", "dropout.hip", "gated_ffn.hip"]
+           "rvq.hip", "surface.hip", "layer_norm.hip", "dropout.hip", "gated_ffn.hip",
+           "gated_ffn_f32.hip", "gated_ffn_f16.hip", "gated_ffn_bf16.hip"]
 
 HIPCC = shutil.which("hipcc") or "/opt/rocm/bin/hipcc"
 ARCH = os.environ.get("NEST_OFFLOAD_ARCH", "gfx950")

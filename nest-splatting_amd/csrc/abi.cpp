@@ -15,6 +15,7 @@
 #include <cstdarg>
 #include <cstdio>
 #include <cstring>
+#include <initializer_list>
 #include <mutex>
 #include <string>
 
@@ -1402,13 +1403,7 @@ int check_norm(int64_t rows, int32_t cols, int32_t dtype, int32_t param_dtype) {
   return NEST_OK;
 }
 
-struct GatedPlan {
-  size_t kept, h, dg, du, own_kept;   // bytes
-  size_t forward() const { return align_up(h); }
-  size_t backward(bool alone) const { return align_up(h) + align_up(dg) + align_up(du) + (alone ? align_up(own_kept) : 0); }
-};
-
-int check_gated(const nest_gated_ffn* f, GatedPlan& plan) {
+int check_gated(const nest_gated_ffn* f) {
   if (!f || f->struct_size != sizeof(nest_gated_ffn)) return fail(NEST_ERR_INVALID_ARGUMENT, "nest_gated_ffn missing or struct_size mismatch");
   if (f->rows < 0 || f->rows >= kMaxRows) return fail(NEST_ERR_INVALID_ARGUMENT, "rows must be in [0, 2^31) (got %lld)", (long long)f->rows);
   const int32_t sides[3] = {f->in_features, f->hidden, f->out_features};
@@ -1417,11 +1412,17 @@ int check_gated(const nest_gated_ffn* f, GatedPlan& plan) {
   if (!element_type(f->dtype)) return fail(NEST_ERR_UNSUPPORTED, "dtype must be float32, float16 or bfloat16");
   if (f->activation != NEST_ACT_RELU && f->activation != NEST_ACT_SILU && f->activation != NEST_ACT_GELU)
     return fail(NEST_ERR_UNSUPPORTED, "activation must be relu, silu or gelu");
-  const size_t es = f->dtype == NEST_DTYPE_F32 ? 4 : 2;
-  const size_t n = (size_t)f->rows * (size_t)f->hidden;
-  plan.kept = plan.own_kept = n * 2 * sizeof(float);
-  plan.h = plan.dg = plan.du = n * es;
   return NEST_OK;
+}
+
+GatedLayout layout_of(const nest_gated_ffn* f, bool backward, bool alone) {
+  return gated_layout(f->rows, f->in_features, f->hidden, f->out_features, f->dtype, backward, alone);
+}
+
+bool aligned16(std::initializer_list<const void*> ps) {
+  for (const void* p : ps)
+    if (reinterpret_cast<uintptr_t>(p) % 16) return false;
+  return true;
 }
 
 GatedParams gated_params(const nest_gated_ffn* f) {
@@ -1517,51 +1518,49 @@ int nest_dropout(int64_t n, int32_t dtype, const void* x, const void* residual, 
 
 int nest_gated_ffn_sizes(const nest_gated_ffn* f, size_t* kept, size_t* forward_ws, size_t* backward_ws,
                          size_t* backward_ws_alone) {
-  GatedPlan plan;
-  if (int rc = check_gated(f, plan); rc != NEST_OK) return rc;
-  if (kept) *kept = plan.kept;
-  if (forward_ws) *forward_ws = plan.forward();
-  if (backward_ws) *backward_ws = plan.backward(false);
-  if (backward_ws_alone) *backward_ws_alone = plan.backward(true);
+  if (int rc = check_gated(f); rc != NEST_OK) return rc;
+  const GatedLayout fwd = layout_of(f, false, false);
+  if (kept) *kept = fwd.kept_bytes;
+  if (forward_ws) *forward_ws = fwd.bytes;
+  if (backward_ws) *backward_ws = layout_of(f, true, false).bytes;
+  if (backward_ws_alone) *backward_ws_alone = layout_of(f, true, true).bytes;
   return NEST_OK;
 }
 
 int nest_gated_ffn_forward(const nest_gated_ffn* f, void* y, void* kept, void* ws, size_t ws_bytes, void* stream) {
-  GatedPlan plan;
-  if (int rc = check_gated(f, plan); rc != NEST_OK) return rc;
+  if (int rc = check_gated(f); rc != NEST_OK) return rc;
   if (f->rows == 0) return NEST_OK;
   if (!f->x || !f->w_gate || !f->w_up || !f->w_down || !y) return fail(NEST_ERR_INVALID_ARGUMENT, "NULL tensor pointer");
-  if (ws_bytes < plan.forward() || !ws) return fail(NEST_ERR_WORKSPACE, "gated ffn workspace too small: %zu < %zu bytes", ws_bytes, plan.forward());
+  const size_t need = layout_of(f, false, false).bytes;
+  if (ws_bytes < need || (need && !ws)) return fail(NEST_ERR_WORKSPACE, "gated ffn workspace too small: %zu < %zu bytes", ws_bytes, need);
+  if (!aligned16({f->x, f->w_gate, f->w_up, f->w_down, y, kept, ws})) return fail(NEST_ERR_INVALID_ARGUMENT, "gated ffn pointers must be 16-byte aligned");
   GatedParams p = gated_params(f);
   p.y = y;
   p.kept = static_cast<float*>(kept);
-  p.h = ws;
+  p.ws = ws;
   hipError_t e = launch_gated_ffn(p, static_cast<hipStream_t>(stream), false);
   return e == hipSuccess ? NEST_OK : hip_fail(e, "gated ffn");
 }
 
 int nest_gated_ffn_backward(const nest_gated_ffn* f, const void* dy, const void* kept, void* dx, void* dw_gate,
                             void* dw_up, void* dw_down, void* ws, size_t ws_bytes, void* stream) {
-  GatedPlan plan;
-  if (int rc = check_gated(f, plan); rc != NEST_OK) return rc;
-  const size_t need = plan.backward(kept == nullptr);
+  if (int rc = check_gated(f); rc != NEST_OK) return rc;
+  if (!dx && !dw_gate && !dw_up && !dw_down) return NEST_OK;
   if (f->rows > 0) {
     if (!f->x || !f->w_gate || !f->w_up || !f->w_down || !dy) return fail(NEST_ERR_INVALID_ARGUMENT, "NULL tensor pointer");
-    if (ws_bytes < need || !ws) return fail(NEST_ERR_WORKSPACE, "gated ffn workspace too small: %zu < %zu bytes", ws_bytes, need);
+    const size_t need = layout_of(f, true, kept == nullptr).bytes;
+    if (ws_bytes < need || (need && !ws)) return fail(NEST_ERR_WORKSPACE, "gated ffn workspace too small: %zu < %zu bytes", ws_bytes, need);
+    if (!aligned16({f->x, f->w_gate, f->w_up, f->w_down, dy, kept, dx, dw_gate, dw_up, dw_down, ws}))
+      return fail(NEST_ERR_INVALID_ARGUMENT, "gated ffn pointers must be 16-byte aligned");
   }
   GatedParams p = gated_params(f);
   p.dy = dy;
+  p.kept = static_cast<float*>(const_cast<void*>(kept));
   p.dx = dx;
   p.dw_gate = dw_gate;
   p.dw_up = dw_up;
   p.dw_down = dw_down;
-  uint8_t* w = static_cast<uint8_t*>(ws);
-  p.h = w;
-  p.dg = w + align_up(plan.h);
-  p.du = w + align_up(plan.h) + align_up(plan.dg);
-  p.kept_here = kept == nullptr;
-  p.kept = p.kept_here ? reinterpret_cast<float*>(w + align_up(plan.h) + align_up(plan.dg) + align_up(plan.du))
-                       : static_cast<float*>(const_cast<void*>(kept));
+  p.ws = ws;
   hipError_t e = launch_gated_ffn(p, static_cast<hipStream_t>(stream), true);
   return e == hipSuccess ? NEST_OK : hip_fail(e, "gated ffn backward");
 }

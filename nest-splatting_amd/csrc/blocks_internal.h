@@ -57,12 +57,28 @@ struct GatedParams {
   void* dw_gate;
   void* dw_up;
   void* dw_down;
-  float* kept;         // [rows][2 hidden] pre-activations, or null
-  int kept_here;       // the backward computes them itself, into its workspace
-  void* h;             // workspace
-  void* dg;
-  void* du;
+  float* kept;         // [rows][2 ldh] pre-activations a forward writes or a backward reads, or null
+  void* ws;
 };
+
+// Tiles of side x side, k split over `splits` workgroups a tile.
+struct TileChoice {
+  int side, splits;
+};
+
+// What a call's sizes fix: row lengths (rounded up to 16 bytes), the
+// workspace's parts (byte offsets) and each product's tiles.
+struct GatedLayout {
+  int64_t ldx, ldh, ldy;
+  size_t h, dg, du, kept, x, wg, wu, wd, dy, part;
+  size_t bytes, kept_bytes;
+  TileChoice y, dx, dw;
+};
+GatedLayout gated_layout(int64_t rows, int in, int hidden, int out, int dtype, bool backward, bool alone);
+TileChoice choose_gate_tile(int64_t M, int64_t N, int64_t K, int es);
 hipError_t launch_gated_ffn(const GatedParams& p, hipStream_t s, bool backward);
+hipError_t gated_ffn_f32(const GatedParams& p, hipStream_t s, bool backward);
+hipError_t gated_ffn_f16(const GatedParams& p, hipStream_t s, bool backward);
+hipError_t gated_ffn_bf16(const GatedParams& p, hipStream_t s, bool backward);
 
 }  // namespace nest

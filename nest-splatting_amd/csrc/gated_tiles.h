@@ -1,0 +1,412 @@
+// The products of a gated feed-forward block as tiles of tile_gemm.h, for one
+// element type: included by gated_ffn_f32.hip, gated_ffn_f16.hip and
+// gated_ffn_bf16.hip.
+//
+//   g = x Wg^T,  u = x Wu^T,  h = act(g) u,  y = h Wd^T
+//   dh = dy Wd,  dg = dh u act'(g),  du = dh act(g)
+//   dx = dg Wg + du Wu,  dWg = dg^T x,  dWu = du^T x,  dWd = dy^T h
+//
+// One kernel makes g and u of the same tile (its weight tile takes 16 rows of
+// Wg, then the same 16 of Wu, so both land in the same lanes), applies the
+// activation and writes h; one makes dh and turns it into dg, du and h with
+// the kept g and u; dx is one sum over both pairs; the three weight gradients
+// share a launch.  Every product is summed in float32.  g and u are kept in
+// float32, because rounding them to 16 bits would make the gradients' error
+// nearly twice one rounding; h, dg and du are rounded to the inputs' type, as
+// operands of the next product.
+//
+// Operands whose rows are no multiple of 16 bytes are copied to padded rows
+// first (pad_kernel), so that the tiles have one way to load.
+#pragma once
+
+#include "blocks_internal.h"
+#include "tile_gemm.h"
+
+namespace nest {
+namespace {
+
+// ---- activations and their slopes ----
+
+__device__ __forceinline__ float act_value(int act, float g) {
+  if (act == NEST_ACT_RELU) return g <= 0.0f ? 0.0f : g;  // NaN stays
+  if (act == NEST_ACT_SILU) return g / (1.0f + expf(-g));
+  return 0.5f * g * (1.0f + erff(g * 0.70710678118654752f));
+}
+
+__device__ __forceinline__ float act_slope(int act, float g) {
+  if (act == NEST_ACT_RELU) return g > 0.0f ? 1.0f : 0.0f;
+  if (act == NEST_ACT_SILU) {
+    const float q = 1.0f / (1.0f + expf(-g));
+    return q * (1.0f + g * (1.0f - q));
+  }
+  return 0.5f * (1.0f + erff(g * 0.70710678118654752f)) + g * expf(-0.5f * g * g) * 0.39894228040143268f;
+}
+
+template <typename T>
+struct alignas(4 * sizeof(T)) Four {
+  T v[4];
+};
+
+// Four columns n .. n + 3 of a row of N values.
+template <typename T>
+__device__ __forceinline__ void store4(T* row, int n, int N, bool aligned, f32x4 v) {
+  if (aligned && n + 4 <= N) {
+    Four<T> t;
+#pragma unroll
+    for (int i = 0; i < 4; i++) t.v[i] = from_f32<T>(v[i]);
+    *reinterpret_cast<Four<T>*>(row + n) = t;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+      if (n + i < N) row[n + i] = from_f32<T>(v[i]);
+  }
+}
+
+// ---- C = A B (+ A2 B2), up to three products in a launch, k split over `splits` ----
+
+template <typename T>
+struct Product {
+  const T *a, *b, *a2, *b2;
+  int64_t lda, ldb;
+  int M, N;
+  int64_t K;
+  T* c;               // [M][N]
+  int tiles_m, tiles_n;
+  int64_t part;       // offset in a slice of the partial sums
+};
+
+template <typename T>
+struct Products {
+  Product<T> p[3];
+  int n, splits;
+  float* part;        // [splits][part_size], or null where splits is 1
+  int64_t part_size;
+};
+
+template <typename T, bool kAK, bool kBK, typename C>
+__global__ __launch_bounds__(C::NT) void product_kernel(Products<T> all) {
+  const int split = all.splits > 1 ? blockIdx.x % all.splits : 0;
+  int id = all.splits > 1 ? blockIdx.x / all.splits : blockIdx.x, which = 0;
+  while (which + 1 < all.n && id >= all.p[which].tiles_m * all.p[which].tiles_n) {
+    id -= all.p[which].tiles_m * all.p[which].tiles_n;
+    which++;
+  }
+  const Product<T>& p = all.p[which];
+  int tm, tn;
+  tile_of(id, p.tiles_m, p.tiles_n, tm, tn);
+  constexpr int kStep = kStepBytes / (int)sizeof(T);
+  const int64_t per = ((p.K + kStep - 1) / kStep + all.splits - 1) / all.splits * kStep;
+  const int64_t k0 = split * per, k = p.K - k0 < per ? p.K - k0 : per;
+  const int64_t m0 = (int64_t)tm * C::BM, n0 = (int64_t)tn * C::BN;
+  f32x4 acc[C::FM][C::FN] = {};
+  if (k > 0) {
+    Loader<T, kAK, C::BM, C::NT> la;
+    Loader<T, kBK, C::BN, C::NT> lb;
+    const int64_t ka = kAK ? k0 : k0 * p.lda, kb = kBK ? k0 : k0 * p.ldb;
+    const char *a2 = nullptr, *b2 = nullptr;
+    if (p.a2) {
+      la.init(p.a2 + ka, p.lda, m0, kAK ? p.M : p.lda);
+      lb.init(p.b2 + kb, p.ldb, n0, kBK ? p.N : p.ldb);
+      a2 = la.base;
+      b2 = lb.base;
+    }
+    la.init(p.a + ka, p.lda, m0, kAK ? p.M : p.lda);
+    lb.init(p.b + kb, p.ldb, n0, kBK ? p.N : p.ldb);
+    tile_product<T, kAK, kBK, C>(la, lb, k, a2, b2, acc);
+  }
+  const int lane = threadIdx.x & 63, w = wave_id();
+  const int64_t m = m0 + (w / C::WN) * C::FM * 16 + (lane & 15);
+  const int n = (int)n0 + (w % C::WN) * C::FN * 16 + (lane >> 4) * 4;
+#pragma unroll
+  for (int i = 0; i < C::FM; i++) {
+    if (m + i * 16 >= p.M) continue;
+#pragma unroll
+    for (int j = 0; j < C::FN; j++) {
+      if (all.part) store4(all.part + split * all.part_size + p.part + (m + i * 16) * p.N, n + j * 16, p.N, p.N % 4 == 0, acc[i][j]);
+      else store4(p.c + (m + i * 16) * p.N, n + j * 16, p.N, p.N % 4 == 0, acc[i][j]);
+    }
+  }
+}
+
+// Joins the partial sums, in the order of the splits.
+template <typename T>
+__global__ __launch_bounds__(256) void join_kernel(Products<T> all) {
+  for (int64_t e = ((int64_t)blockIdx.x * 256 + threadIdx.x); e < all.part_size; e += (int64_t)gridDim.x * 256) {
+    float s = 0.0f;
+    for (int i = 0; i < all.splits; i++) s += all.part[i * all.part_size + e];
+    int which = 0;
+    while (which + 1 < all.n && e >= all.p[which + 1].part) which++;
+    const Product<T>& p = all.p[which];
+    if (e - p.part < (int64_t)p.M * p.N) p.c[e - p.part] = from_f32<T>(s);
+  }
+}
+
+// ---- h = act(g) u ----
+
+template <typename T>
+struct Gate {
+  const T *x, *wg, *wu;   // [M][ldx], [H][ldx]
+  int64_t ldx;
+  int M, H;
+  int64_t ldh;            // H rounded up to 16 bytes: the pad columns are written as zeros
+  T* h;                   // [M][ldh] or null
+  float* kept;            // [M][2 ldh]: g, then u; or null
+  int act, tiles_m, tiles_n;
+};
+
+template <typename T, typename C>
+__global__ __launch_bounds__(C::NT) void gate_kernel(Gate<T> p) {
+  int tm, tn;
+  tile_of(blockIdx.x, p.tiles_m, p.tiles_n, tm, tn);
+  const int64_t m0 = (int64_t)tm * C::BM, n0 = (int64_t)tn * (C::BN / 2);
+  f32x4 acc[C::FM][C::FN] = {};
+  Loader<T, true, C::BM, C::NT> la;
+  Loader<T, true, C::BN, C::NT> lb;
+  la.init(p.x, p.ldx, m0, p.M);
+  lb.init_pair(p.wg, p.wu, p.ldx, n0, p.H);
+  tile_product<T, true, true, C>(la, lb, p.ldx, nullptr, nullptr, acc);
+  const int lane = threadIdx.x & 63, w = wave_id();
+  const int64_t m = m0 + (w / C::WN) * C::FM * 16 + (lane & 15);
+  const int n = (int)n0 + (w % C::WN) * C::FN * 8 + (lane >> 4) * 4;
+#pragma unroll
+  for (int i = 0; i < C::FM; i++) {
+    if (m + i * 16 >= p.M) continue;
+#pragma unroll
+    for (int j = 0; j < C::FN; j += 2) {
+      const f32x4 g = acc[i][j], u = acc[i][j + 1];
+      const int c = n + j * 8;
+      if (p.h) {
+        f32x4 h;
+#pragma unroll
+        for (int e = 0; e < 4; e++) h[e] = act_value(p.act, g[e]) * u[e];
+        store4(p.h + (m + i * 16) * p.ldh, c, (int)p.ldh, true, h);
+      }
+      if (p.kept) {
+        store4(p.kept + (m + i * 16) * 2 * p.ldh, c, (int)p.ldh, true, g);
+        store4(p.kept + (m + i * 16) * 2 * p.ldh + p.ldh, c, (int)p.ldh, true, u);
+      }
+    }
+  }
+}
+
+// ---- dg, du and h from dh = dy Wd ----
+
+template <typename T>
+struct GateBackward {
+  const T *dy, *wd;       // [M][ldy], [O][ldh]
+  int64_t ldy, ldh;
+  int M, O;
+  const float* kept;
+  T *h, *dg, *du;         // [M][ldh]
+  int act, tiles_m, tiles_n;
+};
+
+template <typename T, typename C>
+__global__ __launch_bounds__(C::NT) void gate_backward_kernel(GateBackward<T> p) {
+  int tm, tn;
+  tile_of(blockIdx.x, p.tiles_m, p.tiles_n, tm, tn);
+  const int64_t m0 = (int64_t)tm * C::BM, n0 = (int64_t)tn * C::BN;
+  f32x4 acc[C::FM][C::FN] = {};
+  Loader<T, true, C::BM, C::NT> la;
+  Loader<T, false, C::BN, C::NT> lb;
+  la.init(p.dy, p.ldy, m0, p.M);
+  lb.init(p.wd, p.ldh, n0, p.ldh);
+  tile_product<T, true, false, C>(la, lb, p.O, nullptr, nullptr, acc);
+  const int lane = threadIdx.x & 63, w = wave_id();
+  const int64_t m = m0 + (w / C::WN) * C::FM * 16 + (lane & 15);
+  const int n = (int)n0 + (w % C::WN) * C::FN * 16 + (lane >> 4) * 4;
+#pragma unroll
+  for (int i = 0; i < C::FM; i++) {
+    const int64_t row = m + i * 16;
+    if (row >= p.M) continue;
+#pragma unroll
+    for (int j = 0; j < C::FN; j++) {
+      const int c = n + j * 16;
+      if (c >= p.ldh) continue;   // ldh is a multiple of 4: a lane's four columns are in or out together
+      const f32x4 g = *reinterpret_cast<const f32x4*>(p.kept + row * 2 * p.ldh + c);
+      const f32x4 u = *reinterpret_cast<const f32x4*>(p.kept + row * 2 * p.ldh + p.ldh + c);
+      f32x4 h, dg, du;
+#pragma unroll
+      for (int e = 0; e < 4; e++) {
+        const float a = act_value(p.act, g[e]), d = acc[i][j][e];
+        h[e] = a * u[e];
+        dg[e] = d * u[e] * act_slope(p.act, g[e]);
+        du[e] = d * a;
+      }
+      store4(p.h + row * p.ldh, c, (int)p.ldh, true, h);
+      store4(p.dg + row * p.ldh, c, (int)p.ldh, true, dg);
+      store4(p.du + row * p.ldh, c, (int)p.ldh, true, du);
+    }
+  }
+}
+
+// ---- padded copies ----
+
+template <typename T>
+struct Pads {
+  const T* from[4];
+  T* to[4];
+  int64_t rows[4];
+  int n[4], ld[4];   // row lengths
+};
+
+template <typename T>
+__global__ __launch_bounds__(256) void pad_kernel(Pads<T> p) {
+  constexpr int N = Vec16<T>::kN;
+  const int k = blockIdx.y, n = p.n[k], chunks = p.ld[k] / N;
+  const int64_t total = p.rows[k] * chunks;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+    const int64_t row = i / chunks;
+    const int c = (int)(i % chunks) * N;
+    float v[N];
+    load_vec<T>(v, p.from[k] + row * n + c, n - c);
+    store_vec<T>(p.to[k] + row * p.ld[k] + c, v, N);
+  }
+}
+
+// ---- the choice of tiles, and launches ----
+
+template <typename T, bool kAK, bool kBK>
+hipError_t launch_products(Products<T>& all, TileChoice t, hipStream_t s) {
+  int64_t tiles = 0, part = 0;
+  for (int i = 0; i < all.n; i++) {
+    all.p[i].tiles_m = (all.p[i].M + t.side - 1) / t.side;
+    all.p[i].tiles_n = (all.p[i].N + t.side - 1) / t.side;
+    all.p[i].part = part;
+    tiles += (int64_t)all.p[i].tiles_m * all.p[i].tiles_n;
+    part += ((int64_t)all.p[i].M * all.p[i].N + 3) / 4 * 4;
+  }
+  all.splits = t.splits;
+  all.part_size = part;
+  if (t.splits == 1) all.part = nullptr;
+  const unsigned grid = (unsigned)(tiles * t.splits);
+  if (t.side == 256) {
+    if constexpr (sizeof(T) == 2) product_kernel<T, kAK, kBK, TileL><<<grid, TileL::NT, 0, s>>>(all);
+  } else if (t.side == 128) product_kernel<T, kAK, kBK, TileM><<<grid, TileM::NT, 0, s>>>(all);
+  else product_kernel<T, kAK, kBK, TileS><<<grid, TileS::NT, 0, s>>>(all);
+  if (t.splits > 1) {
+    const int64_t need = (part + 255) / 256;
+    join_kernel<T><<<(unsigned)(need < 65536 ? need : 65536), 256, 0, s>>>(all);
+  }
+  return hipGetLastError();
+}
+
+template <typename T>
+hipError_t launch_gate(Gate<T> p, hipStream_t s) {
+  const TileChoice t = choose_gate_tile(p.M, p.H * 2, p.ldx, sizeof(T));
+  p.tiles_m = (p.M + t.side - 1) / t.side;
+  p.tiles_n = (int)((p.ldh + t.side / 2 - 1) / (t.side / 2));
+  const unsigned grid = (unsigned)((int64_t)p.tiles_m * p.tiles_n);
+  if (t.side == 256) {
+    if constexpr (sizeof(T) == 2) gate_kernel<T, TileL><<<grid, TileL::NT, 0, s>>>(p);
+  } else if (t.side == 128) gate_kernel<T, TileM><<<grid, TileM::NT, 0, s>>>(p);
+  else gate_kernel<T, TileS><<<grid, TileS::NT, 0, s>>>(p);
+  return hipGetLastError();
+}
+
+template <typename T>
+hipError_t launch_gate_backward(GateBackward<T> p, hipStream_t s) {
+  const TileChoice t = choose_gate_tile(p.M, (int)p.ldh, p.O, sizeof(T));
+  p.tiles_m = (p.M + t.side - 1) / t.side;
+  p.tiles_n = (int)((p.ldh + t.side - 1) / t.side);
+  const unsigned grid = (unsigned)((int64_t)p.tiles_m * p.tiles_n);
+  if (t.side == 256) {
+    if constexpr (sizeof(T) == 2) gate_backward_kernel<T, TileL><<<grid, TileL::NT, 0, s>>>(p);
+  } else if (t.side == 128) gate_backward_kernel<T, TileM><<<grid, TileM::NT, 0, s>>>(p);
+  else gate_backward_kernel<T, TileS><<<grid, TileS::NT, 0, s>>>(p);
+  return hipGetLastError();
+}
+
+// The padded operands of a call: x and the weights, dy in a backward.
+template <typename T>
+struct Operands {
+  const T *x, *wg, *wu, *wd, *dy;
+};
+
+template <typename T>
+hipError_t pad_operands(const GatedParams& p, const GatedLayout& l, uint8_t* ws, bool back, Operands<T>& o, hipStream_t s) {
+  o = {static_cast<const T*>(p.x), static_cast<const T*>(p.w_gate), static_cast<const T*>(p.w_up),
+       static_cast<const T*>(p.w_down), static_cast<const T*>(p.dy)};
+  Pads<T> q{};
+  int n = 0;
+  int64_t most = 0;
+  auto add = [&](const T*& src, size_t at, int64_t rows, int len, int64_t ld) {
+    T* to = reinterpret_cast<T*>(ws + at);
+    q.from[n] = src;
+    q.to[n] = to;
+    q.rows[n] = rows;
+    q.n[n] = len;
+    q.ld[n++] = (int)ld;
+    if (rows * ld > most) most = rows * ld;
+    src = to;
+  };
+  if (l.ldx != p.in) {
+    add(o.x, l.x, p.rows, p.in, l.ldx);
+    add(o.wg, l.wg, p.hidden, p.in, l.ldx);
+    add(o.wu, l.wu, p.hidden, p.in, l.ldx);
+  }
+  if (l.ldh != p.hidden) add(o.wd, l.wd, p.out, p.hidden, l.ldh);
+  auto go = [&]() {
+    const int64_t need = (most / Vec16<T>::kN + 255) / 256;
+    pad_kernel<T><<<dim3((unsigned)(need < 4096 ? need : 4096), n), 256, 0, s>>>(q);
+  };
+  if (n == 4 && back && l.ldy != p.out) {   // five copies: the fifth by itself
+    go();
+    n = 0;
+    most = 0;
+  }
+  if (back && l.ldy != p.out) add(o.dy, l.dy, p.rows, p.out, l.ldy);
+  if (n) go();
+  return hipGetLastError();
+}
+
+template <typename T>
+hipError_t gated_forward(const GatedParams& p, hipStream_t s) {
+  const GatedLayout l = gated_layout(p.rows, p.in, p.hidden, p.out, p.dtype, false, false);
+  uint8_t* ws = static_cast<uint8_t*>(p.ws);
+  Operands<T> o;
+  if (hipError_t e = pad_operands(p, l, ws, false, o, s); e != hipSuccess) return e;
+  T* h = reinterpret_cast<T*>(ws + l.h);
+  Gate<T> g{o.x, o.wg, o.wu, l.ldx, (int)p.rows, p.hidden, l.ldh, h, p.kept, p.activation, 0, 0};
+  if (hipError_t e = launch_gate(g, s); e != hipSuccess) return e;
+  Products<T> y{};
+  y.n = 1;
+  y.p[0] = {h, o.wd, nullptr, nullptr, l.ldh, l.ldh, (int)p.rows, p.out, l.ldh, static_cast<T*>(p.y)};
+  y.part = reinterpret_cast<float*>(ws + l.part);
+  return launch_products<T, true, true>(y, l.y, s);
+}
+
+template <typename T>
+hipError_t gated_backward(const GatedParams& p, hipStream_t s) {
+  const bool alone = p.kept == nullptr;
+  const GatedLayout l = gated_layout(p.rows, p.in, p.hidden, p.out, p.dtype, true, alone);
+  uint8_t* ws = static_cast<uint8_t*>(p.ws);
+  T *h = reinterpret_cast<T*>(ws + l.h), *dg = reinterpret_cast<T*>(ws + l.dg), *du = reinterpret_cast<T*>(ws + l.du);
+  Operands<T> o;
+  if (hipError_t e = pad_operands(p, l, ws, true, o, s); e != hipSuccess) return e;
+  float* kept = p.kept;
+  if (alone) {
+    kept = reinterpret_cast<float*>(ws + l.kept);
+    Gate<T> g{o.x, o.wg, o.wu, l.ldx, (int)p.rows, p.hidden, l.ldh, nullptr, kept, p.activation, 0, 0};
+    if (hipError_t e = launch_gate(g, s); e != hipSuccess) return e;
+  }
+  GateBackward<T> b{o.dy, o.wd, l.ldy, l.ldh, (int)p.rows, p.out, kept, h, dg, du, p.activation, 0, 0};
+  if (hipError_t e = launch_gate_backward(b, s); e != hipSuccess) return e;
+  if (p.dx) {
+    Products<T> q{};
+    q.n = 1;
+    q.p[0] = {dg, o.wg, du, o.wu, l.ldh, l.ldx, (int)p.rows, p.in, p.hidden, static_cast<T*>(p.dx)};
+    q.part = reinterpret_cast<float*>(ws + l.part);
+    if (hipError_t e = launch_products<T, true, false>(q, l.dx, s); e != hipSuccess) return e;
+  }
+  Products<T> w{};
+  if (p.dw_gate) w.p[w.n++] = {dg, o.x, nullptr, nullptr, l.ldh, l.ldx, p.hidden, p.in, p.rows, static_cast<T*>(p.dw_gate)};
+  if (p.dw_up) w.p[w.n++] = {du, o.x, nullptr, nullptr, l.ldh, l.ldx, p.hidden, p.in, p.rows, static_cast<T*>(p.dw_up)};
+  if (p.dw_down) w.p[w.n++] = {o.dy, h, nullptr, nullptr, l.ldy, l.ldh, p.out, p.hidden, p.rows, static_cast<T*>(p.dw_down)};
+  if (!w.n) return hipSuccess;
+  w.part = reinterpret_cast<float*>(ws + l.part);
+  return launch_products<T, false, false>(w, l.dw, s);
+}
+
+}  // namespace
+}  // namespace nest

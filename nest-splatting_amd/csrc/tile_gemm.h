@@ -1,0 +1,247 @@
+// Matrix products on MFMA with operands staged by direct loads into LDS: the
+// tiles behind gated_ffn.
+//
+//   C[m][n] = sum_k A(m, k) B(n, k),  float32 sums
+//
+// An operand is stored with k contiguous ("kKM", rows of m or n) or with its
+// own index contiguous (rows of k); every row length is a multiple of 16
+// bytes.  A step takes 128 bytes of k (64 16-bit or 32 float32 values) of each
+// row.  Two LDS buffers: the loads of the next step are in flight while the
+// current one is multiplied, one barrier a step.
+//
+// LDS layouts.  k contiguous: rows of 128 bytes, the 16-byte chunk c of row r
+// at slot c ^ (r & 7), so the 16 rows one fragment load touches fall on
+// different banks.  k outermost: rows of R elements, 16-element units permuted
+// by the row so that the rows one transposing load touches do too.  The
+// permutation is done by the choice of what each lane loads: a direct load
+// always writes 64 x 16 consecutive bytes.
+//
+// Out of range: a lane whose chunk lies outside its operand gives the buffer
+// load an offset past the resource's size, which the hardware answers with
+// zero; zeros add nothing, whatever the other operand holds there being
+// finite or zero itself.
+#pragma once
+
+#include "vec_io.h"
+
+namespace nest {
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef short i16x4 __attribute__((ext_vector_type(4)));
+typedef short i16x8 __attribute__((ext_vector_type(8)));
+
+constexpr int kStepBytes = 128;
+constexpr uint32_t kOutside = 0x80000000u, kRecords = 0x7fffffffu;
+
+template <typename T>
+struct Mma;
+template <>
+struct Mma<bf16_t> {
+  typedef bf16x8 Frag;
+  static __device__ __forceinline__ f32x4 run(Frag a, Frag b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+};
+template <>
+struct Mma<f16_t> {
+  typedef f16x8 Frag;
+  static __device__ __forceinline__ f32x4 run(Frag a, Frag b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+};
+template <>
+struct Mma<float> {
+  typedef f32x4 Frag;   // k = 4 (lane / 16) + j in element j: any order that both operands share
+  static __device__ __forceinline__ f32x4 run(Frag a, Frag b, f32x4 c) {
+#pragma unroll
+    for (int j = 0; j < 4; j++) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[j], b[j], c, 0, 0, 0);
+    return c;
+  }
+};
+
+typedef __attribute__((address_space(3))) void LdsVoid;
+typedef __attribute__((address_space(3))) i16x4 LdsI16x4;
+
+__device__ __forceinline__ int wave_id() { return __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)); }
+
+// Unit permutation of a k-outermost row, for R / 16 units (a power of two).
+template <typename T, int R>
+__device__ __forceinline__ int unit_swizzle(int k) {
+  const int s = sizeof(T) == 2 ? (k & 3) | ((k >> 3) & 1) << 2 : (k >> 2) & 3;
+  return s & (R / 16 - 1);
+}
+
+// The direct loads of one operand's tile of R rows (kKM) or R columns.
+template <typename T, bool kKM, int R, int NT>
+struct Loader {
+  static constexpr int kVec = 16 / (int)sizeof(T), kLoads = R * 8 / NT;
+  static constexpr int kRow = R / kVec;              // chunks of a k-outermost row
+  static constexpr int kStep = kStepBytes / (int)sizeof(T);
+  static constexpr int kPer = kKM ? 0 : NT / kRow;   // rows of k between a lane's loads
+  uint32_t off[kLoads];
+  int k_first;            // this lane's first k inside a step
+  const char* base;
+  int64_t advance;
+
+  // Rows first .. first + R - 1 of n (kKM), or columns of a matrix of `n` columns.
+  __device__ __forceinline__ void init(const T* p, int64_t ld, int64_t first, int64_t n) {
+    const int t = threadIdx.x;
+    if constexpr (kKM) {
+      const int r = t >> 3, c = (t & 7) ^ (r & 7);
+      k_first = c * kVec;
+      base = reinterpret_cast<const char*>(p + first * ld);
+      advance = kStepBytes;
+#pragma unroll
+      for (int i = 0; i < kLoads; i++) {
+        const int row = r + i * (NT / 8);
+        off[i] = first + row < n ? (uint32_t)((row * ld + k_first) * (int64_t)sizeof(T)) : kOutside;
+      }
+    } else {
+      const int k = t / kRow, c = t % kRow;
+      constexpr int kUnit = (int)sizeof(T);          // chunks of a 16-element unit
+      k_first = k;
+      base = reinterpret_cast<const char*>(p + first);
+      advance = ld * kStepBytes;                     // kStep rows
+#pragma unroll
+      for (int i = 0; i < kLoads; i++) {
+        const int row = k + i * kPer;
+        const int col = ((c / kUnit) ^ unit_swizzle<T, R>(row)) * 16 + (c % kUnit) * kVec;
+        off[i] = first + col < n ? (uint32_t)((row * ld + col) * (int64_t)sizeof(T)) : kOutside;
+      }
+    }
+  }
+
+  // Two weight matrices as one tile of R rows: 16 rows of the first, the same
+  // 16 of the second, and so on; rows first .. first + R / 2 - 1 of n of each.
+  __device__ __forceinline__ void init_pair(const T* p0, const T* p1, int64_t ld, int64_t first, int64_t n) {
+    static_assert(!kKM || NT % 256 == 0, "a wave's loads stay with one matrix");
+    const int t = threadIdx.x;
+    const int r = t >> 3, c = (t & 7) ^ (r & 7);
+    k_first = c * kVec;
+    base = reinterpret_cast<const char*>(((wave_id() >> 1) & 1 ? p1 : p0) + first * ld);
+    advance = kStepBytes;
+#pragma unroll
+    for (int i = 0; i < kLoads; i++) {
+      const int lrow = r + i * (NT / 8);
+      const int row = (lrow >> 5) * 16 + (lrow & 15);
+      off[i] = first + row < n ? (uint32_t)((row * ld + k_first) * (int64_t)sizeof(T)) : kOutside;
+    }
+  }
+
+  // Loads the step at base into lds; k_left values of k remain.
+  __device__ __forceinline__ void issue(uint8_t* lds, int64_t k_left) const {
+    auto rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(base), (short)0, (int)kRecords, 0x00020000);
+    uint8_t* at = lds + wave_id() * 1024;
+#pragma unroll
+    for (int i = 0; i < kLoads; i++) {
+      const uint32_t v = k_first + i * kPer < k_left ? off[i] : kOutside;
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (LdsVoid*)(at + i * NT * 16), 16, (int)v, 0, 0, 0);
+    }
+  }
+};
+
+// The fragment of 16 rows (first a multiple of 16) at half kb of a step.
+template <typename T, bool kKM, int R>
+__device__ __forceinline__ typename Mma<T>::Frag fragment(const uint8_t* lds, int first, int kb) {
+  const int lane = threadIdx.x & 63, r = lane & 15, q = lane >> 4;
+  if constexpr (kKM) {
+    return *reinterpret_cast<const typename Mma<T>::Frag*>(lds + (first + r) * kStepBytes + (((kb * 4 + q) ^ (r & 7)) << 4));
+  } else if constexpr (sizeof(T) == 2) {
+    // each group of 16 lanes reads 4 rows of 16 values and gets them transposed
+    const int k = kb * 32 + q * 8 + (r >> 2), unit = first >> 4;
+    i16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+        (LdsI16x4*)(lds + k * (R * 2) + (unit ^ unit_swizzle<T, R>(k)) * 32 + (r & 3) * 8));
+    i16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+        (LdsI16x4*)(lds + (k + 4) * (R * 2) + (unit ^ unit_swizzle<T, R>(k + 4)) * 32 + (r & 3) * 8));
+    return __builtin_bit_cast(typename Mma<T>::Frag, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+  } else {
+    f32x4 f;
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+      const int k = kb * 16 + q * 4 + j;
+      f[j] = *reinterpret_cast<const float*>(lds + k * (R * 4) + ((((first >> 4) ^ unit_swizzle<T, R>(k)) * 16) + r) * 4);
+    }
+    return f;
+  }
+}
+
+// BM x BN by WM x WN waves of (16 FM) x (16 FN).
+template <int kBM, int kBN, int kWM, int kWN>
+struct Tile {
+  static constexpr int BM = kBM, BN = kBN, WM = kWM, WN = kWN, NT = 64 * WM * WN, FM = BM / WM / 16, FN = BN / WN / 16;
+};
+typedef Tile<256, 256, 2, 4> TileL;
+typedef Tile<128, 128, 2, 2> TileM;
+typedef Tile<64, 64, 2, 2> TileS;
+
+// acc[i][j]: rows m = 16 i + lane % 16, columns n = 16 j + 4 (lane / 16) + 0..3
+// of the wave's part.  `steps` steps of k from each of `segments` operand
+// pairs; a2 and b2: the second pair's bases.
+template <typename T, bool kAK, bool kBK, typename C>
+__device__ __forceinline__ void tile_product(Loader<T, kAK, C::BM, C::NT>& la, Loader<T, kBK, C::BN, C::NT>& lb, int64_t K,
+                                             const char* a2, const char* b2, f32x4 (&acc)[C::FM][C::FN]) {
+  __shared__ __attribute__((aligned(16))) uint8_t a_lds0[C::BM * kStepBytes];
+  __shared__ __attribute__((aligned(16))) uint8_t b_lds0[C::BN * kStepBytes];
+  __shared__ __attribute__((aligned(16))) uint8_t a_lds1[C::BM * kStepBytes];
+  __shared__ __attribute__((aligned(16))) uint8_t b_lds1[C::BN * kStepBytes];
+  constexpr int kStep = kStepBytes / (int)sizeof(T);
+  const int steps = (int)((K + kStep - 1) / kStep);
+  const int total = a2 ? 2 * steps : steps;
+  int64_t k_left = K;
+  int next = 0;
+  auto issue = [&](uint8_t* a, uint8_t* b) {
+    if (next == steps) {   // the second pair
+      la.base = a2;
+      lb.base = b2;
+      k_left = K;
+    }
+    la.issue(a, k_left);
+    lb.issue(b, k_left);
+    la.base += la.advance;
+    lb.base += lb.advance;
+    k_left -= kStep;
+    next++;
+  };
+  const int w = wave_id(), wm = (w / C::WN) * C::FM * 16, wn = (w % C::WN) * C::FN * 16;
+  auto multiply = [&](const uint8_t* a, const uint8_t* b) {
+#pragma unroll
+    for (int kb = 0; kb < 2; kb++) {
+      typename Mma<T>::Frag fa[C::FM], fb[C::FN];
+#pragma unroll
+      for (int i = 0; i < C::FM; i++) fa[i] = fragment<T, kAK, C::BM>(a, wm + i * 16, kb);
+#pragma unroll
+      for (int j = 0; j < C::FN; j++) fb[j] = fragment<T, kBK, C::BN>(b, wn + j * 16, kb);
+#pragma unroll
+      for (int i = 0; i < C::FM; i++)
+#pragma unroll
+        for (int j = 0; j < C::FN; j++) acc[i][j] = Mma<T>::run(fb[j], fa[i], acc[i][j]);
+    }
+  };
+  issue(a_lds0, b_lds0);
+  int s = 0;
+  for (; s + 1 < total; s += 2) {
+    __syncthreads();   // buffer 0 has landed, buffer 1 is no longer read
+    issue(a_lds1, b_lds1);
+    multiply(a_lds0, b_lds0);
+    __syncthreads();
+    if (s + 2 < total) issue(a_lds0, b_lds0);
+    multiply(a_lds1, b_lds1);
+  }
+  if (s < total) {
+    __syncthreads();
+    multiply(a_lds0, b_lds0);
+  }
+}
+
+// The tile of a workgroup.  Workgroups go to the eight XCDs in turn, each with
+// an L2 of its own: XCD x takes the x-th contiguous part of the tiles, and
+// runs through them 4 rows at a time, so that the 32 tiles in flight there
+// share 4 row panels and 8 column panels.
+__device__ __forceinline__ void tile_of(int id, int tiles_m, int tiles_n, int& tm, int& tn) {
+  const int n = tiles_m * tiles_n, q = n / 8, r = n % 8, x = id % 8, l = id / 8;
+  const int t = x < r ? x * (q + 1) + l : r * (q + 1) + (x - r) * q + l;
+  const int group = t / (4 * tiles_n), rest = t % (4 * tiles_n);
+  const int rows = tiles_m - group * 4 < 4 ? tiles_m - group * 4 : 4;
+  tm = group * 4 + rest % rows;
+  tn = rest / rows;
+}
+
+}  // namespace nest

@@ -55,6 +55,11 @@ def _like(t: torch.Tensor, ref: torch.Tensor, shape, name: str, dtype=None) -> t
     return t.detach().contiguous()
 
 
+def _aligned(t: torch.Tensor) -> torch.Tensor:
+    """t at an address of a multiple of 16 bytes: a view into the middle of another tensor is copied."""
+    return t.clone() if t.data_ptr() % 16 else t
+
+
 class _on:
     """Makes the tensors' device the current one around a launch, where it is not already."""
 
@@ -199,8 +204,8 @@ def _gated(x, w_gate, w_up, w_down, activation):
     I, H, O = x.shape[-1], w_gate.shape[0], w_down.shape[0]
     if min(I, H, O) < 1:
         raise ValueError("in_features, hidden and out_features must be at least 1")
-    x = x.detach().contiguous()
-    ws = (_like(w_gate, x, (H, I), "w_gate"), _like(w_up, x, (H, I), "w_up"), _like(w_down, x, (O, H), "w_down"))
+    x = _aligned(x.detach().contiguous())
+    ws = tuple(_aligned(_like(w, x, s, n)) for w, s, n in ((w_gate, (H, I), "w_gate"), (w_up, (H, I), "w_up"), (w_down, (O, H), "w_down")))
     rows = x.numel() // I
     f = L.GatedFfn(ct.sizeof(L.GatedFfn), code, _ACT[activation], I, H, O, rows, x.data_ptr(), *(w.data_ptr() for w in ws))
     return f, x, ws
@@ -234,7 +239,7 @@ def gated_ffn_backward(dy: torch.Tensor, x: torch.Tensor, w_gate: torch.Tensor, 
     """(dx, dw_gate, dw_up, dw_down); ``needs``: which of them are wanted, the others are None. ``kept``: what the
     forward call with the same arguments returned; None computes it again."""
     f, x, ws = _gated(x, w_gate, w_up, w_down, activation)
-    dy = _like(dy, x, x.shape[:-1] + (f.out_features,), "dy")
+    dy = _aligned(_like(dy, x, x.shape[:-1] + (f.out_features,), "dy"))
     kept_bytes, _, bwd_bytes, alone_bytes = _gated_sizes(f)
     if kept is not None and (kept.dtype != torch.uint8 or kept.numel() != kept_bytes or not kept.is_contiguous()
                              or kept.device != x.device):
