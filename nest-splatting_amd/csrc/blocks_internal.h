@@ -57,7 +57,7 @@ struct GatedParams {
   void* dw_gate;
   void* dw_up;
   void* dw_down;
-  float* kept;         // [rows][2 ldh] pre-activations a forward writes or a backward reads, or null
+  float* kept;         // pre-activations a forward writes or a backward reads, or null
   void* ws;
 };
 

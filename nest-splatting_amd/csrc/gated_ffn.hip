@@ -67,6 +67,7 @@ GatedLayout gated_layout(int64_t rows, int in, int hidden, int out, int dtype, b
   l.ldx = up(in);
   l.ldh = up(hidden);
   l.ldy = up(out);
+  const int64_t kept_bytes = cdiv(rows, 16) * cdiv(l.ldh, 16) * 2048;   // blocks of 16 x 16 g and u
   size_t at = 0;
   auto take = [&](int64_t bytes) {
     const size_t o = at;
@@ -96,7 +97,7 @@ GatedLayout gated_layout(int64_t rows, int in, int hidden, int out, int dtype, b
     const int64_t WM[3] = {hidden, hidden, out}, WN[3] = {in, in, hidden};
     l.dw = choose_tile(3, WM, WN, rows, es, true);
     partial(l.dw, 3, WM, WN);
-    if (alone) l.kept = take(rows * 2 * l.ldh * 4);
+    if (alone) l.kept = take(kept_bytes);
     if (l.ldy != out) l.dy = take(rows * l.ldy * es);
   }
   if (l.ldx != in) {
@@ -107,7 +108,7 @@ GatedLayout gated_layout(int64_t rows, int in, int hidden, int out, int dtype, b
   if (l.ldh != hidden) l.wd = take(out * l.ldh * es);
   l.part = take(part);
   l.bytes = at;
-  l.kept_bytes = (size_t)rows * 2 * (size_t)l.ldh * 4;
+  l.kept_bytes = (size_t)kept_bytes;
   return l;
 }
 

@@ -27,19 +27,48 @@ namespace {
 
 // ---- activations and their slopes ----
 
-__device__ __forceinline__ float act_value(int act, float g) {
-  if (act == NEST_ACT_RELU) return g <= 0.0f ? 0.0f : g;  // NaN stays
-  if (act == NEST_ACT_SILU) return g / (1.0f + expf(-g));
-  return 0.5f * g * (1.0f + erff(g * 0.70710678118654752f));
+// exp and 1 / x: for 16-bit results the hardware's (1 ulp each, exp's argument
+// rounded once more); for float32 the library's and a division.
+template <typename T>
+__device__ __forceinline__ float exp_of(float x) {
+  if constexpr (sizeof(T) == 4) return expf(x);
+  return __builtin_amdgcn_exp2f(x * 1.4426950408889634f);
+}
+template <typename T>
+__device__ __forceinline__ float inverse(float x) {
+  if constexpr (sizeof(T) == 4) return 1.0f / x;
+  return __builtin_amdgcn_rcpf(x);
 }
 
-__device__ __forceinline__ float act_slope(int act, float g) {
-  if (act == NEST_ACT_RELU) return g > 0.0f ? 1.0f : 0.0f;
-  if (act == NEST_ACT_SILU) {
-    const float q = 1.0f / (1.0f + expf(-g));
-    return q * (1.0f + g * (1.0f - q));
+// act(g), and its slope where it is asked for.  Phi(g) of GELU: for float32 by
+// erf; for 16-bit results by Hastings' rational form (Abramowitz and Stegun
+// 7.1.26, absolute error 1.5e-7 of erf), which shares exp(-g^2 / 2) with the
+// slope's density.
+template <typename T, bool kSlope>
+__device__ __forceinline__ float act_value(int act, float g, float& slope) {
+  if (act == NEST_ACT_RELU) {
+    if constexpr (kSlope) slope = g > 0.0f ? 1.0f : 0.0f;
+    return g <= 0.0f ? 0.0f : g;  // NaN stays
   }
-  return 0.5f * (1.0f + erff(g * 0.70710678118654752f)) + g * expf(-0.5f * g * g) * 0.39894228040143268f;
+  if (act == NEST_ACT_SILU) {
+    const float q = inverse<T>(1.0f + exp_of<T>(-g));
+    if constexpr (kSlope) slope = q * fmaf(g, 1.0f - q, 1.0f);
+    return g * q;
+  }
+  float phi, e = 0.0f;
+  if constexpr (sizeof(T) == 4) {
+    phi = 0.5f * (1.0f + erff(g * 0.70710678118654752f));
+    if constexpr (kSlope) e = expf(-0.5f * g * g);
+  } else {
+    const float x = fabsf(g) * 0.70710678118654752f;
+    const float t = __builtin_amdgcn_rcpf(fmaf(0.3275911f, x, 1.0f));
+    e = exp_of<T>(-x * x);
+    const float tail = 0.5f * e * t *
+        fmaf(t, fmaf(t, fmaf(t, fmaf(t, 1.061405429f, -1.453152027f), 1.421413741f), -0.284496736f), 0.254829592f);
+    phi = g < 0.0f ? tail : 1.0f - tail;
+  }
+  if constexpr (kSlope) slope = fmaf(g * e, 0.39894228040143268f, phi);
+  return g * phi;
 }
 
 template <typename T>
@@ -99,21 +128,19 @@ __global__ __launch_bounds__(C::NT) void product_kernel(Products<T> all) {
   const int64_t k0 = split * per, k = p.K - k0 < per ? p.K - k0 : per;
   const int64_t m0 = (int64_t)tm * C::BM, n0 = (int64_t)tn * C::BN;
   f32x4 acc[C::FM][C::FN] = {};
-  if (k > 0) {
-    Loader<T, kAK, C::BM, C::NT> la;
-    Loader<T, kBK, C::BN, C::NT> lb;
-    const int64_t ka = kAK ? k0 : k0 * p.lda, kb = kBK ? k0 : k0 * p.ldb;
-    const char *a2 = nullptr, *b2 = nullptr;
-    if (p.a2) {
-      la.init(p.a2 + ka, p.lda, m0, kAK ? p.M : p.lda);
-      lb.init(p.b2 + kb, p.ldb, n0, kBK ? p.N : p.ldb);
-      a2 = la.base;
-      b2 = lb.base;
-    }
-    la.init(p.a + ka, p.lda, m0, kAK ? p.M : p.lda);
-    lb.init(p.b + kb, p.ldb, n0, kBK ? p.N : p.ldb);
-    tile_product<T, kAK, kBK, C>(la, lb, k, a2, b2, acc);
+  Loader<T, kAK, C::BM, C::NT> la;
+  Loader<T, kBK, C::BN, C::NT> lb;
+  const int64_t ka = kAK ? k0 : k0 * p.lda, kb = kBK ? k0 : k0 * p.ldb;
+  const char *a2 = nullptr, *b2 = nullptr;
+  if (p.a2) {
+    la.init(p.a2 + ka, p.lda, m0, kAK ? p.M : p.lda);
+    lb.init(p.b2 + kb, p.ldb, n0, kBK ? p.N : p.ldb);
+    a2 = la.base;
+    b2 = lb.base;
   }
+  la.init(p.a + ka, p.lda, m0, kAK ? p.M : p.lda);
+  lb.init(p.b + kb, p.ldb, n0, kBK ? p.N : p.ldb);
+  tile_product<T, kAK, kBK, C>(la, lb, k, a2, b2, acc);   // a split past the end has k <= 0: it loads zeros
   const int lane = threadIdx.x & 63, w = wave_id();
   const int64_t m = m0 + (w / C::WN) * C::FM * 16 + (lane & 15);
   const int n = (int)n0 + (w % C::WN) * C::FN * 16 + (lane >> 4) * 4;
@@ -143,6 +170,50 @@ __global__ __launch_bounds__(256) void join_kernel(Products<T> all) {
 
 // ---- h = act(g) u ----
 
+// The kept pre-activations in the order the accumulators hold them: a block of
+// 16 rows and 16 columns is 1 KB of g, then 1 KB of u, lane l's four columns
+// (4 (l / 16) .. + 3) of row l % 16 at 16 l.  Row-major float32 rows would be
+// touched 64 bytes at a time at a stride of a whole row; on 8192 rows of 8192
+// that took the backward's kernel 3.3 ms, of which 0.3 is the product.
+__device__ __forceinline__ float* kept_block(float* kept, int64_t row, int col, int64_t ldh) {
+  return kept + ((row >> 4) * ((ldh + 15) >> 4) + (col >> 4)) * 512 + (threadIdx.x & 63) * 4;
+}
+
+// 16 x 16-column fragments of a wave to row-major rows, through LDS of its own
+// so that a row's columns leave in 16-byte stores side by side.
+template <typename T, int FN>
+struct RowStage {
+  static constexpr int kPitch = FN * 16 + 16 / (int)sizeof(T);   // elements
+  T v[16 * kPitch];
+};
+
+// Rows row .. row + 15 and columns col .. col + 16 FN - 1 of out [rows][ld]; ld
+// is a multiple of 16 bytes and out aligned.  Element f(j)[e] is column
+// 16 j + 4 (lane / 16) + e of row lane % 16.
+template <typename T, int FN, typename F>
+__device__ __forceinline__ void store_rows(RowStage<T, FN>& stage, T* out, int64_t row, int64_t rows, int col, int64_t ld, F f) {
+  constexpr int kVec = 16 / (int)sizeof(T), kRow = FN * 16 / kVec;
+  const int lane = threadIdx.x & 63;
+#pragma unroll
+  for (int j = 0; j < FN; j++) {
+    const f32x4 v = f(j);
+    Four<T> t;
+#pragma unroll
+    for (int e = 0; e < 4; e++) t.v[e] = from_f32<T>(v[e]);
+    *reinterpret_cast<Four<T>*>(&stage.v[(lane & 15) * RowStage<T, FN>::kPitch + j * 16 + (lane >> 4) * 4]) = t;
+  }
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+#pragma unroll
+  for (int k = lane; k < 16 * kRow; k += 64) {
+    const int r = k / kRow, c = (k % kRow) * kVec;
+    const uint4 v = *reinterpret_cast<const uint4*>(&stage.v[r * RowStage<T, FN>::kPitch + c]);
+    if (row + r < rows && col + c < ld) *reinterpret_cast<uint4*>(out + (row + r) * ld + col + c) = v;
+  }
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
+
 template <typename T>
 struct Gate {
   const T *x, *wg, *wu;   // [M][ldx], [H][ldx]
@@ -150,7 +221,7 @@ struct Gate {
   int M, H;
   int64_t ldh;            // H rounded up to 16 bytes: the pad columns are written as zeros
   T* h;                   // [M][ldh] or null
-  float* kept;            // [M][2 ldh]: g, then u; or null
+  float* kept;            // g and u, see kept_block; or null
   int act, tiles_m, tiles_n;
 };
 
@@ -165,28 +236,32 @@ __global__ __launch_bounds__(C::NT) void gate_kernel(Gate<T> p) {
   la.init(p.x, p.ldx, m0, p.M);
   lb.init_pair(p.wg, p.wu, p.ldx, n0, p.H);
   tile_product<T, true, true, C>(la, lb, p.ldx, nullptr, nullptr, acc);
-  const int lane = threadIdx.x & 63, w = wave_id();
-  const int64_t m = m0 + (w / C::WN) * C::FM * 16 + (lane & 15);
-  const int n = (int)n0 + (w % C::WN) * C::FN * 8 + (lane >> 4) * 4;
+  const int w = wave_id();
+  const int64_t m = m0 + (w / C::WN) * C::FM * 16;
+  const int n = (int)n0 + (w % C::WN) * C::FN * 8;
+  if (p.kept) {
 #pragma unroll
-  for (int i = 0; i < C::FM; i++) {
-    if (m + i * 16 >= p.M) continue;
+    for (int i = 0; i < C::FM; i++)
 #pragma unroll
-    for (int j = 0; j < C::FN; j += 2) {
-      const f32x4 g = acc[i][j], u = acc[i][j + 1];
-      const int c = n + j * 8;
-      if (p.h) {
-        f32x4 h;
-#pragma unroll
-        for (int e = 0; e < 4; e++) h[e] = act_value(p.act, g[e]) * u[e];
-        store4(p.h + (m + i * 16) * p.ldh, c, (int)p.ldh, true, h);
+      for (int j = 0; j < C::FN; j += 2) {
+        if (m + i * 16 >= p.M || n + j * 8 >= p.ldh) continue;
+        float* at = kept_block(p.kept, m + i * 16, n + j * 8, p.ldh);
+        *reinterpret_cast<f32x4*>(at) = acc[i][j];
+        *reinterpret_cast<f32x4*>(at + 256) = acc[i][j + 1];
       }
-      if (p.kept) {
-        store4(p.kept + (m + i * 16) * 2 * p.ldh, c, (int)p.ldh, true, g);
-        store4(p.kept + (m + i * 16) * 2 * p.ldh + p.ldh, c, (int)p.ldh, true, u);
-      }
-    }
   }
+  if (!p.h) return;
+  __syncthreads();   // the operands' LDS is free
+  auto& stage = reinterpret_cast<RowStage<T, C::FN / 2>*>(tile_lds<C>())[w];
+#pragma unroll
+  for (int i = 0; i < C::FM; i++)
+    store_rows<T, C::FN / 2>(stage, p.h, m + i * 16, p.M, n, p.ldh, [&](int j) {
+      f32x4 h;
+      float unused;
+#pragma unroll
+      for (int e = 0; e < 4; e++) h[e] = act_value<T, false>(p.act, acc[i][2 * j][e], unused) * acc[i][2 * j + 1][e];
+      return h;
+    });
 }
 
 // ---- dg, du and h from dh = dy Wd ----
@@ -196,7 +271,7 @@ struct GateBackward {
   const T *dy, *wd;       // [M][ldy], [O][ldh]
   int64_t ldy, ldh;
   int M, O;
-  const float* kept;
+  float* kept;
   T *h, *dg, *du;         // [M][ldh]
   int act, tiles_m, tiles_n;
 };
@@ -212,31 +287,37 @@ __global__ __launch_bounds__(C::NT) void gate_backward_kernel(GateBackward<T> p)
   la.init(p.dy, p.ldy, m0, p.M);
   lb.init(p.wd, p.ldh, n0, p.ldh);
   tile_product<T, true, false, C>(la, lb, p.O, nullptr, nullptr, acc);
-  const int lane = threadIdx.x & 63, w = wave_id();
-  const int64_t m = m0 + (w / C::WN) * C::FM * 16 + (lane & 15);
-  const int n = (int)n0 + (w % C::WN) * C::FN * 16 + (lane >> 4) * 4;
+  const int w = wave_id();
+  const int64_t m = m0 + (w / C::WN) * C::FM * 16;
+  const int n = (int)n0 + (w % C::WN) * C::FN * 16;
+  __syncthreads();   // the operands' LDS is free
+  auto& stage = reinterpret_cast<RowStage<T, C::FN>*>(tile_lds<C>())[w];
 #pragma unroll
   for (int i = 0; i < C::FM; i++) {
     const int64_t row = m + i * 16;
-    if (row >= p.M) continue;
+    if (row >= p.M) break;
+    f32x4 g[C::FN], u[C::FN];
 #pragma unroll
     for (int j = 0; j < C::FN; j++) {
-      const int c = n + j * 16;
-      if (c >= p.ldh) continue;   // ldh is a multiple of 4: a lane's four columns are in or out together
-      const f32x4 g = *reinterpret_cast<const f32x4*>(p.kept + row * 2 * p.ldh + c);
-      const f32x4 u = *reinterpret_cast<const f32x4*>(p.kept + row * 2 * p.ldh + p.ldh + c);
-      f32x4 h, dg, du;
-#pragma unroll
-      for (int e = 0; e < 4; e++) {
-        const float a = act_value(p.act, g[e]), d = acc[i][j][e];
-        h[e] = a * u[e];
-        dg[e] = d * u[e] * act_slope(p.act, g[e]);
-        du[e] = d * a;
-      }
-      store4(p.h + row * p.ldh, c, (int)p.ldh, true, h);
-      store4(p.dg + row * p.ldh, c, (int)p.ldh, true, dg);
-      store4(p.du + row * p.ldh, c, (int)p.ldh, true, du);
+      g[j] = u[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+      if (n + j * 16 >= p.ldh) continue;
+      const float* at = kept_block(p.kept, row, n + j * 16, p.ldh);
+      g[j] = *reinterpret_cast<const f32x4*>(at);
+      u[j] = *reinterpret_cast<const f32x4*>(at + 256);
     }
+#pragma unroll
+    for (int j = 0; j < C::FN; j++)
+#pragma unroll
+      for (int e = 0; e < 4; e++) {   // g: h, u: dg, acc: du
+        float slope;
+        const float a = act_value<T, true>(p.act, g[j][e], slope), d = acc[i][j][e], h = a * u[j][e];
+        u[j][e] = d * u[j][e] * slope;
+        acc[i][j][e] = d * a;
+        g[j][e] = h;
+      }
+    store_rows<T, C::FN>(stage, p.h, row, p.M, n, p.ldh, [&](int j) { return g[j]; });
+    store_rows<T, C::FN>(stage, p.dg, row, p.M, n, p.ldh, [&](int j) { return u[j]; });
+    store_rows<T, C::FN>(stage, p.du, row, p.M, n, p.ldh, [&](int j) { return acc[i][j]; });
   }
 }
 

@@ -138,27 +138,36 @@ struct Loader {
   }
 };
 
-// The fragment of 16 rows (first a multiple of 16) at half kb of a step.
+// Where a lane reads its part of the fragments of a wave whose first row (or
+// column) is `first`, a multiple of 16 times the wave's power-of-two number of
+// fragments: fragment i is at an XOR of this with a constant and a constant
+// offset, so the addresses cost one register a fragment at most.
 template <typename T, bool kKM, int R>
-__device__ __forceinline__ typename Mma<T>::Frag fragment(const uint8_t* lds, int first, int kb) {
+__device__ __forceinline__ int fragment_base(int first) {
   const int lane = threadIdx.x & 63, r = lane & 15, q = lane >> 4;
-  if constexpr (kKM) {
-    return *reinterpret_cast<const typename Mma<T>::Frag*>(lds + (first + r) * kStepBytes + (((kb * 4 + q) ^ (r & 7)) << 4));
-  } else if constexpr (sizeof(T) == 2) {
+  if constexpr (kKM) return (first + r) * kStepBytes + ((q ^ (r & 7)) << 4);
+  if constexpr (sizeof(T) == 2) {
     // each group of 16 lanes reads 4 rows of 16 values and gets them transposed
-    const int k = kb * 32 + q * 8 + (r >> 2), unit = first >> 4;
-    i16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-        (LdsI16x4*)(lds + k * (R * 2) + (unit ^ unit_swizzle<T, R>(k)) * 32 + (r & 3) * 8));
-    i16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-        (LdsI16x4*)(lds + (k + 4) * (R * 2) + (unit ^ unit_swizzle<T, R>(k + 4)) * 32 + (r & 3) * 8));
+    const int k = q * 8 + (r >> 2);
+    return (k * (R * 2) + (unit_swizzle<T, R>(k) << 5) + (r & 3) * 8) ^ (first >> 4 << 5);
+  }
+  return (q * 4 * (R * 4) + (unit_swizzle<T, R>(q * 4) << 6) + r * 4) ^ (first >> 4 << 6);
+}
+
+// Fragment i (16 rows or columns) at half kb of a step.
+template <typename T, bool kKM, int R>
+__device__ __forceinline__ typename Mma<T>::Frag fragment(const uint8_t* lds, int base, int i, int kb) {
+  if constexpr (kKM) {
+    return *reinterpret_cast<const typename Mma<T>::Frag*>(lds + (base ^ (kb << 6)) + i * 16 * kStepBytes);
+  } else if constexpr (sizeof(T) == 2) {
+    const uint8_t* at = lds + (base ^ (i << 5)) + kb * 32 * (R * 2);
+    i16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsI16x4*)at);
+    i16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsI16x4*)(at + 4 * (R * 2)));
     return __builtin_bit_cast(typename Mma<T>::Frag, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
   } else {
     f32x4 f;
 #pragma unroll
-    for (int j = 0; j < 4; j++) {
-      const int k = kb * 16 + q * 4 + j;
-      f[j] = *reinterpret_cast<const float*>(lds + k * (R * 4) + ((((first >> 4) ^ unit_swizzle<T, R>(k)) * 16) + r) * 4);
-    }
+    for (int j = 0; j < 4; j++) f[j] = *reinterpret_cast<const float*>(lds + (base ^ (i << 6)) + (kb * 16 + j) * (R * 4));
     return f;
   }
 }
@@ -172,18 +181,31 @@ typedef Tile<256, 256, 2, 4> TileL;
 typedef Tile<128, 128, 2, 2> TileM;
 typedef Tile<64, 64, 2, 2> TileS;
 
+// The two LDS buffers of a step.  They are separate arrays, so that the
+// compiler knows a direct load into one not to touch a fragment of the other.
+template <typename C>
+__device__ __forceinline__ uint8_t* tile_lds() {
+  __shared__ __attribute__((aligned(16))) uint8_t lds[(C::BM + C::BN) * kStepBytes];
+  return lds;
+}
+template <typename C>
+__device__ __forceinline__ uint8_t* tile_lds_next() {
+  __shared__ __attribute__((aligned(16))) uint8_t lds[(C::BM + C::BN) * kStepBytes];
+  return lds;
+}
+
 // acc[i][j]: rows m = 16 i + lane % 16, columns n = 16 j + 4 (lane / 16) + 0..3
 // of the wave's part.  `steps` steps of k from each of `segments` operand
 // pairs; a2 and b2: the second pair's bases.
 template <typename T, bool kAK, bool kBK, typename C>
 __device__ __forceinline__ void tile_product(Loader<T, kAK, C::BM, C::NT>& la, Loader<T, kBK, C::BN, C::NT>& lb, int64_t K,
                                              const char* a2, const char* b2, f32x4 (&acc)[C::FM][C::FN]) {
-  __shared__ __attribute__((aligned(16))) uint8_t a_lds0[C::BM * kStepBytes];
-  __shared__ __attribute__((aligned(16))) uint8_t b_lds0[C::BN * kStepBytes];
-  __shared__ __attribute__((aligned(16))) uint8_t a_lds1[C::BM * kStepBytes];
-  __shared__ __attribute__((aligned(16))) uint8_t b_lds1[C::BN * kStepBytes];
+  uint8_t* const a_lds0 = tile_lds<C>();
+  uint8_t* const b_lds0 = a_lds0 + C::BM * kStepBytes;
+  uint8_t* const a_lds1 = tile_lds_next<C>();
+  uint8_t* const b_lds1 = a_lds1 + C::BM * kStepBytes;
   constexpr int kStep = kStepBytes / (int)sizeof(T);
-  const int steps = (int)((K + kStep - 1) / kStep);
+  const int steps = K > kStep ? (int)((K + kStep - 1) / kStep) : 1;
   const int total = a2 ? 2 * steps : steps;
   int64_t k_left = K;
   int next = 0;
@@ -201,33 +223,55 @@ __device__ __forceinline__ void tile_product(Loader<T, kAK, C::BM, C::NT>& la, L
     next++;
   };
   const int w = wave_id(), wm = (w / C::WN) * C::FM * 16, wn = (w % C::WN) * C::FN * 16;
-  auto multiply = [&](const uint8_t* a, const uint8_t* b) {
+  const int ba = fragment_base<T, kAK, C::BM>(wm), bb = fragment_base<T, kBK, C::BN>(wn);
+  // A step is four phases: half kb of k times half of the wave's rows.  Each
+  // phase reads the next one's fragments before its own products, so LDS works
+  // beside the matrix cores; the barrier stands before the last phase, whose
+  // fragments are in registers by then.
+  constexpr int kHalf = C::FM / 2;
+  typename Mma<T>::Frag fa[2][kHalf], fb[2][C::FN];
+  auto load_a = [&](int to, const uint8_t* a, int kb, int half) {
 #pragma unroll
-    for (int kb = 0; kb < 2; kb++) {
-      typename Mma<T>::Frag fa[C::FM], fb[C::FN];
+    for (int i = 0; i < kHalf; i++) fa[to][i] = fragment<T, kAK, C::BM>(a, ba, half * kHalf + i, kb);
+  };
+  auto load_b = [&](int to, const uint8_t* b, int kb) {
 #pragma unroll
-      for (int i = 0; i < C::FM; i++) fa[i] = fragment<T, kAK, C::BM>(a, wm + i * 16, kb);
+    for (int j = 0; j < C::FN; j++) fb[to][j] = fragment<T, kBK, C::BN>(b, bb, j, kb);
+  };
+  auto products = [&](int half, int from_a, int from_b) {
 #pragma unroll
-      for (int j = 0; j < C::FN; j++) fb[j] = fragment<T, kBK, C::BN>(b, wn + j * 16, kb);
+    for (int i = 0; i < kHalf; i++)
 #pragma unroll
-      for (int i = 0; i < C::FM; i++)
-#pragma unroll
-        for (int j = 0; j < C::FN; j++) acc[i][j] = Mma<T>::run(fb[j], fa[i], acc[i][j]);
-    }
+      for (int j = 0; j < C::FN; j++)
+        acc[half * kHalf + i][j] = Mma<T>::run(fb[from_b][j], fa[from_a][i], acc[half * kHalf + i][j]);
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  int s = 0;
+  auto step = [&](uint8_t* a, uint8_t* b, uint8_t* a_next, uint8_t* b_next) {
+    load_a(1, a, 0, 1);
+    products(0, 0, 0);
+    load_a(0, a, 1, 0);
+    load_b(1, b, 1);
+    products(1, 1, 0);
+    load_a(1, a, 1, 1);
+    products(0, 0, 1);
+    __syncthreads();   // the next step has landed; this one's fragments are all read
+    if (s + 2 < total) issue(a, b);
+    load_a(0, a_next, 0, 0);   // after the last step: of no use, and of no harm
+    load_b(0, b_next, 0);
+    products(1, 1, 1);
+    s++;
   };
   issue(a_lds0, b_lds0);
-  int s = 0;
-  for (; s + 1 < total; s += 2) {
-    __syncthreads();   // buffer 0 has landed, buffer 1 is no longer read
-    issue(a_lds1, b_lds1);
-    multiply(a_lds0, b_lds0);
-    __syncthreads();
-    if (s + 2 < total) issue(a_lds0, b_lds0);
-    multiply(a_lds1, b_lds1);
-  }
-  if (s < total) {
-    __syncthreads();
-    multiply(a_lds0, b_lds0);
+  __syncthreads();
+  if (total > 1) issue(a_lds1, b_lds1);
+  load_a(0, a_lds0, 0, 0);
+  load_b(0, b_lds0, 0);
+  while (true) {
+    step(a_lds0, b_lds0, a_lds1, b_lds1);
+    if (s == total) break;
+    step(a_lds1, b_lds1, a_lds0, b_lds0);
+    if (s == total) break;
   }
 }
 
