@@ -66,6 +66,24 @@ struct TileChoice {
   int side, splits;
 };
 
+constexpr int kNarrowPad = 8;   // elements: rows of 16 bytes more fall on different banks
+
+// LDS of the forward, in elements: gate and up rows (32 of each in turn), down
+// rows, a stage for each wave's stores.
+struct NarrowLds {
+  int pitch_in, pitch_h, down, stage, total;
+};
+__host__ __device__ inline NarrowLds narrow_lds(int ki, int hidden, int waves) {
+  const int h32 = (hidden + 31) / 32 * 32;
+  NarrowLds l;
+  l.pitch_in = ki * 32 + kNarrowPad;
+  l.pitch_h = h32 + kNarrowPad;
+  l.down = 2 * h32 * l.pitch_in;
+  l.stage = l.down + ki * 32 * l.pitch_h;
+  l.total = l.stage + waves * 16 * (ki * 32 + 8);
+  return l;
+}
+
 // What a call's sizes fix: row lengths (rounded up to 16 bytes), the
 // workspace's parts (byte offsets) and each product's tiles.
 struct GatedLayout {
@@ -73,6 +91,7 @@ struct GatedLayout {
   size_t h, dg, du, kept, x, wg, wu, wd, dy, part;
   size_t bytes, kept_bytes;
   TileChoice y, dx, dw;
+  bool narrow;         // gated_narrow.h
 };
 GatedLayout gated_layout(int64_t rows, int in, int hidden, int out, int dtype, bool backward, bool alone);
 TileChoice choose_gate_tile(int64_t M, int64_t N, int64_t K, int es);

@@ -58,6 +58,14 @@ TileChoice choose_tile(int n, const int64_t* M, const int64_t* N, int64_t K, int
   return best;
 }
 
+// Whether whole rows stay on the chip (gated_narrow.h): 16-bit rows of at most
+// 128 features whose weights fit a CU's LDS.
+bool narrow_rows(int64_t rows, int in, int hidden, int out, int es) {
+  const int side = in > out ? in : out;
+  if (es != 2 || side > 128 || rows < 64) return false;
+  return narrow_lds((side + 31) / 32, hidden, 8).total * 2 <= 160 * 1024;
+}
+
 TileChoice choose_gate_tile(int64_t M, int64_t N, int64_t K, int es) { return choose_tile(1, &M, &N, K, es, false); }
 
 GatedLayout gated_layout(int64_t rows, int in, int hidden, int out, int dtype, bool back, bool alone) {
@@ -74,6 +82,8 @@ GatedLayout gated_layout(int64_t rows, int in, int hidden, int out, int dtype, b
     at = (at + (size_t)bytes + 255) / 256 * 256;
     return o;
   };
+  l.narrow = narrow_rows(rows, in, hidden, out, es);
+  if (l.narrow && !back) return l;
   l.h = take(rows * l.ldh * es);
   int64_t part = 0;
   auto partial = [&](const TileChoice& t, int n, const int64_t* M, const int64_t* N) {
@@ -97,7 +107,7 @@ GatedLayout gated_layout(int64_t rows, int in, int hidden, int out, int dtype, b
     const int64_t WM[3] = {hidden, hidden, out}, WN[3] = {in, in, hidden};
     l.dw = choose_tile(3, WM, WN, rows, es, true);
     partial(l.dw, 3, WM, WN);
-    if (alone) l.kept = take(kept_bytes);
+    if (alone || l.narrow) l.kept = take(kept_bytes);
     if (l.ldy != out) l.dy = take(rows * l.ldy * es);
   }
   if (l.ldx != in) {
@@ -108,7 +118,7 @@ GatedLayout gated_layout(int64_t rows, int in, int hidden, int out, int dtype, b
   if (l.ldh != hidden) l.wd = take(out * l.ldh * es);
   l.part = take(part);
   l.bytes = at;
-  l.kept_bytes = (size_t)kept_bytes;
+  l.kept_bytes = l.narrow ? 0 : (size_t)kept_bytes;   // the narrow backward makes them again
   return l;
 }
 

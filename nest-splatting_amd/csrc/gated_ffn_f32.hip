@@ -1,5 +1,5 @@
-// The gated feed-forward block for float: see gated_tiles.h.
-#include "gated_tiles.h"
+// The gated feed-forward block for float: see gated_calls.h.
+#include "gated_calls.h"
 
 namespace nest {
 

@@ -1,6 +1,5 @@
 // The products of a gated feed-forward block as tiles of tile_gemm.h, for one
-// element type: included by gated_ffn_f32.hip, gated_ffn_f16.hip and
-// gated_ffn_bf16.hip.
+// element type.
 //
 //   g = x Wg^T,  u = x Wu^T,  h = act(g) u,  y = h Wd^T
 //   dh = dy Wd,  dg = dh u act'(g),  du = dh act(g)
@@ -44,13 +43,13 @@ __device__ __forceinline__ float inverse(float x) {
 // erf; for 16-bit results by Hastings' rational form (Abramowitz and Stegun
 // 7.1.26, absolute error 1.5e-7 of erf), which shares exp(-g^2 / 2) with the
 // slope's density.
-template <typename T, bool kSlope>
-__device__ __forceinline__ float act_value(int act, float g, float& slope) {
-  if (act == NEST_ACT_RELU) {
+template <typename T, int kAct, bool kSlope>
+__device__ __forceinline__ float act_value(float g, float& slope) {
+  if constexpr (kAct == NEST_ACT_RELU) {
     if constexpr (kSlope) slope = g > 0.0f ? 1.0f : 0.0f;
     return g <= 0.0f ? 0.0f : g;  // NaN stays
   }
-  if (act == NEST_ACT_SILU) {
+  if constexpr (kAct == NEST_ACT_SILU) {
     const float q = inverse<T>(1.0f + exp_of<T>(-g));
     if constexpr (kSlope) slope = q * fmaf(g, 1.0f - q, 1.0f);
     return g * q;
@@ -69,6 +68,18 @@ __device__ __forceinline__ float act_value(int act, float g, float& slope) {
   }
   if constexpr (kSlope) slope = fmaf(g * e, 0.39894228040143268f, phi);
   return g * phi;
+}
+
+// f with the activation as a constant, so that no element branches on it.
+template <int kAct>
+struct ActConstant {
+  static constexpr int value = kAct;
+};
+template <typename F>
+__host__ __device__ __forceinline__ auto with_act(int act, F f) {
+  if (act == NEST_ACT_RELU) return f(ActConstant<NEST_ACT_RELU>());
+  if (act == NEST_ACT_SILU) return f(ActConstant<NEST_ACT_SILU>());
+  return f(ActConstant<NEST_ACT_GELU>());
 }
 
 template <typename T>
@@ -253,15 +264,17 @@ __global__ __launch_bounds__(C::NT) void gate_kernel(Gate<T> p) {
   if (!p.h) return;
   __syncthreads();   // the operands' LDS is free
   auto& stage = reinterpret_cast<RowStage<T, C::FN / 2>*>(tile_lds<C>())[w];
+  with_act(p.act, [&](auto act) {
 #pragma unroll
-  for (int i = 0; i < C::FM; i++)
-    store_rows<T, C::FN / 2>(stage, p.h, m + i * 16, p.M, n, p.ldh, [&](int j) {
-      f32x4 h;
-      float unused;
+    for (int i = 0; i < C::FM; i++)
+      store_rows<T, C::FN / 2>(stage, p.h, m + i * 16, p.M, n, p.ldh, [&](int j) {
+        f32x4 h;
+        float unused;
 #pragma unroll
-      for (int e = 0; e < 4; e++) h[e] = act_value<T, false>(p.act, acc[i][2 * j][e], unused) * acc[i][2 * j + 1][e];
-      return h;
-    });
+        for (int e = 0; e < 4; e++) h[e] = act_value<T, act.value, false>(acc[i][2 * j][e], unused) * acc[i][2 * j + 1][e];
+        return h;
+      });
+  });
 }
 
 // ---- dg, du and h from dh = dy Wd ----
@@ -292,33 +305,35 @@ __global__ __launch_bounds__(C::NT) void gate_backward_kernel(GateBackward<T> p)
   const int n = (int)n0 + (w % C::WN) * C::FN * 16;
   __syncthreads();   // the operands' LDS is free
   auto& stage = reinterpret_cast<RowStage<T, C::FN>*>(tile_lds<C>())[w];
+  with_act(p.act, [&](auto act) {
 #pragma unroll
-  for (int i = 0; i < C::FM; i++) {
-    const int64_t row = m + i * 16;
-    if (row >= p.M) break;
-    f32x4 g[C::FN], u[C::FN];
+    for (int i = 0; i < C::FM; i++) {
+      const int64_t row = m + i * 16;
+      if (row >= p.M) break;
+      f32x4 g[C::FN], u[C::FN];
 #pragma unroll
-    for (int j = 0; j < C::FN; j++) {
-      g[j] = u[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-      if (n + j * 16 >= p.ldh) continue;
-      const float* at = kept_block(p.kept, row, n + j * 16, p.ldh);
-      g[j] = *reinterpret_cast<const f32x4*>(at);
-      u[j] = *reinterpret_cast<const f32x4*>(at + 256);
-    }
-#pragma unroll
-    for (int j = 0; j < C::FN; j++)
-#pragma unroll
-      for (int e = 0; e < 4; e++) {   // g: h, u: dg, acc: du
-        float slope;
-        const float a = act_value<T, true>(p.act, g[j][e], slope), d = acc[i][j][e], h = a * u[j][e];
-        u[j][e] = d * u[j][e] * slope;
-        acc[i][j][e] = d * a;
-        g[j][e] = h;
+      for (int j = 0; j < C::FN; j++) {
+        g[j] = u[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        if (n + j * 16 >= p.ldh) continue;
+        const float* at = kept_block(p.kept, row, n + j * 16, p.ldh);
+        g[j] = *reinterpret_cast<const f32x4*>(at);
+        u[j] = *reinterpret_cast<const f32x4*>(at + 256);
       }
-    store_rows<T, C::FN>(stage, p.h, row, p.M, n, p.ldh, [&](int j) { return g[j]; });
-    store_rows<T, C::FN>(stage, p.dg, row, p.M, n, p.ldh, [&](int j) { return u[j]; });
-    store_rows<T, C::FN>(stage, p.du, row, p.M, n, p.ldh, [&](int j) { return acc[i][j]; });
-  }
+#pragma unroll
+      for (int j = 0; j < C::FN; j++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) {   // g: h, u: dg, acc: du
+          float slope;
+          const float a = act_value<T, act.value, true>(g[j][e], slope), d = acc[i][j][e], h = a * u[j][e];
+          u[j][e] = d * u[j][e] * slope;
+          acc[i][j][e] = d * a;
+          g[j][e] = h;
+        }
+      store_rows<T, C::FN>(stage, p.h, row, p.M, n, p.ldh, [&](int j) { return g[j]; });
+      store_rows<T, C::FN>(stage, p.dg, row, p.M, n, p.ldh, [&](int j) { return u[j]; });
+      store_rows<T, C::FN>(stage, p.du, row, p.M, n, p.ldh, [&](int j) { return acc[i][j]; });
+    }
+  });
 }
 
 // ---- padded copies ----
@@ -439,54 +454,6 @@ hipError_t pad_operands(const GatedParams& p, const GatedLayout& l, uint8_t* ws,
   if (back && l.ldy != p.out) add(o.dy, l.dy, p.rows, p.out, l.ldy);
   if (n) go();
   return hipGetLastError();
-}
-
-template <typename T>
-hipError_t gated_forward(const GatedParams& p, hipStream_t s) {
-  const GatedLayout l = gated_layout(p.rows, p.in, p.hidden, p.out, p.dtype, false, false);
-  uint8_t* ws = static_cast<uint8_t*>(p.ws);
-  Operands<T> o;
-  if (hipError_t e = pad_operands(p, l, ws, false, o, s); e != hipSuccess) return e;
-  T* h = reinterpret_cast<T*>(ws + l.h);
-  Gate<T> g{o.x, o.wg, o.wu, l.ldx, (int)p.rows, p.hidden, l.ldh, h, p.kept, p.activation, 0, 0};
-  if (hipError_t e = launch_gate(g, s); e != hipSuccess) return e;
-  Products<T> y{};
-  y.n = 1;
-  y.p[0] = {h, o.wd, nullptr, nullptr, l.ldh, l.ldh, (int)p.rows, p.out, l.ldh, static_cast<T*>(p.y)};
-  y.part = reinterpret_cast<float*>(ws + l.part);
-  return launch_products<T, true, true>(y, l.y, s);
-}
-
-template <typename T>
-hipError_t gated_backward(const GatedParams& p, hipStream_t s) {
-  const bool alone = p.kept == nullptr;
-  const GatedLayout l = gated_layout(p.rows, p.in, p.hidden, p.out, p.dtype, true, alone);
-  uint8_t* ws = static_cast<uint8_t*>(p.ws);
-  T *h = reinterpret_cast<T*>(ws + l.h), *dg = reinterpret_cast<T*>(ws + l.dg), *du = reinterpret_cast<T*>(ws + l.du);
-  Operands<T> o;
-  if (hipError_t e = pad_operands(p, l, ws, true, o, s); e != hipSuccess) return e;
-  float* kept = p.kept;
-  if (alone) {
-    kept = reinterpret_cast<float*>(ws + l.kept);
-    Gate<T> g{o.x, o.wg, o.wu, l.ldx, (int)p.rows, p.hidden, l.ldh, nullptr, kept, p.activation, 0, 0};
-    if (hipError_t e = launch_gate(g, s); e != hipSuccess) return e;
-  }
-  GateBackward<T> b{o.dy, o.wd, l.ldy, l.ldh, (int)p.rows, p.out, kept, h, dg, du, p.activation, 0, 0};
-  if (hipError_t e = launch_gate_backward(b, s); e != hipSuccess) return e;
-  if (p.dx) {
-    Products<T> q{};
-    q.n = 1;
-    q.p[0] = {dg, o.wg, du, o.wu, l.ldh, l.ldx, (int)p.rows, p.in, p.hidden, static_cast<T*>(p.dx)};
-    q.part = reinterpret_cast<float*>(ws + l.part);
-    if (hipError_t e = launch_products<T, true, false>(q, l.dx, s); e != hipSuccess) return e;
-  }
-  Products<T> w{};
-  if (p.dw_gate) w.p[w.n++] = {dg, o.x, nullptr, nullptr, l.ldh, l.ldx, p.hidden, p.in, p.rows, static_cast<T*>(p.dw_gate)};
-  if (p.dw_up) w.p[w.n++] = {du, o.x, nullptr, nullptr, l.ldh, l.ldx, p.hidden, p.in, p.rows, static_cast<T*>(p.dw_up)};
-  if (p.dw_down) w.p[w.n++] = {o.dy, h, nullptr, nullptr, l.ldy, l.ldh, p.out, p.hidden, p.rows, static_cast<T*>(p.dw_down)};
-  if (!w.n) return hipSuccess;
-  w.part = reinterpret_cast<float*>(ws + l.part);
-  return launch_products<T, false, false>(w, l.dw, s);
 }
 
 }  // namespace
