@@ -84,6 +84,31 @@ __host__ __device__ inline NarrowLds narrow_lds(int ki, int hidden, int waves) {
   return l;
 }
 
+// Groups of 32 hidden features, one a wave, of the narrow backward: a power of two.
+__host__ __device__ constexpr int narrow_slices(int hidden) {
+  return hidden <= 32 ? 1 : hidden <= 64 ? 2 : hidden <= 128 ? 4 : hidden <= 256 ? 8 : 16;
+}
+
+// LDS of the narrow backward, in elements: weights, then for each group of
+// waves x, dy [32][pitch_in] and dg, du, h [32][pitch_h]; at its end the
+// groups' sums.
+struct NarrowBackLds {
+  int groups, pitch_in, pitch_h, tiles, tile_stride, total;
+};
+__host__ __device__ constexpr NarrowBackLds narrow_back_lds(int ki, int slices) {
+  NarrowBackLds l{};
+  const int h = slices * 32;
+  l.groups = (ki <= 2 ? 8 : 4) / slices;
+  l.pitch_in = ki * 32 + kNarrowPad;
+  l.pitch_h = h + kNarrowPad;
+  l.tiles = 2 * h * l.pitch_in + ki * 32 * l.pitch_h;
+  l.tile_stride = 2 * 32 * l.pitch_in + 3 * 32 * l.pitch_h;
+  l.total = l.tiles + l.groups * l.tile_stride;
+  const int sums = l.groups > 1 ? slices * 12 * ki * 256 * 2 : 0;   // float32: two elements each
+  if (sums > l.total) l.total = sums;
+  return l;
+}
+
 // What a call's sizes fix: row lengths (rounded up to 16 bytes), the
 // workspace's parts (byte offsets) and each product's tiles.
 struct GatedLayout {
@@ -91,7 +116,8 @@ struct GatedLayout {
   size_t h, dg, du, kept, x, wg, wu, wd, dy, part;
   size_t bytes, kept_bytes;
   TileChoice y, dx, dw;
-  bool narrow;         // gated_narrow.h
+  bool narrow, narrow_back;   // gated_narrow.h
+  int narrow_groups;          // workgroups of its backward
 };
 GatedLayout gated_layout(int64_t rows, int in, int hidden, int out, int dtype, bool backward, bool alone);
 TileChoice choose_gate_tile(int64_t M, int64_t N, int64_t K, int es);

@@ -66,6 +66,14 @@ bool narrow_rows(int64_t rows, int in, int hidden, int out, int es) {
   return narrow_lds((side + 31) / 32, hidden, 8).total * 2 <= 160 * 1024;
 }
 
+// Whether the backward does too: the accumulators of the weight gradients fit
+// the registers and everything else the LDS.
+bool narrow_rows_back(int in, int hidden, int out) {
+  const int side = in > out ? in : out, ki = (side + 31) / 32, slices = narrow_slices(hidden);
+  if (slices > (ki == 1 ? 8 : 4)) return false;
+  return narrow_back_lds(ki, slices).total * 2 <= 160 * 1024;
+}
+
 TileChoice choose_gate_tile(int64_t M, int64_t N, int64_t K, int es) { return choose_tile(1, &M, &N, K, es, false); }
 
 GatedLayout gated_layout(int64_t rows, int in, int hidden, int out, int dtype, bool back, bool alone) {
@@ -84,6 +92,15 @@ GatedLayout gated_layout(int64_t rows, int in, int hidden, int out, int dtype, b
   };
   l.narrow = narrow_rows(rows, in, hidden, out, es);
   if (l.narrow && !back) return l;
+  l.narrow_back = l.narrow && narrow_rows_back(in, hidden, out);
+  if (l.narrow_back) {
+    const int ki = ((in > out ? in : out) + 31) / 32, slices = narrow_slices(hidden);
+    const int64_t need = cdiv(rows, 32 * narrow_back_lds(ki, slices).groups);
+    l.narrow_groups = (int)(need < 256 ? need : 256);
+    l.part = take((int64_t)l.narrow_groups * 3 * slices * 32 * ki * 32 * 4);
+    l.bytes = at;
+    return l;
+  }
   l.h = take(rows * l.ldh * es);
   int64_t part = 0;
   auto partial = [&](const TileChoice& t, int n, const int64_t* M, const int64_t* N) {

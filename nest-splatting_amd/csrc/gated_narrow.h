@@ -156,5 +156,278 @@ hipError_t launch_narrow_forward(const GatedParams& g, hipStream_t s) {
   return narrow_forward<T, 4>(p, s);
 }
 
+// ---- backward ----
+//
+// One kernel makes g, u and dh again, dx, and the weight gradients' sums, so
+// that a step reads x and dy and writes dx and nothing of the size of h.  A
+// group of SL waves takes 32 rows at a time, wave s the hidden features
+// 32 s .. 32 s + 31 of all of them; its share of the three weight gradients
+// stays in its accumulators over all rows (96 registers for 64 features).
+// dg, du and h go through LDS as [row][hidden]: read along a row they are
+// operands of dx, whose sum over all hidden features is dealt out by its own
+// columns; read transposed (32 rows as the product's k) they are operands of
+// the weight gradients, as are x and dy.  One copy of the weights in LDS
+// serves both directions for the same reason.
+
+template <typename T>
+struct NarrowBack {
+  const T *x, *wg, *wu, *wd, *dy;
+  T* dx;            // or null
+  float* part;      // [workgroups][dWg, dWu: slices 32 x in padded; dWd: out padded x slices 32]
+  int64_t rows;
+  int in, hidden, out, act;
+};
+
+// Eight values of a lane's row (or column) that lie down a column of a
+// row-major array: rows k .. k + 7 for the lanes of quarter q at k = 8 q, column
+// `col` + lane % 16.
+template <typename T>
+__device__ __forceinline__ typename Mma<T>::Frag down_column(const T* at, int pitch) {
+  const int lane = threadIdx.x & 63, r = lane & 15, q = lane >> 4;
+  const T* p = at + (q * 8 + (r >> 2)) * pitch + (r & 3) * 4;
+  i16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsI16x4*)p);
+  i16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsI16x4*)(p + 4 * pitch));
+  return __builtin_bit_cast(typename Mma<T>::Frag, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+}
+
+template <typename T, int KI, int SL>
+__global__ __launch_bounds__(KI <= 2 ? 512 : 256, KI <= 2 ? 2 : 1) void narrow_backward_kernel(NarrowBack<T> p) {
+  typedef typename Mma<T>::Frag Frag;
+  constexpr int kWaves = KI <= 2 ? 8 : 4, kGroups = kWaves / SL, kThreads = 64 * kWaves;
+  constexpr NarrowBackLds l = narrow_back_lds(KI, SL);
+  constexpr int H = SL * 32, PI = l.pitch_in, PH = l.pitch_h, FI = 2 * KI;
+  static_assert(l.groups == kGroups, "");
+  extern __shared__ __attribute__((aligned(16))) uint8_t narrow_mem[];
+  T* const lds = reinterpret_cast<T*>(narrow_mem);
+  T *const wg = lds, *const wu = lds + H * PI, *const wd = lds + 2 * H * PI;
+  for (int c = threadIdx.x; c < 2 * H * KI * 4; c += kThreads) {
+    const int row = c / (KI * 4), k = c % (KI * 4) * 8, h = row < H ? row : row - H;
+    *reinterpret_cast<Frag*>(lds + row * PI + k) =
+        load8<T>((row < H ? p.wg : p.wu) + (int64_t)h * p.in + k, h < p.hidden ? p.in - k : 0);
+  }
+  for (int c = threadIdx.x; c < KI * 32 * (H / 8); c += kThreads) {
+    const int o = c / (H / 8), k = c % (H / 8) * 8;
+    *reinterpret_cast<Frag*>(wd + o * PH + k) = load8<T>(p.wd + (int64_t)o * p.hidden + k, o < p.out ? p.hidden - k : 0);
+  }
+  const int lane = threadIdx.x & 63, r = lane & 15, q = lane >> 4;
+  const int group = wave_id() / SL, slice = wave_id() % SL, t = threadIdx.x % (SL * 64);
+  T* const xs = lds + l.tiles + group * l.tile_stride;
+  T* const dys = xs + 32 * PI;
+  T* const dg = dys + 32 * PI;
+  T* const du = dg + 32 * PH;
+  T* const hh = du + 32 * PH;
+  // x and dy of the next rows, in registers until their place in LDS is free
+  constexpr int kChunks = 256 * KI, kLoads = (kChunks + SL * 64 - 1) / (SL * 64);
+  Frag next[kLoads];
+  auto load = [&](int64_t row) {
+#pragma unroll
+    for (int i = 0; i < kLoads; i++) {
+      const int c = t + i * SL * 64, half = c / (kChunks / 2), e = c % (kChunks / 2);
+      const int64_t n = row + e / (KI * 4);
+      const int k = e % (KI * 4) * 8, len = half ? p.out : p.in;
+      next[i] = load8<T>((half ? p.dy : p.x) + n * len + k, c < kChunks && n < p.rows ? len - k : 0);
+    }
+  };
+  auto place = [&]() {
+#pragma unroll
+    for (int i = 0; i < kLoads; i++) {
+      const int c = t + i * SL * 64, half = c / (kChunks / 2), e = c % (kChunks / 2);
+      if (c < kChunks) *reinterpret_cast<Frag*>((half ? dys : xs) + e / (KI * 4) * PI + e % (KI * 4) * 8) = next[i];
+    }
+  };
+  f32x4 dwg[2][FI] = {}, dwu[2][FI] = {}, dwd[FI][2] = {};
+  // every group of the workgroup takes the same number of turns: barriers stand inside
+  const int64_t first = ((int64_t)blockIdx.x * kGroups) * 32, step = (int64_t)gridDim.x * kGroups * 32;
+  load(first + group * 32);
+  place();
+  __syncthreads();
+  for (int64_t base = first; base < p.rows; base += step) {
+    const int64_t row = base + group * 32;
+    load(row + step);
+    f32x4 g[2][2] = {}, u[2][2] = {}, dh[2][2] = {};   // [16 hidden][16 rows]
+#pragma unroll
+    for (int k = 0; k < KI; k++) {
+      Frag fx[2], fy[2];
+#pragma unroll
+      for (int i = 0; i < 2; i++) {
+        fx[i] = *reinterpret_cast<const Frag*>(xs + (i * 16 + r) * PI + k * 32 + q * 8);
+        fy[i] = *reinterpret_cast<const Frag*>(dys + (i * 16 + r) * PI + k * 32 + q * 8);
+      }
+#pragma unroll
+      for (int b = 0; b < 2; b++) {
+        const int h = slice * 32 + b * 16;
+        const Frag fg = *reinterpret_cast<const Frag*>(wg + (h + r) * PI + k * 32 + q * 8);
+        const Frag fu = *reinterpret_cast<const Frag*>(wu + (h + r) * PI + k * 32 + q * 8);
+        const Frag fd = down_column<T>(wd + k * 32 * PH + h, PH);
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+          g[b][i] = Mma<T>::run(fg, fx[i], g[b][i]);
+          u[b][i] = Mma<T>::run(fu, fx[i], u[b][i]);
+          dh[b][i] = Mma<T>::run(fd, fy[i], dh[b][i]);
+        }
+      }
+    }
+    with_act(p.act, [&](auto act) {
+#pragma unroll
+      for (int b = 0; b < 2; b++)
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+          Four<T> vg, vu, vh;
+#pragma unroll
+          for (int e = 0; e < 4; e++) {
+            float slope;
+            const float a = act_value<T, act.value, true>(g[b][i][e], slope), d = dh[b][i][e];
+            vg.v[e] = from_f32<T>(d * u[b][i][e] * slope);
+            vu.v[e] = from_f32<T>(d * a);
+            vh.v[e] = from_f32<T>(a * u[b][i][e]);
+          }
+          const int at = (i * 16 + r) * PH + slice * 32 + b * 16 + q * 4;
+          *reinterpret_cast<Four<T>*>(dg + at) = vg;
+          *reinterpret_cast<Four<T>*>(du + at) = vu;
+          *reinterpret_cast<Four<T>*>(hh + at) = vh;
+        }
+    });
+    // this wave's own columns of dg, du and h: no other wave's writes are read
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    {
+      Frag fg[2], fu[2], fh[2];
+#pragma unroll
+      for (int b = 0; b < 2; b++) {
+        fg[b] = down_column<T>(dg + slice * 32 + b * 16, PH);
+        fu[b] = down_column<T>(du + slice * 32 + b * 16, PH);
+        fh[b] = down_column<T>(hh + slice * 32 + b * 16, PH);
+      }
+#pragma unroll
+      for (int j = 0; j < FI; j++) {
+        const Frag fx = down_column<T>(xs + j * 16, PI), fy = down_column<T>(dys + j * 16, PI);
+#pragma unroll
+        for (int b = 0; b < 2; b++) {
+          dwg[b][j] = Mma<T>::run(fg[b], fx, dwg[b][j]);
+          dwu[b][j] = Mma<T>::run(fu[b], fx, dwu[b][j]);
+          dwd[j][b] = Mma<T>::run(fy, fh[b], dwd[j][b]);
+        }
+      }
+    }
+    __syncthreads();   // dg and du are whole; x and dy are no longer read
+    place();
+    if (p.dx) {
+      for (int tile = slice; tile < FI * 2; tile += SL) {
+        const int j = tile >> 1, i = tile & 1;
+        f32x4 acc = {};
+#pragma unroll
+        for (int k = 0; k < SL; k++) {
+          const int at = (i * 16 + r) * PH + k * 32 + q * 8;
+          acc = Mma<T>::run(down_column<T>(wg + k * 32 * PI + j * 16, PI), *reinterpret_cast<const Frag*>(dg + at), acc);
+          acc = Mma<T>::run(down_column<T>(wu + k * 32 * PI + j * 16, PI), *reinterpret_cast<const Frag*>(du + at), acc);
+        }
+        const int64_t n = row + i * 16 + r;
+        if (n < p.rows) store4(p.dx + n * p.in, j * 16 + q * 4, p.in, p.in % 4 == 0, acc);
+      }
+    }
+    __syncthreads();   // the next x and dy are whole; dg and du are no longer read
+  }
+  // the groups' sums, in their order, through the LDS that the weights had
+  f32x4* const sums = reinterpret_cast<f32x4*>(narrow_mem) + slice * (6 * FI * 64) + lane;
+  for (int other = 1; other < kGroups; other++) {
+    if (group == other) {
+#pragma unroll
+      for (int j = 0; j < FI; j++)
+#pragma unroll
+        for (int b = 0; b < 2; b++) {
+          sums[((j * 2 + b) * 3 + 0) * 64] = dwg[b][j];
+          sums[((j * 2 + b) * 3 + 1) * 64] = dwu[b][j];
+          sums[((j * 2 + b) * 3 + 2) * 64] = dwd[j][b];
+        }
+    }
+    __syncthreads();
+    if (group == 0) {
+#pragma unroll
+      for (int j = 0; j < FI; j++)
+#pragma unroll
+        for (int b = 0; b < 2; b++) {
+          dwg[b][j] += sums[((j * 2 + b) * 3 + 0) * 64];
+          dwu[b][j] += sums[((j * 2 + b) * 3 + 1) * 64];
+          dwd[j][b] += sums[((j * 2 + b) * 3 + 2) * 64];
+        }
+    }
+    __syncthreads();
+  }
+  if (group != 0) return;
+  constexpr int D = KI * 32;
+  float* const part = p.part + (int64_t)blockIdx.x * (3 * H * D);
+#pragma unroll
+  for (int j = 0; j < FI; j++)
+#pragma unroll
+    for (int b = 0; b < 2; b++)
+#pragma unroll
+      for (int e = 0; e < 4; e++) {
+        const int h = slice * 32 + b * 16 + q * 4 + e;
+        part[h * D + j * 16 + r] = dwg[b][j][e];
+        part[H * D + h * D + j * 16 + r] = dwu[b][j][e];
+        part[2 * H * D + (j * 16 + q * 4 + e) * H + slice * 32 + b * 16 + r] = dwd[j][b][e];
+      }
+}
+
+// The weight gradients from the workgroups' sums: 32 places a workgroup, 32
+// slices of the sums, joined in LDS in a fixed order.
+template <typename T>
+__global__ __launch_bounds__(1024) void narrow_join_kernel(const float* part, int n, int H, int D, int in, int hidden, int out,
+                                                           T* dwg, T* dwu, T* dwd) {
+  __shared__ float lds[32][33];
+  const int size = 3 * H * D, col = blockIdx.x * 32 + (threadIdx.x & 31), slice = threadIdx.x >> 5;
+  float s = 0.0f;
+  for (int i = slice; i < n; i += 32) s += part[(int64_t)i * size + col];   // size is a multiple of 32
+  lds[slice][threadIdx.x & 31] = s;
+  __syncthreads();
+  if (slice) return;
+  float v = 0.0f;
+#pragma unroll
+  for (int i = 0; i < 32; i++) v += lds[i][threadIdx.x];
+  const int which = col / (H * D), e = col % (H * D);
+  if (which < 2) {
+    T* to = which ? dwu : dwg;
+    const int h = e / D, i = e % D;
+    if (to && h < hidden && i < in) to[(int64_t)h * in + i] = from_f32<T>(v);
+  } else {
+    const int o = e / H, h = e % H;
+    if (dwd && o < out && h < hidden) dwd[(int64_t)o * hidden + h] = from_f32<T>(v);
+  }
+}
+
+template <typename T, int KI, int SL>
+hipError_t narrow_backward(const GatedParams& g, const GatedLayout& l, hipStream_t s) {
+  constexpr NarrowBackLds m = narrow_back_lds(KI, SL);
+  NarrowBack<T> p{static_cast<const T*>(g.x), static_cast<const T*>(g.w_gate), static_cast<const T*>(g.w_up),
+                  static_cast<const T*>(g.w_down), static_cast<const T*>(g.dy), static_cast<T*>(g.dx),
+                  reinterpret_cast<float*>(static_cast<uint8_t*>(g.ws) + l.part), g.rows, g.in, g.hidden, g.out, g.activation};
+  narrow_backward_kernel<T, KI, SL><<<l.narrow_groups, KI <= 2 ? 512 : 256, m.total * sizeof(T), s>>>(p);
+  if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
+  constexpr int H = SL * 32, D = KI * 32;
+  if (g.dw_gate || g.dw_up || g.dw_down)
+    narrow_join_kernel<T><<<3 * H * D / 32, 1024, 0, s>>>(p.part, l.narrow_groups, H, D, g.in, g.hidden, g.out, static_cast<T*>(g.dw_gate),
+                                                          static_cast<T*>(g.dw_up), static_cast<T*>(g.dw_down));
+  return hipGetLastError();
+}
+
+template <typename T, int KI>
+hipError_t narrow_backward_slices(const GatedParams& g, const GatedLayout& l, hipStream_t s) {
+  const int slices = narrow_slices(g.hidden);
+  if (slices == 1) return narrow_backward<T, KI, 1>(g, l, s);
+  if (slices == 2) return narrow_backward<T, KI, 2>(g, l, s);
+  if constexpr (KI == 1)
+    if (slices == 8) return narrow_backward<T, KI, 8>(g, l, s);
+  return narrow_backward<T, KI, 4>(g, l, s);
+}
+
+template <typename T>
+hipError_t launch_narrow_backward(const GatedParams& g, const GatedLayout& l, hipStream_t s) {
+  const int side = g.in > g.out ? g.in : g.out;
+  if (side <= 32) return narrow_backward_slices<T, 1>(g, l, s);
+  if (side <= 64) return narrow_backward_slices<T, 2>(g, l, s);
+  if (side <= 96) return narrow_backward_slices<T, 3>(g, l, s);
+  return narrow_backward_slices<T, 4>(g, l, s);
+}
+
 }  // namespace
 }  // namespace nest
