@@ -117,6 +117,7 @@ struct GatedLayout {
   size_t bytes, kept_bytes;
   TileChoice y, dx, dw;
   bool narrow, narrow_back;   // gated_narrow.h
+  bool few;                   // gated_few.h (forward)
   int narrow_groups;          // workgroups of its backward
 };
 GatedLayout gated_layout(int64_t rows, int in, int hidden, int out, int dtype, bool backward, bool alone);

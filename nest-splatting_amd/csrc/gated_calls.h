@@ -2,6 +2,7 @@
 // gated_ffn_f32.hip, gated_ffn_f16.hip and gated_ffn_bf16.hip.
 #pragma once
 
+#include "gated_few.h"
 #include "gated_narrow.h"
 #include "gated_tiles.h"
 
@@ -13,6 +14,7 @@ hipError_t gated_forward(const GatedParams& p, hipStream_t s) {
   const GatedLayout l = gated_layout(p.rows, p.in, p.hidden, p.out, p.dtype, false, false);
   if constexpr (sizeof(T) == 2)
     if (l.narrow) return launch_narrow_forward<T>(p, s);
+  if (l.few) return launch_few_forward<T>(p, l, s);
   uint8_t* ws = static_cast<uint8_t*>(p.ws);
   Operands<T> o;
   if (hipError_t e = pad_operands(p, l, ws, false, o, s); e != hipSuccess) return e;

@@ -6,6 +6,11 @@ namespace {
 
 constexpr double kCus = 256.0;
 
+// Rows up to which the forward streams the weights through registers
+// (gated_few.h).  2048 -> 8192, us, streamed and in tiles: 32 rows of 16 bits
+// 36 and 38, 33 rows 47 (tiles); 16 rows of float32 70, 32 rows 104 and 87.
+int64_t few_rows(int es) { return es == 2 ? 32 : 16; }
+
 // Products of the rate a library product reaches that each tile size reaches
 // on a full chip, and flops a second of one CU.
 double tile_rate(int side, int es) {
@@ -102,6 +107,12 @@ GatedLayout gated_layout(int64_t rows, int in, int hidden, int out, int dtype, b
     return l;
   }
   l.h = take(rows * l.ldh * es);
+  l.few = !back && rows <= few_rows(es);
+  if (l.few) {
+    l.bytes = at;
+    l.kept_bytes = (size_t)kept_bytes;
+    return l;
+  }
   int64_t part = 0;
   auto partial = [&](const TileChoice& t, int n, const int64_t* M, const int64_t* N) {
     if (t.splits == 1) return;

@@ -13,17 +13,21 @@
 //
 // A row of up to 128 vectors of 16 bytes belongs to a group of 1 to 64 lanes
 // (several rows a wave for narrow rows), a longer one to a workgroup; past
-// the registers of a workgroup the row is read again for each pass.
+// the registers of a workgroup the row is read again for each pass.  A group
+// strides over its rows with the weights in registers and the next row on its
+// way.
 #include "blocks_internal.h"
 #include "vec_io.h"
+
+#include <type_traits>
 
 namespace nest {
 namespace {
 
-constexpr int kLnThreads = 256;
-constexpr int kLnWaves = kLnThreads / 64;
-
-constexpr int64_t kLnGrid = 1 << 22;
+constexpr int kLnThreads = 256;      // of rows that stay with a wave, and of the long kernels
+constexpr int kLnMost = 512;         // of rows a workgroup shares
+constexpr int kLnWaves = kLnMost / 64;
+constexpr int64_t kLnForwardGrid = 2048;   // workgroups
 
 // Sums over the lanes of one row; every lane gets the result.
 template <bool kBlock>
@@ -34,8 +38,7 @@ __device__ __forceinline__ float row_sum(float v, int lanes, float* lds) {
     if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
     __syncthreads();
     v = 0.0f;
-#pragma unroll
-    for (int w = 0; w < kLnWaves; w++) v += lds[w];
+    for (int w = 0; w < (int)blockDim.x / 64; w++) v += lds[w];
   } else {
     for (int o = lanes >> 1; o > 0; o >>= 1) v += __shfl_xor(v, o);
   }
@@ -43,58 +46,64 @@ __device__ __forceinline__ float row_sum(float v, int lanes, float* lds) {
 }
 
 template <typename T, typename P, int NV, bool kBlock>
-__global__ __launch_bounds__(kLnThreads) void layer_norm_kernel(LayerNormParams p, int lanes) {
+__global__ __launch_bounds__(kBlock ? kLnMost : kLnThreads) void layer_norm_kernel(LayerNormParams p, int lanes) {
   constexpr int N = Vec16<T>::kN;
   __shared__ float lds[2][kLnWaves];
   const int rows_wg = kBlock ? 1 : kLnThreads / lanes;
   const int lane = kBlock ? threadIdx.x : threadIdx.x & (lanes - 1);
   const int D = p.cols;
   const float inv = 1.0f / (float)D;
-  // The grid covers all rows up to kLnGrid workgroups; past that it strides.
-  for (int64_t row = (int64_t)blockIdx.x * rows_wg + (kBlock ? 0 : threadIdx.x / lanes); row < p.rows;
-       row += (int64_t)gridDim.x * rows_wg) {
-  const T* x = static_cast<const T*>(p.x) + row * D;
-  float v[NV][N];
-  float s = 0.0f;
+  const int64_t step = (int64_t)gridDim.x * rows_wg;
+  int64_t row = (int64_t)blockIdx.x * rows_wg + (kBlock ? 0 : threadIdx.x / lanes);
+  Vec16<T> next[NV];
+  auto load = [&](int64_t at) {
+    const T* x = static_cast<const T*>(p.x) + at * D;
+#pragma unroll
+    for (int k = 0; k < NV; k++) next[k] = load_raw(x + (k * lanes + lane) * N, at < p.rows ? D - (k * lanes + lane) * N : 0);
+  };
+  load(row);
+  float w[NV][N], b[NV][N];
 #pragma unroll
   for (int k = 0; k < NV; k++) {
     const int c = (k * lanes + lane) * N;
-    load_vec<T>(v[k], x + c, D - c);
+    load_param(w[k], static_cast<const P*>(p.weight) + c, D - c);
+    load_param(b[k], static_cast<const P*>(p.bias) + c, p.bias ? D - c : 0);
   }
+  for (; row < p.rows; row += step) {   // in kBlock the same number of turns for all threads
+    float v[NV][N];
+    float s = 0.0f;
 #pragma unroll
-  for (int k = 0; k < NV; k++)
+    for (int k = 0; k < NV; k++)
 #pragma unroll
-    for (int i = 0; i < N; i++) s += v[k][i];
-  const float mean = row_sum<kBlock>(s, lanes, lds[0]) * inv;
-  float q = 0.0f;
+      for (int i = 0; i < N; i++) {
+        v[k][i] = to_f32(next[k].v[i]);
+        s += v[k][i];
+      }
+    load(row + step);   // on its way while this row is worked on
+    const float mean = row_sum<kBlock>(s, lanes, lds[0]) * inv;
+    float q = 0.0f;
 #pragma unroll
-  for (int k = 0; k < NV; k++) {
-    const int c = (k * lanes + lane) * N;
+    for (int k = 0; k < NV; k++) {
+      const int c = (k * lanes + lane) * N;
 #pragma unroll
-    for (int i = 0; i < N; i++) {
-      v[k][i] -= mean;
-      if (c + i < D) q = fmaf(v[k][i], v[k][i], q);
+      for (int i = 0; i < N; i++) {
+        v[k][i] -= mean;
+        if (c + i < D) q = fmaf(v[k][i], v[k][i], q);
+      }
     }
-  }
-  const float rstd = 1.0f / sqrtf(row_sum<kBlock>(q, lanes, lds[1]) * inv + p.eps);
-  T* y = static_cast<T*>(p.y) + row * D;
+    const float rstd = 1.0f / sqrtf(row_sum<kBlock>(q, lanes, lds[1]) * inv + p.eps);
+    T* y = static_cast<T*>(p.y) + row * D;
 #pragma unroll
-  for (int k = 0; k < NV; k++) {
-    const int c = (k * lanes + lane) * N;
-    float w[N], b[N];
-    load_param(w, static_cast<const P*>(p.weight) + c, D - c);
-    if (p.bias) load_param(b, static_cast<const P*>(p.bias) + c, D - c);
+    for (int k = 0; k < NV; k++) {
+      const int c = (k * lanes + lane) * N;
 #pragma unroll
-    for (int i = 0; i < N; i++) {
-      const float h = v[k][i] * rstd;
-      v[k][i] = p.bias ? fmaf(h, w[i], b[i]) : h * w[i];
+      for (int i = 0; i < N; i++) v[k][i] = fmaf(v[k][i] * rstd, w[k][i], b[k][i]);
+      store_vec<T>(y + c, v[k], D - c);
     }
-    store_vec<T>(y + c, v[k], D - c);
-  }
-  if (lane == 0) {
-    if (p.mean) p.mean[row] = mean;
-    if (p.rstd) p.rstd[row] = rstd;
-  }
+    if (lane == 0) {
+      if (p.mean) p.mean[row] = mean;
+      if (p.rstd) p.rstd[row] = rstd;
+    }
   }
 }
 
@@ -158,8 +167,7 @@ __device__ __forceinline__ void row_sum2(float& a, float& b, int lanes, float (*
     }
     __syncthreads();
     a = b = 0.0f;
-#pragma unroll
-    for (int w = 0; w < kLnWaves; w++) {
+    for (int w = 0; w < (int)blockDim.x / 64; w++) {
       a += lds[0][w];
       b += lds[1][w];
     }
@@ -176,7 +184,7 @@ __device__ __forceinline__ void row_sum2(float& a, float& b, int lanes, float (*
 // row of partial sums: part[workgroup][dw, db][D].  The sums' order depends on
 // the launch shape alone, so results repeat bit for bit.
 template <typename T, typename P, int NV, bool kBlock>
-__global__ __launch_bounds__(kLnThreads) void layer_norm_backward_kernel(LayerNormParams p, int lanes) {
+__global__ __launch_bounds__(kBlock ? kLnMost : kLnThreads) void layer_norm_backward_kernel(LayerNormParams p, int lanes) {
   constexpr int N = Vec16<T>::kN;
   __shared__ float lds[2][2][kLnWaves];
   __shared__ float gather[kBlock ? 1 : kLnThreads][N + 1];
@@ -194,17 +202,35 @@ __global__ __launch_bounds__(kLnThreads) void layer_norm_backward_kernel(LayerNo
     for (int i = 0; i < N; i++) dw[k][i] = db[k][i] = 0.0f;
   }
   int turn = 0;
-  for (int64_t row = (int64_t)blockIdx.x * rows_wg + sub; row < p.rows; row += (int64_t)gridDim.x * rows_wg, turn ^= 1) {
-    const T* x = static_cast<const T*>(p.x) + row * D;
-    const T* dy = static_cast<const T*>(p.dy) + row * D;
-    float h[NV][N], g[NV][N];
+  const int64_t step = (int64_t)gridDim.x * rows_wg;
+  int64_t row = (int64_t)blockIdx.x * rows_wg + sub;
+  Vec16<T> nx[NV], ny[NV];
+  float next_mean = 0.0f, next_rstd = 0.0f;
+  auto load = [&](int64_t at) {
+    const bool in = at < p.rows;
 #pragma unroll
     for (int k = 0; k < NV; k++) {
       const int c = (k * lanes + lane) * N;
-      load_vec<T>(h[k], x + c, D - c);
-      load_vec<T>(g[k], dy + c, D - c);
+      nx[k] = load_raw(static_cast<const T*>(p.x) + at * D + c, in ? D - c : 0);
+      ny[k] = load_raw(static_cast<const T*>(p.dy) + at * D + c, in ? D - c : 0);
     }
-    const float mean = p.mean[row], rstd = p.rstd[row];
+    if (in) {
+      next_mean = p.mean[at];
+      next_rstd = p.rstd[at];
+    }
+  };
+  load(row);
+  for (; row < p.rows; row += step, turn ^= 1) {
+    float h[NV][N], g[NV][N];
+#pragma unroll
+    for (int k = 0; k < NV; k++)
+#pragma unroll
+      for (int i = 0; i < N; i++) {
+        h[k][i] = to_f32(nx[k].v[i]);
+        g[k][i] = to_f32(ny[k].v[i]);
+      }
+    const float mean = next_mean, rstd = next_rstd;
+    load(row + step);   // on its way while this row is worked on
     float a = 0.0f, b = 0.0f;
 #pragma unroll
     for (int k = 0; k < NV; k++)
@@ -312,8 +338,17 @@ __global__ __launch_bounds__(1024) void layer_norm_reduce_kernel(const float* pa
   __shared__ float lds[32][33];
   const int col = blockIdx.x * 32 + (threadIdx.x & 31), slice = threadIdx.x >> 5;
   float s = 0.0f;
-  if (col < 2 * D)
-    for (int r = slice; r < n; r += 32) s += part[(int64_t)r * 2 * D + col];
+  if (col < 2 * D) {
+    int r = slice;
+    for (; r + 7 * 32 < n; r += 8 * 32) {   // eight loads in flight
+      float v[8];
+#pragma unroll
+      for (int i = 0; i < 8; i++) v[i] = part[(int64_t)(r + i * 32) * 2 * D + col];
+#pragma unroll
+      for (int i = 0; i < 8; i++) s += v[i];
+    }
+    for (; r < n; r += 32) s += part[(int64_t)r * 2 * D + col];
+  }
   lds[slice][threadIdx.x & 31] = s;
   __syncthreads();
   if (slice == 0 && col < 2 * D) {
@@ -324,8 +359,6 @@ __global__ __launch_bounds__(1024) void layer_norm_reduce_kernel(const float* pa
     else if (db) db[col - D] = from_f32<P>(t);
   }
 }
-
-unsigned groups(int64_t n) { return (unsigned)(n < kLnGrid ? n : kLnGrid); }
 
 int pow2_at_least(int v) {
   int p = 1;
@@ -338,21 +371,49 @@ int vectors(int cols, int dtype) {
   return (cols + n - 1) / n;
 }
 
+// A row's lanes, and vectors a lane: up to 128 vectors stay with one wave (no
+// barrier), up to 1024 with a workgroup of as many waves as they need; nv 0:
+// past the registers.
+struct LnShape {
+  int lanes, nv;
+  bool block;
+};
+LnShape shape_of(int cols, int dtype) {
+  const int vecs = vectors(cols, dtype);
+  if (vecs <= 128) return {vecs <= 64 ? pow2_at_least(vecs) : 64, vecs <= 64 ? 1 : 2, false};
+  if (vecs <= 2 * kLnMost) {
+    const int nv = vecs <= kLnMost ? 1 : 2;
+    return {(vecs + 64 * nv - 1) / (64 * nv) * 64, nv, true};
+  }
+  return {kLnThreads, 0, true};
+}
+
+// Calls f with the shape as constants.
+template <typename F>
+void with_shape(const LnShape& h, F f) {
+  using std::integral_constant;
+  if (!h.block) {
+    if (h.nv == 1) f(integral_constant<int, 1>(), integral_constant<bool, false>());
+    else f(integral_constant<int, 2>(), integral_constant<bool, false>());
+  } else if (h.nv == 1) f(integral_constant<int, 1>(), integral_constant<bool, true>());
+  else if (h.nv == 2) f(integral_constant<int, 2>(), integral_constant<bool, true>());
+  else f(integral_constant<int, 0>(), integral_constant<bool, true>());
+}
+
+int64_t row_groups(int64_t rows, const LnShape& h) {
+  const int rows_wg = h.block ? 1 : kLnThreads / h.lanes;
+  return (rows + rows_wg - 1) / rows_wg;
+}
+
 template <typename T, typename P>
 hipError_t forward(const LayerNormParams& p, hipStream_t s) {
-  const int vecs = vectors(p.cols, p.dtype);
-  if (vecs <= 128) {
-    const int lanes = vecs <= 64 ? pow2_at_least(vecs) : 64;
-    const unsigned grid = groups((p.rows + kLnThreads / lanes - 1) / (kLnThreads / lanes));
-    if (vecs <= 64) layer_norm_kernel<T, P, 1, false><<<grid, kLnThreads, 0, s>>>(p, lanes);
-    else layer_norm_kernel<T, P, 2, false><<<grid, kLnThreads, 0, s>>>(p, lanes);
-  } else {
-    const unsigned grid = groups(p.rows);
-    if (vecs <= 256) layer_norm_kernel<T, P, 1, true><<<grid, kLnThreads, 0, s>>>(p, kLnThreads);
-    else if (vecs <= 512) layer_norm_kernel<T, P, 2, true><<<grid, kLnThreads, 0, s>>>(p, kLnThreads);
-    else if (vecs <= 1024) layer_norm_kernel<T, P, 4, true><<<grid, kLnThreads, 0, s>>>(p, kLnThreads);
-    else layer_norm_long_kernel<T, P><<<grid, kLnThreads, 0, s>>>(p);
-  }
+  const LnShape h = shape_of(p.cols, p.dtype);
+  const int64_t need = row_groups(p.rows, h);
+  const unsigned grid = (unsigned)(need < kLnForwardGrid ? need : kLnForwardGrid);
+  with_shape(h, [&](auto nv, auto block) {
+    if constexpr (nv == 0) layer_norm_long_kernel<T, P><<<grid, kLnThreads, 0, s>>>(p);
+    else layer_norm_kernel<T, P, nv, block><<<grid, block ? h.lanes : kLnThreads, 0, s>>>(p, h.lanes);
+  });
   return hipGetLastError();
 }
 
@@ -360,15 +421,11 @@ template <typename T, typename P>
 hipError_t backward(const LayerNormParams& p, hipStream_t s) {
   const int n = layer_norm_partials(p.rows, p.cols, p.dtype);
   if (n > 0) {
-    const int vecs = vectors(p.cols, p.dtype);
-    if (vecs <= 128) {
-      const int lanes = vecs <= 64 ? pow2_at_least(vecs) : 64;
-      if (vecs <= 64) layer_norm_backward_kernel<T, P, 1, false><<<n, kLnThreads, 0, s>>>(p, lanes);
-      else layer_norm_backward_kernel<T, P, 2, false><<<n, kLnThreads, 0, s>>>(p, lanes);
-    } else if (vecs <= 256) layer_norm_backward_kernel<T, P, 1, true><<<n, kLnThreads, 0, s>>>(p, kLnThreads);
-    else if (vecs <= 512) layer_norm_backward_kernel<T, P, 2, true><<<n, kLnThreads, 0, s>>>(p, kLnThreads);
-    else if (vecs <= 1024) layer_norm_backward_kernel<T, P, 4, true><<<n, kLnThreads, 0, s>>>(p, kLnThreads);
-    else layer_norm_backward_long_kernel<T, P><<<n, kLnThreads, 0, s>>>(p);
+    const LnShape h = shape_of(p.cols, p.dtype);
+    with_shape(h, [&](auto nv, auto block) {
+      if constexpr (nv == 0) layer_norm_backward_long_kernel<T, P><<<n, kLnThreads, 0, s>>>(p);
+      else layer_norm_backward_kernel<T, P, nv, block><<<n, block ? h.lanes : kLnThreads, 0, s>>>(p, h.lanes);
+    });
     if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
   }
   layer_norm_reduce_kernel<P><<<(2 * p.cols + 31) / 32, 1024, 0, s>>>(p.part, n, p.cols, static_cast<P*>(p.dweight),
@@ -378,11 +435,12 @@ hipError_t backward(const LayerNormParams& p, hipStream_t s) {
 
 }  // namespace
 
+// Workgroups of the backward: as many as the registers let run at once, five a
+// CU where a lane has one vector of a narrow row, else three.
 int layer_norm_partials(int64_t rows, int cols, int dtype) {
-  const int vecs = vectors(cols, dtype);
-  const int rows_wg = vecs <= 64 ? kLnThreads / pow2_at_least(vecs) : vecs <= 128 ? kLnThreads / 64 : 1;
-  const int64_t need = (rows + rows_wg - 1) / rows_wg;
-  return (int)(need < 1024 ? need : 1024);
+  const LnShape h = shape_of(cols, dtype);
+  const int64_t need = row_groups(rows, h), most = h.nv == 1 && !h.block ? 1280 : 768;
+  return (int)(need < most ? need : most);
 }
 
 #define NEST_LN_DISPATCH(fn)                                                                                   \

@@ -29,17 +29,23 @@ __device__ __forceinline__ T from_f32(float v) { return (T)v; }
 
 // n valid elements at p (n may be <= 0 or above kN): the rest read as zero.
 template <typename T>
-__device__ __forceinline__ void load_vec(float (&f)[Vec16<T>::kN], const T* p, int n) {
+__device__ __forceinline__ Vec16<T> load_raw(const T* p, int n) {
   constexpr int N = Vec16<T>::kN;
+  Vec16<T> t;
   if (n >= N) {
-    Vec16<T> t;
     __builtin_memcpy(&t, p, 16);
-#pragma unroll
-    for (int i = 0; i < N; i++) f[i] = to_f32(t.v[i]);
   } else {
 #pragma unroll
-    for (int i = 0; i < N; i++) f[i] = i < n ? to_f32(p[i]) : 0.0f;
+    for (int i = 0; i < N; i++) t.v[i] = i < n ? p[i] : (T)0.0f;
   }
+  return t;
+}
+
+template <typename T>
+__device__ __forceinline__ void load_vec(float (&f)[Vec16<T>::kN], const T* p, int n) {
+  const Vec16<T> t = load_raw(p, n);
+#pragma unroll
+  for (int i = 0; i < Vec16<T>::kN; i++) f[i] = to_f32(t.v[i]);
 }
 
 template <typename T>
@@ -57,11 +63,21 @@ __device__ __forceinline__ void store_vec(T* p, const float (&f)[Vec16<T>::kN], 
   }
 }
 
-// kN parameters (weights, biases) of a type of their own as float32.
+// N parameters (weights, biases) of a type of their own as float32.
 template <typename P, int N>
 __device__ __forceinline__ void load_param(float (&f)[N], const P* p, int n) {
+  constexpr int K = Vec16<P>::kN;
+  if constexpr (K <= N) {
 #pragma unroll
-  for (int i = 0; i < N; i++) f[i] = i < n ? to_f32(p[i]) : 0.0f;
+    for (int v = 0; v < N / K; v++) {
+      const Vec16<P> t = load_raw(p + v * K, n - v * K);
+#pragma unroll
+      for (int i = 0; i < K; i++) f[v * K + i] = to_f32(t.v[i]);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; i++) f[i] = i < n ? to_f32(p[i]) : 0.0f;
+  }
 }
 
 }  // namespace nest

@@ -50,9 +50,9 @@ def _like(t: torch.Tensor, ref: torch.Tensor, shape, name: str, dtype=None) -> t
         raise ValueError(f"{name} is on {t.device}, expected {ref.device}")
     if t.dtype != (dtype or ref.dtype):
         raise TypeError(f"{name} is {t.dtype}, expected {dtype or ref.dtype}")
-    if tuple(t.shape) != tuple(shape):
+    if t.shape != shape:
         raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {tuple(shape)}")
-    return t.detach().contiguous()
+    return _whole(t)
 
 
 def _aligned(t: torch.Tensor) -> torch.Tensor:
@@ -60,19 +60,29 @@ def _aligned(t: torch.Tensor) -> torch.Tensor:
     return t.clone() if t.data_ptr() % 16 else t
 
 
-class _on:
-    """Makes the tensors' device the current one around a launch, where it is not already."""
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
-    def __init__(self, device: torch.device):
-        self.guard = None if device.index == torch.cuda.current_device() else torch.cuda.device(device)
 
-    def __enter__(self):
-        if self.guard is not None:
-            self.guard.__enter__()
+def _call(name: str, device: torch.device, *args) -> None:
+    """Calls a library function on the device's current stream, with the device current."""
+    lib = L.lib()
+    index = device.index
+    stream = _raw_stream(index) if _raw_stream is not None else torch.cuda.current_stream(device).cuda_stream
+    if index == torch.cuda.current_device():
+        rc = getattr(lib, name)(*args, stream)
+    else:
+        with torch.cuda.device(index):
+            rc = getattr(lib, name)(*args, stream)
+    if rc != L.NEST_OK:
+        L.check(rc, name)
 
-    def __exit__(self, *exc):
-        if self.guard is not None:
-            self.guard.__exit__(*exc)
+
+def _at(t: Optional[torch.Tensor]):
+    return None if t is None else t.data_ptr()
+
+
+def _whole(t: torch.Tensor) -> torch.Tensor:
+    return t if t.is_contiguous() else t.detach().contiguous()
 
 
 def _workspace(nbytes: int, device) -> Optional[torch.Tensor]:
@@ -94,19 +104,16 @@ def _norm_args(x, weight, bias, eps):
         bias = _like(bias, x, (D,), "bias", pdt)
     if eps is not None and not eps >= 0:
         raise ValueError("eps must not be negative")
-    return code, _CODE[pdt], x.detach().contiguous(), weight, bias, x.numel() // D, D
+    return code, _CODE[pdt], _whole(x), weight, bias, x.numel() // D, D
 
 
 def layer_norm_forward(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None, eps: float = 1e-5):
     """(y, mean, rstd): y = (x - mean) rstd weight + bias over the last dimension; mean and rstd are float32 [rows]."""
     code, pcode, x, weight, bias, rows, D = _norm_args(x, weight, bias, eps)
     y = torch.empty_like(x)
-    stats = torch.empty((2, rows), dtype=torch.float32, device=x.device)
-    with _on(x.device):
-        L.check(L.lib().nest_layer_norm(rows, D, code, pcode, L.ptr(x), L.ptr(weight), L.ptr(bias), float(eps),
-                                        L.ptr(y), L.ptr(stats[0]), L.ptr(stats[1]), L.stream_ptr(x.device)),
-                "nest_layer_norm")
-    return y, stats[0], stats[1]
+    mean, rstd = torch.empty((2, rows), dtype=torch.float32, device=x.device).unbind(0)
+    _call("nest_layer_norm", x.device, rows, D, code, pcode, _at(x), _at(weight), _at(bias), eps, _at(y), _at(mean), _at(rstd))
+    return y, mean, rstd
 
 
 def layer_norm_backward(dy: torch.Tensor, x: torch.Tensor, weight: torch.Tensor, mean: torch.Tensor,
@@ -117,13 +124,10 @@ def layer_norm_backward(dy: torch.Tensor, x: torch.Tensor, weight: torch.Tensor,
     mean, rstd = (_like(t, x, (rows,), n, torch.float32) for t, n in ((mean, "mean"), (rstd, "rstd")))
     dx, dw = torch.empty_like(x), torch.empty_like(weight)
     db = torch.empty_like(weight) if with_bias else None
-    lib = L.lib()
-    nbytes = lib.nest_layer_norm_backward_workspace_size(rows, D, code)
+    nbytes = L.lib().nest_layer_norm_backward_workspace_size(rows, D, code)
     ws = _workspace(nbytes, x.device)
-    with _on(x.device):
-        L.check(lib.nest_layer_norm_backward(rows, D, code, pcode, L.ptr(dy), L.ptr(x), L.ptr(weight), L.ptr(mean),
-                                             L.ptr(rstd), L.ptr(dx), L.ptr(dw), L.ptr(db), L.ptr(ws), nbytes,
-                                             L.stream_ptr(x.device)), "nest_layer_norm_backward")
+    _call("nest_layer_norm_backward", x.device, rows, D, code, pcode, _at(dy), _at(x), _at(weight), _at(mean), _at(rstd), _at(dx),
+          _at(dw), _at(db), _at(ws), nbytes)
     return dx, dw, db
 
 
@@ -162,11 +166,9 @@ def dropout_forward(x: torch.Tensor, p: float, seed: int, offset: int = 0,
         raise ValueError("seed and offset are unsigned 64-bit numbers")
     if residual is not None:
         residual = _like(residual, x, x.shape, "residual")
-    x = x.detach().contiguous()
+    x = _whole(x)
     y = torch.empty_like(x)
-    with _on(x.device):
-        L.check(L.lib().nest_dropout(x.numel(), code, L.ptr(x), L.ptr(residual), float(p), seed, offset, L.ptr(y),
-                                     L.stream_ptr(x.device)), "nest_dropout")
+    _call("nest_dropout", x.device, x.numel(), code, _at(x), _at(residual), p, seed, offset, _at(y))
     return y
 
 
@@ -204,7 +206,7 @@ def _gated(x, w_gate, w_up, w_down, activation):
     I, H, O = x.shape[-1], w_gate.shape[0], w_down.shape[0]
     if min(I, H, O) < 1:
         raise ValueError("in_features, hidden and out_features must be at least 1")
-    x = _aligned(x.detach().contiguous())
+    x = _aligned(_whole(x))
     ws = tuple(_aligned(_like(w, x, s, n)) for w, s, n in ((w_gate, (H, I), "w_gate"), (w_up, (H, I), "w_up"), (w_down, (O, H), "w_down")))
     rows = x.numel() // I
     f = L.GatedFfn(ct.sizeof(L.GatedFfn), code, _ACT[activation], I, H, O, rows, x.data_ptr(), *(w.data_ptr() for w in ws))
@@ -212,9 +214,12 @@ def _gated(x, w_gate, w_up, w_down, activation):
 
 
 def _gated_sizes(f):
-    s = [ct.c_size_t() for _ in range(4)]
-    L.check(L.lib().nest_gated_ffn_sizes(ct.byref(f), *(ct.byref(v) for v in s)), "nest_gated_ffn_sizes")
-    return [v.value for v in s]
+    """Bytes of (kept, a forward's workspace, a backward's with kept, without)."""
+    kept, fwd, bwd, alone = ct.c_size_t(), ct.c_size_t(), ct.c_size_t(), ct.c_size_t()
+    rc = L.lib().nest_gated_ffn_sizes(f, kept, fwd, bwd, alone)
+    if rc != L.NEST_OK:
+        L.check(rc, "nest_gated_ffn_sizes")
+    return kept.value, fwd.value, bwd.value, alone.value
 
 
 def gated_ffn_forward(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down: torch.Tensor,
@@ -227,9 +232,7 @@ def gated_ffn_forward(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor,
     y = torch.empty(x.shape[:-1] + (f.out_features,), dtype=x.dtype, device=x.device)
     kept = _workspace(kept_bytes, x.device) if training else None
     work = _workspace(fwd_bytes, x.device)
-    with _on(x.device):
-        L.check(L.lib().nest_gated_ffn_forward(ct.byref(f), L.ptr(y), L.ptr(kept), L.ptr(work), fwd_bytes,
-                                               L.stream_ptr(x.device)), "nest_gated_ffn_forward")
+    _call("nest_gated_ffn_forward", x.device, f, _at(y), _at(kept), _at(work), fwd_bytes)
     return y, kept
 
 
@@ -247,9 +250,7 @@ def gated_ffn_backward(dy: torch.Tensor, x: torch.Tensor, w_gate: torch.Tensor, 
     grads = [torch.empty_like(t) if n else None for t, n in zip((x, *ws), needs)]
     nbytes = bwd_bytes if kept is not None else alone_bytes
     work = _workspace(nbytes, x.device)
-    with _on(x.device):
-        L.check(L.lib().nest_gated_ffn_backward(ct.byref(f), L.ptr(dy), L.ptr(kept), *(L.ptr(g) for g in grads),
-                                                L.ptr(work), nbytes, L.stream_ptr(x.device)), "nest_gated_ffn_backward")
+    _call("nest_gated_ffn_backward", x.device, f, _at(dy), _at(kept), *(_at(g) for g in grads), _at(work), nbytes)
     return tuple(grads)
 
 
