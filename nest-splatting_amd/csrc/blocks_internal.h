@@ -66,6 +66,7 @@ struct TileChoice {
   int side, splits;
 };
 
+constexpr int kNarrowLdsBytes = 160 * 1024;
 constexpr int kNarrowPad = 8;   // elements: rows of 16 bytes more fall on different banks
 
 // LDS of the forward, in elements: gate and up rows (32 of each in turn), down
@@ -84,14 +85,9 @@ __host__ __device__ inline NarrowLds narrow_lds(int ki, int hidden, int waves) {
   return l;
 }
 
-// Groups of 32 hidden features, one a wave, of the narrow backward: a power of two.
-__host__ __device__ constexpr int narrow_slices(int hidden) {
-  return hidden <= 32 ? 1 : hidden <= 64 ? 2 : hidden <= 128 ? 4 : hidden <= 256 ? 8 : 16;
-}
-
 // LDS of the narrow backward, in elements: weights, then for each group of
-// waves x, dy [32][pitch_in] and dg, du, h [32][pitch_h]; at its end the
-// groups' sums.
+// waves x, dy [32][pitch_in] and dg, du [32][pitch_h]; at its end the groups'
+// sums.  slices: of 32 hidden features, one a wave.
 struct NarrowBackLds {
   int groups, pitch_in, pitch_h, tiles, tile_stride, total;
 };
@@ -102,7 +98,7 @@ __host__ __device__ constexpr NarrowBackLds narrow_back_lds(int ki, int slices) 
   l.pitch_in = ki * 32 + kNarrowPad;
   l.pitch_h = h + kNarrowPad;
   l.tiles = 2 * h * l.pitch_in + ki * 32 * l.pitch_h;
-  l.tile_stride = 2 * 32 * l.pitch_in + 3 * 32 * l.pitch_h;
+  l.tile_stride = 2 * 32 * l.pitch_in + 2 * 32 * l.pitch_h;
   l.total = l.tiles + l.groups * l.tile_stride;
   const int sums = l.groups > 1 ? slices * 12 * ki * 256 * 2 : 0;   // float32: two elements each
   if (sums > l.total) l.total = sums;
@@ -116,7 +112,9 @@ struct GatedLayout {
   size_t h, dg, du, kept, x, wg, wu, wd, dy, part;
   size_t bytes, kept_bytes;
   TileChoice y, dx, dw;
-  bool narrow, narrow_back;   // gated_narrow.h
+  bool narrow;                // gated_narrow.h
+  size_t dx_sum;              // of its backward: sums of dx between launches,
+  int narrow_parts, narrow_slices;   // launches, and slices of 32 hidden features in each
   bool few;                   // gated_few.h (forward)
   int narrow_groups;          // workgroups of its backward
 };

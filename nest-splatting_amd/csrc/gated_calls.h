@@ -32,8 +32,8 @@ template <typename T>
 hipError_t gated_backward(const GatedParams& p, hipStream_t s) {
   const GatedLayout l = gated_layout(p.rows, p.in, p.hidden, p.out, p.dtype, true, p.kept == nullptr);
   if constexpr (sizeof(T) == 2)
-    if (l.narrow_back) return launch_narrow_backward<T>(p, l, s);
-  const bool alone = p.kept == nullptr || l.narrow;
+    if (l.narrow) return launch_narrow_backward<T>(p, l, s);
+  const bool alone = p.kept == nullptr;
   uint8_t* ws = static_cast<uint8_t*>(p.ws);
   T *h = reinterpret_cast<T*>(ws + l.h), *dg = reinterpret_cast<T*>(ws + l.dg), *du = reinterpret_cast<T*>(ws + l.du);
   Operands<T> o;

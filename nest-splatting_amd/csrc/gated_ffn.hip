@@ -64,19 +64,22 @@ TileChoice choose_tile(int n, const int64_t* M, const int64_t* N, int64_t K, int
 }
 
 // Whether whole rows stay on the chip (gated_narrow.h): 16-bit rows of at most
-// 128 features whose weights fit a CU's LDS.
-bool narrow_rows(int64_t rows, int in, int hidden, int out, int es) {
-  const int side = in > out ? in : out;
-  if (es != 2 || side > 128 || rows < 64) return false;
-  return narrow_lds((side + 31) / 32, hidden, 8).total * 2 <= 160 * 1024;
-}
+// 128 features.
+bool narrow_rows(int64_t rows, int in, int out, int es) { return es == 2 && in <= 128 && out <= 128 && rows >= 64; }
 
-// Whether the backward does too: the accumulators of the weight gradients fit
-// the registers and everything else the LDS.
-bool narrow_rows_back(int in, int hidden, int out) {
-  const int side = in > out ? in : out, ki = (side + 31) / 32, slices = narrow_slices(hidden);
-  if (slices > (ki == 1 ? 8 : 4)) return false;
-  return narrow_back_lds(ki, slices).total * 2 <= 160 * 1024;
+// Launches of the narrow backward and slices of 32 hidden features in each: the
+// least slices in all, then the fewest launches.
+void narrow_parts(int ki, int hidden, int& parts, int& slices) {
+  const int most = ki <= 2 ? 8 : 4;
+  parts = slices = 1 << 20;
+  for (int s = most; s >= (ki == 2 ? 2 : 1); s /= 2) {   // one slice of 33 to 64 features: past the registers
+    const int n = (hidden + 32 * s - 1) / (32 * s);
+    if (n > 1 && s < most / 2) break;   // each launch reads x and dy again
+    if (parts == 1 << 20 || n * s < parts * slices) {
+      parts = n;
+      slices = s;
+    }
+  }
 }
 
 TileChoice choose_gate_tile(int64_t M, int64_t N, int64_t K, int es) { return choose_tile(1, &M, &N, K, es, false); }
@@ -95,14 +98,15 @@ GatedLayout gated_layout(int64_t rows, int in, int hidden, int out, int dtype, b
     at = (at + (size_t)bytes + 255) / 256 * 256;
     return o;
   };
-  l.narrow = narrow_rows(rows, in, hidden, out, es);
-  if (l.narrow && !back) return l;
-  l.narrow_back = l.narrow && narrow_rows_back(in, hidden, out);
-  if (l.narrow_back) {
-    const int ki = ((in > out ? in : out) + 31) / 32, slices = narrow_slices(hidden);
-    const int64_t need = cdiv(rows, 32 * narrow_back_lds(ki, slices).groups);
+  l.narrow = narrow_rows(rows, in, out, es);
+  if (l.narrow) {
+    if (!back) return l;
+    const int ki = ((in > out ? in : out) + 31) / 32;
+    narrow_parts(ki, hidden, l.narrow_parts, l.narrow_slices);
+    const int64_t need = cdiv(rows, 32 * narrow_back_lds(ki, l.narrow_slices).groups);
     l.narrow_groups = (int)(need < 256 ? need : 256);
-    l.part = take((int64_t)l.narrow_groups * 3 * slices * 32 * ki * 32 * 4);
+    l.part = take((int64_t)l.narrow_groups * 3 * l.narrow_slices * 32 * ki * 32 * 4);
+    if (l.narrow_parts > 1) l.dx_sum = take(cdiv(rows, 32) * 32 * ki * 32 * 4);
     l.bytes = at;
     return l;
   }
@@ -135,7 +139,7 @@ GatedLayout gated_layout(int64_t rows, int in, int hidden, int out, int dtype, b
     const int64_t WM[3] = {hidden, hidden, out}, WN[3] = {in, in, hidden};
     l.dw = choose_tile(3, WM, WN, rows, es, true);
     partial(l.dw, 3, WM, WN);
-    if (alone || l.narrow) l.kept = take(kept_bytes);
+    if (alone) l.kept = take(kept_bytes);
     if (l.ldy != out) l.dy = take(rows * l.ldy * es);
   }
   if (l.ldx != in) {
@@ -146,7 +150,7 @@ GatedLayout gated_layout(int64_t rows, int in, int hidden, int out, int dtype, b
   if (l.ldh != hidden) l.wd = take(out * l.ldh * es);
   l.part = take(part);
   l.bytes = at;
-  l.kept_bytes = l.narrow ? 0 : (size_t)kept_bytes;   // the narrow backward makes them again
+  l.kept_bytes = (size_t)kept_bytes;
   return l;
 }
 

@@ -38,40 +38,45 @@ __device__ __forceinline__ typename Mma<T>::Frag load8(const T* p, int n) {
 }
 
 template <typename T, int kAct, int KI, int RG>
-__global__ __launch_bounds__(512, 2) void narrow_forward_kernel(Narrow<T> p) {
+__global__ __launch_bounds__(512, 2) void narrow_forward_kernel(Narrow<T> p, int chunk) {
   typedef typename Mma<T>::Frag Frag;
   constexpr int FO = 2 * KI;
   extern __shared__ __attribute__((aligned(16))) uint8_t narrow_mem[];
   T* lds = reinterpret_cast<T*>(narrow_mem);
   const int waves = blockDim.x >> 6;
-  const NarrowLds l = narrow_lds(KI, p.hidden, waves);
+  const NarrowLds l = narrow_lds(KI, chunk, waves);
   const int h32 = (p.hidden + 31) & ~31;
-  // weights; what lies past a matrix is zero
-  for (int c = threadIdx.x; c < 2 * h32 * (KI * 4); c += blockDim.x) {
-    const int row = c / (KI * 4), k = c % (KI * 4) * 8;
-    const int h = (row >> 6) * 32 + (row & 31);
-    const T* w = row & 32 ? p.wu : p.wg;
-    const Frag f = load8<T>(w + (int64_t)h * p.in + k, h < p.hidden ? p.in - k : 0);
-    *reinterpret_cast<Frag*>(lds + row * l.pitch_in + k) = f;
-  }
-  for (int c = threadIdx.x; c < KI * 32 * (h32 / 8); c += blockDim.x) {
-    const int o = c / (h32 / 8), k = c % (h32 / 8) * 8;   // elements k .. k + 7 of a row in LDS: a chunk's quarter
-    const int base = (k & ~31) + ((k >> 3) & 3) * 4;
-    Frag f;
-#pragma unroll
-    for (int e = 0; e < 8; e++) {
-      const int h = base + (e & 3) + (e >> 2) * 16;
-      f[e] = o < p.out && h < p.hidden ? p.wd[(int64_t)o * p.hidden + h] : (T)0.0f;
+  // weights of hidden features from h0 on; what lies past a matrix is zero
+  auto load_weights = [&](int h0) {
+    for (int c = threadIdx.x; c < 2 * chunk * (KI * 4); c += blockDim.x) {
+      const int row = c / (KI * 4), k = c % (KI * 4) * 8;
+      const int h = h0 + (row >> 6) * 32 + (row & 31);
+      const T* w = row & 32 ? p.wu : p.wg;
+      *reinterpret_cast<Frag*>(lds + row * l.pitch_in + k) = load8<T>(w + (int64_t)h * p.in + k, h < p.hidden ? p.in - k : 0);
     }
-    *reinterpret_cast<Frag*>(lds + l.down + o * l.pitch_h + k) = f;
-  }
-  __syncthreads();
+    for (int c = threadIdx.x; c < KI * 32 * (chunk / 8); c += blockDim.x) {
+      const int o = c / (chunk / 8), k = c % (chunk / 8) * 8;   // elements k .. k + 7 of a row in LDS: a quarter's
+      const int base = h0 + (k & ~31) + ((k >> 3) & 3) * 4;
+      Frag f;
+#pragma unroll
+      for (int e = 0; e < 8; e++) {
+        const int h = base + (e & 3) + (e >> 2) * 16;
+        f[e] = o < p.out && h < p.hidden ? p.wd[(int64_t)o * p.hidden + h] : (T)0.0f;
+      }
+      *reinterpret_cast<Frag*>(lds + l.down + o * l.pitch_h + k) = f;
+    }
+    __syncthreads();
+  };
+  const bool whole = chunk >= h32;
+  if (whole) load_weights(0);
   const int lane = threadIdx.x & 63, r = lane & 15, q = lane >> 4;
   const T* w_in = lds + r * l.pitch_in + q * 8;
   const T* w_down = lds + l.down + r * l.pitch_h + q * 8;
   auto& stage = *reinterpret_cast<RowStage<T, FO>*>(lds + l.stage + wave_id() * 16 * RowStage<T, FO>::kPitch);
+  // every wave of a workgroup takes the same number of turns: there may be barriers inside
   const int64_t step = (int64_t)gridDim.x * waves * (16 * RG);
-  int64_t row = ((int64_t)blockIdx.x * waves + wave_id()) * (16 * RG);
+  int64_t base = (int64_t)blockIdx.x * waves * (16 * RG);
+  int64_t row = base + wave_id() * (16 * RG);
   Frag x[RG][KI];
   auto load_x = [&](int64_t at) {
 #pragma unroll
@@ -82,40 +87,47 @@ __global__ __launch_bounds__(512, 2) void narrow_forward_kernel(Narrow<T> p) {
         x[i][k] = load8<T>(p.x + n * p.in + k * 32 + q * 8, n < p.rows ? p.in - k * 32 - q * 8 : 0);
       }
   };
-  if (row < p.rows) load_x(row);
-  for (; row < p.rows; row += step) {
+  load_x(row);
+  for (; base < p.rows; base += step, row += step) {
     f32x4 y[RG][FO] = {};
-    for (int hc = 0; hc < h32; hc += 32) {
-      f32x4 g[RG][2] = {}, u[RG][2] = {};
-      const T* w = w_in + hc * 2 * l.pitch_in;
+    for (int h0 = 0; h0 < h32; h0 += chunk) {
+      if (!whole) {
+        __syncthreads();   // the last chunk is no longer read
+        load_weights(h0);
+      }
+      const int end = h32 - h0 < chunk ? h32 - h0 : chunk;
+      for (int hc = 0; hc < end; hc += 32) {
+        f32x4 g[RG][2] = {}, u[RG][2] = {};
+        const T* w = w_in + hc * 2 * l.pitch_in;
 #pragma unroll
-      for (int k = 0; k < KI; k++)
+        for (int k = 0; k < KI; k++)
 #pragma unroll
-        for (int b = 0; b < 2; b++) {
-          const Frag fg = *reinterpret_cast<const Frag*>(w + b * 16 * l.pitch_in + k * 32);
-          const Frag fu = *reinterpret_cast<const Frag*>(w + (32 + b * 16) * l.pitch_in + k * 32);
+          for (int b = 0; b < 2; b++) {
+            const Frag fg = *reinterpret_cast<const Frag*>(w + b * 16 * l.pitch_in + k * 32);
+            const Frag fu = *reinterpret_cast<const Frag*>(w + (32 + b * 16) * l.pitch_in + k * 32);
 #pragma unroll
-          for (int i = 0; i < RG; i++) {
-            g[i][b] = Mma<T>::run(fg, x[i][k], g[i][b]);
-            u[i][b] = Mma<T>::run(fu, x[i][k], u[i][b]);
+            for (int i = 0; i < RG; i++) {
+              g[i][b] = Mma<T>::run(fg, x[i][k], g[i][b]);
+              u[i][b] = Mma<T>::run(fu, x[i][k], u[i][b]);
+            }
           }
+        Frag h[RG];
+#pragma unroll
+        for (int i = 0; i < RG; i++)
+#pragma unroll
+          for (int e = 0; e < 8; e++) {
+            float unused;
+            h[i][e] = from_f32<T>(act_value<T, kAct, false>(g[i][e >> 2][e & 3], unused) * u[i][e >> 2][e & 3]);
+          }
+#pragma unroll
+        for (int o = 0; o < FO; o++) {
+          const Frag fd = *reinterpret_cast<const Frag*>(w_down + o * 16 * l.pitch_h + hc);
+#pragma unroll
+          for (int i = 0; i < RG; i++) y[i][o] = Mma<T>::run(fd, h[i], y[i][o]);
         }
-      Frag h[RG];
-#pragma unroll
-      for (int i = 0; i < RG; i++)
-#pragma unroll
-        for (int e = 0; e < 8; e++) {
-          float unused;
-          h[i][e] = from_f32<T>(act_value<T, kAct, false>(g[i][e >> 2][e & 3], unused) * u[i][e >> 2][e & 3]);
-        }
-#pragma unroll
-      for (int o = 0; o < FO; o++) {
-        const Frag fd = *reinterpret_cast<const Frag*>(w_down + o * 16 * l.pitch_h + hc);
-#pragma unroll
-        for (int i = 0; i < RG; i++) y[i][o] = Mma<T>::run(fd, h[i], y[i][o]);
       }
     }
-    if (row + step < p.rows) load_x(row + step);   // on its way while y is stored
+    load_x(row + step);   // on its way while y is stored
     if (p.out % 8 == 0) {
 #pragma unroll
       for (int i = 0; i < RG; i++)
@@ -135,12 +147,18 @@ hipError_t narrow_forward(const Narrow<T>& p, hipStream_t s) {
   // 64 rows a wave where registers allow: each weight fragment read from LDS is used RG times
   constexpr int RG = KI <= 2 ? 4 : 2;
   const bool small = p.rows < (int64_t)256 * 8 * 16 * RG;   // fewer rows than a full chip's waves take: smaller workgroups
-  const int waves = small ? 4 : 8;
+  const int waves = small ? 4 : 8, h32 = (p.hidden + 31) / 32 * 32;
+  // hidden features in LDS at a time: all, or equal parts that fit
+  int parts = 1, chunk = h32;
+  while (narrow_lds(KI, chunk, waves).total * sizeof(T) > kNarrowLdsBytes) {
+    parts++;
+    chunk = (h32 / 32 + parts - 1) / parts * 32;
+  }
   const int64_t tiles = (p.rows + 16 * RG * waves - 1) / (16 * RG * waves);
-  const size_t lds = (size_t)narrow_lds(KI, p.hidden, waves).total * sizeof(T);
+  const size_t lds = (size_t)narrow_lds(KI, chunk, waves).total * sizeof(T);
   const int64_t full = 256 * (lds <= 80 * 1024 ? 2 : 1);
   with_act(p.act, [&](auto act) {
-    narrow_forward_kernel<T, act.value, KI, RG><<<(unsigned)(tiles < full ? tiles : full), waves * 64, lds, s>>>(p);
+    narrow_forward_kernel<T, act.value, KI, RG><<<(unsigned)(tiles < full ? tiles : full), waves * 64, lds, s>>>(p, chunk);
   });
   return hipGetLastError();
 }
@@ -168,14 +186,20 @@ hipError_t launch_narrow_forward(const GatedParams& g, hipStream_t s) {
 // columns; read transposed (32 rows as the product's k) they are operands of
 // the weight gradients, as are x and dy.  One copy of the weights in LDS
 // serves both directions for the same reason.
+//
+// More hidden features than a group's waves have (256, or 128 for over 64
+// features) take a launch each for equal parts of them; dx is summed between
+// the launches in float32, in the order the accumulators hold it.
 
 template <typename T>
 struct NarrowBack {
   const T *x, *wg, *wu, *wd, *dy;
   T* dx;            // or null
+  float* dx_sum;    // sums of dx between launches, see below
   float* part;      // [workgroups][dWg, dWu: slices 32 x in padded; dWd: out padded x slices 32]
   int64_t rows;
   int in, hidden, out, act;
+  int first, last;  // hidden features of this launch
 };
 
 // Eight values of a lane's row (or column) that lie down a column of a
@@ -203,11 +227,11 @@ __global__ __launch_bounds__(KI <= 2 ? 512 : 256, KI <= 2 ? 2 : 1) void narrow_b
   for (int c = threadIdx.x; c < 2 * H * KI * 4; c += kThreads) {
     const int row = c / (KI * 4), k = c % (KI * 4) * 8, h = row < H ? row : row - H;
     *reinterpret_cast<Frag*>(lds + row * PI + k) =
-        load8<T>((row < H ? p.wg : p.wu) + (int64_t)h * p.in + k, h < p.hidden ? p.in - k : 0);
+        load8<T>((row < H ? p.wg : p.wu) + (int64_t)(p.first + h) * p.in + k, p.first + h < p.last ? p.in - k : 0);
   }
   for (int c = threadIdx.x; c < KI * 32 * (H / 8); c += kThreads) {
-    const int o = c / (H / 8), k = c % (H / 8) * 8;
-    *reinterpret_cast<Frag*>(wd + o * PH + k) = load8<T>(p.wd + (int64_t)o * p.hidden + k, o < p.out ? p.hidden - k : 0);
+    const int o = c / (H / 8), k = p.first + c % (H / 8) * 8;
+    *reinterpret_cast<Frag*>(wd + o * PH + k - p.first) = load8<T>(p.wd + (int64_t)o * p.hidden + k, o < p.out ? p.last - k : 0);
   }
   const int lane = threadIdx.x & 63, r = lane & 15, q = lane >> 4;
   const int group = wave_id() / SL, slice = wave_id() % SL, t = threadIdx.x % (SL * 64);
@@ -215,7 +239,6 @@ __global__ __launch_bounds__(KI <= 2 ? 512 : 256, KI <= 2 ? 2 : 1) void narrow_b
   T* const dys = xs + 32 * PI;
   T* const dg = dys + 32 * PI;
   T* const du = dg + 32 * PH;
-  T* const hh = du + 32 * PH;
   // x and dy of the next rows, in registers until their place in LDS is free
   constexpr int kChunks = 256 * KI, kLoads = (kChunks + SL * 64 - 1) / (SL * 64);
   Frag next[kLoads];
@@ -267,37 +290,48 @@ __global__ __launch_bounds__(KI <= 2 ? 512 : 256, KI <= 2 ? 2 : 1) void narrow_b
         }
       }
     }
+    // dg, du and h of this wave's own columns, which no other wave reads before
+    // the barrier: h first takes dg's place to be read transposed
+    Four<T> vg[2][2], vu[2][2], vh[2][2];
     with_act(p.act, [&](auto act) {
 #pragma unroll
       for (int b = 0; b < 2; b++)
 #pragma unroll
-        for (int i = 0; i < 2; i++) {
-          Four<T> vg, vu, vh;
+        for (int i = 0; i < 2; i++)
 #pragma unroll
           for (int e = 0; e < 4; e++) {
             float slope;
             const float a = act_value<T, act.value, true>(g[b][i][e], slope), d = dh[b][i][e];
-            vg.v[e] = from_f32<T>(d * u[b][i][e] * slope);
-            vu.v[e] = from_f32<T>(d * a);
-            vh.v[e] = from_f32<T>(a * u[b][i][e]);
+            vg[b][i].v[e] = from_f32<T>(d * u[b][i][e] * slope);
+            vu[b][i].v[e] = from_f32<T>(d * a);
+            vh[b][i].v[e] = from_f32<T>(a * u[b][i][e]);
           }
-          const int at = (i * 16 + r) * PH + slice * 32 + b * 16 + q * 4;
-          *reinterpret_cast<Four<T>*>(dg + at) = vg;
-          *reinterpret_cast<Four<T>*>(du + at) = vu;
-          *reinterpret_cast<Four<T>*>(hh + at) = vh;
-        }
     });
-    // this wave's own columns of dg, du and h: no other wave's writes are read
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
+    auto put = [&](T* to, const Four<T> (&v)[2][2]) {
+#pragma unroll
+      for (int b = 0; b < 2; b++)
+#pragma unroll
+        for (int i = 0; i < 2; i++) *reinterpret_cast<Four<T>*>(to + (i * 16 + r) * PH + slice * 32 + b * 16 + q * 4) = v[b][i];
+    };
+    auto settle = [&]() {
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+    };
     {
       Frag fg[2], fu[2], fh[2];
+      put(dg, vh);
+      put(du, vu);
+      settle();
 #pragma unroll
       for (int b = 0; b < 2; b++) {
-        fg[b] = down_column<T>(dg + slice * 32 + b * 16, PH);
+        fh[b] = down_column<T>(dg + slice * 32 + b * 16, PH);
         fu[b] = down_column<T>(du + slice * 32 + b * 16, PH);
-        fh[b] = down_column<T>(hh + slice * 32 + b * 16, PH);
       }
+      settle();
+      put(dg, vg);
+      settle();
+#pragma unroll
+      for (int b = 0; b < 2; b++) fg[b] = down_column<T>(dg + slice * 32 + b * 16, PH);
 #pragma unroll
       for (int j = 0; j < FI; j++) {
         const Frag fx = down_column<T>(xs + j * 16, PI), fy = down_column<T>(dys + j * 16, PI);
@@ -311,10 +345,12 @@ __global__ __launch_bounds__(KI <= 2 ? 512 : 256, KI <= 2 ? 2 : 1) void narrow_b
     }
     __syncthreads();   // dg and du are whole; x and dy are no longer read
     place();
-    if (p.dx) {
+    if (p.dx && row < p.rows) {   // the whole group, and no barrier inside
       for (int tile = slice; tile < FI * 2; tile += SL) {
         const int j = tile >> 1, i = tile & 1;
+        float* const sum = p.dx_sum + (((row >> 4) + i) * FI + j) * 256 + lane * 4;   // rows in whole 32s
         f32x4 acc = {};
+        if (p.first) acc = *reinterpret_cast<const f32x4*>(sum);
 #pragma unroll
         for (int k = 0; k < SL; k++) {
           const int at = (i * 16 + r) * PH + k * 32 + q * 8;
@@ -322,7 +358,8 @@ __global__ __launch_bounds__(KI <= 2 ? 512 : 256, KI <= 2 ? 2 : 1) void narrow_b
           acc = Mma<T>::run(down_column<T>(wu + k * 32 * PI + j * 16, PI), *reinterpret_cast<const Frag*>(du + at), acc);
         }
         const int64_t n = row + i * 16 + r;
-        if (n < p.rows) store4(p.dx + n * p.in, j * 16 + q * 4, p.in, p.in % 4 == 0, acc);
+        if (p.last < p.hidden) *reinterpret_cast<f32x4*>(sum) = acc;
+        else if (n < p.rows) store4(p.dx + n * p.in, j * 16 + q * 4, p.in, p.in % 4 == 0, acc);
       }
     }
     __syncthreads();   // the next x and dy are whole; dg and du are no longer read
@@ -373,7 +410,7 @@ __global__ __launch_bounds__(KI <= 2 ? 512 : 256, KI <= 2 ? 2 : 1) void narrow_b
 // slices of the sums, joined in LDS in a fixed order.
 template <typename T>
 __global__ __launch_bounds__(1024) void narrow_join_kernel(const float* part, int n, int H, int D, int in, int hidden, int out,
-                                                           T* dwg, T* dwu, T* dwd) {
+                                                           int first, int last, T* dwg, T* dwu, T* dwd) {
   __shared__ float lds[32][33];
   const int size = 3 * H * D, col = blockIdx.x * 32 + (threadIdx.x & 31), slice = threadIdx.x >> 5;
   float s = 0.0f;
@@ -387,35 +424,43 @@ __global__ __launch_bounds__(1024) void narrow_join_kernel(const float* part, in
   const int which = col / (H * D), e = col % (H * D);
   if (which < 2) {
     T* to = which ? dwu : dwg;
-    const int h = e / D, i = e % D;
-    if (to && h < hidden && i < in) to[(int64_t)h * in + i] = from_f32<T>(v);
+    const int h = first + e / D, i = e % D;
+    if (to && h < last && i < in) to[(int64_t)h * in + i] = from_f32<T>(v);
   } else {
-    const int o = e / H, h = e % H;
-    if (dwd && o < out && h < hidden) dwd[(int64_t)o * hidden + h] = from_f32<T>(v);
+    const int o = e / H, h = first + e % H;
+    if (dwd && o < out && h < last) dwd[(int64_t)o * hidden + h] = from_f32<T>(v);
   }
 }
 
 template <typename T, int KI, int SL>
 hipError_t narrow_backward(const GatedParams& g, const GatedLayout& l, hipStream_t s) {
   constexpr NarrowBackLds m = narrow_back_lds(KI, SL);
-  NarrowBack<T> p{static_cast<const T*>(g.x), static_cast<const T*>(g.w_gate), static_cast<const T*>(g.w_up),
-                  static_cast<const T*>(g.w_down), static_cast<const T*>(g.dy), static_cast<T*>(g.dx),
-                  reinterpret_cast<float*>(static_cast<uint8_t*>(g.ws) + l.part), g.rows, g.in, g.hidden, g.out, g.activation};
-  narrow_backward_kernel<T, KI, SL><<<l.narrow_groups, KI <= 2 ? 512 : 256, m.total * sizeof(T), s>>>(p);
-  if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
-  constexpr int H = SL * 32, D = KI * 32;
-  if (g.dw_gate || g.dw_up || g.dw_down)
-    narrow_join_kernel<T><<<3 * H * D / 32, 1024, 0, s>>>(p.part, l.narrow_groups, H, D, g.in, g.hidden, g.out, static_cast<T*>(g.dw_gate),
-                                                          static_cast<T*>(g.dw_up), static_cast<T*>(g.dw_down));
-  return hipGetLastError();
+  uint8_t* const ws = static_cast<uint8_t*>(g.ws);
+  const int per = (g.hidden + l.narrow_parts - 1) / l.narrow_parts;
+  for (int first = 0; first < g.hidden; first += per) {
+    const int last = first + per < g.hidden ? first + per : g.hidden;
+    const NarrowBack<T> p{static_cast<const T*>(g.x), static_cast<const T*>(g.w_gate), static_cast<const T*>(g.w_up),
+                          static_cast<const T*>(g.w_down), static_cast<const T*>(g.dy), static_cast<T*>(g.dx),
+                          reinterpret_cast<float*>(ws + l.dx_sum), reinterpret_cast<float*>(ws + l.part), g.rows, g.in, g.hidden, g.out,
+                          g.activation, first, last};
+    narrow_backward_kernel<T, KI, SL><<<l.narrow_groups, KI <= 2 ? 512 : 256, m.total * sizeof(T), s>>>(p);
+    if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
+    constexpr int H = SL * 32, D = KI * 32;
+    if (g.dw_gate || g.dw_up || g.dw_down)
+      narrow_join_kernel<T><<<3 * H * D / 32, 1024, 0, s>>>(p.part, l.narrow_groups, H, D, g.in, g.hidden, g.out, first, last,
+                                                            static_cast<T*>(g.dw_gate), static_cast<T*>(g.dw_up), static_cast<T*>(g.dw_down));
+    if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
+  }
+  return hipSuccess;
 }
 
 template <typename T, int KI>
 hipError_t narrow_backward_slices(const GatedParams& g, const GatedLayout& l, hipStream_t s) {
-  const int slices = narrow_slices(g.hidden);
-  if (slices == 1) return narrow_backward<T, KI, 1>(g, l, s);
+  const int slices = l.narrow_slices;
+  if constexpr (KI != 2)
+    if (slices == 1) return narrow_backward<T, KI, 1>(g, l, s);
   if (slices == 2) return narrow_backward<T, KI, 2>(g, l, s);
-  if constexpr (KI == 1)
+  if constexpr (KI <= 2)
     if (slices == 8) return narrow_backward<T, KI, 8>(g, l, s);
   return narrow_backward<T, KI, 4>(g, l, s);
 }

@@ -202,6 +202,30 @@ def test_ffn_values_and_gradients(B, size, dtype):
     ffn_check(B, *ffn_case(*size, dtype), kind)
 
 
+# Rows of at most 128 features: every padded width, every number of waves that share the hidden features, hidden
+# features past one launch of the backward and past the forward's LDS, unlike widths, the last rows of a workgroup.
+NARROW_SIZES = [(64, 16, 20, 16), (65, 33, 30, 40), (100, 64, 60, 33), (777, 96, 32, 96), (129, 128, 64, 100), (2100, 32, 256, 8),
+                (300, 64, 256, 64), (90, 40, 300, 64), (333, 128, 256, 128), (200, 96, 400, 72), (150, 5, 700, 128), (4099, 24, 96, 24)]
+
+
+@pytest.mark.parametrize("dtype", TYPES[1:])
+@pytest.mark.parametrize("size", NARROW_SIZES, ids=lambda s: "x".join(map(str, s)))
+def test_ffn_narrow_rows(B, size, dtype):
+    kind = ("silu", "gelu", "relu")[(NARROW_SIZES.index(size) + TYPES.index(dtype)) % 3]
+    ffn_check(B, *ffn_case(*size, dtype), kind)
+
+
+FEW_ROWS = [1, 2, 4, 5, 8, 9, 16, 17, 31, 32, 33]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows", FEW_ROWS)
+def test_ffn_few_rows(B, rows, dtype):
+    """Each way of dealing k to lanes and waves, with odd and even lengths of it."""
+    i, h, o = (264, 520, 200) if rows % 2 else (301, 2060, 77)
+    ffn_check(B, *ffn_case(rows, i, h, o, dtype), "silu")
+
+
 @pytest.mark.parametrize("kind", ["silu", "gelu", "relu"])
 @pytest.mark.parametrize("dtype", TYPES)
 def test_ffn_activations_over_their_range(B, dtype, kind):
