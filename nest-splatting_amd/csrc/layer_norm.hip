@@ -11,7 +11,7 @@
 // mean (a second pass over registers), never as a difference of squares.  All
 // sums are float32; y, dx, dw and db are rounded once.
 //
-// A row of up to 128 vectors of 16 bytes belongs to a group of 1 to 64 lanes
+// A row of up to 192 vectors of 16 bytes belongs to a group of 1 to 64 lanes
 // (several rows a wave for narrow rows), a longer one to a workgroup; past
 // the registers of a workgroup the row is read again for each pass.  A group
 // strides over its rows with the weights in registers and the next row on its
@@ -25,8 +25,10 @@ namespace nest {
 namespace {
 
 constexpr int kLnThreads = 256;      // of rows that stay with a wave, and of the long kernels
-constexpr int kLnMost = 512;         // of rows a workgroup shares
+constexpr int kLnMost = 1024;        // of rows a workgroup shares (512 for 16-bit rows: their lanes hold twice the values)
 constexpr int kLnWaves = kLnMost / 64;
+template <typename T>
+constexpr int most_threads() { return sizeof(T) == 4 ? kLnMost : kLnMost / 2; }
 constexpr int64_t kLnForwardGrid = 2048;   // workgroups
 
 // Sums over the lanes of one row; every lane gets the result.
@@ -46,7 +48,7 @@ __device__ __forceinline__ float row_sum(float v, int lanes, float* lds) {
 }
 
 template <typename T, typename P, int NV, bool kBlock>
-__global__ __launch_bounds__(kBlock ? kLnMost : kLnThreads) void layer_norm_kernel(LayerNormParams p, int lanes) {
+__global__ __launch_bounds__(kBlock ? most_threads<T>() : kLnThreads) void layer_norm_kernel(LayerNormParams p, int lanes) {
   constexpr int N = Vec16<T>::kN;
   __shared__ float lds[2][kLnWaves];
   const int rows_wg = kBlock ? 1 : kLnThreads / lanes;
@@ -184,7 +186,7 @@ __device__ __forceinline__ void row_sum2(float& a, float& b, int lanes, float (*
 // row of partial sums: part[workgroup][dw, db][D].  The sums' order depends on
 // the launch shape alone, so results repeat bit for bit.
 template <typename T, typename P, int NV, bool kBlock>
-__global__ __launch_bounds__(kBlock ? kLnMost : kLnThreads) void layer_norm_backward_kernel(LayerNormParams p, int lanes) {
+__global__ __launch_bounds__(kBlock ? most_threads<T>() : kLnThreads) void layer_norm_backward_kernel(LayerNormParams p, int lanes) {
   constexpr int N = Vec16<T>::kN;
   __shared__ float lds[2][2][kLnWaves];
   __shared__ float gather[kBlock ? 1 : kLnThreads][N + 1];
@@ -371,18 +373,18 @@ int vectors(int cols, int dtype) {
   return (cols + n - 1) / n;
 }
 
-// A row's lanes, and vectors a lane: up to 128 vectors stay with one wave (no
-// barrier), up to 1024 with a workgroup of as many waves as they need; nv 0:
-// past the registers.
+// A row's lanes, and vectors a lane: up to 192 vectors stay with one wave (no
+// barrier), up to 1024 (2048 of float32) with a workgroup of as many waves as
+// they need; nv 0: past the registers.
 struct LnShape {
   int lanes, nv;
   bool block;
 };
 LnShape shape_of(int cols, int dtype) {
-  const int vecs = vectors(cols, dtype);
-  if (vecs <= 128) return {vecs <= 64 ? pow2_at_least(vecs) : 64, vecs <= 64 ? 1 : 2, false};
-  if (vecs <= 2 * kLnMost) {
-    const int nv = vecs <= kLnMost ? 1 : 2;
+  const int vecs = vectors(cols, dtype), most = dtype == NEST_DTYPE_F32 ? kLnMost : kLnMost / 2;
+  if (vecs <= 192) return {vecs <= 64 ? pow2_at_least(vecs) : 64, (vecs + 63) / 64, false};
+  if (vecs <= 2 * most) {
+    const int nv = vecs <= 512 ? 1 : 2;
     return {(vecs + 64 * nv - 1) / (64 * nv) * 64, nv, true};
   }
   return {kLnThreads, 0, true};
@@ -394,7 +396,8 @@ void with_shape(const LnShape& h, F f) {
   using std::integral_constant;
   if (!h.block) {
     if (h.nv == 1) f(integral_constant<int, 1>(), integral_constant<bool, false>());
-    else f(integral_constant<int, 2>(), integral_constant<bool, false>());
+    else if (h.nv == 2) f(integral_constant<int, 2>(), integral_constant<bool, false>());
+    else f(integral_constant<int, 3>(), integral_constant<bool, false>());
   } else if (h.nv == 1) f(integral_constant<int, 1>(), integral_constant<bool, true>());
   else if (h.nv == 2) f(integral_constant<int, 2>(), integral_constant<bool, true>());
   else f(integral_constant<int, 0>(), integral_constant<bool, true>());
@@ -435,11 +438,14 @@ hipError_t backward(const LayerNormParams& p, hipStream_t s) {
 
 }  // namespace
 
-// Workgroups of the backward: as many as the registers let run at once, five a
-// CU where a lane has one vector of a narrow row, else three.
+// Workgroups of the backward: as many as the registers let run at once (waves
+// a CU), so that none waits for a turn of its own.
 int layer_norm_partials(int64_t rows, int cols, int dtype) {
   const LnShape h = shape_of(cols, dtype);
-  const int64_t need = row_groups(rows, h), most = h.nv == 1 && !h.block ? 1280 : 768;
+  const bool wide = dtype == NEST_DTYPE_F32;
+  const int waves = h.block ? h.lanes / 64 : kLnThreads / 64;
+  const int a_cu = h.block ? (h.nv == 1 || wide ? 16 : 8) : h.nv == 1 ? 20 : h.nv == 2 || wide ? 12 : 8;
+  const int64_t need = row_groups(rows, h), most = 256 * a_cu / waves;
   return (int)(need < most ? need : most);
 }
 
