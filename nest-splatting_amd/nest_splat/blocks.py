@@ -272,3 +272,98 @@ class _GatedFfn(torch.autograd.Function):
 def gated_ffn(x, w_gate, w_up, w_down, activation: str = "silu") -> torch.Tensor:
     """gated_ffn_forward's y under autograd (x and the three weights)."""
     return _GatedFfn.apply(x, w_gate, w_up, w_down, activation)
+
+
+# ---- modules ----
+
+class LayerNorm(nn.Module):
+    """layer_norm over the last dimension with float32 weight and bias, for rows of any of the types."""
+
+    def __init__(self, features: int, eps: float = 1e-5, bias: bool = True):
+        super().__init__()
+        self.eps = float(eps)
+        self.weight = nn.Parameter(torch.ones(features))
+        self.bias = nn.Parameter(torch.zeros(features)) if bias else None
+
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        return layer_norm(x, self.weight, self.bias, self.eps)
+
+
+class Dropout(nn.Module):
+    """dropout while training, with a new offset each call; the place in the sequence is part of the state dict, so a
+    resumed run draws the masks that follow. In evaluation x passes through (plus the residual)."""
+
+    def __init__(self, p: float = 0.1, seed: int = 0):
+        super().__init__()
+        if not 0.0 <= p <= 1.0:
+            raise ValueError(f"p must be in [0, 1], got {p}")
+        self.p, self.seed, self.offset = float(p), int(seed), 0
+
+    def get_extra_state(self):
+        return {"seed": self.seed, "offset": self.offset}
+
+    def set_extra_state(self, state):
+        self.seed, self.offset = state["seed"], state["offset"]
+
+    def forward(self, x: torch.Tensor, residual: Optional[torch.Tensor] = None) -> torch.Tensor:
+        if not self.training or self.p == 0.0:
+            return x if residual is None else residual + x
+        offset, self.offset = self.offset, self.offset + 1
+        return dropout(x, self.p, self.seed, offset, residual)
+
+
+class GatedFFN(nn.Module):
+    """gated_ffn with float32 weights, computed in ``dtype`` (x and the weights are cast to it, y has it)."""
+
+    def __init__(self, features: int, hidden: int, out_features: Optional[int] = None, activation: str = "silu", dtype="bf16",
+                 seed: int = 0):
+        super().__init__()
+        if activation not in _ACT:
+            raise ValueError(f"activation must be one of {sorted(_ACT)}, got {activation!r}")
+        self.activation = activation
+        self.dtype = _NAMED.get(dtype, dtype)
+        if self.dtype not in _CODE:
+            raise TypeError(f"dtype {dtype!r}: float32, float16 and bfloat16 are supported")
+        g = torch.Generator().manual_seed(seed)
+
+        def xavier(o, i):
+            return nn.Parameter((torch.rand((o, i), generator=g) * 2 - 1) * math.sqrt(6.0 / (i + o)))
+        self.w_gate, self.w_up = xavier(hidden, features), xavier(hidden, features)
+        self.w_down = xavier(features if out_features is None else out_features, hidden)
+
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        t = self.dtype
+        return gated_ffn(x.to(t), self.w_gate.to(t), self.w_up.to(t), self.w_down.to(t), self.activation)
+
+
+class GatedRefiner(nn.Module):
+    """``depth`` residual blocks x + dropout(ffn(norm(x))) over the feature channels of every pixel.
+
+    The rows run through the blocks in ``dtype``. The down projections start at zero, so a new refiner returns its input
+    rounded to dtype; with the colour MLP's own 16-bit type that leaves the decoded image as it was, since the MLP
+    rounds its features to that type."""
+
+    def __init__(self, features: int, hidden: Optional[int] = None, depth: int = 1, p: float = 0.1, activation: str = "silu",
+                 dtype="bf16", seed: int = 0):
+        super().__init__()
+        self.features = int(features)
+        self.dtype = _NAMED.get(dtype, dtype)
+        self.norms = nn.ModuleList(LayerNorm(features) for _ in range(depth))
+        self.ffns = nn.ModuleList(GatedFFN(features, hidden or 2 * features, None, activation, dtype, seed + k) for k in range(depth))
+        self.drops = nn.ModuleList(Dropout(p, seed + (k << 32)) for k in range(depth))
+        for f in self.ffns:
+            nn.init.zeros_(f.w_down)
+
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        """x [..., features] of any of the types -> the same shape and type."""
+        if x.shape[-1] != self.features:
+            raise ValueError(f"expected {self.features} feature channels, got {x.shape[-1]}")
+        y = x.to(self.dtype)
+        for norm, ffn, drop in zip(self.norms, self.ffns, self.drops):
+            y = drop(ffn(norm(y)), residual=y)
+        return y.to(x.dtype)
+
+    def refine_image(self, color: torch.Tensor) -> torch.Tensor:
+        """A feature map [C, H, W] refined pixel by pixel."""
+        C, H, W = color.shape
+        return self(color.reshape(C, -1).t()).t().reshape(C, H, W).contiguous()

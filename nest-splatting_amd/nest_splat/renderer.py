@@ -116,11 +116,14 @@ class SplatModel:
 class HashINGP:
     """The INGP attributes the baseline render reads (hash_encoder/modules.py):
     hash_encoding (a GridEncoder), gridrange, contract, active_levels, levels,
-    level_dim and rgb_decode."""
+    level_dim and rgb_decode.  refiner: an optional blocks.GatedRefiner that
+    render() passes the composited features through before the MLP."""
 
-    def __init__(self, encoding, mlp: NestMLP, gridrange, contract: bool = False, active_levels: Optional[int] = None):
+    def __init__(self, encoding, mlp: NestMLP, gridrange, contract: bool = False, active_levels: Optional[int] = None,
+                 refiner=None):
         self.hash_encoding = encoding
         self.mlp_rgb = mlp
+        self.refiner = refiner
         self.gridrange = torch.as_tensor(np.asarray(gridrange, dtype=np.float32))
         self._gridrange_host = np.asarray(gridrange, dtype=np.float32)
         self.contract = contract
@@ -300,7 +303,9 @@ def render(viewpoint_camera, pc, pipe, bg_color: torch.Tensor, scaling_modifier=
             rgb = rgb + (1.0 - render_alpha) * bg_color.to(dev).unsqueeze(-1).unsqueeze(-1)
     else:
         bg = bg_color if float(bg_color.sum()) > 0 else None
-        rgb = ingp.mlp_rgb.decode_image(rendered_image, view_ray_matrix(viewpoint_camera), alpha=render_alpha, bg=bg)
+        refiner = getattr(ingp, "refiner", None)
+        decoded = rendered_image if refiner is None else refiner.refine_image(rendered_image.detach())
+        rgb = ingp.mlp_rgb.decode_image(decoded, view_ray_matrix(viewpoint_camera), alpha=render_alpha, bg=bg)
     rets["render"] = rgb
 
     if with_surface:

@@ -377,3 +377,63 @@ def test_refusals(B):
     g, = torch.autograd.grad(B.layer_norm(a, w, b).float().sum(), a, create_graph=True)
     with pytest.raises(RuntimeError):
         g.sum().backward()
+
+
+# ---- modules and the path that runs them together ----
+
+def test_modules_against_the_definitions(B):
+    torch.manual_seed(0)
+    norm = B.LayerNorm(48).to(DEV)
+    with torch.no_grad():
+        norm.weight.normal_(1, 0.2)
+        norm.bias.normal_(0, 0.2)
+    x = rand(5, 7, 48, dtype=torch.float16, seed=1)
+    ref = R.norm(x.view(-1, 48), norm.weight.detach(), norm.bias.detach(), 1e-5)
+    R.check(norm(x).detach().view(-1, 48), *ref["y"], "LayerNorm")
+    ffn = B.GatedFFN(48, 96, 40, "gelu", "f16").to(DEV)
+    ws = [w.detach().half() for w in (ffn.w_gate, ffn.w_up, ffn.w_down)]
+    y = ffn(x.float())
+    assert y.shape == (5, 7, 40) and y.dtype == torch.float16
+    R.check(y.detach().view(-1, 40), *R.ffn(x.view(-1, 48), *ws, "gelu")["y"], "GatedFFN")
+    y.sum().backward()
+    assert all(w.grad is not None and w.grad.dtype == torch.float32 and w.grad.any() for w in ffn.parameters())
+    drop = B.Dropout(0.25, seed=5).to(DEV)
+    flat = rand(1000, dtype=torch.float32, seed=2)
+    first, second = drop(flat), drop(flat)
+    assert torch.equal(first, B.dropout_forward(flat, 0.25, 5, 0)) and torch.equal(second, B.dropout_forward(flat, 0.25, 5, 1))
+    other = B.Dropout(0.25)
+    other.load_state_dict(drop.state_dict())
+    assert torch.equal(other(flat), B.dropout_forward(flat, 0.25, 5, 2))
+    assert drop.eval()(flat) is flat
+    with pytest.raises(ValueError):
+        B.GatedFFN(8, 8, activation="tanh")
+    with pytest.raises(ValueError):
+        B.GatedRefiner(16).to(DEV)(rand(4, 15, dtype=torch.float32, seed=1))
+
+
+def test_a_new_refiner_leaves_the_frame_as_it_was():
+    """Its blocks add zero, and the MLP rounds its features to the refiner's type in any case."""
+    from nest_splat import blocks, renderer
+    from nest_splat.mlp import NestMLP
+    from nest_splat.scene import get_spec, make_scene
+    sc = make_scene(get_spec("cfg1"))
+    pc, ingp = renderer.scene_to_device(sc, DEV)
+    bg = torch.zeros(3, device=DEV)
+    ingp.mlp_rgb = NestMLP(sc.spec.C, 64, "f16").to(DEV)
+    want = renderer.render(sc.cameras[0], pc, renderer.Pipe(), bg, ingp=ingp, with_surface=False)
+    ingp.refiner = blocks.GatedRefiner(sc.spec.C, depth=2, dtype="f16").to(DEV).eval()
+    got = renderer.render(sc.cameras[0], pc, renderer.Pipe(), bg, ingp=ingp, with_surface=False)
+    assert torch.equal(got["features"], want["features"]) and torch.equal(got["render"], want["render"])
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_training_a_refiner(dtype):
+    import importlib.util
+    import os
+    path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "examples", "train_refiner.py")
+    spec = importlib.util.spec_from_file_location("train_refiner", path)
+    m = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(m)
+    refiner, before, after = m.train(steps=60, dtype=dtype, device=str(DEV), log=lambda s: None)
+    assert after < 0.9 * before
+    assert all(torch.isfinite(p).all() for p in refiner.parameters())
