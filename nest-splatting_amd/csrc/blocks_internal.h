@@ -85,6 +85,9 @@ __host__ __device__ inline NarrowLds narrow_lds(int ki, int hidden, int waves) {
   return l;
 }
 
+// Waves of a workgroup of the narrow backward, as its registers allow.
+__host__ __device__ constexpr int narrow_back_waves(int ki) { return ki <= 2 ? 8 : 4; }
+
 // LDS of the narrow backward, in elements: weights, then for each group of
 // waves x, dy [32][pitch_in] and dg, du [32][pitch_h]; at its end the groups'
 // sums.  slices: of 32 hidden features, one a wave.
@@ -94,7 +97,7 @@ struct NarrowBackLds {
 __host__ __device__ constexpr NarrowBackLds narrow_back_lds(int ki, int slices) {
   NarrowBackLds l{};
   const int h = slices * 32;
-  l.groups = (ki <= 2 ? 8 : 4) / slices;
+  l.groups = narrow_back_waves(ki) / slices;
   l.pitch_in = ki * 32 + kNarrowPad;
   l.pitch_h = h + kNarrowPad;
   l.tiles = 2 * h * l.pitch_in + ki * 32 * l.pitch_h;

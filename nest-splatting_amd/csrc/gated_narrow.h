@@ -38,7 +38,7 @@ __device__ __forceinline__ typename Mma<T>::Frag load8(const T* p, int n) {
 }
 
 template <typename T, int kAct, int KI, int RG>
-__global__ __launch_bounds__(512, 2) void narrow_forward_kernel(Narrow<T> p, int chunk) {
+__global__ __launch_bounds__(512, KI <= 2 ? 4 : 2) void narrow_forward_kernel(Narrow<T> p, int chunk) {
   typedef typename Mma<T>::Frag Frag;
   constexpr int FO = 2 * KI;
   extern __shared__ __attribute__((aligned(16))) uint8_t narrow_mem[];
@@ -144,8 +144,9 @@ __global__ __launch_bounds__(512, 2) void narrow_forward_kernel(Narrow<T> p, int
 
 template <typename T, int KI>
 hipError_t narrow_forward(const Narrow<T>& p, hipStream_t s) {
-  // 64 rows a wave where registers allow: each weight fragment read from LDS is used RG times
-  constexpr int RG = KI <= 2 ? 4 : 2;
+  // 32 rows a wave: up to 64 features that leaves registers for four waves a SIMD, one's activation beside
+  // another's products.  64 rows a wave and two waves: 145 us instead of 124 on 1,702,400 x 64, hidden 128 bf16.
+  constexpr int RG = 2;
   const bool small = p.rows < (int64_t)256 * 8 * 16 * RG;   // fewer rows than a full chip's waves take: smaller workgroups
   const int waves = small ? 4 : 8, h32 = (p.hidden + 31) / 32 * 32;
   // hidden features in LDS at a time: all, or equal parts that fit
@@ -215,9 +216,9 @@ __device__ __forceinline__ typename Mma<T>::Frag down_column(const T* at, int pi
 }
 
 template <typename T, int KI, int SL>
-__global__ __launch_bounds__(KI <= 2 ? 512 : 256, KI <= 2 ? 2 : 1) void narrow_backward_kernel(NarrowBack<T> p) {
+__global__ __launch_bounds__(64 * narrow_back_waves(KI), KI <= 2 ? 2 : 1) void narrow_backward_kernel(NarrowBack<T> p) {
   typedef typename Mma<T>::Frag Frag;
-  constexpr int kWaves = KI <= 2 ? 8 : 4, kGroups = kWaves / SL, kThreads = 64 * kWaves;
+  constexpr int kWaves = narrow_back_waves(KI), kGroups = kWaves / SL, kThreads = 64 * kWaves;
   constexpr NarrowBackLds l = narrow_back_lds(KI, SL);
   constexpr int H = SL * 32, PI = l.pitch_in, PH = l.pitch_h, FI = 2 * KI;
   static_assert(l.groups == kGroups, "");
@@ -317,29 +318,37 @@ __global__ __launch_bounds__(KI <= 2 ? 512 : 256, KI <= 2 ? 2 : 1) void narrow_b
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
       __builtin_amdgcn_wave_barrier();
     };
+    put(dg, vh);
+    put(du, vu);
+    settle();
     {
-      Frag fg[2], fu[2], fh[2];
-      put(dg, vh);
-      put(du, vu);
-      settle();
+      Frag fh[2];
 #pragma unroll
-      for (int b = 0; b < 2; b++) {
-        fh[b] = down_column<T>(dg + slice * 32 + b * 16, PH);
-        fu[b] = down_column<T>(du + slice * 32 + b * 16, PH);
-      }
-      settle();
-      put(dg, vg);
-      settle();
-#pragma unroll
-      for (int b = 0; b < 2; b++) fg[b] = down_column<T>(dg + slice * 32 + b * 16, PH);
+      for (int b = 0; b < 2; b++) fh[b] = down_column<T>(dg + slice * 32 + b * 16, PH);
 #pragma unroll
       for (int j = 0; j < FI; j++) {
-        const Frag fx = down_column<T>(xs + j * 16, PI), fy = down_column<T>(dys + j * 16, PI);
+        const Frag fy = down_column<T>(dys + j * 16, PI);
+#pragma unroll
+        for (int b = 0; b < 2; b++) dwd[j][b] = Mma<T>::run(fy, fh[b], dwd[j][b]);
+      }
+    }
+    settle();
+    put(dg, vg);
+    settle();
+    {
+      Frag fg[2], fu[2];
+#pragma unroll
+      for (int b = 0; b < 2; b++) {
+        fg[b] = down_column<T>(dg + slice * 32 + b * 16, PH);
+        fu[b] = down_column<T>(du + slice * 32 + b * 16, PH);
+      }
+#pragma unroll
+      for (int j = 0; j < FI; j++) {
+        const Frag fx = down_column<T>(xs + j * 16, PI);
 #pragma unroll
         for (int b = 0; b < 2; b++) {
           dwg[b][j] = Mma<T>::run(fg[b], fx, dwg[b][j]);
           dwu[b][j] = Mma<T>::run(fu[b], fx, dwu[b][j]);
-          dwd[j][b] = Mma<T>::run(fy, fh[b], dwd[j][b]);
         }
       }
     }
@@ -443,7 +452,7 @@ hipError_t narrow_backward(const GatedParams& g, const GatedLayout& l, hipStream
                           static_cast<const T*>(g.w_down), static_cast<const T*>(g.dy), static_cast<T*>(g.dx),
                           reinterpret_cast<float*>(ws + l.dx_sum), reinterpret_cast<float*>(ws + l.part), g.rows, g.in, g.hidden, g.out,
                           g.activation, first, last};
-    narrow_backward_kernel<T, KI, SL><<<l.narrow_groups, KI <= 2 ? 512 : 256, m.total * sizeof(T), s>>>(p);
+    narrow_backward_kernel<T, KI, SL><<<l.narrow_groups, 64 * narrow_back_waves(KI), m.total * sizeof(T), s>>>(p);
     if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
     constexpr int H = SL * 32, D = KI * 32;
     if (g.dw_gate || g.dw_up || g.dw_down)

@@ -102,6 +102,41 @@ __device__ __forceinline__ void store4(T* row, int n, int N, bool aligned, f32x4
   }
 }
 
+// 16 x 16-column fragments of a wave to row-major rows, through LDS of its own
+// so that a row's columns leave in 16-byte stores side by side.
+template <typename T, int FN>
+struct RowStage {
+  static constexpr int kPitch = FN * 16 + 16 / (int)sizeof(T);   // elements
+  T v[16 * kPitch];
+};
+
+// Rows row .. row + 15 and columns col .. col + 16 FN - 1 of out [rows][ld]; ld
+// is a multiple of 16 bytes and out aligned.  Element f(j)[e] is column
+// 16 j + 4 (lane / 16) + e of row lane % 16.
+template <typename T, int FN, typename F>
+__device__ __forceinline__ void store_rows(RowStage<T, FN>& stage, T* out, int64_t row, int64_t rows, int col, int64_t ld, F f) {
+  constexpr int kVec = 16 / (int)sizeof(T), kRow = FN * 16 / kVec;
+  const int lane = threadIdx.x & 63;
+#pragma unroll
+  for (int j = 0; j < FN; j++) {
+    const f32x4 v = f(j);
+    Four<T> t;
+#pragma unroll
+    for (int e = 0; e < 4; e++) t.v[e] = from_f32<T>(v[e]);
+    *reinterpret_cast<Four<T>*>(&stage.v[(lane & 15) * RowStage<T, FN>::kPitch + j * 16 + (lane >> 4) * 4]) = t;
+  }
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+#pragma unroll
+  for (int k = lane; k < 16 * kRow; k += 64) {
+    const int r = k / kRow, c = (k % kRow) * kVec;
+    const uint4 v = *reinterpret_cast<const uint4*>(&stage.v[r * RowStage<T, FN>::kPitch + c]);
+    if (row + r < rows && col + c < ld) *reinterpret_cast<uint4*>(out + (row + r) * ld + col + c) = v;
+  }
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
+
 // ---- C = A B (+ A2 B2), up to three products in a launch, k split over `splits` ----
 
 template <typename T>
@@ -153,15 +188,25 @@ __global__ __launch_bounds__(C::NT) void product_kernel(Products<T> all) {
   lb.init(p.b + kb, p.ldb, n0, kBK ? p.N : p.ldb);
   tile_product<T, kAK, kBK, C>(la, lb, k, a2, b2, acc);   // a split past the end has k <= 0: it loads zeros
   const int lane = threadIdx.x & 63, w = wave_id();
-  const int64_t m = m0 + (w / C::WN) * C::FM * 16 + (lane & 15);
-  const int n = (int)n0 + (w % C::WN) * C::FN * 16 + (lane >> 4) * 4;
+  const int64_t m = m0 + (w / C::WN) * C::FM * 16;
+  const int n = (int)n0 + (w % C::WN) * C::FN * 16;
+  constexpr int kVec = 16 / (int)sizeof(T);
+  if (!all.part && p.N % kVec == 0) {   // whole 16-byte pieces of the rows of C
+    __syncthreads();   // the operands' LDS is free
+    auto& stage = reinterpret_cast<RowStage<T, C::FN>*>(tile_lds<C>())[w];
+#pragma unroll
+    for (int i = 0; i < C::FM; i++)
+      store_rows<T, C::FN>(stage, p.c, m + i * 16, p.M, n, p.N, [&](int j) { return acc[i][j]; });
+    return;
+  }
+  const int r = lane & 15, q = lane >> 4;
 #pragma unroll
   for (int i = 0; i < C::FM; i++) {
-    if (m + i * 16 >= p.M) continue;
+    if (m + i * 16 + r >= p.M) continue;
 #pragma unroll
     for (int j = 0; j < C::FN; j++) {
-      if (all.part) store4(all.part + split * all.part_size + p.part + (m + i * 16) * p.N, n + j * 16, p.N, p.N % 4 == 0, acc[i][j]);
-      else store4(p.c + (m + i * 16) * p.N, n + j * 16, p.N, p.N % 4 == 0, acc[i][j]);
+      if (all.part) store4(all.part + split * all.part_size + p.part + (m + i * 16 + r) * p.N, n + j * 16 + q * 4, p.N, p.N % 4 == 0, acc[i][j]);
+      else store4(p.c + (m + i * 16 + r) * p.N, n + j * 16 + q * 4, p.N, p.N % 4 == 0, acc[i][j]);
     }
   }
 }
@@ -188,41 +233,6 @@ __global__ __launch_bounds__(256) void join_kernel(Products<T> all) {
 // that took the backward's kernel 3.3 ms, of which 0.3 is the product.
 __device__ __forceinline__ float* kept_block(float* kept, int64_t row, int col, int64_t ldh) {
   return kept + ((row >> 4) * ((ldh + 15) >> 4) + (col >> 4)) * 512 + (threadIdx.x & 63) * 4;
-}
-
-// 16 x 16-column fragments of a wave to row-major rows, through LDS of its own
-// so that a row's columns leave in 16-byte stores side by side.
-template <typename T, int FN>
-struct RowStage {
-  static constexpr int kPitch = FN * 16 + 16 / (int)sizeof(T);   // elements
-  T v[16 * kPitch];
-};
-
-// Rows row .. row + 15 and columns col .. col + 16 FN - 1 of out [rows][ld]; ld
-// is a multiple of 16 bytes and out aligned.  Element f(j)[e] is column
-// 16 j + 4 (lane / 16) + e of row lane % 16.
-template <typename T, int FN, typename F>
-__device__ __forceinline__ void store_rows(RowStage<T, FN>& stage, T* out, int64_t row, int64_t rows, int col, int64_t ld, F f) {
-  constexpr int kVec = 16 / (int)sizeof(T), kRow = FN * 16 / kVec;
-  const int lane = threadIdx.x & 63;
-#pragma unroll
-  for (int j = 0; j < FN; j++) {
-    const f32x4 v = f(j);
-    Four<T> t;
-#pragma unroll
-    for (int e = 0; e < 4; e++) t.v[e] = from_f32<T>(v[e]);
-    *reinterpret_cast<Four<T>*>(&stage.v[(lane & 15) * RowStage<T, FN>::kPitch + j * 16 + (lane >> 4) * 4]) = t;
-  }
-  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-  __builtin_amdgcn_wave_barrier();
-#pragma unroll
-  for (int k = lane; k < 16 * kRow; k += 64) {
-    const int r = k / kRow, c = (k % kRow) * kVec;
-    const uint4 v = *reinterpret_cast<const uint4*>(&stage.v[r * RowStage<T, FN>::kPitch + c]);
-    if (row + r < rows && col + c < ld) *reinterpret_cast<uint4*>(out + (row + r) * ld + col + c) = v;
-  }
-  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-  __builtin_amdgcn_wave_barrier();
 }
 
 template <typename T>

@@ -60,19 +60,20 @@ def _aligned(t: torch.Tensor) -> torch.Tensor:
     return t.clone() if t.data_ptr() % 16 else t
 
 
-_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+# the current stream and device without the objects around them, where this torch has them
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
+_raw_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 
 
 def _call(name: str, device: torch.device, *args) -> None:
     """Calls a library function on the device's current stream, with the device current."""
-    lib = L.lib()
+    function = getattr(L.lib(), name)
     index = device.index
-    stream = _raw_stream(index) if _raw_stream is not None else torch.cuda.current_stream(device).cuda_stream
-    if index == torch.cuda.current_device():
-        rc = getattr(lib, name)(*args, stream)
+    if index == _raw_device():
+        rc = function(*args, _raw_stream(index))
     else:
         with torch.cuda.device(index):
-            rc = getattr(lib, name)(*args, stream)
+            rc = function(*args, _raw_stream(index))
     if rc != L.NEST_OK:
         L.check(rc, name)
 
