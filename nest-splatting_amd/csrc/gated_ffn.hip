@@ -12,17 +12,20 @@ int64_t few_rows(int es) { return es == 2 ? 32 : 16; }
 int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 // Seconds that `groups` workgroups of tiles of side x side and `steps` steps of
-// 128 bytes of k take: rounds of what the LDS lets run at once, a step of a
-// round bound by its products (the share of a CU's peak that each tile size
-// reaches alone) or by the latency of its loads.
+// 128 bytes of k take, in rounds of what the LDS lets run at once.  A step of a
+// round takes its products' time at the rate a full CU reaches, or what a lone
+// workgroup's step takes: its loads' latency, and for float32 the cutting into
+// parts beside the products.  Rates and times as measured.
 double seconds(int64_t groups, int64_t steps, int side, int es) {
-  const double peak = (es == 2 ? 1400e12 : 150e12) / 256, latency = 0.42e-6;
-  const double share = es == 2 ? (side == 256 ? 0.8 : side == 128 ? 0.62 : 0.42) : (side == 128 ? 0.9 : 0.85);
-  const int at_once = side == 256 ? 1 : side == 128 ? 2 : 5;
-  const double step = 2.0 * side * side * (128 / es) / (peak * share);
-  auto round = [&](int64_t a_cu) { return (double)steps * (step * a_cu > latency ? step * a_cu : latency); };
-  const int64_t full = groups / (256 * at_once), rest = groups % (256 * at_once);
-  return (double)full * round(at_once) + (rest ? round(cdiv(rest, 256)) : 0.0);
+  const int i = side == 256 ? 0 : side == 128 ? 1 : 2;
+  static constexpr double kRate[2][3] = {{4.4e12, 3.4e12, 2.3e12}, {1.05e12, 0.88e12, 0.53e12}};   // of a CU
+  static constexpr double kLone[2][3] = {{0.42e-6, 0.42e-6, 0.42e-6}, {4.0e-6, 1.69e-6, 0.73e-6}};
+  static constexpr int kAtOnce[3] = {1, 2, 5};
+  const int f32 = es == 4;
+  const double step = 2.0 * side * side * (128 / es) / kRate[f32][i];
+  auto round = [&](int64_t a_cu) { return (double)steps * (step * a_cu > kLone[f32][i] ? step * a_cu : kLone[f32][i]); };
+  const int64_t full = groups / (256 * kAtOnce[i]), rest = groups % (256 * kAtOnce[i]);
+  return (double)full * round(kAtOnce[i]) + (rest ? round(cdiv(rest, 256)) : 0.0);
 }
 
 __global__ __launch_bounds__(256) void clear_kernel(uint16_t* p, int64_t n) {
@@ -39,14 +42,14 @@ hipError_t launch_clear(void* p, size_t bytes, hipStream_t s) {
 }  // namespace
 
 // Tiles for up to three products that share a launch and K.  Against every
-// tile and split timed on eleven sizes of the down projection (64 to 8192
-// rows, 256 to 2048 columns, k of 512 to 8192, both kinds of types) the choice
-// is within 2% of the best on average, 18% at worst.
+// tile and split timed on eight sizes of the down projection of 16-bit types
+// and eight of float32 (64 to 300,000 rows, 64 to 2048 columns, k of 128 to
+// 8192) the choice is within 2% of the best on average, 18% at worst.
 TileChoice choose_tile(int n, const int64_t* M, const int64_t* N, int64_t K, int es, bool may_split) {
   TileChoice best{64, 1};
   double least = 1e30;
   const int64_t steps = cdiv(K, 128 / es);
-  for (int side = es == 2 ? 256 : 128; side >= 64; side /= 2) {
+  for (int side = 256; side >= 64; side /= 2) {
     int64_t tiles = 0, size = 0;
     for (int i = 0; i < n; i++) {
       tiles += cdiv(M[i], side) * cdiv(N[i], side);

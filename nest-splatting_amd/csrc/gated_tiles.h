@@ -387,7 +387,7 @@ hipError_t launch_products(Products<T>& all, TileChoice t, hipStream_t s) {
   if (t.splits == 1) all.part = nullptr;
   const unsigned grid = (unsigned)(tiles * t.splits);
   if (t.side == 256) {
-    if constexpr (sizeof(T) == 2) product_kernel<T, kAK, kBK, TileL><<<grid, TileL::NT, 0, s>>>(all);
+    product_kernel<T, kAK, kBK, TileL><<<grid, TileL::NT, 0, s>>>(all);
   } else if (t.side == 128) product_kernel<T, kAK, kBK, TileM><<<grid, TileM::NT, 0, s>>>(all);
   else product_kernel<T, kAK, kBK, TileS><<<grid, TileS::NT, 0, s>>>(all);
   if (t.splits > 1) {
@@ -404,7 +404,7 @@ hipError_t launch_gate(Gate<T> p, hipStream_t s) {
   p.tiles_n = (int)((p.ldh + t.side / 2 - 1) / (t.side / 2));
   const unsigned grid = (unsigned)((int64_t)p.tiles_m * p.tiles_n);
   if (t.side == 256) {
-    if constexpr (sizeof(T) == 2) gate_kernel<T, TileL><<<grid, TileL::NT, 0, s>>>(p);
+    gate_kernel<T, TileL><<<grid, TileL::NT, 0, s>>>(p);
   } else if (t.side == 128) gate_kernel<T, TileM><<<grid, TileM::NT, 0, s>>>(p);
   else gate_kernel<T, TileS><<<grid, TileS::NT, 0, s>>>(p);
   return hipGetLastError();
@@ -417,7 +417,7 @@ hipError_t launch_gate_backward(GateBackward<T> p, hipStream_t s) {
   p.tiles_n = (int)((p.ldh + t.side - 1) / t.side);
   const unsigned grid = (unsigned)((int64_t)p.tiles_m * p.tiles_n);
   if (t.side == 256) {
-    if constexpr (sizeof(T) == 2) gate_backward_kernel<T, TileL><<<grid, TileL::NT, 0, s>>>(p);
+    gate_backward_kernel<T, TileL><<<grid, TileL::NT, 0, s>>>(p);
   } else if (t.side == 128) gate_backward_kernel<T, TileM><<<grid, TileM::NT, 0, s>>>(p);
   else gate_backward_kernel<T, TileS><<<grid, TileS::NT, 0, s>>>(p);
   return hipGetLastError();

@@ -57,6 +57,45 @@ struct Mma<float> {
   }
 };
 
+// Eight float32 values of a lane as three bfloat16 parts of 8 bits each, their
+// sum exact: the leading 8 bits, the next 8, the rest (Henry, Tang, Heinecke,
+// "Leveraging the bfloat16 artificial intelligence datatype for higher-precision
+// computations", 2019).  Parts are cut off, not rounded, so none overflows.
+struct Parts {
+  bf16x8 p[3];
+};
+
+__device__ __forceinline__ Parts split(f32x4 lo, f32x4 hi) {
+  uint32_t w[3][4];
+#pragma unroll
+  for (int i = 0; i < 4; i++) {   // pairs of values: the upper halves of two words are a word of parts
+    float a = i < 2 ? lo[2 * i] : hi[2 * i - 4], b = i < 2 ? lo[2 * i + 1] : hi[2 * i - 3];
+#pragma unroll
+    for (int k = 0; k < 3; k++) {
+      const uint32_t ua = __builtin_bit_cast(uint32_t, a), ub = __builtin_bit_cast(uint32_t, b);
+      w[k][i] = __builtin_amdgcn_perm(ub, ua, 0x07060302);
+      if (k < 2) {
+        a -= __builtin_bit_cast(float, ua & 0xffff0000u);
+        b -= __builtin_bit_cast(float, ub & 0xffff0000u);
+      }
+    }
+  }
+  Parts r;
+#pragma unroll
+  for (int k = 0; k < 3; k++) r.p[k] = __builtin_bit_cast(bf16x8, w[k]);
+  return r;
+}
+
+// The product of all parts but those below 2^-23 of the whole, smallest first.
+__device__ __forceinline__ f32x4 run_parts(const Parts& a, const Parts& b, f32x4 c) {
+  c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.p[1], b.p[1], c, 0, 0, 0);
+  c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.p[0], b.p[2], c, 0, 0, 0);
+  c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.p[2], b.p[0], c, 0, 0, 0);
+  c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.p[0], b.p[1], c, 0, 0, 0);
+  c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.p[1], b.p[0], c, 0, 0, 0);
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.p[0], b.p[0], c, 0, 0, 0);
+}
+
 typedef __attribute__((address_space(3))) void LdsVoid;
 typedef __attribute__((address_space(3))) i16x4 LdsI16x4;
 
@@ -224,6 +263,32 @@ __device__ __forceinline__ void tile_product(Loader<T, kAK, C::BM, C::NT>& la, L
   };
   const int w = wave_id(), wm = (w / C::WN) * C::FM * 16, wn = (w % C::WN) * C::FN * 16;
   const int ba = fragment_base<T, kAK, C::BM>(wm), bb = fragment_base<T, kBK, C::BN>(wn);
+  int s = 0;
+  if constexpr (sizeof(T) == 4) {
+    // Both halves of a step's k make one 32-wide product of the parts.
+    auto multiply = [&](const uint8_t* a, const uint8_t* b) {
+      Parts pb[C::FN];
+#pragma unroll
+      for (int j = 0; j < C::FN; j++) pb[j] = split(fragment<T, kBK, C::BN>(b, bb, j, 0), fragment<T, kBK, C::BN>(b, bb, j, 1));
+#pragma unroll
+      for (int i = 0; i < C::FM; i++) {
+        const Parts pa = split(fragment<T, kAK, C::BM>(a, ba, i, 0), fragment<T, kAK, C::BM>(a, ba, i, 1));
+#pragma unroll
+        for (int j = 0; j < C::FN; j++) acc[i][j] = run_parts(pb[j], pa, acc[i][j]);
+      }
+    };
+    issue(a_lds0, b_lds0);
+    while (true) {
+      __syncthreads();   // this step has landed, the last one is all read
+      if (s + 1 < total) issue(a_lds1, b_lds1);
+      multiply(a_lds0, b_lds0);
+      if (++s == total) return;
+      __syncthreads();
+      if (s + 1 < total) issue(a_lds0, b_lds0);
+      multiply(a_lds1, b_lds1);
+      if (++s == total) return;
+    }
+  }
   // A step is four phases: half kb of k times half of the wave's rows.  Each
   // phase reads the next one's fragments before its own products, so LDS works
   // beside the matrix cores; the barrier stands before the last phase, whose
@@ -246,7 +311,6 @@ __device__ __forceinline__ void tile_product(Loader<T, kAK, C::BM, C::NT>& la, L
         acc[half * kHalf + i][j] = Mma<T>::run(fb[from_b][j], fa[from_a][i], acc[half * kHalf + i][j]);
     __builtin_amdgcn_sched_barrier(0);
   };
-  int s = 0;
   auto step = [&](uint8_t* a, uint8_t* b, uint8_t* a_next, uint8_t* b_next) {
     load_a(1, a, 0, 1);
     products(0, 0, 0);
