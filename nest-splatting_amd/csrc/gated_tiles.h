@@ -211,16 +211,18 @@ __global__ __launch_bounds__(C::NT) void product_kernel(Products<T> all) {
   }
 }
 
-// Joins the partial sums, in the order of the splits.
+// Joins the partial sums, in the order of the splits, four places a thread
+// (each product's part of a slice is a multiple of four).
 template <typename T>
 __global__ __launch_bounds__(256) void join_kernel(Products<T> all) {
-  for (int64_t e = ((int64_t)blockIdx.x * 256 + threadIdx.x); e < all.part_size; e += (int64_t)gridDim.x * 256) {
-    float s = 0.0f;
-    for (int i = 0; i < all.splits; i++) s += all.part[i * all.part_size + e];
+  for (int64_t e = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4; e < all.part_size; e += (int64_t)gridDim.x * 1024) {
+    f32x4 s = *reinterpret_cast<const f32x4*>(all.part + e);
+    for (int i = 1; i < all.splits; i++) s += *reinterpret_cast<const f32x4*>(all.part + i * all.part_size + e);
     int which = 0;
     while (which + 1 < all.n && e >= all.p[which + 1].part) which++;
     const Product<T>& p = all.p[which];
-    if (e - p.part < (int64_t)p.M * p.N) p.c[e - p.part] = from_f32<T>(s);
+    const int64_t at = e - p.part, left = (int64_t)p.M * p.N - at;
+    if (left > 0) store4(p.c + at, 0, left < 4 ? (int)left : 4, true, s);
   }
 }
 
@@ -350,10 +352,10 @@ __global__ __launch_bounds__(C::NT) void gate_backward_kernel(GateBackward<T> p)
 
 template <typename T>
 struct Pads {
-  const T* from[4];
-  T* to[4];
-  int64_t rows[4];
-  int n[4], ld[4];   // row lengths
+  const T* from[5];
+  T* to[5];
+  int64_t rows[5];
+  int n[5], ld[5];   // row lengths
 };
 
 template <typename T>
@@ -391,7 +393,7 @@ hipError_t launch_products(Products<T>& all, TileChoice t, hipStream_t s) {
   } else if (t.side == 128) product_kernel<T, kAK, kBK, TileM><<<grid, TileM::NT, 0, s>>>(all);
   else product_kernel<T, kAK, kBK, TileS><<<grid, TileS::NT, 0, s>>>(all);
   if (t.splits > 1) {
-    const int64_t need = (part + 255) / 256;
+    const int64_t need = (part + 1023) / 1024;
     join_kernel<T><<<(unsigned)(need < 65536 ? need : 65536), 256, 0, s>>>(all);
   }
   return hipGetLastError();
@@ -452,17 +454,11 @@ hipError_t pad_operands(const GatedParams& p, const GatedLayout& l, uint8_t* ws,
     add(o.wu, l.wu, p.hidden, p.in, l.ldx);
   }
   if (l.ldh != p.hidden) add(o.wd, l.wd, p.out, p.hidden, l.ldh);
-  auto go = [&]() {
+  if (back && l.ldy != p.out) add(o.dy, l.dy, p.rows, p.out, l.ldy);
+  if (n) {
     const int64_t need = (most / Vec16<T>::kN + 255) / 256;
     pad_kernel<T><<<dim3((unsigned)(need < 4096 ? need : 4096), n), 256, 0, s>>>(q);
-  };
-  if (n == 4 && back && l.ldy != p.out) {   // five copies: the fifth by itself
-    go();
-    n = 0;
-    most = 0;
   }
-  if (back && l.ldy != p.out) add(o.dy, l.dy, p.rows, p.out, l.ldy);
-  if (n) go();
   return hipGetLastError();
 }
 
