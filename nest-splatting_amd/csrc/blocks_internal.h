@@ -67,7 +67,7 @@ struct TileChoice {
 };
 
 constexpr int kNarrowLdsBytes = 160 * 1024;
-constexpr int kNarrowPad = 8;   // elements: rows of 16 bytes more fall on different banks
+constexpr int kNarrowPad = 16;   // elements past a multiple of 64 bytes: 16-byte reads of 16 rows fall on different banks
 
 // LDS of the forward, in elements: gate and up rows (32 of each in turn), down
 // rows, a stage for each wave's stores.
@@ -89,19 +89,18 @@ __host__ __device__ inline NarrowLds narrow_lds(int ki, int hidden, int waves) {
 __host__ __device__ constexpr int narrow_back_waves(int ki) { return ki <= 2 ? 8 : 4; }
 
 // LDS of the narrow backward, in elements: weights, then for each group of
-// waves x, dy [32][pitch_in] and dg, du [32][pitch_h]; at its end the groups'
-// sums.  slices: of 32 hidden features, one a wave.
+// waves x, dy [32][row_in] and dg, du [32][row_h]; at its end the groups' sums.
+// slices: of 32 hidden features, one a wave.  Rows are a power of two long.
 struct NarrowBackLds {
-  int groups, pitch_in, pitch_h, tiles, tile_stride, total;
+  int groups, row_in, row_h, tiles, tile_stride, total;
 };
 __host__ __device__ constexpr NarrowBackLds narrow_back_lds(int ki, int slices) {
   NarrowBackLds l{};
-  const int h = slices * 32;
   l.groups = narrow_back_waves(ki) / slices;
-  l.pitch_in = ki * 32 + kNarrowPad;
-  l.pitch_h = h + kNarrowPad;
-  l.tiles = 2 * h * l.pitch_in + ki * 32 * l.pitch_h;
-  l.tile_stride = 2 * 32 * l.pitch_in + 2 * 32 * l.pitch_h;
+  l.row_in = ki == 3 ? 128 : ki * 32;
+  l.row_h = slices * 32;
+  l.tiles = 2 * l.row_h * l.row_in + ki * 32 * l.row_h;
+  l.tile_stride = 2 * 32 * l.row_in + 2 * 32 * l.row_h;
   l.total = l.tiles + l.groups * l.tile_stride;
   const int sums = l.groups > 1 ? slices * 12 * ki * 256 * 2 : 0;   // float32: two elements each
   if (sums > l.total) l.total = sums;

@@ -203,36 +203,73 @@ struct NarrowBack {
   int first, last;  // hidden features of this launch
 };
 
-// Eight values of a lane's row (or column) that lie down a column of a
-// row-major array: rows k .. k + 7 for the lanes of quarter q at k = 8 q, column
-// `col` + lane % 16.
-template <typename T>
-__device__ __forceinline__ typename Mma<T>::Frag down_column(const T* at, int pitch) {
-  const int lane = threadIdx.x & 63, r = lane & 15, q = lane >> 4;
-  const T* p = at + (q * 8 + (r >> 2)) * pitch + (r & 3) * 4;
-  i16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsI16x4*)p);
-  i16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsI16x4*)(p + 4 * pitch));
-  return __builtin_bit_cast(typename Mma<T>::Frag, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
-}
+// Rows of n elements in LDS, n a power of two, their 16-byte chunks permuted by
+// the row (its low four bits) such that none of the three ways they are touched
+// meets a bank twice: 16-byte reads of 16 rows, transposing reads of rows 0 to 3
+// and 8 to 11 at once, 8-byte writes of 16 rows.  Each is an address of the lane
+// XOR a multiple of 16 columns, plus whole rows.
+template <int n>
+struct Rows {
+  static __device__ __forceinline__ int permute(int row) {
+    const int b0 = row & 1, b1 = row >> 1 & 1, b2 = row >> 2 & 1, b3 = row >> 3 & 1;
+    if constexpr (n == 32) return b2 * 2 ^ b3 * 3;
+    if constexpr (n == 64) return b1 * 2 ^ b2 * 4 ^ b3 * 5;
+    return b0 * 2 ^ b1 * 4 ^ b2 * 8 ^ b3 * 9;
+  }
+  static __device__ __forceinline__ int at(int row, int col) { return row * n + (((col >> 3) ^ permute(row)) << 3) + (col & 7); }
+
+  int along_, down_[2], put_;
+  __device__ __forceinline__ Rows() {
+    const int lane = threadIdx.x & 63, r = lane & 15, q = lane >> 4;
+    along_ = at(r, q * 8);
+    down_[0] = at(q * 8 + (r >> 2), (r & 3) * 4);
+    down_[1] = at(q * 8 + (r >> 2) + 4, (r & 3) * 4);
+    put_ = at(r, q * 4);
+  }
+  // Hides the lane's addresses from the compiler, which would otherwise keep
+  // every one of their XORs in registers over a loop.
+  __device__ __forceinline__ void renew() { asm volatile("" : "+v"(along_), "+v"(down_[0]), "+v"(down_[1]), "+v"(put_)); }
+  // Eight values along row `row` + lane % 16 from column `col` + 8 (lane / 16) on; row a multiple of 16, col of 32.
+  template <typename T>
+  __device__ __forceinline__ typename Mma<T>::Frag along(const T* p, int row, int col) const {
+    return *reinterpret_cast<const typename Mma<T>::Frag*>(p + (along_ ^ col) + row * n);
+  }
+  // Eight values down column `col` + lane % 16 from row `row` + 8 (lane / 16) on; row a multiple of 32, col of 16.
+  template <typename T>
+  __device__ __forceinline__ typename Mma<T>::Frag down(const T* p, int row, int col) const {
+    i16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsI16x4*)(p + (down_[0] ^ col) + row * n));
+    i16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsI16x4*)(p + (down_[1] ^ col) + row * n));
+    return __builtin_bit_cast(typename Mma<T>::Frag, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+  }
+  // Four values at row `row` + lane % 16, column `col` + 4 (lane / 16).
+  template <typename T>
+  __device__ __forceinline__ void put(T* p, int row, int col, const Four<T>& v) const {
+    *reinterpret_cast<Four<T>*>(p + (put_ ^ col) + row * n) = v;
+  }
+};
 
 template <typename T, int KI, int SL>
 __global__ __launch_bounds__(64 * narrow_back_waves(KI), KI <= 2 ? 2 : 1) void narrow_backward_kernel(NarrowBack<T> p) {
   typedef typename Mma<T>::Frag Frag;
   constexpr int kWaves = narrow_back_waves(KI), kGroups = kWaves / SL, kThreads = 64 * kWaves;
   constexpr NarrowBackLds l = narrow_back_lds(KI, SL);
-  constexpr int H = SL * 32, PI = l.pitch_in, PH = l.pitch_h, FI = 2 * KI;
+  constexpr int H = SL * 32, PI = l.row_in, PH = l.row_h, FI = 2 * KI;
+  typedef Rows<PI> In;
+  typedef Rows<PH> Hid;
+  In in;
+  Hid hid;
   static_assert(l.groups == kGroups, "");
   extern __shared__ __attribute__((aligned(16))) uint8_t narrow_mem[];
   T* const lds = reinterpret_cast<T*>(narrow_mem);
   T *const wg = lds, *const wu = lds + H * PI, *const wd = lds + 2 * H * PI;
   for (int c = threadIdx.x; c < 2 * H * KI * 4; c += kThreads) {
     const int row = c / (KI * 4), k = c % (KI * 4) * 8, h = row < H ? row : row - H;
-    *reinterpret_cast<Frag*>(lds + row * PI + k) =
+    *reinterpret_cast<Frag*>((row < H ? wg : wu) + In::at(h, k)) =
         load8<T>((row < H ? p.wg : p.wu) + (int64_t)(p.first + h) * p.in + k, p.first + h < p.last ? p.in - k : 0);
   }
   for (int c = threadIdx.x; c < KI * 32 * (H / 8); c += kThreads) {
-    const int o = c / (H / 8), k = p.first + c % (H / 8) * 8;
-    *reinterpret_cast<Frag*>(wd + o * PH + k - p.first) = load8<T>(p.wd + (int64_t)o * p.hidden + k, o < p.out ? p.last - k : 0);
+    const int o = c / (H / 8), k = c % (H / 8) * 8, h = p.first + k;
+    *reinterpret_cast<Frag*>(wd + Hid::at(o, k)) = load8<T>(p.wd + (int64_t)o * p.hidden + h, o < p.out ? p.last - h : 0);
   }
   const int lane = threadIdx.x & 63, r = lane & 15, q = lane >> 4;
   const int group = wave_id() / SL, slice = wave_id() % SL, t = threadIdx.x % (SL * 64);
@@ -256,7 +293,7 @@ __global__ __launch_bounds__(64 * narrow_back_waves(KI), KI <= 2 ? 2 : 1) void n
 #pragma unroll
     for (int i = 0; i < kLoads; i++) {
       const int c = t + i * SL * 64, half = c / (kChunks / 2), e = c % (kChunks / 2);
-      if (c < kChunks) *reinterpret_cast<Frag*>((half ? dys : xs) + e / (KI * 4) * PI + e % (KI * 4) * 8) = next[i];
+      if (c < kChunks) *reinterpret_cast<Frag*>((half ? dys : xs) + In::at(e / (KI * 4), e % (KI * 4) * 8)) = next[i];
     }
   };
   f32x4 dwg[2][FI] = {}, dwu[2][FI] = {}, dwd[FI][2] = {};
@@ -267,6 +304,8 @@ __global__ __launch_bounds__(64 * narrow_back_waves(KI), KI <= 2 ? 2 : 1) void n
   __syncthreads();
   for (int64_t base = first; base < p.rows; base += step) {
     const int64_t row = base + group * 32;
+    in.renew();
+    hid.renew();
     load(row + step);
     f32x4 g[2][2] = {}, u[2][2] = {}, dh[2][2] = {};   // [16 hidden][16 rows]
 #pragma unroll
@@ -274,15 +313,13 @@ __global__ __launch_bounds__(64 * narrow_back_waves(KI), KI <= 2 ? 2 : 1) void n
       Frag fx[2], fy[2];
 #pragma unroll
       for (int i = 0; i < 2; i++) {
-        fx[i] = *reinterpret_cast<const Frag*>(xs + (i * 16 + r) * PI + k * 32 + q * 8);
-        fy[i] = *reinterpret_cast<const Frag*>(dys + (i * 16 + r) * PI + k * 32 + q * 8);
+        fx[i] = in.along(xs, i * 16, k * 32);
+        fy[i] = in.along(dys, i * 16, k * 32);
       }
 #pragma unroll
       for (int b = 0; b < 2; b++) {
         const int h = slice * 32 + b * 16;
-        const Frag fg = *reinterpret_cast<const Frag*>(wg + (h + r) * PI + k * 32 + q * 8);
-        const Frag fu = *reinterpret_cast<const Frag*>(wu + (h + r) * PI + k * 32 + q * 8);
-        const Frag fd = down_column<T>(wd + k * 32 * PH + h, PH);
+        const Frag fg = in.along(wg, h, k * 32), fu = in.along(wu, h, k * 32), fd = hid.down(wd, k * 32, h);
 #pragma unroll
         for (int i = 0; i < 2; i++) {
           g[b][i] = Mma<T>::run(fg, fx[i], g[b][i]);
@@ -312,7 +349,7 @@ __global__ __launch_bounds__(64 * narrow_back_waves(KI), KI <= 2 ? 2 : 1) void n
 #pragma unroll
       for (int b = 0; b < 2; b++)
 #pragma unroll
-        for (int i = 0; i < 2; i++) *reinterpret_cast<Four<T>*>(to + (i * 16 + r) * PH + slice * 32 + b * 16 + q * 4) = v[b][i];
+        for (int i = 0; i < 2; i++) hid.put(to, i * 16, slice * 32 + b * 16, v[b][i]);
     };
     auto settle = [&]() {
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
@@ -324,10 +361,10 @@ __global__ __launch_bounds__(64 * narrow_back_waves(KI), KI <= 2 ? 2 : 1) void n
     {
       Frag fh[2];
 #pragma unroll
-      for (int b = 0; b < 2; b++) fh[b] = down_column<T>(dg + slice * 32 + b * 16, PH);
+      for (int b = 0; b < 2; b++) fh[b] = hid.down(dg, 0, slice * 32 + b * 16);
 #pragma unroll
       for (int j = 0; j < FI; j++) {
-        const Frag fy = down_column<T>(dys + j * 16, PI);
+        const Frag fy = in.down(dys, 0, j * 16);
 #pragma unroll
         for (int b = 0; b < 2; b++) dwd[j][b] = Mma<T>::run(fy, fh[b], dwd[j][b]);
       }
@@ -339,12 +376,12 @@ __global__ __launch_bounds__(64 * narrow_back_waves(KI), KI <= 2 ? 2 : 1) void n
       Frag fg[2], fu[2];
 #pragma unroll
       for (int b = 0; b < 2; b++) {
-        fg[b] = down_column<T>(dg + slice * 32 + b * 16, PH);
-        fu[b] = down_column<T>(du + slice * 32 + b * 16, PH);
+        fg[b] = hid.down(dg, 0, slice * 32 + b * 16);
+        fu[b] = hid.down(du, 0, slice * 32 + b * 16);
       }
 #pragma unroll
       for (int j = 0; j < FI; j++) {
-        const Frag fx = down_column<T>(xs + j * 16, PI);
+        const Frag fx = in.down(xs, 0, j * 16);
 #pragma unroll
         for (int b = 0; b < 2; b++) {
           dwg[b][j] = Mma<T>::run(fg[b], fx, dwg[b][j]);
@@ -362,9 +399,8 @@ __global__ __launch_bounds__(64 * narrow_back_waves(KI), KI <= 2 ? 2 : 1) void n
         if (p.first) acc = *reinterpret_cast<const f32x4*>(sum);
 #pragma unroll
         for (int k = 0; k < SL; k++) {
-          const int at = (i * 16 + r) * PH + k * 32 + q * 8;
-          acc = Mma<T>::run(down_column<T>(wg + k * 32 * PI + j * 16, PI), *reinterpret_cast<const Frag*>(dg + at), acc);
-          acc = Mma<T>::run(down_column<T>(wu + k * 32 * PI + j * 16, PI), *reinterpret_cast<const Frag*>(du + at), acc);
+          acc = Mma<T>::run(in.down(wg, k * 32, j * 16), hid.along(dg, i * 16, k * 32), acc);
+          acc = Mma<T>::run(in.down(wu, k * 32, j * 16), hid.along(du, i * 16, k * 32), acc);
         }
         const int64_t n = row + i * 16 + r;
         if (p.last < p.hidden) *reinterpret_cast<f32x4*>(sum) = acc;
