@@ -380,9 +380,13 @@ struct LnShape {
   int lanes, nv;
   bool block;
 };
-LnShape shape_of(int cols, int dtype) {
+//
+// A forward of few rows takes a workgroup from 65 vectors on, for more loads
+// in flight: 5003 x 1155 f16 13.3 us instead of 15.8 with a wave a row, while
+// 50,000 rows take 73 instead of 68.
+LnShape shape_of(int cols, int dtype, bool few_rows = false) {
   const int vecs = vectors(cols, dtype), most = dtype == NEST_DTYPE_F32 ? kLnMost : kLnMost / 2;
-  if (vecs <= 192) return {vecs <= 64 ? pow2_at_least(vecs) : 64, (vecs + 63) / 64, false};
+  if (vecs <= (few_rows ? 64 : 192)) return {vecs <= 64 ? pow2_at_least(vecs) : 64, (vecs + 63) / 64, false};
   if (vecs <= 2 * most) {
     const int nv = vecs <= 512 ? 1 : 2;
     return {(vecs + 64 * nv - 1) / (64 * nv) * 64, nv, true};
@@ -410,7 +414,7 @@ int64_t row_groups(int64_t rows, const LnShape& h) {
 
 template <typename T, typename P>
 hipError_t forward(const LayerNormParams& p, hipStream_t s) {
-  const LnShape h = shape_of(p.cols, p.dtype);
+  const LnShape h = shape_of(p.cols, p.dtype, p.rows < 16384);
   const int64_t need = row_groups(p.rows, h);
   const unsigned grid = (unsigned)(need < kLnForwardGrid ? need : kLnForwardGrid);
   with_shape(h, [&](auto nv, auto block) {

@@ -48,11 +48,11 @@ def _like(t: torch.Tensor, ref: torch.Tensor, shape, name: str, dtype=None) -> t
     """t checked against the main tensor's device, a type and a shape, and made contiguous."""
     if t.device != ref.device:
         raise ValueError(f"{name} is on {t.device}, expected {ref.device}")
-    if t.dtype != (dtype or ref.dtype):
+    if t.dtype is not (dtype or ref.dtype):
         raise TypeError(f"{name} is {t.dtype}, expected {dtype or ref.dtype}")
     if t.shape != shape:
         raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {tuple(shape)}")
-    return _whole(t)
+    return t if t.is_contiguous() else t.detach().contiguous()
 
 
 def _aligned(t: torch.Tensor) -> torch.Tensor:
@@ -112,7 +112,8 @@ def layer_norm_forward(x: torch.Tensor, weight: torch.Tensor, bias: Optional[tor
     """(y, mean, rstd): y = (x - mean) rstd weight + bias over the last dimension; mean and rstd are float32 [rows]."""
     code, pcode, x, weight, bias, rows, D = _norm_args(x, weight, bias, eps)
     y = torch.empty_like(x)
-    mean, rstd = torch.empty((2, rows), dtype=torch.float32, device=x.device).unbind(0)
+    mean = torch.empty(rows, dtype=torch.float32, device=x.device)
+    rstd = torch.empty_like(mean)
     _call("nest_layer_norm", x.device, rows, D, code, pcode, _at(x), _at(weight), _at(bias), eps, _at(y), _at(mean), _at(rstd))
     return y, mean, rstd
 
