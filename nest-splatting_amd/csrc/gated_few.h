@@ -13,6 +13,10 @@
 // the L1 may lose it: 38 us instead of 29 for 16 rows of 2048 -> 8192 bf16.
 // Waves of a workgroup share k and join their sums in LDS in their order.  One
 // launch for the gate, one for the down projection.
+//
+// Measured, 2048 -> 8192: one row bf16 13.3 us for the gate (67 MB, 5.0 TB/s)
+// and 9.6 for the down projection (33 MB); 32 rows f16 18.8 and 15.2, where x
+// is read from L2 by every workgroup.
 #pragma once
 
 #include "gated_tiles.h"

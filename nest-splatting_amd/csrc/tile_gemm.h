@@ -3,6 +3,11 @@
 //
 //   C[m][n] = sum_k A(m, k) B(n, k),  float32 sums
 //
+// 16-bit operands multiply on v_mfma_f32_16x16x32; float32 ones as three
+// bfloat16 parts each on the same instruction (split, run_parts), which passes
+// the rate of the float32 instructions.  An infinity has no such parts: the
+// float32 results that it enters are NaN.
+//
 // An operand is stored with k contiguous ("kKM", rows of m or n) or with its
 // own index contiguous (rows of k); every row length is a multiple of 16
 // bytes.  A step takes 128 bytes of k (64 16-bit or 32 float32 values) of each
@@ -18,8 +23,14 @@
 //
 // Out of range: a lane whose chunk lies outside its operand gives the buffer
 // load an offset past the resource's size, which the hardware answers with
-// zero; zeros add nothing, whatever the other operand holds there being
-// finite or zero itself.
+// zero.  k past the end is outside in both operands (or a zero of one's row
+// padding), so nothing an operand does not hold is multiplied.
+//
+// Measured: 8192 x 2048 x 8192 bf16 1130 TFLOP/s, 8192 x 2048 x 16384 1210,
+// where the library's 8192^3 product reaches 1395 on this card; the matrix
+// cores are busy 61 to 68% of the cycles, no LDS bank conflicts; the rest is
+// the barrier and the wait for loads that two buffers leave.  float32
+// 4096 x 2048, 4096: 210 TFLOP/s, 155 the library's product.
 #pragma once
 
 #include "vec_io.h"
@@ -30,7 +41,6 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef short i16x4 __attribute__((ext_vector_type(4)));
-typedef short i16x8 __attribute__((ext_vector_type(8)));
 
 constexpr int kStepBytes = 128;
 constexpr uint32_t kOutside = 0x80000000u, kRecords = 0x7fffffffu;

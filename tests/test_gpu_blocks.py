@@ -437,3 +437,52 @@ def test_training_a_refiner(dtype):
     refiner, before, after = m.train(steps=60, dtype=dtype, device=str(DEV), log=lambda s: None)
     assert after < 0.9 * before
     assert all(torch.isfinite(p).all() for p in refiner.parameters())
+
+
+# ---- offsets past 32 bits, float32 values that are not finite ----
+
+def test_rows_past_4_gib(B):
+    """The last rows of arrays over 4 GiB come out as the same rows by themselves: a row's result does not depend on its place."""
+    for dtype, rows in ((torch.bfloat16, 34_000_003), (torch.float32, 17_000_003)):
+        ws = ffn_case(1, 64, 96, 64, dtype)[1:4]
+        x, dy = torch.zeros(rows, 64, dtype=dtype, device=DEV), torch.zeros(rows, 64, dtype=dtype, device=DEV)
+        assert x.numel() * x.element_size() > 1 << 32
+        x[-200:], dy[-200:] = rand(200, 64, dtype=dtype, seed=1), rand(200, 64, dtype=dtype, seed=2)
+        tail = x[-200:].clone(), dy[-200:].clone()
+        w = rand(64, dtype=dtype, seed=3)
+        y, mean, rstd = B.layer_norm_forward(x, w)
+        want = B.layer_norm_forward(tail[0], w)
+        assert torch.equal(y[-200:], want[0])
+        assert torch.equal(B.layer_norm_backward(dy, x, w, mean, rstd)[0][-200:], B.layer_norm_backward(tail[1], tail[0], w, *want[1:])[0])
+        del y, mean, rstd
+        assert torch.equal(B.gated_ffn_forward(x, *ws)[0][-200:], B.gated_ffn_forward(tail[0], *ws)[0])
+        dx = B.gated_ffn_backward(dy, x, *ws)
+        alone = B.gated_ffn_backward(tail[1], tail[0], *ws)
+        assert torch.equal(dx[0][-200:], alone[0])
+        for d, a in zip(dx[1:], alone[1:]):  # rows of zeros add nothing: the sums differ by their order alone
+            assert torch.allclose(d.float(), a.float(), rtol=0, atol=float(a.float().abs().max()) * (2e-5 if dtype == torch.float32 else 2e-2))
+        del x, dy, dx
+        torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
+@pytest.mark.parametrize("rows", [4, 150])
+def test_ffn_values_that_are_not_finite_stay_in_their_rows(B, rows, dtype):
+    x, wg, wu, wd, dy = ffn_case(rows, 72, 200, 72, dtype)
+    clean, cx = B.gated_ffn_forward(x, wg, wu, wd)[0], B.gated_ffn_backward(dy, x, wg, wu, wd)[0]
+    x[1, 3], x[3, 71] = float("nan"), float("inf")
+    keep = torch.ones(rows, dtype=torch.bool, device=DEV)
+    keep[[1, 3]] = False
+    y, dx = B.gated_ffn_forward(x, wg, wu, wd)[0], B.gated_ffn_backward(dy, x, wg, wu, wd)[0]
+    assert torch.equal(y[keep], clean[keep]) and torch.equal(dx[keep], cx[keep])
+    assert torch.isnan(y[1]).all() and not torch.isfinite(y[3]).any()
+
+
+def test_ffn_float32_over_its_range(B):
+    """Values from 2^-60 to 2^60 in one product: each is cut into parts by itself, the largest does not overflow."""
+    x, wg, wu, wd, dy = ffn_case(100, 64, 96, 64, torch.float32)
+    scale = torch.exp2(torch.arange(100, device=DEV, dtype=torch.float32).fmod(21) - 10)[:, None]
+    ffn_check(B, x * scale, wg, wu, wd, dy, "relu")
+    big = torch.full((70, 64), 2.0 ** 60, device=DEV)
+    y = B.gated_ffn_forward(big, wg * 2.0 ** -60, wu * 2.0 ** -60, wd, "relu")[0]
+    R.check(y, *R.ffn(big, wg * 2.0 ** -60, wu * 2.0 ** -60, wd, "relu")["y"], "y of 2^60")
