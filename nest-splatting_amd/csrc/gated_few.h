@@ -8,15 +8,14 @@
 // are the 16 columns: the diagonal blocks of the result, where both parts
 // agree, are summed, the rest is of no use.  With S = 16 (one row of x) a load
 // takes 1 KB of one weight row, with S = 4 (up to four) 256 bytes of four, with
-// S = 2 (up to 32) 128 bytes of eight.  S = 1, 64 bytes of sixteen rows, would
+// S = 2 (up to 16) 128 bytes of eight.  S = 1, 64 bytes of sixteen rows, would
 // fit 16 rows of x, but a line's halves then come by two loads between which
 // the L1 may lose it: 38 us instead of 29 for 16 rows of 2048 -> 8192 bf16.
 // Waves of a workgroup share k and join their sums in LDS in their order.  One
 // launch for the gate, one for the down projection.
 //
 // Measured, 2048 -> 8192: one row bf16 13.3 us for the gate (67 MB, 5.0 TB/s)
-// and 9.6 for the down projection (33 MB); 32 rows f16 18.8 and 15.2, where x
-// is read from L2 by every workgroup.
+// and 9.6 for the down projection (33 MB).
 #pragma once
 
 #include "gated_tiles.h"
@@ -176,8 +175,7 @@ hipError_t launch_few(const Few<T>& p, hipStream_t s) {
   if (p.M == 1) return launch_few_shape<T, FewShape<16, 1, 2 * kMore, 4>, kGate>(p, s);
   if (p.M <= 4) return launch_few_shape<T, FewShape<4, 1, 2 * kMore, 4>, kGate>(p, s);
   if (p.M <= 8) return launch_few_shape<T, FewShape<2, 1, 1, 8>, kGate>(p, s);
-  if (p.M <= 16) return launch_few_shape<T, FewShape<2, 2, 1, 4>, kGate>(p, s);
-  return launch_few_shape<T, FewShape<2, 4, kGate ? 2 : 1, kGate ? 2 : 4>, kGate>(p, s);
+  return launch_few_shape<T, FewShape<2, 2, 1, 4>, kGate>(p, s);
 }
 
 template <typename T>

@@ -5,25 +5,29 @@ namespace nest {
 namespace {
 
 // Rows up to which the forward streams the weights through registers
-// (gated_few.h).  2048 -> 8192, us, streamed and in tiles: 32 rows of 16 bits
-// 36 and 38, 33 rows 47 (tiles); 16 rows of float32 70, 32 rows 104 and 87.
-int64_t few_rows(int es) { return es == 2 ? 32 : 16; }
+// (gated_few.h).  2048 -> 8192, weights from memory, us, streamed and in tiles:
+// 8 rows bf16 24 and 33, 16 rows 28 and 30, 32 rows 37 and 30; float32 45 and
+// 75 for one row, 67 and 70 for 16.
+constexpr int64_t kFewRows = 16;
 
 int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 // Seconds that `groups` workgroups of tiles of side x side and `steps` steps of
 // 128 bytes of k take, in rounds of what the LDS lets run at once.  A step of a
 // round takes its products' time at the rate a full CU reaches, or what a lone
-// workgroup's step takes: its loads' latency, and for float32 the cutting into
-// parts beside the products.  Rates and times as measured.
+// workgroup's step takes: its loads' latency (less with four buffers), and for
+// float32 the cutting into parts beside the products.  Rates and times are
+// fitted to the choices of choose_tile.
 double seconds(int64_t groups, int64_t steps, int side, int es) {
   const int i = side == 256 ? 0 : side == 128 ? 1 : 2;
-  static constexpr double kRate[2][3] = {{4.4e12, 3.4e12, 2.3e12}, {1.05e12, 0.88e12, 0.53e12}};   // of a CU
-  static constexpr double kLone[2][3] = {{0.42e-6, 0.42e-6, 0.42e-6}, {4.0e-6, 1.69e-6, 0.73e-6}};
+  static constexpr double kRate[2][3] = {{5.2e12, 4.1e12, 2.2e12}, {0.95e12, 0.86e12, 0.59e12}};   // of a CU
+  static constexpr double kLone[2][3] = {{0.31e-6, 0.95e-6, 0.44e-6}, {1.9e-6, 1.8e-6, 0.73e-6}};
+  static constexpr double kLoneMore[2] = {0.26e-6, 0.70e-6};
   static constexpr int kAtOnce[3] = {1, 2, 5};
   const int f32 = es == 4;
   const double step = 2.0 * side * side * (128 / es) / kRate[f32][i];
-  auto round = [&](int64_t a_cu) { return (double)steps * (step * a_cu > kLone[f32][i] ? step * a_cu : kLone[f32][i]); };
+  const double lone = side == 64 && groups <= kMoreBuffers ? kLoneMore[f32] : kLone[f32][i];
+  auto round = [&](int64_t a_cu) { return (double)steps * (step * a_cu > lone ? step * a_cu : lone); };
   const int64_t full = groups / (256 * kAtOnce[i]), rest = groups % (256 * kAtOnce[i]);
   return (double)full * round(kAtOnce[i]) + (rest ? round(cdiv(rest, 256)) : 0.0);
 }
@@ -42,9 +46,9 @@ hipError_t launch_clear(void* p, size_t bytes, hipStream_t s) {
 }  // namespace
 
 // Tiles for up to three products that share a launch and K.  Against every
-// tile and split timed on eight sizes of the down projection of 16-bit types
-// and eight of float32 (64 to 300,000 rows, 64 to 2048 columns, k of 128 to
-// 8192) the choice is within 2% of the best on average, 18% at worst.
+// tile and split timed at 200 sizes of all five launches (33 to 8192 rows, 160
+// to 2048 features, 256 to 8192 hidden; half of them float32) the choice costs
+// 1% of a call on average (0.3% for float32), 24% at worst (calls of 20 us).
 TileChoice choose_tile(int n, const int64_t* M, const int64_t* N, int64_t K, int es, bool may_split) {
   TileChoice best{64, 1};
   double least = 1e30;
@@ -58,7 +62,7 @@ TileChoice choose_tile(int n, const int64_t* M, const int64_t* N, int64_t K, int
     for (int splits = 1; splits <= (may_split ? 256 : 1); splits *= 2) {
       if (splits > 1 && steps < 4 * splits) break;   // at least four steps each
       double t = seconds(tiles * splits, cdiv(steps, splits), side, es);
-      if (splits > 1) t += 3.5e-6 + 8.0 * (double)size * splits / 5e12;   // the partial sums' way to memory and back
+      if (splits > 1) t += 4.5e-6 + 8.0 * (double)size * splits / 5e12;   // the partial sums' way to memory and back
       if (t < least) {
         least = t;
         best = {side, splits};
@@ -116,7 +120,7 @@ GatedLayout gated_layout(int64_t rows, int in, int hidden, int out, int dtype, b
     return l;
   }
   l.h = take(rows * l.ldh * es);
-  l.few = !back && rows <= few_rows(es);
+  l.few = !back && rows <= kFewRows;
   if (l.few) {
     l.bytes = at;
     l.kept_bytes = (size_t)kept_bytes;

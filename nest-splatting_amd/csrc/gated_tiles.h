@@ -378,6 +378,14 @@ __global__ __launch_bounds__(256) void pad_kernel(Pads<T> p) {
 
 // ---- the choice of tiles, and launches ----
 
+// f with the tile of a launch of `groups` workgroups.
+template <typename F>
+void with_tile(int side, int64_t groups, F f) {
+  if (side == 256) f(TileL());
+  else if (side == 128) f(TileM());
+  else groups <= kMoreBuffers ? f(TileS4()) : f(TileS());
+}
+
 template <typename T, bool kAK, bool kBK>
 hipError_t launch_products(Products<T>& all, TileChoice t, hipStream_t s) {
   int64_t tiles = 0, part = 0;
@@ -392,10 +400,10 @@ hipError_t launch_products(Products<T>& all, TileChoice t, hipStream_t s) {
   all.part_size = part;
   if (t.splits == 1) all.part = nullptr;
   const unsigned grid = (unsigned)(tiles * t.splits);
-  if (t.side == 256) {
-    product_kernel<T, kAK, kBK, TileL><<<grid, TileL::NT, 0, s>>>(all);
-  } else if (t.side == 128) product_kernel<T, kAK, kBK, TileM><<<grid, TileM::NT, 0, s>>>(all);
-  else product_kernel<T, kAK, kBK, TileS><<<grid, TileS::NT, 0, s>>>(all);
+  with_tile(t.side, grid, [&](auto c) {
+    typedef decltype(c) C;
+    product_kernel<T, kAK, kBK, C><<<grid, C::NT, 0, s>>>(all);
+  });
   if (t.splits > 1) {
     const int64_t need = (part + 1023) / 1024;
     join_kernel<T><<<(unsigned)(need < 65536 ? need : 65536), 256, 0, s>>>(all);
@@ -409,10 +417,10 @@ hipError_t launch_gate(Gate<T> p, hipStream_t s) {
   p.tiles_m = (p.M + t.side - 1) / t.side;
   p.tiles_n = (int)((p.ldh + t.side / 2 - 1) / (t.side / 2));
   const unsigned grid = (unsigned)((int64_t)p.tiles_m * p.tiles_n);
-  if (t.side == 256) {
-    gate_kernel<T, TileL><<<grid, TileL::NT, 0, s>>>(p);
-  } else if (t.side == 128) gate_kernel<T, TileM><<<grid, TileM::NT, 0, s>>>(p);
-  else gate_kernel<T, TileS><<<grid, TileS::NT, 0, s>>>(p);
+  with_tile(t.side, grid, [&](auto c) {
+    typedef decltype(c) C;
+    gate_kernel<T, C><<<grid, C::NT, 0, s>>>(p);
+  });
   return hipGetLastError();
 }
 
@@ -422,10 +430,10 @@ hipError_t launch_gate_backward(GateBackward<T> p, hipStream_t s) {
   p.tiles_m = (p.M + t.side - 1) / t.side;
   p.tiles_n = (int)((p.ldh + t.side - 1) / t.side);
   const unsigned grid = (unsigned)((int64_t)p.tiles_m * p.tiles_n);
-  if (t.side == 256) {
-    gate_backward_kernel<T, TileL><<<grid, TileL::NT, 0, s>>>(p);
-  } else if (t.side == 128) gate_backward_kernel<T, TileM><<<grid, TileM::NT, 0, s>>>(p);
-  else gate_backward_kernel<T, TileS><<<grid, TileS::NT, 0, s>>>(p);
+  with_tile(t.side, grid, [&](auto c) {
+    typedef decltype(c) C;
+    gate_backward_kernel<T, C><<<grid, C::NT, 0, s>>>(p);
+  });
   return hipGetLastError();
 }
 

@@ -11,8 +11,8 @@
 // An operand is stored with k contiguous ("kKM", rows of m or n) or with its
 // own index contiguous (rows of k); every row length is a multiple of 16
 // bytes.  A step takes 128 bytes of k (64 16-bit or 32 float32 values) of each
-// row.  Two LDS buffers: the loads of the next step are in flight while the
-// current one is multiplied, one barrier a step.
+// row.  Two or four LDS buffers: the loads of the next one or three steps are in
+// flight while the current one is multiplied, one barrier a step.
 //
 // LDS layouts.  k contiguous: rows of 128 bytes, the 16-byte chunk c of row r
 // at slot c ^ (r & 7), so the 16 rows one fragment load touches fall on
@@ -221,62 +221,104 @@ __device__ __forceinline__ typename Mma<T>::Frag fragment(const uint8_t* lds, in
   }
 }
 
-// BM x BN by WM x WN waves of (16 FM) x (16 FN).
-template <int kBM, int kBN, int kWM, int kWN>
+// BM x BN by WM x WN waves of (16 FM) x (16 FN), with `stages` LDS buffers.
+template <int kBM, int kBN, int kWM, int kWN, int kStages>
 struct Tile {
   static constexpr int BM = kBM, BN = kBN, WM = kWM, WN = kWN, NT = 64 * WM * WN, FM = BM / WM / 16, FN = BN / WN / 16;
+  static constexpr int stages = kStages;
 };
-typedef Tile<256, 256, 2, 4> TileL;
-typedef Tile<128, 128, 2, 2> TileM;
-typedef Tile<64, 64, 2, 2> TileS;
+typedef Tile<256, 256, 2, 4, 2> TileL;
+typedef Tile<128, 128, 2, 2, 2> TileM;
+typedef Tile<64, 64, 2, 2, 2> TileS;
+typedef Tile<64, 64, 2, 2, 4> TileS4;
 
-// The two LDS buffers of a step.  They are separate arrays, so that the
-// compiler knows a direct load into one not to touch a fragment of the other.
-template <typename C>
+// LDS buffer kBuf of a step.  They are separate arrays, so that the compiler
+// knows a direct load into one not to touch a fragment of another.
+template <typename C, int kBuf = 0>
 __device__ __forceinline__ uint8_t* tile_lds() {
   __shared__ __attribute__((aligned(16))) uint8_t lds[(C::BM + C::BN) * kStepBytes];
   return lds;
 }
-template <typename C>
-__device__ __forceinline__ uint8_t* tile_lds_next() {
-  __shared__ __attribute__((aligned(16))) uint8_t lds[(C::BM + C::BN) * kStepBytes];
-  return lds;
+
+template <int n>
+struct Number {
+  static constexpr int value = n;
+};
+
+// f(Number<0>()), f(Number<1>()), ... f(Number<n - 1>()).
+template <int n, int i = 0, typename F>
+__device__ __forceinline__ void each(F f) {
+  if constexpr (i < n) {
+    f(Number<i>());
+    each<n, i + 1>(f);
+  }
+}
+
+// step(Number<s % n>()) for each s < total.  One loop with one way out: what is
+// left stands behind it, because a jump from the middle would make the compiler
+// wait for all loads at its top.
+template <int n, typename F>
+__device__ __forceinline__ void each_step(int total, F step) {
+  int left = total;
+  for (; left >= n; left -= n) each<n>(step);
+  each<n - 1>([&](auto i) {
+    if (i.value < left) step(i);
+  });
+}
+
+// A barrier after all but this wave's last n direct loads have landed; its LDS
+// reads are done.
+template <int n>
+__device__ __forceinline__ void landed_barrier() {
+  if constexpr (n == 0) {
+    __syncthreads();
+  } else {
+    static_assert(n < 64, "");
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(n) : "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+  }
 }
 
 // acc[i][j]: rows m = 16 i + lane % 16, columns n = 16 j + 4 (lane / 16) + 0..3
 // of the wave's part.  `steps` steps of k from each of `segments` operand
-// pairs; a2 and b2: the second pair's bases.
+// pairs; a2 and b2: the second pair's bases.  Loads are issued past the last
+// step, where all of their lanes are outside, so that each wait counts the
+// same; a barrier has to follow before the LDS is used again.
 template <typename T, bool kAK, bool kBK, typename C>
 __device__ __forceinline__ void tile_product(Loader<T, kAK, C::BM, C::NT>& la, Loader<T, kBK, C::BN, C::NT>& lb, int64_t K,
                                              const char* a2, const char* b2, f32x4 (&acc)[C::FM][C::FN]) {
-  uint8_t* const a_lds0 = tile_lds<C>();
-  uint8_t* const b_lds0 = a_lds0 + C::BM * kStepBytes;
-  uint8_t* const a_lds1 = tile_lds_next<C>();
-  uint8_t* const b_lds1 = a_lds1 + C::BM * kStepBytes;
-  constexpr int kStep = kStepBytes / (int)sizeof(T);
+  constexpr int kStep = kStepBytes / (int)sizeof(T), kBufs = C::stages;
+  constexpr int kStepLoads = Loader<T, kAK, C::BM, C::NT>::kLoads + Loader<T, kBK, C::BN, C::NT>::kLoads;
   const int steps = K > kStep ? (int)((K + kStep - 1) / kStep) : 1;
   const int total = a2 ? 2 * steps : steps;
   int64_t k_left = K;
   int next = 0;
-  auto issue = [&](uint8_t* a, uint8_t* b) {
-    if (next == steps) {   // the second pair
+  auto issue = [&](auto buf) {
+    if (a2 && next == steps) {   // the second pair
       la.base = a2;
       lb.base = b2;
       k_left = K;
     }
-    la.issue(a, k_left);
-    lb.issue(b, k_left);
+    uint8_t* const lds = tile_lds<C, buf.value>();
+    la.issue(lds, k_left);
+    lb.issue(lds + C::BM * kStepBytes, k_left);
     la.base += la.advance;
     lb.base += lb.advance;
     k_left -= kStep;
     next++;
+    __builtin_amdgcn_sched_barrier(0);   // first of all, not among the products
   };
   const int w = wave_id(), wm = (w / C::WN) * C::FM * 16, wn = (w % C::WN) * C::FN * 16;
   const int ba = fragment_base<T, kAK, C::BM>(wm), bb = fragment_base<T, kBK, C::BN>(wn);
-  int s = 0;
   if constexpr (sizeof(T) == 4) {
     // Both halves of a step's k make one 32-wide product of the parts.
-    auto multiply = [&](const uint8_t* a, const uint8_t* b) {
+    each<kBufs - 1>(issue);
+    each_step<kBufs>(total, [&](auto buf) {
+      landed_barrier<(kBufs - 2) * kStepLoads>();   // this step has landed, the last one is all read
+      issue(Number<(buf.value + kBufs - 1) % kBufs>());
+      const uint8_t* a = tile_lds<C, buf.value>();
+      const uint8_t* b = a + C::BM * kStepBytes;
       Parts pb[C::FN];
 #pragma unroll
       for (int j = 0; j < C::FN; j++) pb[j] = split(fragment<T, kBK, C::BN>(b, bb, j, 0), fragment<T, kBK, C::BN>(b, bb, j, 1));
@@ -286,18 +328,9 @@ __device__ __forceinline__ void tile_product(Loader<T, kAK, C::BM, C::NT>& la, L
 #pragma unroll
         for (int j = 0; j < C::FN; j++) acc[i][j] = run_parts(pb[j], pa, acc[i][j]);
       }
-    };
-    issue(a_lds0, b_lds0);
-    while (true) {
-      __syncthreads();   // this step has landed, the last one is all read
-      if (s + 1 < total) issue(a_lds1, b_lds1);
-      multiply(a_lds0, b_lds0);
-      if (++s == total) return;
-      __syncthreads();
-      if (s + 1 < total) issue(a_lds0, b_lds0);
-      multiply(a_lds1, b_lds1);
-      if (++s == total) return;
-    }
+    });
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    return;
   }
   // A step is four phases: half kb of k times half of the wave's rows.  Each
   // phase reads the next one's fragments before its own products, so LDS works
@@ -309,9 +342,9 @@ __device__ __forceinline__ void tile_product(Loader<T, kAK, C::BM, C::NT>& la, L
 #pragma unroll
     for (int i = 0; i < kHalf; i++) fa[to][i] = fragment<T, kAK, C::BM>(a, ba, half * kHalf + i, kb);
   };
-  auto load_b = [&](int to, const uint8_t* b, int kb) {
+  auto load_b = [&](int to, const uint8_t* a, int kb) {
 #pragma unroll
-    for (int j = 0; j < C::FN; j++) fb[to][j] = fragment<T, kBK, C::BN>(b, bb, j, kb);
+    for (int j = 0; j < C::FN; j++) fb[to][j] = fragment<T, kBK, C::BN>(a + C::BM * kStepBytes, bb, j, kb);
   };
   auto products = [&](int half, int from_a, int from_b) {
 #pragma unroll
@@ -321,32 +354,27 @@ __device__ __forceinline__ void tile_product(Loader<T, kAK, C::BM, C::NT>& la, L
         acc[half * kHalf + i][j] = Mma<T>::run(fb[from_b][j], fa[from_a][i], acc[half * kHalf + i][j]);
     __builtin_amdgcn_sched_barrier(0);
   };
-  auto step = [&](uint8_t* a, uint8_t* b, uint8_t* a_next, uint8_t* b_next) {
-    load_a(1, a, 0, 1);
+  each<kBufs>(issue);
+  landed_barrier<(kBufs - 1) * kStepLoads>();
+  load_a(0, tile_lds<C>(), 0, 0);
+  load_b(0, tile_lds<C>(), 0);
+  each_step<kBufs>(total, [&](auto buf) {
+    const uint8_t* const at = tile_lds<C, buf.value>();
+    const uint8_t* const at_next = tile_lds<C, (buf.value + 1) % kBufs>();
+    load_a(1, at, 0, 1);
     products(0, 0, 0);
-    load_a(0, a, 1, 0);
-    load_b(1, b, 1);
+    load_a(0, at, 1, 0);
+    load_b(1, at, 1);
     products(1, 1, 0);
-    load_a(1, a, 1, 1);
+    load_a(1, at, 1, 1);
     products(0, 0, 1);
-    __syncthreads();   // the next step has landed; this one's fragments are all read
-    if (s + 2 < total) issue(a, b);
-    load_a(0, a_next, 0, 0);   // after the last step: of no use, and of no harm
-    load_b(0, b_next, 0);
+    landed_barrier<(kBufs - 2) * kStepLoads>();   // the next step has landed; this one's fragments are all read
+    issue(buf);
+    load_a(0, at_next, 0, 0);   // after the last step: of no use, and of no harm
+    load_b(0, at_next, 0);
     products(1, 1, 1);
-    s++;
-  };
-  issue(a_lds0, b_lds0);
-  __syncthreads();
-  if (total > 1) issue(a_lds1, b_lds1);
-  load_a(0, a_lds0, 0, 0);
-  load_b(0, b_lds0, 0);
-  while (true) {
-    step(a_lds0, b_lds0, a_lds1, b_lds1);
-    if (s == total) break;
-    step(a_lds1, b_lds1, a_lds0, b_lds0);
-    if (s == total) break;
-  }
+  });
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // no load into LDS outlives the workgroup
 }
 
 // The tile of a workgroup.  Workgroups go to the eight XCDs in turn, each with
