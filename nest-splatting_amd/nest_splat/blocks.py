@@ -32,6 +32,7 @@ from . import _lib as L
 
 _CODE = {torch.float32: L.DTYPE_F32, torch.float16: L.DTYPE_F16, torch.bfloat16: L.DTYPE_BF16}
 _NAMED = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}
+_STRUCT_SIZE = ct.sizeof(L.GatedFfn)
 _ACT = {"relu": L.ACT_RELU, "silu": L.ACT_SILU, "gelu": L.ACT_GELU}
 
 
@@ -46,7 +47,7 @@ def _code(t: torch.Tensor, name: str) -> int:
 
 def _like(t: torch.Tensor, ref: torch.Tensor, shape, name: str, dtype=None) -> torch.Tensor:
     """t checked against the main tensor's device, a type and a shape, and made contiguous."""
-    if t.device != ref.device:
+    if t.get_device() != ref.get_device():   # -1 off the GPU; less to build than two devices
         raise ValueError(f"{name} is on {t.device}, expected {ref.device}")
     if t.dtype is not (dtype or ref.dtype):
         raise TypeError(f"{name} is {t.dtype}, expected {dtype or ref.dtype}")
@@ -199,20 +200,25 @@ def dropout(x, p: float, seed: int, offset: int = 0, residual=None) -> torch.Ten
 
 # ---- gated feed-forward ----
 
+def _weight(t, ref, shape, name):
+    return _aligned(_like(t, ref, shape, name))
+
+
 def _gated(x, w_gate, w_up, w_down, activation):
     code = _code(x, "x")
-    if activation not in _ACT:
+    act = _ACT.get(activation)
+    if act is None:
         raise ValueError(f"activation must be one of {sorted(_ACT)}, got {activation!r}")
     if x.dim() < 1 or w_gate.dim() != 2 or w_down.dim() != 2:
         raise ValueError("x needs a last dimension, the weights are [out, in] matrices")
-    I, H, O = x.shape[-1], w_gate.shape[0], w_down.shape[0]
-    if min(I, H, O) < 1:
+    I, (H, _), (O, _) = x.shape[-1], w_gate.shape, w_down.shape
+    if I < 1 or H < 1 or O < 1:
         raise ValueError("in_features, hidden and out_features must be at least 1")
     x = _aligned(_whole(x))
-    ws = tuple(_aligned(_like(w, x, s, n)) for w, s, n in ((w_gate, (H, I), "w_gate"), (w_up, (H, I), "w_up"), (w_down, (O, H), "w_down")))
-    rows = x.numel() // I
-    f = L.GatedFfn(ct.sizeof(L.GatedFfn), code, _ACT[activation], I, H, O, rows, x.data_ptr(), *(w.data_ptr() for w in ws))
-    return f, x, ws
+    up = (H, I)
+    w_gate, w_up, w_down = _weight(w_gate, x, up, "w_gate"), _weight(w_up, x, up, "w_up"), _weight(w_down, x, (O, H), "w_down")
+    f = L.GatedFfn(_STRUCT_SIZE, code, act, I, H, O, x.numel() // I, x.data_ptr(), w_gate.data_ptr(), w_up.data_ptr(), w_down.data_ptr())
+    return f, x, (w_gate, w_up, w_down)
 
 
 def _gated_sizes(f):
@@ -231,7 +237,8 @@ def gated_ffn_forward(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor,
     where computing it again costs less); it is None otherwise."""
     f, x, ws = _gated(x, w_gate, w_up, w_down, activation)
     kept_bytes, fwd_bytes, _, _ = _gated_sizes(f)
-    y = torch.empty(x.shape[:-1] + (f.out_features,), dtype=x.dtype, device=x.device)
+    O = f.out_features
+    y = torch.empty_like(x) if O == x.shape[-1] else torch.empty(x.shape[:-1] + (O,), dtype=x.dtype, device=x.device)
     kept = _workspace(kept_bytes, x.device) if training else None
     work = _workspace(fwd_bytes, x.device)
     _call("nest_gated_ffn_forward", x.device, f, _at(y), _at(kept), _at(work), fwd_bytes)
