@@ -226,6 +226,21 @@ def test_ffn_few_rows(B, rows, dtype):
     ffn_check(B, *ffn_case(rows, i, h, o, dtype), "silu")
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("steps", range(1, 10))
+def test_ffn_every_count_of_steps(B, steps, dtype):
+    """Sums of 1 to 9 steps of 128 bytes, the last one short: each way in and out of two and four LDS buffers."""
+    n = steps * (32 if dtype is torch.float32 else 64)
+    ffn_check(B, *ffn_case(n - 1, n - 5, n - 3, 136, dtype), "silu")
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("size", [(1500, 200, 1400, 136), (3000, 140, 2000, 132)], ids=lambda s: "x".join(map(str, s)))
+def test_ffn_many_tiles(B, size, dtype):
+    """More tiles than run at once, at sizes whose sides end inside a tile."""
+    ffn_check(B, *ffn_case(*size, dtype), "gelu")
+
+
 @pytest.mark.parametrize("kind", ["silu", "gelu", "relu"])
 @pytest.mark.parametrize("dtype", TYPES)
 def test_ffn_activations_over_their_range(B, dtype, kind):
