@@ -71,6 +71,7 @@ struct TileChoice {
 // With more workgroups the others' loads do as well: five of two buffers fit a
 // CU, and 1777 x 515, 1365 float32 backward takes 167 us against 188 with four.
 constexpr int64_t kMoreBuffers = 512;
+constexpr int64_t kJoinGroup = 1024;   // partial sums that a workgroup joins
 
 constexpr int kNarrowLdsBytes = 160 * 1024;
 constexpr int kNarrowPad = 16;   // elements past a multiple of 64 bytes: 16-byte reads of 16 rows fall on different banks

@@ -130,7 +130,7 @@ GatedLayout gated_layout(int64_t rows, int in, int hidden, int out, int dtype, b
   auto partial = [&](const TileChoice& t, int n, const int64_t* M, const int64_t* N) {
     if (t.splits == 1) return;
     int64_t size = 0;
-    for (int i = 0; i < n; i++) size += cdiv(M[i] * N[i], 4) * 4;
+    for (int i = 0; i < n; i++) size += cdiv(M[i] * N[i], kJoinGroup) * kJoinGroup;
     if (size * t.splits * 4 > part) part = size * t.splits * 4;
   };
   if (!back) {

@@ -215,18 +215,35 @@ __global__ __launch_bounds__(C::NT) void product_kernel(Products<T> all) {
   }
 }
 
-// Joins the partial sums, in the order of the splits, four places a thread
-// (each product's part of a slice is a multiple of four).
+// s + the n slices of a power of two, all loads before the first sum.
+template <int n>
+__device__ __forceinline__ f32x4 add_slices(f32x4 s, const float* part, int64_t slice) {
+  f32x4 v[n];
+#pragma unroll
+  for (int i = 0; i < n; i++) v[i] = *reinterpret_cast<const f32x4*>(part + i * slice);
+#pragma unroll
+  for (int i = 0; i < n; i++) s += v[i];
+  return s;
+}
+
+// Joins the partial sums, in the order of the splits (a power of two), four
+// places a thread; the products' parts of a slice are whole workgroups.
+// 32 x 2048 in eight splits 3.3 us, with one load after another 4.1.
 template <typename T>
 __global__ __launch_bounds__(256) void join_kernel(Products<T> all) {
-  for (int64_t e = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4; e < all.part_size; e += (int64_t)gridDim.x * 1024) {
-    f32x4 s = *reinterpret_cast<const f32x4*>(all.part + e);
-    for (int i = 1; i < all.splits; i++) s += *reinterpret_cast<const f32x4*>(all.part + i * all.part_size + e);
+  for (int64_t first = (int64_t)blockIdx.x * kJoinGroup; first < all.part_size; first += (int64_t)gridDim.x * kJoinGroup) {
     int which = 0;
-    while (which + 1 < all.n && e >= all.p[which + 1].part) which++;
+    while (which + 1 < all.n && first >= all.p[which + 1].part) which++;
     const Product<T>& p = all.p[which];
-    const int64_t at = e - p.part, left = (int64_t)p.M * p.N - at;
-    if (left > 0) store4(p.c + at, 0, left < 4 ? (int)left : 4, true, s);
+    const int64_t e = first + threadIdx.x * 4, at = e - p.part, left = (int64_t)p.M * p.N - at;
+    if (left <= 0) continue;
+    const float* part = all.part + e;
+    f32x4 s = {};
+    if (all.splits == 2) s = add_slices<2>(s, part, all.part_size);
+    else if (all.splits == 4) s = add_slices<4>(s, part, all.part_size);
+    else
+      for (int i = 0; i < all.splits; i += 8) s = add_slices<8>(s, part + i * all.part_size, all.part_size);
+    store4(p.c + at, 0, left < 4 ? (int)left : 4, true, s);
   }
 }
 
@@ -367,9 +384,10 @@ __global__ __launch_bounds__(256) void pad_kernel(Pads<T> p) {
   constexpr int N = Vec16<T>::kN;
   const int k = blockIdx.y, n = p.n[k], chunks = p.ld[k] / N;
   const int64_t total = p.rows[k] * chunks;
+  const bool small = total < (int64_t)1 << 32;   // a division of 32 bits does
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
-    const int64_t row = i / chunks;
-    const int c = (int)(i % chunks) * N;
+    const int64_t row = small ? (int64_t)((uint32_t)i / (uint32_t)chunks) : i / chunks;
+    const int c = (int)(i - row * chunks) * N;
     float v[N];
     load_vec<T>(v, p.from[k] + row * n + c, n - c);
     store_vec<T>(p.to[k] + row * p.ld[k] + c, v, N);
@@ -394,7 +412,7 @@ hipError_t launch_products(Products<T>& all, TileChoice t, hipStream_t s) {
     all.p[i].tiles_n = (all.p[i].N + t.side - 1) / t.side;
     all.p[i].part = part;
     tiles += (int64_t)all.p[i].tiles_m * all.p[i].tiles_n;
-    part += ((int64_t)all.p[i].M * all.p[i].N + 3) / 4 * 4;
+    part += ((int64_t)all.p[i].M * all.p[i].N + kJoinGroup - 1) / kJoinGroup * kJoinGroup;
   }
   all.splits = t.splits;
   all.part_size = part;
@@ -405,7 +423,7 @@ hipError_t launch_products(Products<T>& all, TileChoice t, hipStream_t s) {
     product_kernel<T, kAK, kBK, C><<<grid, C::NT, 0, s>>>(all);
   });
   if (t.splits > 1) {
-    const int64_t need = (part + 1023) / 1024;
+    const int64_t need = part / kJoinGroup;
     join_kernel<T><<<(unsigned)(need < 65536 ? need : 65536), 256, 0, s>>>(all);
   }
   return hipGetLastError();
