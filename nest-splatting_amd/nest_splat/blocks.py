@@ -298,15 +298,24 @@ class LayerNorm(nn.Module):
         return layer_norm(x, self.weight, self.bias, self.eps)
 
 
-class Dropout(nn.Module):
-    """dropout while training, with a new offset each call; the place in the sequence is part of the state dict, so a
-    resumed run draws the masks that follow. In evaluation x passes through (plus the residual)."""
+# the backward pass that this call is made from, -1 outside of any
+_backward_id = getattr(torch._C, "_current_graph_task_id", lambda: -1)
 
-    def __init__(self, p: float = 0.1, seed: int = 0):
+
+class Dropout(nn.Module):
+    """dropout while training, with a new mask each call. In evaluation x passes through (plus the residual).
+
+    Without ``seed`` each call draws its key from torch's CPU generator: torch.manual_seed governs the masks, modules and
+    differently seeded ranks have masks of their own, and a forward that torch.utils.checkpoint recomputes, with the
+    generator's state restored, draws its mask again. With ``seed`` the module counts its calls under that key, and its
+    state dict keeps the count, so a resumed run draws the masks that follow; such a count cannot be taken back for a
+    recomputed forward, and replicas would count on copies: both raise."""
+
+    def __init__(self, p: float = 0.1, seed: Optional[int] = None):
         super().__init__()
         if not 0.0 <= p <= 1.0:
             raise ValueError(f"p must be in [0, 1], got {p}")
-        self.p, self.seed, self.offset = float(p), int(seed), 0
+        self.p, self.seed, self.offset = float(p), None if seed is None else int(seed), 0
 
     def get_extra_state(self):
         return {"seed": self.seed, "offset": self.offset}
@@ -314,11 +323,22 @@ class Dropout(nn.Module):
     def set_extra_state(self, state):
         self.seed, self.offset = state["seed"], state["offset"]
 
+    def _key(self):
+        """(seed, offset) of this call."""
+        if self.seed is None:
+            return int(torch.empty((), dtype=torch.int64, device="cpu").random_()), 0
+        if _backward_id() != -1:
+            raise RuntimeError("a recomputed forward would draw another mask from a Dropout with a seed of its own: leave seed "
+                               "out (torch's generator then repeats the mask), or call dropout with an offset")
+        if getattr(self, "_is_replica", False):
+            raise RuntimeError("a replica of a Dropout with a seed of its own would repeat its masks each step: leave seed out")
+        self.offset += 1
+        return self.seed, self.offset - 1
+
     def forward(self, x: torch.Tensor, residual: Optional[torch.Tensor] = None) -> torch.Tensor:
         if not self.training or self.p == 0.0:
             return x if residual is None else residual + x
-        offset, self.offset = self.offset, self.offset + 1
-        return dropout(x, self.p, self.seed, offset, residual)
+        return dropout(x, self.p, *self._key(), residual)
 
 
 class GatedFFN(nn.Module):
@@ -350,7 +370,7 @@ class GatedRefiner(nn.Module):
 
     The rows run through the blocks in ``dtype``. The down projections start at zero, so a new refiner returns its input
     rounded to dtype; with the colour MLP's own 16-bit type that leaves the decoded image as it was, since the MLP
-    rounds its features to that type."""
+    rounds its features to that type. ``seed`` makes the weights; the masks come from torch's generator (see Dropout)."""
 
     def __init__(self, features: int, hidden: Optional[int] = None, depth: int = 1, p: float = 0.1, activation: str = "silu",
                  dtype="bf16", seed: int = 0):
@@ -359,7 +379,7 @@ class GatedRefiner(nn.Module):
         self.dtype = _NAMED.get(dtype, dtype)
         self.norms = nn.ModuleList(LayerNorm(features) for _ in range(depth))
         self.ffns = nn.ModuleList(GatedFFN(features, hidden or 2 * features, None, activation, dtype, seed + k) for k in range(depth))
-        self.drops = nn.ModuleList(Dropout(p, seed + (k << 32)) for k in range(depth))
+        self.drops = nn.ModuleList(Dropout(p) for _ in range(depth))
         for f in self.ffns:
             nn.init.zeros_(f.w_down)
 
