@@ -136,7 +136,7 @@ __global__ __launch_bounds__(512, KI <= 2 ? 4 : 2) void narrow_forward_kernel(Na
     if (p.out % 8 == 0) {
 #pragma unroll
       for (int i = 0; i < RG; i++)
-        store_rows<T, FO>(stage, p.y, row + i * 16, p.rows, 0, p.out, [&](int j) { return y[i][j]; });
+        store_rows<T, FO>(stage, p.y, row + i * 16, p.rows, 0, p.out, [&](int j) { return y[i][j]; }, lane);
     } else {
 #pragma unroll
       for (int i = 0; i < RG; i++)

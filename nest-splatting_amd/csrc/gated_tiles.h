@@ -118,9 +118,9 @@ struct RowStage {
 // is a multiple of 16 bytes and out aligned.  Element f(j)[e] is column
 // 16 j + 4 (lane / 16) + e of row lane % 16.
 template <typename T, int FN, typename F>
-__device__ __forceinline__ void store_rows(RowStage<T, FN>& stage, T* out, int64_t row, int64_t rows, int col, int64_t ld, F f) {
+__device__ __forceinline__ void store_rows(RowStage<T, FN>& stage, T* out, int64_t row, int64_t rows, int col, int64_t ld, F f,
+                                           int lane) {
   constexpr int kVec = 16 / (int)sizeof(T), kRow = FN * 16 / kVec;
-  const int lane = threadIdx.x & 63;
 #pragma unroll
   for (int j = 0; j < FN; j++) {
     const f32x4 v = f(j);
@@ -200,7 +200,7 @@ __global__ __launch_bounds__(C::NT) void product_kernel(Products<T> all) {
     auto& stage = reinterpret_cast<RowStage<T, C::FN>*>(tile_lds<C>())[w];
 #pragma unroll
     for (int i = 0; i < C::FM; i++)
-      store_rows<T, C::FN>(stage, p.c, m + i * 16, p.M, n, p.N, [&](int j) { return acc[i][j]; });
+      store_rows<T, C::FN>(stage, p.c, m + i * 16, p.M, n, p.N, [&](int j) { return acc[i][j]; }, lane);
     return;
   }
   const int r = lane & 15, q = lane >> 4;
@@ -306,7 +306,7 @@ __global__ __launch_bounds__(C::NT) void gate_kernel(Gate<T> p) {
 #pragma unroll
         for (int e = 0; e < 4; e++) h[e] = act_value<T, act.value, false>(acc[i][2 * j][e], unused) * acc[i][2 * j + 1][e];
         return h;
-      });
+      }, threadIdx.x & 63);
   });
 }
 
@@ -338,6 +338,8 @@ __global__ __launch_bounds__(C::NT) void gate_backward_kernel(GateBackward<T> p)
   const int n = (int)n0 + (w % C::WN) * C::FN * 16;
   __syncthreads();   // the operands' LDS is free
   auto& stage = reinterpret_cast<RowStage<T, C::FN>*>(tile_lds<C>())[w];
+  int lane = threadIdx.x & 63;
+  asm volatile("" : "+v"(lane));   // made again here, not held in a register over the products
   with_act(p.act, [&](auto act) {
 #pragma unroll
     for (int i = 0; i < C::FM; i++) {
@@ -362,9 +364,9 @@ __global__ __launch_bounds__(C::NT) void gate_backward_kernel(GateBackward<T> p)
           acc[i][j][e] = d * a;
           g[j][e] = h;
         }
-      store_rows<T, C::FN>(stage, p.h, row, p.M, n, p.ldh, [&](int j) { return g[j]; });
-      store_rows<T, C::FN>(stage, p.dg, row, p.M, n, p.ldh, [&](int j) { return u[j]; });
-      store_rows<T, C::FN>(stage, p.du, row, p.M, n, p.ldh, [&](int j) { return acc[i][j]; });
+      store_rows<T, C::FN>(stage, p.h, row, p.M, n, p.ldh, [&](int j) { return g[j]; }, lane);
+      store_rows<T, C::FN>(stage, p.dg, row, p.M, n, p.ldh, [&](int j) { return u[j]; }, lane);
+      store_rows<T, C::FN>(stage, p.du, row, p.M, n, p.ldh, [&](int j) { return acc[i][j]; }, lane);
     }
   });
 }
