@@ -22,6 +22,7 @@ from __future__ import annotations
 
 import ctypes as ct
 import math
+from contextlib import contextmanager
 from dataclasses import dataclass
 from typing import Optional
 
@@ -117,7 +118,8 @@ class HashINGP:
     """The INGP attributes the baseline render reads (hash_encoder/modules.py):
     hash_encoding (a GridEncoder), gridrange, contract, active_levels, levels,
     level_dim and rgb_decode.  refiner: an optional blocks.GatedRefiner that
-    render() passes the composited features through before the MLP."""
+    render() passes the composited features through before the MLP, as in
+    evaluation (no dropout, no gradient): render() does not train it."""
 
     def __init__(self, encoding, mlp: NestMLP, gridrange, contract: bool = False, active_levels: Optional[int] = None,
                  refiner=None):
@@ -163,6 +165,20 @@ class HashINGP:
             x = (x + 2.0) * 0.25
         out = self.hash_encoding(x.reshape(-1, 3))
         return out.view(*x.shape[:-1], out.shape[-1])
+
+
+@contextmanager
+def _evaluating(module: torch.nn.Module):
+    """No gradients, and the module in evaluation; its parts' modes come back as they were."""
+    training = [m for m in module.modules() if m.training]
+    for m in training:
+        m.training = False
+    try:
+        with torch.no_grad():
+            yield
+    finally:
+        for m in training:
+            m.training = True
 
 
 @dataclass
@@ -304,7 +320,11 @@ def render(viewpoint_camera, pc, pipe, bg_color: torch.Tensor, scaling_modifier=
     else:
         bg = bg_color if float(bg_color.sum()) > 0 else None
         refiner = getattr(ingp, "refiner", None)
-        decoded = rendered_image if refiner is None else refiner.refine_image(rendered_image.detach())
+        if refiner is None:
+            decoded = rendered_image
+        else:
+            with _evaluating(refiner):
+                decoded = refiner.refine_image(rendered_image.detach())
         rgb = ingp.mlp_rgb.decode_image(decoded, view_ray_matrix(viewpoint_camera), alpha=render_alpha, bg=bg)
     rets["render"] = rgb
 
