@@ -118,8 +118,9 @@ class HashINGP:
     """The INGP attributes the baseline render reads (hash_encoder/modules.py):
     hash_encoding (a GridEncoder), gridrange, contract, active_levels, levels,
     level_dim and rgb_decode.  refiner: an optional blocks.GatedRefiner that
-    render() passes the composited features through before the MLP, as in
-    evaluation (no dropout, no gradient): render() does not train it."""
+    features pass through before the MLP, the composited ones of render() as
+    well as rgb_decode's, as in evaluation (no dropout, no gradient: neither
+    trains it).  The modes that decode no features do not use it."""
 
     def __init__(self, encoding, mlp: NestMLP, gridrange, contract: bool = False, active_levels: Optional[int] = None,
                  refiner=None):
@@ -134,6 +135,9 @@ class HashINGP:
         self.active_levels = self.levels if active_levels is None else active_levels
 
     def rgb_decode(self, features, ray_unit):
+        if self.refiner is not None:
+            with _evaluating(self.refiner):
+                features = self.refiner(features)
         return self.mlp_rgb.rgb_decode(features, ray_unit)
 
     def __call__(self, points_3D: torch.Tensor, with_xyz: bool = False) -> torch.Tensor:

@@ -53,3 +53,39 @@ def test_render_keeps_nothing_for_a_backward_pass():
     out = frame()
     assert torch.cuda.max_memory_allocated() <= least
     assert not out["render"].requires_grad
+
+
+@pytest.mark.parametrize("mode", ["diffuse_ngp", "diffuse_offset"])
+def test_deferred_modes_decode_through_the_refiner(mode):
+    import numpy as np
+    from nest_splat import renderer
+    from scenes import scene
+    sc = scene("shell_small")
+    _, ingp = renderer.scene_to_device(sc, DEV)
+    seen = {}
+
+    class Watched(renderer.HashINGP):
+        def __call__(self, points, with_xyz=False):
+            seen["features"] = super().__call__(points, with_xyz)
+            return seen["features"]
+
+        def rgb_decode(self, features, ray_unit):
+            seen["rays"] = ray_unit
+            return super().rgb_decode(features, ray_unit)
+
+    ingp.__class__ = Watched
+    arrays = (sc.means, sc.scales, sc.rotations, sc.opacity, sc.ap_level, sc.homotrans,
+              np.random.default_rng(7).normal(0, 0.5, (sc.spec.P, 16, 3)).astype(np.float32))
+    means, scales, rotations, opacity, ap, homotrans, shs = (torch.from_numpy(np.ascontiguousarray(a)).to(DEV) for a in arrays)
+    pc = renderer.SplatModel(means, scales, rotations, opacity, ap, homotrans=homotrans, features=shs, active_sh_degree=3)
+
+    def frame():
+        return renderer.render(sc.cameras[0], pc, renderer.Pipe(), torch.zeros(3, device=DEV), ingp=ingp, mode=mode, with_surface=False)
+
+    plain = frame()["ngp_rgb"]
+    ingp.refiner = trained(sc.spec.C, dtype="f32")
+    got = frame()
+    with torch.no_grad():
+        refined = ingp.refiner.eval()(seen["features"])
+    want = ingp.mlp_rgb.rgb_decode(refined, seen["rays"]).view(*got["ngp_rgb"].shape[1:], 3).permute(2, 0, 1) * (got["allmap"][1:2] > 0)
+    assert torch.equal(got["ngp_rgb"], want) and not torch.equal(want, plain)
