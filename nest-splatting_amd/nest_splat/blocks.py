@@ -265,8 +265,9 @@ def gated_ffn_backward(dy: torch.Tensor, x: torch.Tensor, w_gate: torch.Tensor, 
 
 class _GatedFfn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, w_gate, w_up, w_down, activation):
-        y, kept = gated_ffn_forward(x, w_gate, w_up, w_down, activation, training=any(ctx.needs_input_grad))
+    def forward(ctx, x, w_gate, w_up, w_down, activation, recording):
+        # needs_input_grad is that of the tensors, whether or not gradients are recorded
+        y, kept = gated_ffn_forward(x, w_gate, w_up, w_down, activation, training=recording and any(ctx.needs_input_grad))
         ctx.save_for_backward(x, w_gate, w_up, w_down, kept)
         ctx.activation = activation
         return y
@@ -275,12 +276,12 @@ class _GatedFfn(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, dy):
         grads = gated_ffn_backward(dy, *ctx.saved_tensors, ctx.activation, ctx.needs_input_grad[:4])
-        return (*grads, None)
+        return (*grads, None, None)
 
 
 def gated_ffn(x, w_gate, w_up, w_down, activation: str = "silu") -> torch.Tensor:
     """gated_ffn_forward's y under autograd (x and the three weights)."""
-    return _GatedFfn.apply(x, w_gate, w_up, w_down, activation)
+    return _GatedFfn.apply(x, w_gate, w_up, w_down, activation, torch.is_grad_enabled())
 
 
 # ---- modules ----

@@ -114,3 +114,30 @@ def test_checkpointed_blocks_have_the_gradients_of_kept_ones(reentrant):
     else:
         got = grads(lambda: checkpoint(refiner, x, use_reentrant=False))
     assert all(torch.equal(g, w) for g, w in zip(got, want))
+
+
+class _Recorder:
+    """Stands in for the library: sizes and calls of the gated feed-forward block, on the CPU."""
+
+    def __init__(self, blocks, monkeypatch):
+        self.kept = []
+        monkeypatch.setattr(blocks, "gated_ffn_forward", self.forward)
+
+    def forward(self, x, w_gate, w_up, w_down, activation="silu", training=False):
+        self.kept.append(training)
+        return x @ w_down.t() if x.shape[-1] == w_down.shape[1] else x.new_zeros(x.shape[0], w_down.shape[0]), None
+
+
+@pytest.mark.parametrize("mode", [torch.no_grad, torch.inference_mode])
+def test_a_forward_without_gradients_keeps_nothing_for_them(monkeypatch, mode):
+    """Under no_grad a parameter still asks for its gradient, but there will be none."""
+    from nest_splat import blocks
+    seen = _Recorder(blocks, monkeypatch)
+    ffn = blocks.GatedFFN(8, 16, dtype="f32")
+    x = torch.zeros(4, 8)
+    with mode():
+        ffn(x)
+    blocks.gated_ffn(x, *(w.detach() for w in ffn.parameters()))
+    assert seen.kept == [False, False]
+    assert ffn(x).requires_grad
+    assert seen.kept[2]
