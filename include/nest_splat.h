@@ -609,7 +609,9 @@ int nest_dropout(int64_t n, int32_t dtype, const void *x, const void *residual, 
 /* y = (act(x Wg^T) * (x Wu^T)) Wd^T: x [rows, in_features], w_gate and w_up
  * [hidden, in_features], w_down [out_features, hidden], y [rows,
  * out_features], all of dtype.  Float32 results that an infinity enters may be
- * NaN. */
+ * NaN.  Sizes that take 2^32 threads or more at 512 a tile
+ * of 256 rows by 128 hidden or 256 other features, which no launch runs, are
+ * refused as unsupported (not the 16-bit rows of up to 128 features). */
 typedef struct nest_gated_ffn {
   uint32_t struct_size;
   int32_t dtype;

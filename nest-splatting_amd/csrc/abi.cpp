@@ -1419,6 +1419,8 @@ GatedLayout layout_of(const nest_gated_ffn* f, bool backward, bool alone) {
   return gated_layout(f->rows, f->in_features, f->hidden, f->out_features, f->dtype, backward, alone);
 }
 
+int too_many_tiles() { return fail(NEST_ERR_UNSUPPORTED, "rows by features take more tiles than one launch runs: split the rows"); }
+
 bool aligned16(std::initializer_list<const void*> ps) {
   for (const void* p : ps)
     if (reinterpret_cast<uintptr_t>(p) % 16) return false;
@@ -1520,6 +1522,7 @@ int nest_gated_ffn_sizes(const nest_gated_ffn* f, size_t* kept, size_t* forward_
                          size_t* backward_ws_alone) {
   if (int rc = check_gated(f); rc != NEST_OK) return rc;
   const GatedLayout fwd = layout_of(f, false, false);
+  if (!fwd.fits) return too_many_tiles();
   if (kept) *kept = fwd.kept_bytes;
   if (forward_ws) *forward_ws = fwd.bytes;
   if (backward_ws) *backward_ws = layout_of(f, true, false).bytes;
@@ -1531,7 +1534,9 @@ int nest_gated_ffn_forward(const nest_gated_ffn* f, void* y, void* kept, void* w
   if (int rc = check_gated(f); rc != NEST_OK) return rc;
   if (f->rows == 0) return NEST_OK;
   if (!f->x || !f->w_gate || !f->w_up || !f->w_down || !y) return fail(NEST_ERR_INVALID_ARGUMENT, "NULL tensor pointer");
-  const size_t need = layout_of(f, false, false).bytes;
+  const GatedLayout l = layout_of(f, false, false);
+  if (!l.fits) return too_many_tiles();
+  const size_t need = l.bytes;
   if (ws_bytes < need || (need && !ws)) return fail(NEST_ERR_WORKSPACE, "gated ffn workspace too small: %zu < %zu bytes", ws_bytes, need);
   if (!aligned16({f->x, f->w_gate, f->w_up, f->w_down, y, kept, ws})) return fail(NEST_ERR_INVALID_ARGUMENT, "gated ffn pointers must be 16-byte aligned");
   GatedParams p = gated_params(f);
@@ -1548,7 +1553,9 @@ int nest_gated_ffn_backward(const nest_gated_ffn* f, const void* dy, const void*
   if (!dx && !dw_gate && !dw_up && !dw_down) return NEST_OK;
   if (f->rows > 0) {
     if (!f->x || !f->w_gate || !f->w_up || !f->w_down || !dy) return fail(NEST_ERR_INVALID_ARGUMENT, "NULL tensor pointer");
-    const size_t need = layout_of(f, true, kept == nullptr).bytes;
+    const GatedLayout l = layout_of(f, true, kept == nullptr);
+    if (!l.fits) return too_many_tiles();
+    const size_t need = l.bytes;
     if (ws_bytes < need || (need && !ws)) return fail(NEST_ERR_WORKSPACE, "gated ffn workspace too small: %zu < %zu bytes", ws_bytes, need);
     if (!aligned16({f->x, f->w_gate, f->w_up, f->w_down, dy, kept, dx, dw_gate, dw_up, dw_down, ws}))
       return fail(NEST_ERR_INVALID_ARGUMENT, "gated ffn pointers must be 16-byte aligned");

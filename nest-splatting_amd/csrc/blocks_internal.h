@@ -61,10 +61,14 @@ struct GatedParams {
   void* ws;
 };
 
-// Tiles of side x side, k split over `splits` workgroups a tile.
+// Tiles of side x side, k split over `splits` workgroups a tile; side 0: no
+// tiles that one launch takes.
 struct TileChoice {
   int side, splits;
 };
+inline int64_t tiles_along(int64_t n, int side) { return (n + side - 1) / side; }
+constexpr int tile_threads(int side) { return side == 256 ? 512 : 256; }
+constexpr int64_t kMostThreads = ((int64_t)1 << 32) - 1;   // of a launch
 // Launches of up to this many workgroups of 64 x 64 tiles, two a CU, take four
 // LDS buffers (64 KB) for more loads in flight: forward of 128 rows, 2048 ->
 // 8192 bf16, 33 us instead of 39; 1000 rows, 512 -> 2048 f16, 26 instead of 29.
@@ -120,7 +124,8 @@ struct GatedLayout {
   int64_t ldx, ldh, ldy;
   size_t h, dg, du, kept, x, wg, wu, wd, dy, part;
   size_t bytes, kept_bytes;
-  TileChoice y, dx, dw;
+  TileChoice gate, gate_back, y, dx, dw;
+  bool fits;                  // in launches
   bool narrow;                // gated_narrow.h
   size_t dx_sum;              // of its backward: sums of dx between launches,
   int narrow_parts, narrow_slices;   // launches, and slices of 32 hidden features in each
@@ -128,7 +133,6 @@ struct GatedLayout {
   int narrow_groups;          // workgroups of its backward
 };
 GatedLayout gated_layout(int64_t rows, int in, int hidden, int out, int dtype, bool backward, bool alone);
-TileChoice choose_gate_tile(int64_t M, int64_t N, int64_t K, int es);
 hipError_t launch_gated_ffn(const GatedParams& p, hipStream_t s, bool backward);
 hipError_t gated_ffn_f32(const GatedParams& p, hipStream_t s, bool backward);
 hipError_t gated_ffn_f16(const GatedParams& p, hipStream_t s, bool backward);

@@ -20,7 +20,7 @@ hipError_t gated_forward(const GatedParams& p, hipStream_t s) {
   if (hipError_t e = pad_operands(p, l, ws, false, o, s); e != hipSuccess) return e;
   T* h = reinterpret_cast<T*>(ws + l.h);
   Gate<T> g{o.x, o.wg, o.wu, l.ldx, (int)p.rows, p.hidden, l.ldh, h, p.kept, p.activation, 0, 0};
-  if (hipError_t e = launch_gate(g, s); e != hipSuccess) return e;
+  if (hipError_t e = launch_gate(g, l.gate, s); e != hipSuccess) return e;
   Products<T> y{};
   y.n = 1;
   y.p[0] = {h, o.wd, nullptr, nullptr, l.ldh, l.ldh, (int)p.rows, p.out, l.ldh, static_cast<T*>(p.y)};
@@ -42,10 +42,10 @@ hipError_t gated_backward(const GatedParams& p, hipStream_t s) {
   if (alone) {
     kept = reinterpret_cast<float*>(ws + l.kept);
     Gate<T> g{o.x, o.wg, o.wu, l.ldx, (int)p.rows, p.hidden, l.ldh, nullptr, kept, p.activation, 0, 0};
-    if (hipError_t e = launch_gate(g, s); e != hipSuccess) return e;
+    if (hipError_t e = launch_gate(g, l.gate, s); e != hipSuccess) return e;
   }
   GateBackward<T> b{o.dy, o.wd, l.ldy, l.ldh, (int)p.rows, p.out, kept, h, dg, du, p.activation, 0, 0};
-  if (hipError_t e = launch_gate_backward(b, s); e != hipSuccess) return e;
+  if (hipError_t e = launch_gate_backward(b, l.gate_back, s); e != hipSuccess) return e;
   if (p.dx) {
     Products<T> q{};
     q.n = 1;

@@ -1,6 +1,8 @@
 // Gated feed-forward block: workspace layout, choice of tiles, dispatch.
 #include "blocks_internal.h"
 
+#include <cmath>
+
 namespace nest {
 namespace {
 
@@ -50,17 +52,18 @@ hipError_t launch_clear(void* p, size_t bytes, hipStream_t s) {
 // to 2048 features, 256 to 8192 hidden; half of them float32) the choice costs
 // 1% of a call on average (0.3% for float32), 24% at worst (calls of 20 us).
 TileChoice choose_tile(int n, const int64_t* M, const int64_t* N, int64_t K, int es, bool may_split) {
-  TileChoice best{64, 1};
-  double least = 1e30;
+  TileChoice best{};
+  double least = INFINITY;
   const int64_t steps = cdiv(K, 128 / es);
   for (int side = 256; side >= 64; side /= 2) {
     int64_t tiles = 0, size = 0;
     for (int i = 0; i < n; i++) {
-      tiles += cdiv(M[i], side) * cdiv(N[i], side);
+      tiles += tiles_along(M[i], side) * tiles_along(N[i], side);
       size += M[i] * N[i];
     }
     for (int splits = 1; splits <= (may_split ? 256 : 1); splits *= 2) {
       if (splits > 1 && steps < 4 * splits) break;   // at least four steps each
+      if (tiles * splits * tile_threads(side) > kMostThreads) break;
       double t = seconds(tiles * splits, cdiv(steps, splits), side, es);
       if (splits > 1) t += 4.5e-6 + 8.0 * (double)size * splits / 5e12;   // the partial sums' way to memory and back
       if (t < least) {
@@ -91,8 +94,6 @@ void narrow_parts(int ki, int hidden, int& parts, int& slices) {
   }
 }
 
-TileChoice choose_gate_tile(int64_t M, int64_t N, int64_t K, int es) { return choose_tile(1, &M, &N, K, es, false); }
-
 GatedLayout gated_layout(int64_t rows, int in, int hidden, int out, int dtype, bool back, bool alone) {
   GatedLayout l{};
   const int es = dtype == NEST_DTYPE_F32 ? 4 : 2, v = 16 / es;
@@ -108,6 +109,7 @@ GatedLayout gated_layout(int64_t rows, int in, int hidden, int out, int dtype, b
     return o;
   };
   l.narrow = narrow_rows(rows, in, out, es);
+  l.fits = true;
   if (l.narrow) {
     if (!back) return l;
     const int ki = ((in > out ? in : out) + 31) / 32;
@@ -133,11 +135,18 @@ GatedLayout gated_layout(int64_t rows, int in, int hidden, int out, int dtype, b
     for (int i = 0; i < n; i++) size += cdiv(M[i] * N[i], kJoinGroup) * kJoinGroup;
     if (size * t.splits * 4 > part) part = size * t.splits * 4;
   };
+  if (!back || alone) {
+    const int64_t M = rows, N = 2 * (int64_t)hidden;
+    l.gate = choose_tile(1, &M, &N, l.ldx, es, false);
+    l.fits = l.gate.side != 0;
+  }
   if (!back) {
     const int64_t M = rows, N = out;
     l.y = choose_tile(1, &M, &N, l.ldh, es, true);
     partial(l.y, 1, &M, &N);
+    l.fits &= l.y.side != 0;
   } else {
+    l.gate_back = choose_tile(1, &rows, &l.ldh, out, es, false);
     l.dg = take(rows * l.ldh * es);
     l.du = take(rows * l.ldh * es);
     const int64_t M = rows, N = in;
@@ -148,6 +157,7 @@ GatedLayout gated_layout(int64_t rows, int in, int hidden, int out, int dtype, b
     const int64_t WM[3] = {hidden, hidden, out}, WN[3] = {in, in, hidden};
     l.dw = choose_tile(3, WM, WN, rows, es, true);
     partial(l.dw, 3, WM, WN);
+    l.fits &= l.gate_back.side != 0 && l.dx.side != 0 && l.dw.side != 0;
     if (alone) l.kept = take(kept_bytes);
     if (l.ldy != out) l.dy = take(rows * l.ldy * es);
   }

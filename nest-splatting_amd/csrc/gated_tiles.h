@@ -410,8 +410,8 @@ template <typename T, bool kAK, bool kBK>
 hipError_t launch_products(Products<T>& all, TileChoice t, hipStream_t s) {
   int64_t tiles = 0, part = 0;
   for (int i = 0; i < all.n; i++) {
-    all.p[i].tiles_m = (all.p[i].M + t.side - 1) / t.side;
-    all.p[i].tiles_n = (all.p[i].N + t.side - 1) / t.side;
+    all.p[i].tiles_m = (int)tiles_along(all.p[i].M, t.side);
+    all.p[i].tiles_n = (int)tiles_along(all.p[i].N, t.side);
     all.p[i].part = part;
     tiles += (int64_t)all.p[i].tiles_m * all.p[i].tiles_n;
     part += ((int64_t)all.p[i].M * all.p[i].N + kJoinGroup - 1) / kJoinGroup * kJoinGroup;
@@ -422,6 +422,7 @@ hipError_t launch_products(Products<T>& all, TileChoice t, hipStream_t s) {
   const unsigned grid = (unsigned)(tiles * t.splits);
   with_tile(t.side, grid, [&](auto c) {
     typedef decltype(c) C;
+    static_assert(C::NT == tile_threads(C::BM), "");
     product_kernel<T, kAK, kBK, C><<<grid, C::NT, 0, s>>>(all);
   });
   if (t.splits > 1) {
@@ -432,10 +433,9 @@ hipError_t launch_products(Products<T>& all, TileChoice t, hipStream_t s) {
 }
 
 template <typename T>
-hipError_t launch_gate(Gate<T> p, hipStream_t s) {
-  const TileChoice t = choose_gate_tile(p.M, p.H * 2, p.ldx, sizeof(T));
-  p.tiles_m = (p.M + t.side - 1) / t.side;
-  p.tiles_n = (int)((p.ldh + t.side / 2 - 1) / (t.side / 2));
+hipError_t launch_gate(Gate<T> p, TileChoice t, hipStream_t s) {
+  p.tiles_m = (int)tiles_along(p.M, t.side);
+  p.tiles_n = (int)tiles_along(p.ldh, t.side / 2);
   const unsigned grid = (unsigned)((int64_t)p.tiles_m * p.tiles_n);
   with_tile(t.side, grid, [&](auto c) {
     typedef decltype(c) C;
@@ -445,10 +445,9 @@ hipError_t launch_gate(Gate<T> p, hipStream_t s) {
 }
 
 template <typename T>
-hipError_t launch_gate_backward(GateBackward<T> p, hipStream_t s) {
-  const TileChoice t = choose_gate_tile(p.M, (int)p.ldh, p.O, sizeof(T));
-  p.tiles_m = (p.M + t.side - 1) / t.side;
-  p.tiles_n = (int)((p.ldh + t.side - 1) / t.side);
+hipError_t launch_gate_backward(GateBackward<T> p, TileChoice t, hipStream_t s) {
+  p.tiles_m = (int)tiles_along(p.M, t.side);
+  p.tiles_n = (int)tiles_along(p.ldh, t.side);
   const unsigned grid = (unsigned)((int64_t)p.tiles_m * p.tiles_n);
   with_tile(t.side, grid, [&](auto c) {
     typedef decltype(c) C;
