@@ -44,7 +44,7 @@ hipError_t gated_backward(const GatedParams& p, hipStream_t s) {
     Gate<T> g{o.x, o.wg, o.wu, l.ldx, (int)p.rows, p.hidden, l.ldh, nullptr, kept, p.activation, 0, 0};
     if (hipError_t e = launch_gate(g, l.gate, s); e != hipSuccess) return e;
   }
-  GateBackward<T> b{o.dy, o.wd, l.ldy, l.ldh, (int)p.rows, p.out, kept, h, dg, du, p.activation, 0, 0};
+  GateBackward<T> b{o.dy, o.wd, l.ldy, l.ldh, (int)p.rows, p.out, p.hidden, kept, h, dg, du, p.activation, 0, 0};
   if (hipError_t e = launch_gate_backward(b, l.gate_back, s); e != hipSuccess) return e;
   if (p.dx) {
     Products<T> q{};

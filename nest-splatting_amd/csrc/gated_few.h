@@ -150,7 +150,7 @@ __global__ __launch_bounds__(64 * kFewWaves) void few_kernel(Few<T> p) {
           p.kept[at + 256] = v[1];
         }
         float unused;
-        v[0] = act_value<T, act.value, false>(v[0], unused) * v[1];
+        v[0] = c < p.N ? act_value<T, act.value, false>(v[0], unused) * v[1] : 0.0f;
         if (row < p.M) p.out[row * p.ldo + c] = from_f32<T>(v[0]);
       } else if (row < p.M && c < p.N) {
         p.out[row * p.ldo + c] = from_f32<T>(v[0]);

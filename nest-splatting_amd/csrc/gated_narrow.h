@@ -42,7 +42,9 @@ __device__ __forceinline__ typename Mma<T>::Frag load8(const T* p, int n) {
   return f;
 }
 
-template <typename T, int kAct, int KI, int RG>
+// kEnds: the hidden features end inside the last 32; h past the last one is
+// zero, where an infinity times its weights of zero would make the row NaN.
+template <typename T, int kAct, int KI, int RG, bool kEnds>
 __global__ __launch_bounds__(512, KI <= 2 ? 4 : 2) void narrow_forward_kernel(Narrow<T> p, int chunk) {
   typedef typename Mma<T>::Frag Frag;
   constexpr int FO = 2 * KI;
@@ -122,7 +124,9 @@ __global__ __launch_bounds__(512, KI <= 2 ? 4 : 2) void narrow_forward_kernel(Na
 #pragma unroll
           for (int e = 0; e < 8; e++) {
             float unused;
-            h[i][e] = from_f32<T>(act_value<T, kAct, false>(g[i][e >> 2][e & 3], unused) * u[i][e >> 2][e & 3]);
+            float v = act_value<T, kAct, false>(g[i][e >> 2][e & 3], unused) * u[i][e >> 2][e & 3];
+            if (kEnds && h0 + hc + q * 4 + (e & 3) + (e >> 2) * 16 >= p.hidden) v = 0.0f;
+            h[i][e] = from_f32<T>(v);
           }
 #pragma unroll
         for (int o = 0; o < FO; o++) {
@@ -164,7 +168,9 @@ hipError_t narrow_forward(const Narrow<T>& p, hipStream_t s) {
   const size_t lds = (size_t)narrow_lds(KI, chunk, waves).total * sizeof(T);
   const int64_t full = 256 * (lds <= 80 * 1024 ? 2 : 1);
   with_act(p.act, [&](auto act) {
-    narrow_forward_kernel<T, act.value, KI, RG><<<(unsigned)(tiles < full ? tiles : full), waves * 64, lds, s>>>(p, chunk);
+    const unsigned grid = (unsigned)(tiles < full ? tiles : full);
+    if (p.hidden % 32) narrow_forward_kernel<T, act.value, KI, RG, true><<<grid, waves * 64, lds, s>>>(p, chunk);
+    else narrow_forward_kernel<T, act.value, KI, RG, false><<<grid, waves * 64, lds, s>>>(p, chunk);
   });
   return hipGetLastError();
 }
@@ -258,7 +264,10 @@ struct Rows {
   }
 };
 
-template <typename T, int KI, int SL>
+// kEnds: the launch's hidden features end before its slices do.  dx sums over
+// all of them: dg and du past the last one are zero, where an infinity times
+// its weights of zero would make the row NaN.
+template <typename T, int KI, int SL, bool kEnds>
 __global__ __launch_bounds__(64 * narrow_back_waves(KI), KI <= 2 ? 2 : 1) void narrow_backward_kernel(NarrowBack<T> p) {
   typedef typename Mma<T>::Frag Frag;
   constexpr int kWaves = narrow_back_waves(KI), kGroups = kWaves / SL, kThreads = 64 * kWaves;
@@ -355,6 +364,14 @@ __global__ __launch_bounds__(64 * narrow_back_waves(KI), KI <= 2 ? 2 : 1) void n
             vh[b][i].v[e] = from_f32<T>(a * u[b][i][e]);
           }
     });
+    if constexpr (kEnds) {
+#pragma unroll
+      for (int b = 0; b < 2; b++)
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+          if (p.first + slice * 32 + b * 16 + q * 4 + e >= p.last)
+            vg[b][0].v[e] = vg[b][1].v[e] = vu[b][0].v[e] = vu[b][1].v[e] = (T)0.0f;
+    }
     auto put = [&](T* to, const Four<T> (&v)[2][2]) {
 #pragma unroll
       for (int b = 0; b < 2; b++)
@@ -498,9 +515,10 @@ hipError_t narrow_backward(const GatedParams& g, const GatedLayout& l, hipStream
                           static_cast<const T*>(g.w_down), static_cast<const T*>(g.dy), static_cast<T*>(g.dx),
                           reinterpret_cast<float*>(ws + l.dx_sum), reinterpret_cast<float*>(ws + l.part), g.rows, g.in, g.hidden, g.out,
                           g.activation, first, last};
-    narrow_backward_kernel<T, KI, SL><<<l.narrow_groups, 64 * narrow_back_waves(KI), m.total * sizeof(T), s>>>(p);
-    if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
     constexpr int H = SL * 32, D = KI * 32;
+    if (last - first < H) narrow_backward_kernel<T, KI, SL, true><<<l.narrow_groups, 64 * narrow_back_waves(KI), m.total * sizeof(T), s>>>(p);
+    else narrow_backward_kernel<T, KI, SL, false><<<l.narrow_groups, 64 * narrow_back_waves(KI), m.total * sizeof(T), s>>>(p);
+    if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
     if (g.dw_gate || g.dw_up || g.dw_down)
       narrow_join_kernel<T><<<3 * H * D / 32, 1024, 0, s>>>(p.part, l.narrow_groups, H, D, g.in, g.hidden, g.out, first, last,
                                                             static_cast<T*>(g.dw_gate), static_cast<T*>(g.dw_up), static_cast<T*>(g.dw_down));

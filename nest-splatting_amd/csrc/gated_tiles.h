@@ -106,6 +106,13 @@ __device__ __forceinline__ void store4(T* row, int n, int N, bool aligned, f32x4
   }
 }
 
+// Columns n .. n + 3, those from N on as zero.
+__device__ __forceinline__ f32x4 before(f32x4 v, int n, int N) {
+#pragma unroll
+  for (int e = 0; e < 4; e++) v[e] = n + e < N ? v[e] : 0.0f;
+  return v;
+}
+
 // 16 x 16-column fragments of a wave to row-major rows, through LDS of its own
 // so that a row's columns leave in 16-byte stores side by side.
 template <typename T, int FN>
@@ -263,7 +270,7 @@ struct Gate {
   const T *x, *wg, *wu;   // [M][ldx], [H][ldx]
   int64_t ldx;
   int M, H;
-  int64_t ldh;            // H rounded up to 16 bytes: the pad columns are written as zeros
+  int64_t ldh;            // H rounded up to 16 bytes: the pad columns are written as zeros, also in a row with an infinity
   T* h;                   // [M][ldh] or null
   float* kept;            // g and u, see kept_block; or null
   int act, tiles_m, tiles_n;
@@ -295,6 +302,7 @@ __global__ __launch_bounds__(C::NT) void gate_kernel(Gate<T> p) {
       }
   }
   if (!p.h) return;
+  const int lane = threadIdx.x & 63;
   __syncthreads();   // the operands' LDS is free
   auto& stage = reinterpret_cast<RowStage<T, C::FN / 2>*>(tile_lds<C>())[w];
   with_act(p.act, [&](auto act) {
@@ -305,8 +313,8 @@ __global__ __launch_bounds__(C::NT) void gate_kernel(Gate<T> p) {
         float unused;
 #pragma unroll
         for (int e = 0; e < 4; e++) h[e] = act_value<T, act.value, false>(acc[i][2 * j][e], unused) * acc[i][2 * j + 1][e];
-        return h;
-      }, threadIdx.x & 63);
+        return n + j * 16 + 16 > p.H ? before(h, n + j * 16 + (lane >> 4) * 4, p.H) : h;
+      }, lane);
   });
 }
 
@@ -316,9 +324,9 @@ template <typename T>
 struct GateBackward {
   const T *dy, *wd;       // [M][ldy], [O][ldh]
   int64_t ldy, ldh;
-  int M, O;
+  int M, O, H;
   float* kept;
-  T *h, *dg, *du;         // [M][ldh]
+  T *h, *dg, *du;         // [M][ldh]; the pad columns of dg and du are zeros
   int act, tiles_m, tiles_n;
 };
 
@@ -364,6 +372,13 @@ __global__ __launch_bounds__(C::NT) void gate_backward_kernel(GateBackward<T> p)
           acc[i][j][e] = d * a;
           g[j][e] = h;
         }
+      if (n + C::FN * 16 > p.H) {
+#pragma unroll
+        for (int j = 0; j < C::FN; j++) {
+          u[j] = before(u[j], n + j * 16 + (lane >> 4) * 4, p.H);
+          acc[i][j] = before(acc[i][j], n + j * 16 + (lane >> 4) * 4, p.H);
+        }
+      }
       store_rows<T, C::FN>(stage, p.h, row, p.M, n, p.ldh, [&](int j) { return g[j]; }, lane);
       store_rows<T, C::FN>(stage, p.dg, row, p.M, n, p.ldh, [&](int j) { return u[j]; }, lane);
       store_rows<T, C::FN>(stage, p.du, row, p.M, n, p.ldh, [&](int j) { return acc[i][j]; }, lane);

@@ -43,3 +43,31 @@ def test_float32_ends_of_the_range(B):
     y, _ = B.gated_ffn_forward(x, wg, wg * 0.75, wd, "relu")
     assert torch.isfinite(y).all()
     R.check(y, *R.ffn(x, wg, wg * 0.75, wd, "relu")["y"], "y at the ends of the range")
+
+
+def same_kind(got, want, what):
+    """Infinities and NaN where the formula has them, in 16 bits."""
+    got, want = got.double(), want.to(got.dtype).double()
+    assert torch.equal(torch.isnan(got), torch.isnan(want)), what
+    inf = torch.isinf(want)
+    assert torch.equal(torch.isinf(got), inf) and torch.equal(got[inf], want[inf]), what
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("size", [(70, 24, 20, 16), (300, 64, 100, 40), (200, 128, 300, 128), (3, 72, 77, 40), (16, 72, 75, 24),
+                                  (40, 136, 132, 72), (300, 200, 1001, 136)], ids=str)
+def test_infinities_with_hidden_features_that_end_inside_a_tile(B, size, dtype):
+    """Positive inputs and weights, so that the formula of a row with an infinity has no NaN; what a kernel adds to the hidden
+    features to fill a tile must not bring one in."""
+    rows, i, h, o = size
+    g = torch.Generator(device=DEV).manual_seed(5)
+    x, wg, wu, wd, dy = ((torch.rand(s, generator=g, device=DEV) * 0.1 + 0.01).to(dtype) for s in ((rows, i), (h, i), (h, i), (o, h), (rows, o)))
+    x[1, 3] = float("inf")
+    dy[2, 5] = float("inf")
+    ref = {k: v[0] for k, v in R.ffn(x, wg, wu, wd, "relu", dy).items()}
+    y, kept = B.gated_ffn_forward(x, wg, wu, wd, "relu", training=True)
+    same_kind(y, ref["y"], "y")
+    for k in (kept, None):
+        for name, v in zip(("dx", "dw_gate", "dw_up", "dw_down"), B.gated_ffn_backward(dy, x, wg, wu, wd, k, "relu")):
+            same_kind(v, ref[name], (name, k is not None))
+    assert torch.isinf(y[1]).all() and not torch.isnan(ref["dx"]).any()
