@@ -437,7 +437,9 @@ __global__ __launch_bounds__(64 * narrow_back_waves(KI), KI <= 2 ? 2 : 1) void n
     __syncthreads();   // the next x and dy are whole; dg and du are no longer read
   }
   // the groups' sums, in their order, through the LDS that the weights had
-  f32x4* const sums = reinterpret_cast<f32x4*>(narrow_mem) + slice * (6 * FI * 64) + lane;
+  int last_lane = threadIdx.x & 63;
+  asm volatile("" : "+v"(last_lane));   // made again here, not held in a register over the rows
+  f32x4* const sums = reinterpret_cast<f32x4*>(narrow_mem) + slice * (6 * FI * 64) + last_lane;
   for (int other = 1; other < kGroups; other++) {
     if (group == other) {
 #pragma unroll
@@ -471,10 +473,10 @@ __global__ __launch_bounds__(64 * narrow_back_waves(KI), KI <= 2 ? 2 : 1) void n
     for (int b = 0; b < 2; b++)
 #pragma unroll
       for (int e = 0; e < 4; e++) {
-        const int h = slice * 32 + b * 16 + q * 4 + e;
-        part[h * D + j * 16 + r] = dwg[b][j][e];
-        part[H * D + h * D + j * 16 + r] = dwu[b][j][e];
-        part[2 * H * D + (j * 16 + q * 4 + e) * H + slice * 32 + b * 16 + r] = dwd[j][b][e];
+        const int row4 = (last_lane >> 4) * 4 + e, col = last_lane & 15, h = slice * 32 + b * 16 + row4;
+        part[h * D + j * 16 + col] = dwg[b][j][e];
+        part[H * D + h * D + j * 16 + col] = dwu[b][j][e];
+        part[2 * H * D + (j * 16 + row4) * H + slice * 32 + b * 16 + col] = dwd[j][b][e];
       }
 }
 

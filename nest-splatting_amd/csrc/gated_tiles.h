@@ -198,7 +198,9 @@ __global__ __launch_bounds__(C::NT) void product_kernel(Products<T> all) {
   la.init(p.a + ka, p.lda, m0, kAK ? p.M : p.lda);
   lb.init(p.b + kb, p.ldb, n0, kBK ? p.N : p.ldb);
   tile_product<T, kAK, kBK, C>(la, lb, k, a2, b2, acc);   // a split past the end has k <= 0: it loads zeros
-  const int lane = threadIdx.x & 63, w = wave_id();
+  int lane = threadIdx.x & 63;
+  asm volatile("" : "+v"(lane));   // made again here, not held in a register over the products
+  const int w = wave_id();
   const int64_t m = m0 + (w / C::WN) * C::FM * 16;
   const int n = (int)n0 + (w % C::WN) * C::FN * 16;
   constexpr int kVec = 16 / (int)sizeof(T);

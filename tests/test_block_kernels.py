@@ -79,3 +79,19 @@ def test_waits_of_the_products(objects):
                     waited = None
             seen += 1
     assert seen >= 3 * 4 * 5   # types, tiles, products
+
+
+def test_no_kernel_spills(objects):
+    """Registers hold all that the kernels of these files keep: none has scratch memory."""
+    seen = 0
+    for path, symbols in objects:
+        if not any(re.search(PRODUCTS + r"|layer_norm|dropout_kernel|narrow_|few_kernel", s) for s in symbols):
+            continue
+        notes = subprocess.run([TOOLS["readelf"], "--notes", str(path)], check=True, capture_output=True, text=True).stdout
+        for k in re.split(r"\n  - \.", notes)[1:]:
+            name = re.search(r"\.name: +(_Z\w+)", k)
+            if name:
+                seen += 1
+                spilled = [int(v) for v in re.findall(r"\.(?:private_segment_fixed_size|vgpr_spill_count): +(\d+)", k)]
+                assert len(spilled) == 2 and not any(spilled), (name.group(1), spilled)
+    assert seen > 100
