@@ -48,9 +48,10 @@ hipError_t launch_clear(void* p, size_t bytes, hipStream_t s) {
 }  // namespace
 
 // Tiles for up to three products that share a launch and K.  Against every
-// tile and split timed at 200 sizes of all five launches (33 to 8192 rows, 160
+// tile and split timed at 140 sizes of all five launches (33 to 8192 rows, 160
 // to 2048 features, 256 to 8192 hidden; half of them float32) the choice costs
-// 1% of a call on average (0.3% for float32), 24% at worst (calls of 20 us).
+// 0.7% of a call on average, 18% at worst (calls of 20 us); rates fitted to
+// those timings would save 0.2%.
 TileChoice choose_tile(int n, const int64_t* M, const int64_t* N, int64_t K, int es, bool may_split) {
   TileChoice best{};
   double least = INFINITY;
