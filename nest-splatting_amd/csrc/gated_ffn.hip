@@ -76,10 +76,6 @@ TileChoice choose_tile(int n, const int64_t* M, const int64_t* N, int64_t K, int
   return best;
 }
 
-// Whether whole rows stay on the chip (gated_narrow.h): 16-bit rows of at most
-// 128 features.
-bool narrow_rows(int64_t rows, int in, int out, int es) { return es == 2 && in <= 128 && out <= 128 && rows >= 64; }
-
 // Launches of the narrow backward and slices of 32 hidden features in each: the
 // least slices in all, then the fewest launches.
 void narrow_parts(int ki, int hidden, int& parts, int& slices) {
@@ -93,6 +89,34 @@ void narrow_parts(int ki, int hidden, int& parts, int& slices) {
       slices = s;
     }
   }
+}
+
+// Whether whole rows stay on the chip (gated_narrow.h): 16-bit rows of at most
+// 128 features, where a forward and backward take less time so than in tiles.
+//
+// Estimated in us from 104 sizes of 32, 64 and 128 features, 128 to 8192 hidden
+// and 64 to 640,000 rows, bf16.  Narrow: the weights pass through LDS again for
+// every 65536 rows of a forward; a backward takes a launch and a join of its
+// workgroups' sums for each part of the hidden features, and each further turn
+// of its workgroups.  Tiles: calls of 36 us, or h, g, u and their gradients
+// through memory.  A step, narrow and in tiles: 640,000 x 64, 128 179 and 680;
+// 65,536 x 64, 1024 254 and 512; 8192 x 64, 512 103 and 49; 8192 x 128, 512 205
+// and 55; 64 x 128, 8192 2317 and 42.  The choice costs 0.3% of a step on
+// average and 11% at worst; narrow wherever the types and features allow it
+// would cost 108%.
+bool narrow_rows(int64_t rows, int in, int hidden, int out, int es) {
+  if (es != 2 || in > 128 || out > 128 || rows < 64) return false;
+  static constexpr double kHidden[4] = {0.028, 0.047, 0.075, 0.1};   // forward, a hidden feature
+  static constexpr double kLaunch[4] = {9.5, 13.5, 17.0, 21.0}, kTurn[4] = {2.0, 2.6, 3.5, 4.3};
+  const int ki = ((in > out ? in : out) + 31) / 32;
+  int parts, slices;
+  narrow_parts(ki, hidden, parts, slices);
+  const int64_t need = cdiv(rows, 32 * narrow_back_lds(ki, slices).groups), groups = need < 256 ? need : 256;
+  const double sums = (double)groups * 3 * slices * 32 * ki * 32 * 4;   // bytes, written and read
+  const double forward = hidden * kHidden[ki - 1] * (double)cdiv(rows, 65536);
+  const double backward = parts * (kLaunch[ki - 1] + 2.0 * sums / 4.2e6 + (double)(cdiv(need, 256) - 1) * kTurn[ki - 1]);
+  const double tiles = 8e-6 * (double)rows * hidden;
+  return (forward > 9.0 ? forward : 9.0) + (backward > 19.0 ? backward : 19.0) < (tiles > 36.0 ? tiles : 36.0);
 }
 
 GatedLayout gated_layout(int64_t rows, int in, int hidden, int out, int dtype, bool back, bool alone) {
@@ -109,7 +133,7 @@ GatedLayout gated_layout(int64_t rows, int in, int hidden, int out, int dtype, b
     at = (at + (size_t)bytes + 255) / 256 * 256;
     return o;
   };
-  l.narrow = narrow_rows(rows, in, out, es);
+  l.narrow = narrow_rows(rows, in, hidden, out, es);
   l.fits = true;
   if (l.narrow) {
     if (!back) return l;
