@@ -572,8 +572,9 @@ int nest_rvq_decode_batch(int32_t n, const nest_rvq_attr *attrs, void *stream);
  * colour head, forward and backward.  dtype is that of x, y and their
  * gradients (F32, F16 or BF16); rows are contiguous and row-major, with any
  * row length and any alignment of the element type.  Sums are float32, each
- * result is rounded once.  The pointers of nest_gated_ffn_* are multiples of
- * 16 bytes. */
+ * result is rounded once (nest_gated_ffn_* round their intermediate operands
+ * too, see there).  The pointers of nest_gated_ffn_* are multiples of 16
+ * bytes. */
 
 /* y = (x - mean) rstd w + b over each row of x [rows, cols], rstd =
  * 1/sqrt(var + eps) with the variance about the mean, divided by cols.
@@ -608,10 +609,14 @@ int nest_dropout(int64_t n, int32_t dtype, const void *x, const void *residual, 
 
 /* y = (act(x Wg^T) * (x Wu^T)) Wd^T: x [rows, in_features], w_gate and w_up
  * [hidden, in_features], w_down [out_features, hidden], y [rows,
- * out_features], all of dtype.  Float32 results that an infinity enters may be
- * NaN.  Sizes that take 2^32 threads or more at 512 a tile
- * of 256 rows by 128 hidden or 256 other features, which no launch runs, are
- * refused as unsupported (not the 16-bit rows of up to 128 features). */
+ * out_features], all of dtype.  h = act(g) u, and dg and du in the backward,
+ * are rounded to dtype as operands of the next product: 16-bit results are off
+ * by about 1.4 times what one rounding makes, and in F16 a value of theirs past
+ * 65504 makes the results that it enters infinite or NaN.  Float32 products
+ * leave out at most 2^-24 of each; results that an infinity enters may be NaN.
+ * Sizes that would take 2^32 threads, at 512 a tile of 256 rows by 128 hidden
+ * or 256 other features, are more than a launch runs and refused as
+ * unsupported. */
 typedef struct nest_gated_ffn {
   uint32_t struct_size;
   int32_t dtype;

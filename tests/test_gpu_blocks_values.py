@@ -71,3 +71,25 @@ def test_infinities_with_hidden_features_that_end_inside_a_tile(B, size, dtype):
         for name, v in zip(("dx", "dw_gate", "dw_up", "dw_down"), B.gated_ffn_backward(dy, x, wg, wu, wd, k, "relu")):
             same_kind(v, ref[name], (name, k is not None))
     assert torch.isinf(y[1]).all() and not torch.isnan(ref["dx"]).any()
+
+
+@pytest.mark.parametrize("size", [(4, 64, 128, 64), (16, 72, 200, 40), (300, 64, 128, 64), (300, 100, 90, 128), (150, 200, 520, 136)], ids=str)
+def test_float16_past_its_range_is_seen(B, size):
+    """h = act(g) u is handed on in the inputs' type: past 65504 the rows it enters are infinite or NaN, though the formula's y
+    would fit, never a finite number that is wrong; other rows are as they were, and bfloat16 has the range."""
+    rows, i, h, o = size
+    x, wg, wu, wd = (torch.rand(s, generator=torch.Generator(device=DEV).manual_seed(7), device=DEV) for s in ((rows, i), (h, i), (h, i), (o, h)))
+    x, wd = x * 0.1, wd * 2.0 ** -10
+    half = [t.half() for t in (x, wg, wu, wd)]
+    clean = B.gated_ffn_forward(*half, "relu")[0]
+    assert torch.isfinite(clean).all()
+    big = torch.ones(rows, dtype=torch.bool, device=DEV)
+    big[[0, rows - 2]] = False
+    x[~big] = 800.0 / i
+    half[0] = x.half()
+    want = R.ffn(*half, "relu")["y"][0][~big]
+    y = B.gated_ffn_forward(*half, "relu")[0]
+    assert (want < 65504).all() and (want / wd.half().double().sum(1) > 65504).all()
+    assert torch.equal(y[big], clean[big]) and not torch.isfinite(y[~big]).any()
+    bf = [t.bfloat16() for t in (x, wg, wu, wd)]
+    R.check(B.gated_ffn_forward(*bf, "relu")[0], *R.ffn(*bf, "relu")["y"], "y of bfloat16")
