@@ -18,8 +18,8 @@
 // first (pad_kernel), so that the tiles have one way to load.
 //
 // Measured, 8192 rows, 2048 -> 8192, bf16: gate 525 us (550 GFLOP, 0.67 GB
-// written), y 243, dg, du and h 380 (275 GFLOP, 0.94 GB), dx 430, the weight
-// gradients 690: bound by the products (tile_gemm.h).
+// written), y 235, dg, du and h 385 (275 GFLOP, 0.94 GB), dx 435, the weight
+// gradients 720: bound by the products (tile_gemm.h).
 #pragma once
 
 #include "blocks_internal.h"

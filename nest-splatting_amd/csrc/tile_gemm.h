@@ -26,14 +26,14 @@
 // zero.  k past the end is outside in both operands (or a zero of one's row
 // padding), so nothing an operand does not hold is multiplied.
 //
-// Measured: 8192 x 2048 x 8192 bf16 1130 TFLOP/s, 8192 x 2048 x 16384 1210,
+// Measured: 8192 x 2048 x 8192 bf16 1170 TFLOP/s, 8192 x 2048 x 16384 1260,
 // where the library's 8192^3 product reaches 1395 on this card; the matrix
-// cores are busy 54 to 63% of the cycles, at a clock of 1.9 GHz, without LDS
-// bank conflicts; the rest is the barrier and the wait for loads that two
-// buffers leave.  float32 4096 x 2048, 4096: 216 TFLOP/s, 155 the library's
-// product; that is 1300 of the parts' products, and in 64 x 64 tiles, whose
-// fragments are cut four times for four products, the vector ALU is busy 0.86
-// of the cycles and 150 TFLOP/s come out.
+// cores are busy 54 to 67% of the cycles, at a clock of 1.7 to 1.9 GHz, without
+// LDS bank conflicts; the rest is the barrier and the wait for loads that two
+// buffers leave.  float32 4096 x 2048, 4096: 202 TFLOP/s, 155 the library's
+// product; that is 1210 of the parts' products, and in 64 x 64 tiles, whose
+// fragments are cut four times for four products, the vector ALU is busy 0.64 to
+// 0.85 of the cycles and 125 TFLOP/s come out.
 #pragma once
 
 #include "vec_io.h"
