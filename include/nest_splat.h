@@ -613,7 +613,8 @@ int nest_dropout(int64_t n, int32_t dtype, const void *x, const void *residual, 
  * are rounded to dtype as operands of the next product: 16-bit results are off
  * by about 1.4 times what one rounding makes, and in F16 a value of theirs past
  * 65504 makes the results that it enters infinite or NaN.  Float32 products
- * leave out at most 2^-24 of each; results that an infinity enters may be NaN.
+ * leave out at most 2^-24 of each (operands below 2^-110 keep their bits down
+ * to 2^-133); results that an infinity enters may be NaN.
  * Sizes that would take 2^32 threads, at 512 a tile of 256 rows by 128 hidden
  * or 256 other features, are more than a launch runs and refused as
  * unsupported. */

@@ -19,8 +19,8 @@ rounds what its first products hand to its second ones, h = act(g) u and in
 the backward pass dg and du, to the type: in 16 bits its results are off by
 about 1.4 times what one rounding makes, and in float16 an h, dg or du past
 65504 makes the results that it enters infinite or NaN.  Its float32 products
-leave out at most 2^-24 of each, and a float32 result that an infinity enters
-may be NaN.  Tensors that are not contiguous are copied first.
+leave out at most 2^-24 of each (operands below 2^-110 keep their bits down to
+2^-133), and a float32 result that an infinity enters may be NaN.  Tensors that are not contiguous are copied first.
 Every call is ordered on the current
 stream of the tensors' device.  Gradients of gradients are not available.
 """

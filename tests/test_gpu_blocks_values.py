@@ -93,3 +93,16 @@ def test_float16_past_its_range_is_seen(B, size):
     assert torch.equal(y[big], clean[big]) and not torch.isfinite(y[~big]).any()
     bf = [t.bfloat16() for t in (x, wg, wu, wd)]
     R.check(B.gated_ffn_forward(*bf, "relu")[0], *R.ffn(*bf, "relu")["y"], "y of bfloat16")
+
+
+@pytest.mark.parametrize("e", [0, 60, 100, 109, 112, 118, 126])
+def test_float32_products_of_small_numbers(B, e):
+    """x of 2^-e against weights of 2^e: the bound of one term, and past 2^-110, where x's last part ends below the smallest
+    bfloat16, half of that, 2^-134, for x in each of g and u."""
+    n = 128
+    g = torch.Generator().manual_seed(4)
+    x, w = ((1.0 + torch.rand(n, 1, generator=g)).to(DEV) * 2.0 ** s for s in (-e, e))
+    y, _ = B.gated_ffn_forward(x, w, torch.full_like(w, 2.0 ** e), torch.eye(n, device=DEV), "relu")
+    want = (x.double() @ w.double().T) * (x.double() * 2.0 ** e)
+    off = ((y.double() - want) / want).abs()
+    assert float(off.max()) <= 4.25 * U + 2 * 2.0 ** (e - 134)
