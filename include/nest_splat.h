@@ -33,7 +33,7 @@
 extern "C" {
 #endif
 
-#define NEST_ABI_VERSION 19
+#define NEST_ABI_VERSION 20
 
 #define NEST_OK 0
 #define NEST_ERR_INVALID_ARGUMENT (-1)
@@ -648,6 +648,107 @@ int nest_gated_ffn_forward(const nest_gated_ffn *f, void *y, void *kept, void *w
  * Sums run in a fixed order: results repeat bit for bit. */
 int nest_gated_ffn_backward(const nest_gated_ffn *f, const void *dy, const void *kept, void *dx, void *dw_gate,
                             void *dw_up, void *dw_down, void *ws, size_t ws_bytes, void *stream);
+
+/* ---- Operators of a residual block conditioned on the view (no reference
+ * counterpart) ----
+ * A dense layer with its bias, activation and residual in the epilogue, rows
+ * held in 8 bits for its backward, the residual stream between two norms, and
+ * an embedding of each row's view.  As above: dtype is that of the rows and
+ * their gradients, rows are contiguous, sums are float32 and run in a fixed
+ * order (results repeat bit for bit), and each result is rounded once.  The
+ * pointers of nest_linear_* are multiples of 16 bytes. */
+
+#define NEST_ACT_NONE (-1)
+
+/* y = act(x W^T + b) + residual: x [rows, in_features], weight [out_features,
+ * in_features], bias [out_features] or NULL, residual [rows, out_features] or
+ * NULL, all of dtype.  A training step keeps act'(x W^T + b): one byte an
+ * element for relu, else two (four for F32), and with save8 one (two for F32),
+ * in steps of 1/200 (1/26000).  The backward rounds dz = dy act' to dtype as
+ * operand of its products: in 16 bits dx and dweight are off by about 1.4
+ * times what one rounding makes.  Float32 products leave out at most 2^-24 of
+ * each, as nest_gated_ffn_* do, and give NaN where an infinity enters.  Sizes
+ * that would take 2^32 threads are refused as unsupported. */
+typedef struct nest_linear {
+  uint32_t struct_size;
+  int32_t dtype;
+  int32_t activation;   /* NEST_ACT_* */
+  int32_t save8;
+  int32_t in_features;
+  int32_t out_features;
+  int64_t rows;
+  const void *x;
+  const void *weight;
+  const void *bias;
+  const void *residual;
+} nest_linear;
+
+/* Bytes the calls below need, each may be 0 and each pointer may be NULL: the
+ * slopes a training forward leaves for the backward; the workspaces of a
+ * forward, of a backward, and of a backward whose x is given in 8 bits.  Host
+ * only. */
+int nest_linear_sizes(const nest_linear *f, size_t *kept, size_t *forward_ws, size_t *backward_ws,
+                      size_t *backward_ws_packed);
+
+/* kept: NULL, or the array of that size a training step hands on. */
+int nest_linear_forward(const nest_linear *f, void *y, void *kept, void *ws, size_t ws_bytes, void *stream);
+
+/* dx [rows, in_features], dweight and dbias (each NULL where it is not wanted)
+ * are overwritten; with no rows dweight and dbias are zero.  kept: what the
+ * forward left (NULL only without an activation).  codes and steps: x as
+ * nest_pack8 left it, in place of f->x; or both NULL.  The residual's gradient
+ * is dy. */
+int nest_linear_backward(const nest_linear *f, const void *dy, const void *kept, const int8_t *codes,
+                         const uint8_t *steps, void *dx, void *dweight, void *dbias, void *ws, size_t ws_bytes,
+                         void *stream);
+
+/* Rows of x [rows, cols] in 8 bits: codes [rows, cols] and one step for each
+ * 32 values of a row (the last may be fewer), steps [rows, ceil(cols / 32)].
+ * With e = max(floor(log2(largest magnitude of the 32)), -126), the step is
+ * 2^(e - 6), held as e + 126; a code is x over the step to the nearest (halves
+ * to even), clamped to -127..127.  A step held as 255: an infinity or a NaN
+ * among the 32, which all come back as NaN. */
+int nest_pack8(int64_t rows, int32_t cols, int32_t dtype, const void *x, int8_t *codes, uint8_t *steps,
+               void *stream);
+int nest_unpack8(int64_t rows, int32_t cols, int32_t dtype, const int8_t *codes, const uint8_t *steps, void *x,
+                 void *stream);
+
+/* The residual stream between two root-mean-square norms, over rows of cols
+ * <= 8192 values:
+ *   t = h / sqrt(mean(h^2) + eps) * post   (post NULL: t = h)
+ *   r = scale x + gate t                   (gate NULL: 1; h NULL: r is x, is not
+ *                                           written, and scale is 1)
+ *   y = r / sqrt(mean(r^2) + eps) * pre    (pre NULL: no y)
+ * y is the norm of r as it is stored.  gate is [gates, cols]; rows / gates
+ * consecutive rows share one (gates divides rows).  gate, post and pre are of
+ * param_dtype: F32 or dtype.  rstd_post and rstd_pre [rows] float32 receive
+ * what the backward needs (either may be NULL). */
+int nest_residual_norm(int64_t rows, int32_t cols, int32_t dtype, int32_t param_dtype, const void *x, const void *h,
+                       const void *gate, int64_t gates, const void *post, const void *pre, float scale, float eps,
+                       void *r, void *y, float *rstd_post, float *rstd_pre, void *stream);
+
+/* Gradients of nest_residual_norm from dr and dy (NULL: zero), with the r it
+ * stored (x where h is NULL): dx, dh (with h), dgate (with gate), dpost and
+ * dpre are overwritten; with no rows the parameters' gradients are zero. */
+size_t nest_residual_norm_backward_workspace_size(int64_t rows, int32_t cols, int32_t dtype, int64_t gates);
+int nest_residual_norm_backward(int64_t rows, int32_t cols, int32_t dtype, int32_t param_dtype, const void *dr,
+                                const void *dy, const void *r, const void *h, const void *gate, int64_t gates,
+                                const void *post, const void *pre, float scale, const float *rstd_post,
+                                const float *rstd_pre, void *dx, void *dh, void *dgate, void *dpost, void *dpre,
+                                void *ws, size_t ws_bytes, void *stream);
+
+/* y[i] = residual[i] + scale * table[ids[i]] (residual NULL: 0): ids [rows],
+ * int64 with wide_ids and int32 without; table [table_rows, cols].  An id
+ * outside [0, table_rows) adds nothing.  y may be residual itself. */
+int nest_embedding(int64_t rows, int32_t cols, int64_t table_rows, int32_t dtype, const void *ids, int32_t wide_ids,
+                   const void *table, float scale, const void *residual, void *y, void *stream);
+
+/* dtable[v] = scale * sum of dy[i] over ids[i] == v, in the order of a stable
+ * sort; every row is written.  The residual's gradient is dy. */
+size_t nest_embedding_backward_workspace_size(int64_t rows, int32_t cols, int64_t table_rows, int32_t dtype);
+int nest_embedding_backward(int64_t rows, int32_t cols, int64_t table_rows, int32_t dtype, const void *ids,
+                            int32_t wide_ids, const void *dy, float scale, void *dtable, void *ws, size_t ws_bytes,
+                            void *stream);
 
 #ifdef __cplusplus
 }

@@ -25,7 +25,8 @@ INCLUDE = os.path.join(os.path.dirname(HERE), "include")
 
 SOURCES = ["abi.cpp", "preprocess.hip", "binning.hip", "render.hip", "backward.hip", "grid_encode.hip", "mlp.hip",
            "rvq.hip", "surface.hip", "layer_norm.hip", "dropout.hip", "gated_ffn.hip",
-           "gated_ffn_f32.hip", "gated_ffn_f16.hip", "gated_ffn_bf16.hip"]
+           "gated_ffn_f32.hip", "gated_ffn_f16.hip", "gated_ffn_bf16.hip", "linear.hip", "linear_f32.hip",
+           "linear_f16.hip", "linear_bf16.hip", "pack8.hip", "residual_norm.hip", "embedding.hip"]
 
 HIPCC = shutil.which("hipcc") or "/opt/rocm/bin/hipcc"
 ARCH = os.environ.get("NEST_OFFLOAD_ARCH", "gfx950")

@@ -21,7 +21,9 @@
 
 #include "../../include/nest_splat.h"
 #include "blocks_internal.h"
+#include "residual_internal.h"
 #include "nest_internal.h"
+#include "residual_internal.h"
 
 using namespace nest;
 
@@ -1570,6 +1572,256 @@ int nest_gated_ffn_backward(const nest_gated_ffn* f, const void* dy, const void*
   p.ws = ws;
   hipError_t e = launch_gated_ffn(p, static_cast<hipStream_t>(stream), true);
   return e == hipSuccess ? NEST_OK : hip_fail(e, "gated ffn backward");
+}
+
+// ---- operators of a residual block ----
+
+namespace {
+
+int check_rows(int64_t rows, int32_t cols, int32_t dtype, int32_t most) {
+  if (rows < 0 || rows >= kMaxRows) return fail(NEST_ERR_INVALID_ARGUMENT, "rows must be in [0, 2^31) (got %lld)", (long long)rows);
+  if (cols < 1 || cols > most) return fail(NEST_ERR_INVALID_ARGUMENT, "cols must be in [1, %d] (got %d)", most, cols);
+  if (!element_type(dtype)) return fail(NEST_ERR_UNSUPPORTED, "dtype must be float32, float16 or bfloat16");
+  return NEST_OK;
+}
+
+int check_linear(const nest_linear* f) {
+  if (!f || f->struct_size != sizeof(nest_linear)) return fail(NEST_ERR_INVALID_ARGUMENT, "nest_linear missing or struct_size mismatch");
+  if (f->rows < 0 || f->rows >= kMaxRows) return fail(NEST_ERR_INVALID_ARGUMENT, "rows must be in [0, 2^31) (got %lld)", (long long)f->rows);
+  const int32_t sides[2] = {f->in_features, f->out_features};
+  for (int32_t v : sides)
+    if (v < 1 || v > kMaxFeatures) return fail(NEST_ERR_INVALID_ARGUMENT, "in_features and out_features must be in [1, %d] (got %d)", kMaxFeatures, v);
+  if (!element_type(f->dtype)) return fail(NEST_ERR_UNSUPPORTED, "dtype must be float32, float16 or bfloat16");
+  if (f->activation != NEST_ACT_NONE && f->activation != NEST_ACT_RELU && f->activation != NEST_ACT_SILU && f->activation != NEST_ACT_GELU)
+    return fail(NEST_ERR_UNSUPPORTED, "activation must be none, relu, silu or gelu");
+  return NEST_OK;
+}
+
+LinearParams linear_params(const nest_linear* f) {
+  LinearParams p{};
+  p.rows = f->rows;
+  p.in = f->in_features;
+  p.out = f->out_features;
+  p.dtype = f->dtype;
+  p.activation = f->activation;
+  p.slope_bytes = linear_slope_bytes(f->dtype, f->activation, f->save8 != 0);
+  p.x = f->x;
+  p.w = f->weight;
+  p.bias = f->bias;
+  p.residual = f->residual;
+  return p;
+}
+
+int check_residual_norm(int64_t rows, int32_t cols, int32_t dtype, int32_t param_dtype, int64_t gates) {
+  if (int rc = check_rows(rows, cols, dtype, kResidualNormCols); rc != NEST_OK) return rc;
+  if (param_dtype != NEST_DTYPE_F32 && param_dtype != dtype)
+    return fail(NEST_ERR_UNSUPPORTED, "gate, post and pre must be float32 or of the rows' own type");
+  if (gates < 0 || gates >= kMaxRows || (gates > 0 && rows % gates != 0))
+    return fail(NEST_ERR_INVALID_ARGUMENT, "gates must divide rows (got %lld gates, %lld rows)", (long long)gates, (long long)rows);
+  return NEST_OK;
+}
+
+int check_embedding(int64_t rows, int32_t cols, int64_t table_rows, int32_t dtype) {
+  if (int rc = check_rows(rows, cols, dtype, kMaxFeatures); rc != NEST_OK) return rc;
+  if (table_rows < 1 || table_rows >= kMaxRows - 1)
+    return fail(NEST_ERR_INVALID_ARGUMENT, "table_rows must be in [1, 2^31 - 1) (got %lld)", (long long)table_rows);
+  return NEST_OK;
+}
+
+}  // namespace
+
+int nest_linear_sizes(const nest_linear* f, size_t* kept, size_t* forward_ws, size_t* backward_ws, size_t* backward_ws_packed) {
+  if (int rc = check_linear(f); rc != NEST_OK) return rc;
+  LinearParams p = linear_params(f);
+  const LinearLayout fwd = linear_layout(p, false), bwd = linear_layout(p, true);
+  if (!fwd.fits || !bwd.fits) return too_many_tiles();
+  if (kept) *kept = (size_t)p.rows * p.out * p.slope_bytes;
+  if (forward_ws) *forward_ws = fwd.bytes;
+  if (backward_ws) *backward_ws = bwd.bytes;
+  if (backward_ws_packed) {
+    const int8_t some = 0;
+    p.codes = &some;
+    *backward_ws_packed = linear_layout(p, true).bytes;
+  }
+  return NEST_OK;
+}
+
+int nest_linear_forward(const nest_linear* f, void* y, void* kept, void* ws, size_t ws_bytes, void* stream) {
+  if (int rc = check_linear(f); rc != NEST_OK) return rc;
+  if (f->rows == 0) return NEST_OK;
+  if (!f->x || !f->weight || !y) return fail(NEST_ERR_INVALID_ARGUMENT, "NULL tensor pointer");
+  LinearParams p = linear_params(f);
+  const LinearLayout l = linear_layout(p, false);
+  if (!l.fits) return too_many_tiles();
+  if (ws_bytes < l.bytes || (l.bytes && !ws)) return fail(NEST_ERR_WORKSPACE, "linear workspace too small: %zu < %zu bytes", ws_bytes, l.bytes);
+  if (!aligned16({f->x, f->weight, f->bias, f->residual, y, kept, ws})) return fail(NEST_ERR_INVALID_ARGUMENT, "linear pointers must be 16-byte aligned");
+  p.y = y;
+  p.kept = kept;
+  p.ws = ws;
+  hipError_t e = launch_linear(p, static_cast<hipStream_t>(stream), false);
+  return e == hipSuccess ? NEST_OK : hip_fail(e, "linear");
+}
+
+int nest_linear_backward(const nest_linear* f, const void* dy, const void* kept, const int8_t* codes, const uint8_t* steps, void* dx,
+                         void* dweight, void* dbias, void* ws, size_t ws_bytes, void* stream) {
+  if (int rc = check_linear(f); rc != NEST_OK) return rc;
+  if (!dx && !dweight && !dbias) return NEST_OK;
+  LinearParams p = linear_params(f);
+  p.codes = codes;
+  p.steps = steps;
+  if ((codes == nullptr) != (steps == nullptr)) return fail(NEST_ERR_INVALID_ARGUMENT, "codes and steps come together");
+  if (f->rows > 0) {
+    if (!dy || (dweight && !f->x && !codes) || (dx && !f->weight) || (p.slope_bytes && !kept)) return fail(NEST_ERR_INVALID_ARGUMENT, "NULL tensor pointer");
+    const LinearLayout l = linear_layout(p, true);
+    if (!l.fits) return too_many_tiles();
+    if (ws_bytes < l.bytes || (l.bytes && !ws)) return fail(NEST_ERR_WORKSPACE, "linear workspace too small: %zu < %zu bytes", ws_bytes, l.bytes);
+    if (!aligned16({f->x, f->weight, dy, kept, codes, dx, dweight, dbias, ws})) return fail(NEST_ERR_INVALID_ARGUMENT, "linear pointers must be 16-byte aligned");
+  }
+  p.dy = dy;
+  p.kept = const_cast<void*>(kept);
+  p.dx = dx;
+  p.dw = dweight;
+  p.db = dbias;
+  p.ws = ws;
+  hipError_t e = launch_linear(p, static_cast<hipStream_t>(stream), true);
+  return e == hipSuccess ? NEST_OK : hip_fail(e, "linear backward");
+}
+
+int nest_pack8(int64_t rows, int32_t cols, int32_t dtype, const void* x, int8_t* codes, uint8_t* steps, void* stream) {
+  if (int rc = check_rows(rows, cols, dtype, kMaxFeatures); rc != NEST_OK) return rc;
+  if (rows == 0) return NEST_OK;
+  if (!x || !codes || !steps) return fail(NEST_ERR_INVALID_ARGUMENT, "NULL tensor pointer");
+  hipError_t e = launch_pack8(rows, cols, dtype, x, codes, steps, static_cast<hipStream_t>(stream));
+  return e == hipSuccess ? NEST_OK : hip_fail(e, "pack8");
+}
+
+int nest_unpack8(int64_t rows, int32_t cols, int32_t dtype, const int8_t* codes, const uint8_t* steps, void* x, void* stream) {
+  if (int rc = check_rows(rows, cols, dtype, kMaxFeatures); rc != NEST_OK) return rc;
+  if (rows == 0) return NEST_OK;
+  if (!x || !codes || !steps) return fail(NEST_ERR_INVALID_ARGUMENT, "NULL tensor pointer");
+  hipError_t e = launch_unpack8(rows, cols, dtype, codes, steps, x, cols, static_cast<hipStream_t>(stream));
+  return e == hipSuccess ? NEST_OK : hip_fail(e, "unpack8");
+}
+
+int nest_residual_norm(int64_t rows, int32_t cols, int32_t dtype, int32_t param_dtype, const void* x, const void* h, const void* gate,
+                       int64_t gates, const void* post, const void* pre, float scale, float eps, void* r, void* y, float* rstd_post,
+                       float* rstd_pre, void* stream) {
+  if (int rc = check_residual_norm(rows, cols, dtype, param_dtype, gate ? gates : 0); rc != NEST_OK) return rc;
+  if (!(eps >= 0.0f)) return fail(NEST_ERR_INVALID_ARGUMENT, "eps must not be negative");
+  if (gate && gates < 1 && rows > 0) return fail(NEST_ERR_INVALID_ARGUMENT, "a gate needs at least one row");
+  if (!h && (gate || post || scale != 1.0f)) return fail(NEST_ERR_INVALID_ARGUMENT, "without h there is no gate, no post and a scale of 1");
+  if (!h && !pre) return fail(NEST_ERR_INVALID_ARGUMENT, "nothing to do without h and pre");
+  if (rows == 0) return NEST_OK;
+  if (!x || (h && !r) || (pre && !y)) return fail(NEST_ERR_INVALID_ARGUMENT, "NULL tensor pointer");
+  ResidualNormParams p{};
+  p.rows = rows;
+  p.cols = cols;
+  p.dtype = dtype;
+  p.param_dtype = param_dtype;
+  p.scale = scale;
+  p.eps = eps;
+  p.x = x;
+  p.h = h;
+  p.gate = gate;
+  p.gates = gate ? gates : 0;
+  p.post = post;
+  p.pre = pre;
+  p.r = r;
+  p.y = y;
+  p.rstd_post = rstd_post;
+  p.rstd_pre = rstd_pre;
+  hipError_t e = launch_residual_norm(p, static_cast<hipStream_t>(stream));
+  return e == hipSuccess ? NEST_OK : hip_fail(e, "residual norm");
+}
+
+size_t nest_residual_norm_backward_workspace_size(int64_t rows, int32_t cols, int32_t dtype, int64_t gates) {
+  if (check_residual_norm(rows, cols, dtype, dtype, gates) != NEST_OK) return 0;
+  return residual_norm_ws_bytes(rows, cols, dtype, gates);
+}
+
+int nest_residual_norm_backward(int64_t rows, int32_t cols, int32_t dtype, int32_t param_dtype, const void* dr, const void* dy,
+                                const void* r, const void* h, const void* gate, int64_t gates, const void* post, const void* pre,
+                                float scale, const float* rstd_post, const float* rstd_pre, void* dx, void* dh, void* dgate,
+                                void* dpost, void* dpre, void* ws, size_t ws_bytes, void* stream) {
+  if (!gate) gates = 0;
+  if (int rc = check_residual_norm(rows, cols, dtype, param_dtype, gates); rc != NEST_OK) return rc;
+  if (gate && gates < 1 && rows > 0) return fail(NEST_ERR_INVALID_ARGUMENT, "a gate needs at least one row");
+  if (!h && (gate || post || scale != 1.0f)) return fail(NEST_ERR_INVALID_ARGUMENT, "without h there is no gate, no post and a scale of 1");
+  const size_t need = residual_norm_ws_bytes(rows, cols, dtype, gates);
+  if (ws_bytes < need || (need && !ws)) return fail(NEST_ERR_WORKSPACE, "residual norm workspace too small: %zu < %zu bytes", ws_bytes, need);
+  if ((gate && !dgate && gates > 0) || (post && !dpost) || (pre && !dpre) ||
+      (rows > 0 && (!dx || (h && !dh) || (pre && (!r || !rstd_pre)) || (post && !rstd_post))))
+    return fail(NEST_ERR_INVALID_ARGUMENT, "NULL tensor pointer");
+  ResidualNormParams p{};
+  p.rows = rows;
+  p.cols = cols;
+  p.dtype = dtype;
+  p.param_dtype = param_dtype;
+  p.scale = scale;
+  p.h = h;
+  p.gate = gate;
+  p.gates = gates;
+  p.post = post;
+  p.pre = pre;
+  p.r = const_cast<void*>(r);
+  p.rstd_post = const_cast<float*>(rstd_post);
+  p.rstd_pre = const_cast<float*>(rstd_pre);
+  p.dr = dr;
+  p.dy = dy;
+  p.dx = dx;
+  p.dh = dh;
+  p.dgate = dgate;
+  p.dpost = dpost;
+  p.dpre = dpre;
+  p.ws = static_cast<float*>(ws);
+  hipError_t e = launch_residual_norm_backward(p, static_cast<hipStream_t>(stream));
+  return e == hipSuccess ? NEST_OK : hip_fail(e, "residual norm backward");
+}
+
+int nest_embedding(int64_t rows, int32_t cols, int64_t table_rows, int32_t dtype, const void* ids, int32_t wide_ids, const void* table,
+                   float scale, const void* residual, void* y, void* stream) {
+  if (int rc = check_embedding(rows, cols, table_rows, dtype); rc != NEST_OK) return rc;
+  if (rows == 0) return NEST_OK;
+  if (!ids || !table || !y) return fail(NEST_ERR_INVALID_ARGUMENT, "NULL tensor pointer");
+  EmbeddingParams p{};
+  p.rows = rows;
+  p.cols = cols;
+  p.table_rows = table_rows;
+  p.dtype = dtype;
+  p.wide_ids = wide_ids != 0;
+  p.ids = ids;
+  p.scale = scale;
+  p.table = table;
+  p.residual = residual;
+  p.y = y;
+  hipError_t e = launch_embedding(p, static_cast<hipStream_t>(stream));
+  return e == hipSuccess ? NEST_OK : hip_fail(e, "embedding");
+}
+
+size_t nest_embedding_backward_workspace_size(int64_t rows, int32_t cols, int64_t table_rows, int32_t dtype) {
+  if (check_embedding(rows, cols, table_rows, dtype) != NEST_OK) return 0;
+  return embedding_ws_bytes(rows, cols, table_rows, dtype);
+}
+
+int nest_embedding_backward(int64_t rows, int32_t cols, int64_t table_rows, int32_t dtype, const void* ids, int32_t wide_ids,
+                            const void* dy, float scale, void* dtable, void* ws, size_t ws_bytes, void* stream) {
+  if (int rc = check_embedding(rows, cols, table_rows, dtype); rc != NEST_OK) return rc;
+  const size_t need = embedding_ws_bytes(rows, cols, table_rows, dtype);
+  if (rows > 0 && (ws_bytes < need || !ws)) return fail(NEST_ERR_WORKSPACE, "embedding workspace too small: %zu < %zu bytes", ws_bytes, need);
+  if (!dtable || (rows > 0 && (!ids || !dy))) return fail(NEST_ERR_INVALID_ARGUMENT, "NULL tensor pointer");
+  EmbeddingParams p{};
+  p.rows = rows;
+  p.cols = cols;
+  p.table_rows = table_rows;
+  p.dtype = dtype;
+  p.wide_ids = wide_ids != 0;
+  p.ids = ids;
+  p.scale = scale;
+  p.dy = dy;
+  p.dtable = dtable;
+  p.ws = ws;
+  hipError_t e = launch_embedding_backward(p, static_cast<hipStream_t>(stream));
+  return e == hipSuccess ? NEST_OK : hip_fail(e, "embedding backward");
 }
 
 }  // extern "C"

@@ -766,6 +766,13 @@ hipError_t launch_sort_tiles(const uint32_t* tile_keys, const uint32_t* ids, uin
                                        reinterpret_cast<const uint32_t*>(depth), ws, s, ranges, ntiles);
 }
 
+size_t index_sort_ws_bytes(int64_t n) { return sort_ws_bytes_t<uint32_t, uint32_t>(n); }
+
+hipError_t launch_sort_indices(const uint32_t* keys, uint32_t* keys_out, uint32_t* index_out, int64_t n, int end_bit, void* ws,
+                               hipStream_t s) {
+  return sort_impl<uint32_t, uint32_t>(keys, nullptr, keys_out, index_out, n, end_bit, nullptr, ws, s);
+}
+
 // The reference's sorted keys, tile << 32 | depth bits of the pair's splat
 // (point_list_keys, CR/rasterizer_impl.cu:381-386), from the tile ranges and
 // the sorted point list: one workgroup per tile, its positions in order.

@@ -57,8 +57,14 @@ struct FewShape {
 };
 constexpr int kFewWaves = 8;   // of a workgroup at most
 
-template <typename T, typename C, bool kGate>
-__global__ __launch_bounds__(64 * kFewWaves) void few_kernel(Few<T> p) {
+// What becomes of a sum of the kernel without a gate: column c of a row.
+template <typename T>
+struct StoreSum {
+  __device__ __forceinline__ void operator()(const Few<T>& p, int row, int64_t c, float v) const { p.out[row * p.ldo + c] = from_f32<T>(v); }
+};
+
+template <typename T, typename C, bool kGate, typename F = StoreSum<T>>
+__global__ __launch_bounds__(64 * kFewWaves) void few_kernel(Few<T> p, F finish) {
   typedef typename Mma<T>::Frag Frag;
   constexpr int S = C::S, NB = C::NB, RT = C::RT, U = C::U, TR = C::TR;
   constexpr int kVec = 16 / (int)sizeof(T), kLoad = S * 4 * kVec, kChunk = kLoad * U, kMats = kGate ? 2 : 1;
@@ -153,29 +159,29 @@ __global__ __launch_bounds__(64 * kFewWaves) void few_kernel(Few<T> p) {
         v[0] = c < p.N ? act_value<T, act.value, false>(v[0], unused) * v[1] : 0.0f;
         if (row < p.M) p.out[row * p.ldo + c] = from_f32<T>(v[0]);
       } else if (row < p.M && c < p.N) {
-        p.out[row * p.ldo + c] = from_f32<T>(v[0]);
+        finish(p, row, c, v[0]);
       }
     }
   });
 }
 
-template <typename T, typename C, bool kGate>
-hipError_t launch_few_shape(const Few<T>& p, hipStream_t s) {
+template <typename T, typename C, bool kGate, typename F>
+hipError_t launch_few_shape(const Few<T>& p, F finish, hipStream_t s) {
   constexpr int kChunk = 64 / (int)sizeof(T) * C::S * C::U;
   const int64_t tiles = ((kGate ? p.ldo : p.N) + C::rows - 1) / C::rows;
   int waves = 1;
   while (waves < kFewWaves && waves * kChunk < p.K) waves *= 2;
-  few_kernel<T, C, kGate><<<(unsigned)tiles, waves * 64, 0, s>>>(p);
+  few_kernel<T, C, kGate, F><<<(unsigned)tiles, waves * 64, 0, s>>>(p, finish);
   return hipGetLastError();
 }
 
-template <typename T, bool kGate>
-hipError_t launch_few(const Few<T>& p, hipStream_t s) {
+template <typename T, bool kGate, typename F = StoreSum<T>>
+hipError_t launch_few(const Few<T>& p, hipStream_t s, F finish = F()) {
   constexpr int kMore = kGate ? 1 : 2;
-  if (p.M == 1) return launch_few_shape<T, FewShape<16, 1, 2 * kMore, 4>, kGate>(p, s);
-  if (p.M <= 4) return launch_few_shape<T, FewShape<4, 1, 2 * kMore, 4>, kGate>(p, s);
-  if (p.M <= 8) return launch_few_shape<T, FewShape<2, 1, 1, 8>, kGate>(p, s);
-  return launch_few_shape<T, FewShape<2, 2, 1, 4>, kGate>(p, s);
+  if (p.M == 1) return launch_few_shape<T, FewShape<16, 1, 2 * kMore, 4>, kGate>(p, finish, s);
+  if (p.M <= 4) return launch_few_shape<T, FewShape<4, 1, 2 * kMore, 4>, kGate>(p, finish, s);
+  if (p.M <= 8) return launch_few_shape<T, FewShape<2, 1, 1, 8>, kGate>(p, finish, s);
+  return launch_few_shape<T, FewShape<2, 2, 1, 4>, kGate>(p, finish, s);
 }
 
 template <typename T>

@@ -188,6 +188,11 @@ size_t tile_sort_ws_bytes(int64_t n);
 hipError_t launch_sort_tiles(const uint32_t* tile_keys, const uint32_t* ids, uint64_t* keys_out, uint32_t* vals_out,
                              int64_t n, int tile_bits, const float* depth, uint32_t* ranges, uint32_t ntiles, void* ws,
                              hipStream_t s);
+// Stable sort of 0 .. n - 1 by keys[i] on bits [0, end_bit); the keys are not
+// written.
+size_t index_sort_ws_bytes(int64_t n);
+hipError_t launch_sort_indices(const uint32_t* keys, uint32_t* keys_out, uint32_t* index_out, int64_t n, int end_bit, void* ws,
+                               hipStream_t s);
 // Per-tile [start, end) of the n sorted pairs from those counts ((0, 0) for a
 // tile without pairs); with n == 0, zeroes the ranges.
 hipError_t launch_tile_ranges(uint32_t* ranges, int64_t n, uint32_t ntiles, hipStream_t s);

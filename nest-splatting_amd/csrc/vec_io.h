@@ -63,6 +63,19 @@ __device__ __forceinline__ void store_vec(T* p, const float (&f)[Vec16<T>::kN], 
   }
 }
 
+// The first n of a vector's elements (n may be <= 0 or above kN).
+template <typename T>
+__device__ __forceinline__ void store_raw(T* p, const Vec16<T>& t, int n) {
+  constexpr int N = Vec16<T>::kN;
+  if (n >= N) {
+    __builtin_memcpy(p, &t, 16);
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; i++)
+      if (i < n) p[i] = t.v[i];
+  }
+}
+
 // N parameters (weights, biases) of a type of their own as float32.
 template <typename P, int N>
 __device__ __forceinline__ void load_param(float (&f)[N], const P* p, int n) {
@@ -77,6 +90,20 @@ __device__ __forceinline__ void load_param(float (&f)[N], const P* p, int n) {
   } else {
 #pragma unroll
     for (int i = 0; i < N; i++) f[i] = i < n ? to_f32(p[i]) : 0.0f;
+  }
+}
+
+// The first n of N values as parameters of a type of their own.
+template <typename P, int N>
+__device__ __forceinline__ void store_param(P* p, const float (&f)[N], int n) {
+  constexpr int K = Vec16<P>::kN;
+  static_assert(N % K == 0, "");
+#pragma unroll
+  for (int v = 0; v < N / K; v++) {
+    Vec16<P> t;
+#pragma unroll
+    for (int i = 0; i < K; i++) t.v[i] = from_f32<P>(f[v * K + i]);
+    store_raw(p + v * K, t, n - v * K);
   }
 }
 

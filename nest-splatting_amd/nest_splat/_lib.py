@@ -27,7 +27,7 @@ MAX_LEVELS = 32
 MAX_CHANNELS = 128
 OTHERS_CHANNELS = 14
 
-ABI_VERSION = 19
+ABI_VERSION = 20
 SCAN_NOALLOC_MAX = 268431360
 (GEOM_DEPTH, GEOM_XY, GEOM_TILES, GEOM_OFFSETS, GEOM_RECORDS, GEOM_RADII, GEOM_SCAN_TMP, GEOM_DEPTH_ORDER,
  GEOM_ORDER_OFFSETS, GEOM_ORDER_TMP, GEOM_RGB, GEOM_CLAMPED, GEOM_RECT, GEOM_ORDER_RECT) = range(14)
@@ -136,6 +136,7 @@ class RvqAttr(ct.Structure):
 RVQ_BATCH_MAX = 4
 
 ACT_RELU, ACT_SILU, ACT_GELU = 0, 1, 2
+ACT_NONE = -1
 
 
 class GatedFfn(ct.Structure):
@@ -143,6 +144,12 @@ class GatedFfn(ct.Structure):
                 ("in_features", ct.c_int32), ("hidden", ct.c_int32), ("out_features", ct.c_int32),
                 ("rows", ct.c_int64), ("x", ct.c_void_p), ("w_gate", ct.c_void_p), ("w_up", ct.c_void_p),
                 ("w_down", ct.c_void_p)]
+
+
+class Linear(ct.Structure):
+    _fields_ = [("struct_size", ct.c_uint32), ("dtype", ct.c_int32), ("activation", ct.c_int32), ("save8", ct.c_int32),
+                ("in_features", ct.c_int32), ("out_features", ct.c_int32), ("rows", ct.c_int64), ("x", ct.c_void_p),
+                ("weight", ct.c_void_p), ("bias", ct.c_void_p), ("residual", ct.c_void_p)]
 
 
 EXPORTS = {
@@ -205,6 +212,27 @@ EXPORTS = {
                                           ct.c_void_p]),
     "nest_gated_ffn_backward": (ct.c_int, [ct.POINTER(GatedFfn), ct.c_void_p, ct.c_void_p, ct.c_void_p, ct.c_void_p,
                                            ct.c_void_p, ct.c_void_p, ct.c_void_p, ct.c_size_t, ct.c_void_p]),
+    "nest_linear_sizes": (ct.c_int, [ct.POINTER(Linear), ct.POINTER(ct.c_size_t), ct.POINTER(ct.c_size_t),
+                                     ct.POINTER(ct.c_size_t), ct.POINTER(ct.c_size_t)]),
+    "nest_linear_forward": (ct.c_int, [ct.POINTER(Linear), ct.c_void_p, ct.c_void_p, ct.c_void_p, ct.c_size_t, ct.c_void_p]),
+    "nest_linear_backward": (ct.c_int, [ct.POINTER(Linear), ct.c_void_p, ct.c_void_p, ct.c_void_p, ct.c_void_p, ct.c_void_p,
+                                        ct.c_void_p, ct.c_void_p, ct.c_void_p, ct.c_size_t, ct.c_void_p]),
+    "nest_pack8": (ct.c_int, [ct.c_int64, ct.c_int32, ct.c_int32, ct.c_void_p, ct.c_void_p, ct.c_void_p, ct.c_void_p]),
+    "nest_unpack8": (ct.c_int, [ct.c_int64, ct.c_int32, ct.c_int32, ct.c_void_p, ct.c_void_p, ct.c_void_p, ct.c_void_p]),
+    "nest_residual_norm": (ct.c_int, [ct.c_int64, ct.c_int32, ct.c_int32, ct.c_int32, ct.c_void_p, ct.c_void_p, ct.c_void_p,
+                                      ct.c_int64, ct.c_void_p, ct.c_void_p, ct.c_float, ct.c_float, ct.c_void_p,
+                                      ct.c_void_p, ct.c_void_p, ct.c_void_p, ct.c_void_p]),
+    "nest_residual_norm_backward_workspace_size": (ct.c_size_t, [ct.c_int64, ct.c_int32, ct.c_int32, ct.c_int64]),
+    "nest_residual_norm_backward": (ct.c_int, [ct.c_int64, ct.c_int32, ct.c_int32, ct.c_int32, ct.c_void_p, ct.c_void_p,
+                                               ct.c_void_p, ct.c_void_p, ct.c_void_p, ct.c_int64, ct.c_void_p,
+                                               ct.c_void_p, ct.c_float, ct.c_void_p, ct.c_void_p, ct.c_void_p,
+                                               ct.c_void_p, ct.c_void_p, ct.c_void_p, ct.c_void_p, ct.c_void_p,
+                                               ct.c_size_t, ct.c_void_p]),
+    "nest_embedding": (ct.c_int, [ct.c_int64, ct.c_int32, ct.c_int64, ct.c_int32, ct.c_void_p, ct.c_int32, ct.c_void_p,
+                                  ct.c_float, ct.c_void_p, ct.c_void_p, ct.c_void_p]),
+    "nest_embedding_backward_workspace_size": (ct.c_size_t, [ct.c_int64, ct.c_int32, ct.c_int64, ct.c_int32]),
+    "nest_embedding_backward": (ct.c_int, [ct.c_int64, ct.c_int32, ct.c_int64, ct.c_int32, ct.c_void_p, ct.c_int32,
+                                           ct.c_void_p, ct.c_float, ct.c_void_p, ct.c_void_p, ct.c_size_t, ct.c_void_p]),
 }
 
 _lib = None

@@ -10,6 +10,7 @@ from __future__ import annotations
 
 import math
 from dataclasses import dataclass
+from typing import Optional
 
 import numpy as np
 
@@ -56,6 +57,7 @@ class Camera:
     camera_center: np.ndarray         # float32 [3]
     znear: float = 0.01
     zfar: float = 100.0
+    view: Optional[int] = None        # the row of a ViewRefiner's embedding that the image was taken as, if any
 
     @property
     def tanfovx(self) -> float:

@@ -117,10 +117,12 @@ class SplatModel:
 class HashINGP:
     """The INGP attributes the baseline render reads (hash_encoder/modules.py):
     hash_encoding (a GridEncoder), gridrange, contract, active_levels, levels,
-    level_dim and rgb_decode.  refiner: an optional blocks.GatedRefiner that
-    features pass through before the MLP, the composited ones of render() as
-    well as rgb_decode's, as in evaluation (no dropout, no gradient: neither
-    trains it).  The modes that decode no features do not use it."""
+    level_dim and rgb_decode.  refiner: an optional blocks.GatedRefiner or
+    residual.ViewRefiner that features pass through before the MLP, the
+    composited ones of render() as well as rgb_decode's, as in evaluation (no
+    dropout, no gradient: neither trains it).  render() hands a ViewRefiner the
+    camera's ``view`` (None: of none), rgb_decode none.  The modes that decode
+    no features do not use it."""
 
     def __init__(self, encoding, mlp: NestMLP, gridrange, contract: bool = False, active_levels: Optional[int] = None,
                  refiner=None):
@@ -327,8 +329,9 @@ def render(viewpoint_camera, pc, pipe, bg_color: torch.Tensor, scaling_modifier=
         if refiner is None:
             decoded = rendered_image
         else:
+            view = getattr(viewpoint_camera, "view", None) if hasattr(refiner, "views") else None
             with _evaluating(refiner):
-                decoded = refiner.refine_image(rendered_image.detach())
+                decoded = refiner.refine_image(rendered_image.detach(), *(() if view is None else (view,)))
         rgb = ingp.mlp_rgb.decode_image(decoded, view_ray_matrix(viewpoint_camera), alpha=render_alpha, bg=bg)
     rets["render"] = rgb
 
