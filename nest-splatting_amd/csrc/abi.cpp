@@ -1604,7 +1604,7 @@ LinearParams linear_params(const nest_linear* f) {
   p.out = f->out_features;
   p.dtype = f->dtype;
   p.activation = f->activation;
-  p.slope_bytes = linear_slope_bytes(f->dtype, f->activation, f->save8 != 0);
+  p.slope_bytes = linear_slope_bytes(f->in_features, f->out_features, f->dtype, f->activation, f->save8 != 0);
   p.x = f->x;
   p.w = f->weight;
   p.bias = f->bias;
@@ -1671,11 +1671,13 @@ int nest_linear_backward(const nest_linear* f, const void* dy, const void* kept,
   p.steps = steps;
   if ((codes == nullptr) != (steps == nullptr)) return fail(NEST_ERR_INVALID_ARGUMENT, "codes and steps come together");
   if (f->rows > 0) {
-    if (!dy || (dweight && !f->x && !codes) || (dx && !f->weight) || (p.slope_bytes && !kept)) return fail(NEST_ERR_INVALID_ARGUMENT, "NULL tensor pointer");
+    const bool again = p.slope_bytes == 0 && f->activation != NEST_ACT_NONE;   // the slopes are made from x
+    if (again && codes) return fail(NEST_ERR_INVALID_ARGUMENT, "slopes that are not kept are made again from x, not from its 8 bits");
+    if (!dy || ((dweight || again) && !f->x && !codes) || ((dx || again) && !f->weight) || (p.slope_bytes && !kept)) return fail(NEST_ERR_INVALID_ARGUMENT, "NULL tensor pointer");
     const LinearLayout l = linear_layout(p, true);
     if (!l.fits) return too_many_tiles();
     if (ws_bytes < l.bytes || (l.bytes && !ws)) return fail(NEST_ERR_WORKSPACE, "linear workspace too small: %zu < %zu bytes", ws_bytes, l.bytes);
-    if (!aligned16({f->x, f->weight, dy, kept, codes, dx, dweight, dbias, ws})) return fail(NEST_ERR_INVALID_ARGUMENT, "linear pointers must be 16-byte aligned");
+    if (!aligned16({f->x, f->weight, f->bias, dy, kept, codes, dx, dweight, dbias, ws})) return fail(NEST_ERR_INVALID_ARGUMENT, "linear pointers must be 16-byte aligned");
   }
   p.dy = dy;
   p.kept = const_cast<void*>(kept);

@@ -13,6 +13,7 @@ namespace {
 struct SumTask {
   const float* part;
   int64_t n, groups;
+  int cols;
   const void *weight, *mul0, *mul1;
   void *out0, *out1;
   float* sum;
@@ -23,9 +24,10 @@ struct SumTasks {
 
 // 32 columns a workgroup, 32 slices of the rows, joined in LDS in their order.
 template <typename P>
-__global__ __launch_bounds__(1024) void column_sums_kernel(SumTasks tasks, int D) {
+__global__ __launch_bounds__(1024) void column_sums_kernel(SumTasks tasks) {
   __shared__ float lds[32][33];
   const SumTask& t = tasks.t[blockIdx.z];
+  const int64_t D = t.cols;
   const int col = blockIdx.x * 32 + (threadIdx.x & 31), slice = threadIdx.x >> 5;
   for (int64_t g = blockIdx.y; g < t.groups; g += gridDim.y) {
     const float* part = t.part + g * t.n * D + col;
@@ -63,10 +65,14 @@ __global__ __launch_bounds__(1024) void column_sums_kernel(SumTasks tasks, int D
 }
 
 template <typename P>
-hipError_t launch_column_sums(const SumTasks& tasks, int n, int D, hipStream_t s) {
+hipError_t launch_column_sums(const SumTasks& tasks, int n, hipStream_t s) {
   int64_t groups = 1;
-  for (int i = 0; i < n; i++) groups = tasks.t[i].groups > groups ? tasks.t[i].groups : groups;
-  column_sums_kernel<P><<<dim3((unsigned)((D + 31) / 32), (unsigned)(groups < 4096 ? groups : 4096), n), 1024, 0, s>>>(tasks, D);
+  int cols = 1;
+  for (int i = 0; i < n; i++) {
+    groups = tasks.t[i].groups > groups ? tasks.t[i].groups : groups;
+    cols = tasks.t[i].cols > cols ? tasks.t[i].cols : cols;
+  }
+  column_sums_kernel<P><<<dim3((unsigned)((cols + 31) / 32), (unsigned)(groups < 4096 ? groups : 4096), n), 1024, 0, s>>>(tasks);
   return hipGetLastError();
 }
 

@@ -21,8 +21,8 @@ hipError_t launch_clear(void* p, size_t bytes, hipStream_t s) {
 
 }  // namespace
 
-int linear_slope_bytes(int dtype, int activation, bool save8) {
-  if (activation == NEST_ACT_NONE) return 0;
+int linear_slope_bytes(int in, int out, int dtype, int activation, bool save8) {
+  if (activation == NEST_ACT_NONE || (!save8 && linear_narrow(in, out, dtype))) return 0;
   if (activation == NEST_ACT_RELU) return 1;
   return (save8 ? 1 : 2) * (dtype == NEST_DTYPE_F32 ? 2 : 1);
 }
@@ -39,6 +39,18 @@ LinearLayout linear_layout(const LinearParams& p, bool back) {
     at = (at + (size_t)bytes + 255) / 256 * 256;
     return o;
   };
+  l.narrow = linear_narrow(p.in, p.out, p.dtype);
+  if (l.narrow) {
+    if (!back) return l;
+    // as many workgroups as run at once, by LDS and registers
+    const int ki = (p.in + 31) / 32, ko = (p.out + 31) / 32, a_cu = ki + ko <= 3 ? 3 : ki + ko <= 6 ? 2 : 1;
+    const int64_t turns = cdiv(p.rows, 64 * narrow_groups(ki, ko));
+    l.sum_rows = (int)(turns < 256 * a_cu ? turns : 256 * a_cu);
+    l.sums = take(l.sum_rows * (int64_t)p.out * 4);
+    l.part = take(l.sum_rows * (int64_t)p.out * p.in * 4);
+    l.bytes = at;
+    return l;
+  }
   int64_t part = 0;
   auto partial = [&](const TileChoice& t, int64_t M, int64_t N) {
     const int64_t bytes = t.splits * cdiv(M * N, kJoinGroup) * kJoinGroup * 4;

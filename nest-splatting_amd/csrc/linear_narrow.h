@@ -1,0 +1,390 @@
+// The dense layer for narrow rows (at most 128 features in and out) of a
+// 16-bit type: whole rows stay in registers, the weights in LDS.
+//
+// A frame has a million rows of 16 to 128 features, so a forward is bound by
+// reading x and the residual and writing y, a backward by reading x and dy and
+// writing dx, and nothing of the rows' size is kept between the two: the
+// backward makes z again from x, which it reads anyway, where the tiles would
+// write and read two bytes of slope an element (a third of the traffic).  Only
+// what is kept in 8 bits on request is read instead.
+//
+// A wave takes 32 rows.  It computes transposed products, weights as the first
+// operand and rows as the second, with the first operand's rows in an order by
+// which a lane's accumulators of two fragments are 8 consecutive features of
+// one row: 16 bytes of y, of dy, or of the second operand of the next product,
+// so no value changes lanes between loads, products and stores.  The weights'
+// gradient sums over rows: the four waves of a workgroup put dz and x into LDS
+// and each takes a part of the gradient over all 128 rows with transposing
+// reads; it gathers in registers over the workgroup's turns.
+#pragma once
+
+#include "linear_tiles.h"
+
+namespace nest {
+namespace {
+
+constexpr int kForwardRows = 128;   // of a workgroup's turn: four waves of 32
+
+template <typename T>
+struct NarrowLayer {
+  const T *x, *w, *bias;     // a backward's x may be null: codes hold it, or nothing asks for it
+  const int8_t* codes;       // x in 8 bits, or null
+  const uint8_t* steps;
+  int64_t rows;
+  int in, out, act;
+  Epilogue<T> ep;            // forward
+  const T* dy;               // backward
+  const uint8_t* slopes;     // or null: none, or made again
+  T* dx;
+  float *dw, *db;            // [groups][out][in], [groups][out]; each may be null
+};
+
+// 8 elements of a row with n left at p as a fragment.
+template <typename T>
+__device__ __forceinline__ typename Mma<T>::Frag row_frag(const T* p, int n) {
+  return __builtin_bit_cast(typename Mma<T>::Frag, load_raw(p, n));
+}
+
+// 8 bytes of a row with n left at p, zeros past its end.
+__device__ __forceinline__ uint2 row_bytes(const void* p, int n) {
+  uint2 v = make_uint2(0, 0);
+  if (n >= 8) {
+    __builtin_memcpy(&v, p, 8);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; i++)
+      if (i < n) (i < 4 ? v.x : v.y) |= (uint32_t)static_cast<const uint8_t*>(p)[i] << (i % 4 * 8);
+  }
+  return v;
+}
+__device__ __forceinline__ float byte_of(uint2 v, int i) { return (float)(((i < 4 ? v.x : v.y) >> (i % 4 * 8)) & 0xffu); }
+
+// Feature of the first operand's row m in half jj of 32: lane quarter q's sums
+// of the two halves are features 8 q .. 8 q + 7.
+__device__ __forceinline__ int feature_of(int m, int jj) { return 8 * (m >> 2) + (m & 3) + 4 * jj; }
+
+// A [rows][cols] matrix of the weights (transposed: [cols][rows] in memory) to
+// LDS, zeros around it.
+template <typename T, int R, int C, bool kTransposed>
+__device__ __forceinline__ void stage_weights(T* lds, const T* w, int rows, int cols) {
+  constexpr int kPitch = C + 8;
+  for (int i = threadIdx.x; i < R * C; i += 256) {
+    const int r = kTransposed ? i % R : i / C, c = kTransposed ? i / R : i % C;
+    lds[r * kPitch + c] = r < rows && c < cols ? w[kTransposed ? c * rows + r : r * cols + c] : (T)0.0f;
+  }
+}
+
+// acc[jj][g] over K / 32 steps: features 32 J + 8 (lane / 16) + 4 jj + 0..3 of
+// row lane % 16 of group g.
+template <typename T, int K, int G>
+__device__ __forceinline__ void narrow_product(const T* lds, int J, const typename Mma<T>::Frag (&rows)[G][K / 32], f32x4 (&acc)[2][G]) {
+  const int lane = threadIdx.x & 63, r = lane & 15, q = lane >> 4;
+#pragma unroll
+  for (int jj = 0; jj < 2; jj++)
+#pragma unroll
+    for (int g = 0; g < G; g++) acc[jj][g] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+  for (int k = 0; k < K / 32; k++)
+#pragma unroll
+    for (int jj = 0; jj < 2; jj++) {
+      const auto a = *reinterpret_cast<const typename Mma<T>::Frag*>(lds + (32 * J + feature_of(r, jj)) * (K + 8) + k * 32 + q * 8);
+#pragma unroll
+      for (int g = 0; g < G; g++) acc[jj][g] = Mma<T>::run(a, rows[g][k], acc[jj][g]);
+    }
+}
+
+template <typename T, int KI, int KO>
+__global__ __launch_bounds__(256) void narrow_layer_kernel(NarrowLayer<T> p) {
+  typedef typename Mma<T>::Frag Frag;
+  __shared__ __attribute__((aligned(16))) T w[KO * 32 * (KI * 32 + 8)];
+  stage_weights<T, KO * 32, KI * 32, false>(w, p.w, p.out, p.in);
+  __syncthreads();
+  const int lane = threadIdx.x & 63, r = lane & 15, q = lane >> 4;
+  const int64_t step = (int64_t)gridDim.x * kForwardRows;
+  int64_t row = (int64_t)blockIdx.x * kForwardRows + wave_id() * 32 + r;
+  Frag x[2][KI];
+  auto load = [&](int64_t at) {
+#pragma unroll
+    for (int g = 0; g < 2; g++)
+#pragma unroll
+      for (int k = 0; k < KI; k++) {
+        const int c = k * 32 + q * 8;
+        x[g][k] = row_frag(p.x + (at + g * 16) * p.in + c, at + g * 16 < p.rows ? p.in - c : 0);
+      }
+  };
+  load(row);
+  with_activation(p.act, [&](auto act) {
+    for (; row - r < p.rows; row += step) {
+      Frag now[2][KI];
+#pragma unroll
+      for (int g = 0; g < 2; g++)
+#pragma unroll
+        for (int k = 0; k < KI; k++) now[g][k] = x[g][k];
+      load(row + step);   // on its way while this turn is worked on
+#pragma unroll
+      for (int J = 0; J < KO; J++) {
+        f32x4 acc[2][2];
+        narrow_product<T, KI * 32, 2>(w, J, now, acc);
+        const int c = J * 32 + q * 8;
+#pragma unroll
+        for (int g = 0; g < 2; g++) {
+          float z[8];
+#pragma unroll
+          for (int e = 0; e < 8; e++) z[e] = acc[e >> 2][g][e & 3];
+          if (row + g * 16 < p.rows && c < p.out) p.ep.template finish<8, act.value>(row + g * 16, c, p.out - c, z);
+        }
+      }
+    }
+  });
+}
+
+constexpr int pow2_of(int k) { return k == 3 ? 4 : k; }   // 32s of a tile's row
+
+// LDS of the backward, in elements.
+template <int KI, int KO, bool kSaved>
+struct NarrowLayerLds {
+  static constexpr int rows = 64 * narrow_groups(KI, KO);   // of a workgroup's turn
+  static constexpr int RO = pow2_of(KO) * 32, RI = pow2_of(KI) * 32;
+  static constexpr int wt = kSaved ? 0 : KO * 32 * (KI * 32 + 8);
+  static constexpr int dz = wt + KI * 32 * (KO * 32 + 8);
+  static constexpr int x = dz + rows * RO;
+  static constexpr int total = x + rows * RI;
+};
+
+// Where a lane's 8 elements of a row go in a tile of R columns that is read
+// transposed (tile_gemm.h).
+template <typename T, int R>
+__device__ __forceinline__ int tile_place(int row, int J, int q) {
+  return row * R + (((2 * J + (q >> 1)) ^ unit_swizzle<T, R>(row)) << 4) + (q & 1) * 8;
+}
+
+// kSaved: what the backward needs may lie in 8 bits, x (codes) as well as the
+// slopes, and no slopes are made again.
+template <typename T, int KI, int KO, bool kSaved>
+__global__ __launch_bounds__(256) void narrow_layer_backward_kernel(NarrowLayer<T> p) {
+  typedef typename Mma<T>::Frag Frag;
+  typedef NarrowLayerLds<KI, KO, kSaved> L;
+  constexpr int G = narrow_groups(KI, KO), kRows = L::rows, NO = 2 * KO, NI = 2 * KI;
+  constexpr int WO = NO % 4 == 0 ? 4 : 2, WI = 4 / WO, FO = NO / WO, FI = NI / WI;   // waves and fragments of dW
+  __shared__ __attribute__((aligned(16))) T lds[L::total];
+  if constexpr (!kSaved) stage_weights<T, KO * 32, KI * 32, false>(lds, p.w, p.out, p.in);
+  if (p.dx) stage_weights<T, KI * 32, KO * 32, true>(lds + L::wt, p.w, p.in, p.out);
+  __syncthreads();
+  const int lane = threadIdx.x & 63, r = lane & 15, q = lane >> 4, wave = wave_id();
+  const int64_t step = (int64_t)gridDim.x * kRows;
+  const int64_t first = (int64_t)blockIdx.x * kRows;
+  Frag x[G][KI], dy[G][KO];
+  uint2 slopes[G][KO], codes[G][KI];
+  int steps[G][KI];
+  const int groups_in = (p.in + 31) / 32;
+  const bool again = !kSaved && p.act != NEST_ACT_NONE;
+  auto load = [&](int64_t turn) {
+#pragma unroll
+    for (int g = 0; g < G; g++) {
+      const int64_t at = turn + wave * 16 * G + g * 16 + r;
+      const bool in = at < p.rows;
+#pragma unroll
+      for (int k = 0; k < KI; k++) {
+        const int c = k * 32 + q * 8, n = in ? p.in - c : 0;
+        if (kSaved && p.codes) {
+          codes[g][k] = row_bytes(p.codes + at * p.in + c, n);
+          steps[g][k] = n > 0 ? p.steps[at * groups_in + k] : 0;
+        } else {
+          x[g][k] = row_frag(p.x + at * p.in + c, p.x ? n : 0);
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < KO; k++) {
+        const int c = k * 32 + q * 8, n = in ? p.out - c : 0;
+        dy[g][k] = row_frag(p.dy + at * p.out + c, n);
+        if constexpr (kSaved) slopes[g][k] = row_bytes(p.slopes + at * p.out + c, p.slopes ? n : 0);
+      }
+    }
+  };
+  load(first);
+  f32x4 dw[FO][FI] = {};
+  float db[KO][8] = {};
+  const int wo = wave % WO, wi = wave / WO;
+  const int base_o = fragment_base<T, false, L::RO>(0), base_i = fragment_base<T, false, L::RI>(0);
+  for (int64_t turn = first; turn < p.rows; turn += step) {
+    Frag dz[G][KO];
+    if constexpr (kSaved) {
+      if (p.codes) {
+#pragma unroll
+        for (int g = 0; g < G; g++)
+#pragma unroll
+          for (int k = 0; k < KI; k++) {
+            // a code and 128 as an unsigned byte; what lies past the row's end is of no gradient that is stored
+            const uint2 c = make_uint2(codes[g][k].x ^ 0x80808080u, codes[g][k].y ^ 0x80808080u);
+            const float step = steps[g][k] == 255 ? __builtin_nanf("") : __builtin_amdgcn_ldexpf(1.0f, steps[g][k] - 132);
+#pragma unroll
+            for (int e = 0; e < 8; e++) x[g][k][e] = from_f32<T>((byte_of(c, e) - 128.0f) * step);
+          }
+      }
+    }
+#pragma unroll
+    for (int J = 0; J < KO; J++) {
+      float z[G][8], bias[8];
+      if (again) {
+        f32x4 acc[2][G];
+        narrow_product<T, KI * 32, G>(lds, J, x, acc);
+        load_param(bias, p.bias + J * 32 + q * 8, p.bias ? p.out - J * 32 - q * 8 : 0);
+#pragma unroll
+        for (int g = 0; g < G; g++)
+#pragma unroll
+          for (int e = 0; e < 8; e++) z[g][e] = acc[e >> 2][g][e & 3] + bias[e];
+        with_act(p.act, [&](auto act) {
+#pragma unroll
+          for (int g = 0; g < G; g++)
+#pragma unroll
+            for (int e = 0; e < 8; e++) activate<T, act.value>(z[g][e], z[g][e]);   // the slope in its place
+        });
+      }
+#pragma unroll
+      for (int g = 0; g < G; g++)
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+          float d = to_f32((T)dy[g][J][e]);   // zero past the ends
+          if (kSaved && p.slopes) d *= coarse_slope(byte_of(slopes[g][J], e));
+          else if (again) d *= z[g][e];
+          if (J == KO - 1 && J * 32 + q * 8 + e >= p.out) d = 0.0f;   // of no feature: an infinity in x makes its z NaN
+          dz[g][J][e] = from_f32<T>(d);
+          db[J][e] += d;
+        }
+    }
+#pragma unroll
+    for (int g = 0; g < G; g++) {
+      const int at = wave * 16 * G + g * 16 + r;
+#pragma unroll
+      for (int k = 0; k < KO; k++) *reinterpret_cast<Frag*>(lds + L::dz + tile_place<T, L::RO>(at, k, q)) = dz[g][k];
+#pragma unroll
+      for (int k = 0; k < KI; k++) *reinterpret_cast<Frag*>(lds + L::x + tile_place<T, L::RI>(at, k, q)) = x[g][k];
+    }
+    load(turn + step);   // on its way while this turn is worked on
+    if (p.dx) {
+#pragma unroll
+      for (int J = 0; J < KI; J++) {
+        f32x4 acc[2][G];
+        narrow_product<T, KO * 32, G>(lds + L::wt, J, dz, acc);
+        const int c = J * 32 + q * 8;
+#pragma unroll
+        for (int g = 0; g < G; g++) {
+          const int64_t at = turn + wave * 16 * G + g * 16 + r;
+          float v[8];
+#pragma unroll
+          for (int e = 0; e < 8; e++) v[e] = acc[e >> 2][g][e & 3];
+          store_vec<T>(p.dx + at * p.in + c, v, at < p.rows ? p.in - c : 0);
+        }
+      }
+    }
+    __syncthreads();   // all rows of the turn are in LDS
+    if (p.dw) {
+      const uint8_t *tz = reinterpret_cast<const uint8_t*>(lds + L::dz), *tx = reinterpret_cast<const uint8_t*>(lds + L::x);
+#pragma unroll
+      for (int kb = 0; kb < kRows / 32; kb++) {
+        Frag a[FO];
+#pragma unroll
+        for (int i = 0; i < FO; i++) a[i] = fragment<T, false, L::RO>(tz, base_o, wo * FO + i, kb);
+#pragma unroll
+        for (int j = 0; j < FI; j++) {
+          const Frag b = fragment<T, false, L::RI>(tx, base_i, wi * FI + j, kb);
+#pragma unroll
+          for (int i = 0; i < FO; i++) dw[i][j] = Mma<T>::run(b, a[i], dw[i][j]);
+        }
+      }
+    }
+    __syncthreads();   // and read
+  }
+  if (p.dw) {
+    float* const part = p.dw + (int64_t)blockIdx.x * p.out * p.in;
+#pragma unroll
+    for (int i = 0; i < FO; i++)
+#pragma unroll
+      for (int j = 0; j < FI; j++) {
+        const int o = (wo * FO + i) * 16 + r, c = (wi * FI + j) * 16 + q * 4;
+        if (o < p.out) store4(part + o * p.in, c, p.in, p.in % 4 == 0, dw[i][j]);
+      }
+  }
+  if (p.db) {
+    float* const sums = reinterpret_cast<float*>(lds + L::dz);   // [4][KO * 32]
+#pragma unroll
+    for (int k = 0; k < KO; k++)
+#pragma unroll
+      for (int e = 0; e < 8; e++) {
+        float s = db[k][e];
+#pragma unroll
+        for (int o = 1; o < 16; o <<= 1) s += __shfl_xor(s, o);
+        if (r == 0) sums[wave * KO * 32 + k * 32 + q * 8 + e] = s;
+      }
+    __syncthreads();
+    for (int c = threadIdx.x; c < p.out; c += 256)
+      p.db[(int64_t)blockIdx.x * p.out + c] = sums[c] + sums[KO * 32 + c] + sums[2 * KO * 32 + c] + sums[3 * KO * 32 + c];
+  }
+}
+
+// f with the 32s of features in and out as constants.
+template <typename F>
+void with_widths(int in, int out, F f) {
+  const int ki = (in + 31) / 32, ko = (out + 31) / 32;
+  auto second = [&](auto k) {
+    if (ko == 1) f(k, Number<1>());
+    else if (ko == 2) f(k, Number<2>());
+    else if (ko == 3) f(k, Number<3>());
+    else f(k, Number<4>());
+  };
+  if (ki == 1) second(Number<1>());
+  else if (ki == 2) second(Number<2>());
+  else if (ki == 3) second(Number<3>());
+  else second(Number<4>());
+}
+
+template <typename T>
+hipError_t launch_narrow_layer(const LinearParams& p, const Epilogue<T>& ep, hipStream_t s) {
+  NarrowLayer<T> n{};
+  n.x = static_cast<const T*>(p.x);
+  n.w = static_cast<const T*>(p.w);
+  n.rows = p.rows;
+  n.in = p.in;
+  n.out = p.out;
+  n.act = p.activation;
+  n.ep = ep;
+  const int64_t turns = (p.rows + kForwardRows - 1) / kForwardRows;
+  const unsigned grid = (unsigned)(turns < 1024 ? turns : 1024);
+  with_widths(p.in, p.out, [&](auto ki, auto ko) {
+    narrow_layer_kernel<T, ki.value, ko.value><<<grid, 256, 0, s>>>(n);
+  });
+  return hipGetLastError();
+}
+
+template <typename T>
+hipError_t launch_narrow_layer_backward(const LinearParams& p, const LinearLayout& l, hipStream_t s) {
+  uint8_t* ws = static_cast<uint8_t*>(p.ws);
+  NarrowLayer<T> n{};
+  n.x = static_cast<const T*>(p.x);
+  n.w = static_cast<const T*>(p.w);
+  n.bias = static_cast<const T*>(p.bias);
+  n.codes = p.codes;
+  n.steps = p.steps;
+  n.rows = p.rows;
+  n.in = p.in;
+  n.out = p.out;
+  n.act = p.activation;
+  n.dy = static_cast<const T*>(p.dy);
+  n.slopes = static_cast<const uint8_t*>(p.kept);
+  n.dx = static_cast<T*>(p.dx);
+  n.dw = p.dw ? reinterpret_cast<float*>(ws + l.part) : nullptr;
+  n.db = p.db ? reinterpret_cast<float*>(ws + l.sums) : nullptr;
+  with_widths(p.in, p.out, [&](auto ki, auto ko) {
+    if (p.slope_bytes || p.codes) narrow_layer_backward_kernel<T, ki.value, ko.value, true><<<l.sum_rows, 256, 0, s>>>(n);
+    else narrow_layer_backward_kernel<T, ki.value, ko.value, false><<<l.sum_rows, 256, 0, s>>>(n);
+  });
+  if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
+  SumTasks t{};
+  int k = 0;
+  if (p.dw) t.t[k++] = {n.dw, l.sum_rows, 1, p.in * p.out, nullptr, nullptr, nullptr, p.dw, nullptr, nullptr};
+  if (p.db) t.t[k++] = {n.db, l.sum_rows, 1, p.out, nullptr, nullptr, nullptr, p.db, nullptr, nullptr};
+  return k ? launch_column_sums<T>(t, k, s) : hipSuccess;
+}
+
+}  // namespace
+}  // namespace nest

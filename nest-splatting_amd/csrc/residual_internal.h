@@ -100,13 +100,21 @@ struct LinearLayout {
   int64_t ldx, ldz;
   size_t x, w, dz, sums, part, bytes;
   TileChoice y, dx, dw;
+  bool narrow;             // linear_narrow.h
   bool few;                // gated_few.h (forward)
   bool fits;               // in launches
   bool copy_dz;            // the backward makes dz; it is dy itself otherwise
   int sum_rows;            // workgroups that gather db
 };
 LinearLayout linear_layout(const LinearParams& p, bool backward);
-int linear_slope_bytes(int dtype, int activation, bool save8);
+// Rows that stay on the chip; a backward makes their slopes again from x and
+// the bias unless they are kept in 8 bits.
+inline bool linear_narrow(int in, int out, int dtype) { return dtype != NEST_DTYPE_F32 && in <= 128 && out <= 128; }
+// Groups of 16 rows that a wave of the backward takes, by 32s of features in
+// and out: two share a read of the weights, where their registers leave two
+// waves a SIMD.
+constexpr int narrow_groups(int ki, int ko) { return ki + 2 * ko <= 6 ? 2 : 1; }
+int linear_slope_bytes(int in, int out, int dtype, int activation, bool save8);
 hipError_t launch_linear(const LinearParams& p, hipStream_t s, bool backward);
 hipError_t linear_f32(const LinearParams& p, hipStream_t s, bool backward);
 hipError_t linear_f16(const LinearParams& p, hipStream_t s, bool backward);

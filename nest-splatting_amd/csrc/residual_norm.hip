@@ -426,18 +426,18 @@ hipError_t backward(const ResidualNormParams& p, hipStream_t s) {
   }
   SumTasks tasks{};
   int n = 0;
-  if (p.pre) tasks.t[n++] = {l.items.dpre, l.groups, 1, nullptr, nullptr, nullptr, p.dpre, nullptr, nullptr};
+  if (p.pre) tasks.t[n++] = {l.items.dpre, l.groups, 1, p.cols, nullptr, nullptr, nullptr, p.dpre, nullptr, nullptr};
   if (l.items.s) {
-    if (l.each) tasks.t[n++] = {l.items.s, l.items.n, 1, nullptr, nullptr, nullptr, p.dpost, nullptr, nullptr};
-    else if (many) tasks.t[n++] = {l.items.s, l.items.parts, p.gates, nullptr, p.post, nullptr, p.dgate, nullptr, p.ws + l.sums};
-    else tasks.t[n++] = {l.items.s, l.items.n, 1, nullptr, p.post, p.gate, gate ? p.dgate : nullptr, post ? p.dpost : nullptr, nullptr};
+    if (l.each) tasks.t[n++] = {l.items.s, l.items.n, 1, p.cols, nullptr, nullptr, nullptr, p.dpost, nullptr, nullptr};
+    else if (many) tasks.t[n++] = {l.items.s, l.items.parts, p.gates, p.cols, nullptr, p.post, nullptr, p.dgate, nullptr, p.ws + l.sums};
+    else tasks.t[n++] = {l.items.s, l.items.n, 1, p.cols, nullptr, p.post, p.gate, gate ? p.dgate : nullptr, post ? p.dpost : nullptr, nullptr};
   }
   if (n == 0) return hipSuccess;
-  if (hipError_t e = launch_column_sums<P>(tasks, n, p.cols, s); e != hipSuccess) return e;
+  if (hipError_t e = launch_column_sums<P>(tasks, n, s); e != hipSuccess) return e;
   if (!many || !post) return hipSuccess;
   SumTasks last{};   // dpost, from every gate's S
-  last.t[0] = {p.ws + l.sums, p.gates, 1, p.gate, nullptr, nullptr, p.dpost, nullptr, nullptr};
-  return launch_column_sums<P>(last, 1, p.cols, s);
+  last.t[0] = {p.ws + l.sums, p.gates, 1, p.cols, p.gate, nullptr, nullptr, p.dpost, nullptr, nullptr};
+  return launch_column_sums<P>(last, 1, s);
 }
 
 }  // namespace

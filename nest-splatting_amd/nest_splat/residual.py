@@ -118,6 +118,11 @@ def _slope_type(dtype, activation, save8):
     return torch.uint8 if save8 else torch.int16
 
 
+def _narrow(dtype, features, out_features):
+    """Whether a backward makes the slopes again rather than have them kept: the library's rule."""
+    return dtype is not torch.float32 and features <= 128 and out_features <= 128
+
+
 def _linear_sizes(f):
     """Bytes of (kept slopes, a forward's workspace, a backward's, a backward's with x in 8 bits)."""
     kept, fwd, bwd, packed = ct.c_size_t(), ct.c_size_t(), ct.c_size_t(), ct.c_size_t()
@@ -138,7 +143,9 @@ def linear_forward(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.T
     """(y, kept): y = act(x weight^T + bias) + residual for x [..., in], weight [out, in], bias [out] and residual [..., out] (or
     None), all of one type; activation None, "relu", "silu" or "gelu". ``training``: kept is what linear_backward needs of the
     activation, its slopes, of y's shape: int16 in steps of 1/26000 (float32 for float32 rows), with ``save8`` uint8 in steps of
-    1/200 from -26/200 on (int16 for float32 rows), for relu always uint8. None without an activation."""
+    1/200 from -26/200 on (int16 for float32 rows), for relu always uint8. 16-bit rows of at most 128 features in and out keep
+    none without ``save8``: their backward makes them again, and kept is the bias that it needs (of no elements for no bias).
+    None without an activation."""
     code = _code(x, "x")
     O, I = _matrix(weight).shape
     if x.dim() < 1:
@@ -158,16 +165,22 @@ def linear_forward(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.T
         f.residual = residual.data_ptr()
     _, fwd_bytes, _, _ = _linear_sizes(f)
     y = torch.empty(out_shape, dtype=x.dtype, device=x.device)
-    kept = torch.empty(out_shape, dtype=_slope_type(x.dtype, activation, save8), device=x.device) if training and activation else None
+    kept = slopes = None
+    if training and activation is not None:
+        if not save8 and _narrow(x.dtype, I, O):
+            kept = x.new_empty(0) if bias is None else bias
+        else:
+            kept = slopes = torch.empty(out_shape, dtype=_slope_type(x.dtype, activation, save8), device=x.device)
     work = _workspace(fwd_bytes, x.device)
-    _call("nest_linear_forward", x.device, f, y.data_ptr(), _at(kept), _at(work), fwd_bytes)
+    _call("nest_linear_forward", x.device, f, y.data_ptr(), _at(slopes), _at(work), fwd_bytes)
     return y, kept
 
 
 def linear_backward(dy: torch.Tensor, x: Union[torch.Tensor, Packed8, None], weight: torch.Tensor, kept: Optional[torch.Tensor] = None,
                     activation: Optional[str] = None, with_bias: bool = True, needs=(True, True)):
-    """(dx, dweight, dbias) from dy and the kept slopes of the forward call; the residual's gradient is dy itself. x: the
-    forward's, or its Packed8, or None where dweight is not wanted. ``needs``: whether dx and dweight are wanted, None else."""
+    """(dx, dweight, dbias) from dy and what the forward call kept; the residual's gradient is dy itself. x: the forward's, or
+    its Packed8 (where slopes are kept), or None where neither dweight is wanted nor slopes are made again. ``needs``: whether dx
+    and dweight are wanted, None else."""
     code = _code(dy, "dy")
     O, I = _matrix(weight).shape
     if dy.dim() < 1 or dy.shape[-1] != O:
@@ -187,15 +200,26 @@ def linear_backward(dy: torch.Tensor, x: Union[torch.Tensor, Packed8, None], wei
         else:
             x = _aligned(_like(x, dy, in_shape, "x"))
             f.x = x.data_ptr()
+    slopes = None
     if activation is not None:
         if kept is None:
             raise ValueError(f"the backward of {activation} needs what linear_forward(training=True) kept")
+        narrow = _narrow(dy.dtype, I, O)
         full, half = (_slope_type(dy.dtype, activation, save8) for save8 in (False, True))
-        if kept.dtype not in (full, half) or kept.shape != dy.shape or not kept.is_contiguous() or kept.device != dy.device:
+        if kept.device != dy.device:
+            raise ValueError(f"kept is on {kept.device}, expected {dy.device}")
+        if narrow and kept.dtype is dy.dtype and kept.dim() == 1 and kept.shape[0] in (0, O):
+            if x is None or packed:
+                raise ValueError("slopes that are not kept are made again from x: pass the tensor")
+            x = _aligned(_like(x, dy, in_shape, "x"))
+            kept = _aligned(_whole(kept))
+            f.x = x.data_ptr()
+            f.bias = kept.data_ptr() if kept.shape[0] else None
+        elif kept.dtype in ((half,) if narrow else (full, half)) and kept.shape == dy.shape and kept.is_contiguous():
+            f.save8 = int(kept.dtype is half)
+            slopes = kept = _aligned(kept)
+        else:
             raise ValueError("kept is not what linear_forward(training=True) returned for these arguments")
-        f.save8 = int(kept.dtype is half)
-    else:
-        kept = None
     _, _, bwd_bytes, packed_bytes = _linear_sizes(f)
     dx = torch.empty(in_shape, dtype=dy.dtype, device=dy.device) if needs[0] else None
     dw = torch.empty_like(weight) if needs[1] else None
@@ -203,7 +227,7 @@ def linear_backward(dy: torch.Tensor, x: Union[torch.Tensor, Packed8, None], wei
     use_packed = packed and needs[1]
     nbytes = packed_bytes if use_packed else bwd_bytes
     work = _workspace(nbytes, dy.device)
-    _call("nest_linear_backward", dy.device, f, dy.data_ptr(), _at(kept),
+    _call("nest_linear_backward", dy.device, f, dy.data_ptr(), _at(slopes),
           x.codes.data_ptr() if use_packed else None, x.steps.data_ptr() if use_packed else None, _at(dx), _at(dw), _at(db), _at(work), nbytes)
     return dx, dw, db
 
@@ -216,7 +240,8 @@ class _Linear(torch.autograd.Function):
         y, kept = linear_forward(x, weight, bias, activation, residual, training, save8)
         if training:
             codes = steps = None
-            held = x if need_w else None
+            again = activation is not None and not save8 and _narrow(x.dtype, weight.shape[1], weight.shape[0])
+            held = x if need_w or again else None
             if need_w and save8:
                 p = pack8(x)
                 held, codes, steps = None, p.codes, p.steps

@@ -114,7 +114,7 @@ def test_linear_from_8_bits(B, rows, cols, out, act, dtype):
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("act", ["relu", "silu", "gelu"])
 def test_linear_kept_slopes_are_the_nearest_codes(B, act, dtype, save8):
-    x, w, b, _, _ = linear_case(130, 72, 100, dtype)
+    x, w, b, _, _ = linear_case(130, 72, 100 if save8 else 140, dtype)
     x[::3] *= 6
     _, kept = B.linear_forward(x, w, b, act, training=True, save8=save8)
     z, e_z = R.pre_activation(x, w, b)
@@ -151,15 +151,58 @@ def test_linear_strides_leading_dimensions_and_alignment(B):
     linear_check(B, flat[1:].view(60, 24), w, rand(41, dtype=torch.float16, seed=3)[1:], rand(60, 50, dtype=torch.float16, seed=6)[:, 5:45], dy, "gelu")
 
 
+@pytest.mark.parametrize("dtype", TYPES[1:])
+@pytest.mark.parametrize("cols", [16, 33, 64, 70, 96, 128])
+@pytest.mark.parametrize("out", [1, 32, 48, 64, 90, 128])
+def test_linear_narrow_widths(B, cols, out, dtype):
+    for rows, act in ((333, "silu"), (130, None)):
+        linear_check(B, *linear_case(rows, cols, out, dtype), act)
+        linear_check(B, *linear_case(rows, cols, out, dtype, residual=False), act, save8=True)
+    x, w, b, r, dy = linear_case(70, cols, out, dtype)
+    _, kept = B.linear_forward(x, w, b, "gelu", training=True, save8=True)
+    got = B.linear_backward(dy, x, w, kept, "gelu")   # the slopes alone in 8 bits
+    ref = R.linear(x, w, b, "gelu", None, dy, True)
+    for k, v in zip(("dx", "dw", "db"), got):
+        R.check(v, *ref[k], k)
+
+
+def test_linear_narrow_many_turns(B):
+    """More rows than the workgroups that run at once take in one turn, the last turn partial."""
+    for rows, cols, out in ((256 * 3 * 128 + 77, 16, 32), (256 * 2 * 128 * 2 + 5, 64, 64), (256 * 64 * 2 + 31, 128, 128)):
+        x, w, b, r, dy = linear_case(rows, cols, out, torch.bfloat16)
+        linear_check(B, x, w, b, r, dy, "gelu")
+        linear_check(B, x, w, b, r, dy, "gelu", save8=True)
+
+
 def test_linear_gradients_that_are_not_wanted(B):
-    x, w, b, r, dy = linear_case(50, 24, 40, torch.bfloat16)
-    _, kept = B.linear_forward(x, w, b, "silu", r, training=True)
-    want = B.linear_backward(dy, x, w, kept, "silu")
-    for needs in ((True, False), (False, True), (False, False)):
-        for bias in (True, False):
-            got = B.linear_backward(dy, x if needs[1] else None, w, kept, "silu", with_bias=bias, needs=needs)
-            for g, v, n in zip(got, want, (*needs, bias)):
-                assert torch.equal(g, v) if n else g is None
+    for out in (40, 140):
+        x, w, b, r, dy = linear_case(50, 24, out, torch.bfloat16)
+        _, kept = B.linear_forward(x, w, b, "silu", r, training=True)
+        want = B.linear_backward(dy, x, w, kept, "silu")
+        for needs in ((True, False), (False, True), (False, False)):
+            for bias in (True, False):
+                got = B.linear_backward(dy, x, w, kept, "silu", with_bias=bias, needs=needs)
+                for g, v, n in zip(got, want, (*needs, bias)):
+                    assert torch.equal(g, v) if n else g is None
+
+
+@pytest.mark.parametrize("out", [40, 140])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_linear_without_x(B, dtype, out):
+    """dx and dbias alone need no x where slopes are kept, or there are none."""
+    x, w, b, r, dy = linear_case(50, 24, out, dtype)
+    for act, save8 in ((None, False), ("silu", True), ("relu", True)):
+        _, kept = B.linear_forward(x, w, b, act, r, training=True, save8=save8)
+        want = B.linear_backward(dy, x, w, kept, act)
+        dx, dw, db = B.linear_backward(dy, None, w, kept, act, needs=(True, False))
+        assert torch.equal(dx, want[0]) and dw is None and torch.equal(db, want[2])
+    for act in (None, "gelu"):
+        for save8 in (False, True):
+            ps = [t.clone().requires_grad_(k in (0, 2)) for k, t in enumerate((x, w, b))]
+            got = torch.autograd.grad(B.linear(*ps, act, save8=save8), (ps[0], ps[2]), dy)
+            _, kept = B.linear_forward(x, w, b, act, training=True, save8=save8)
+            want = B.linear_backward(dy, x, w, kept, act)
+            assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[2])
 
 
 @pytest.mark.parametrize("dtype", TYPES[1:])
@@ -174,10 +217,14 @@ def test_linear_values_that_are_not_finite_stay_in_their_rows(B, dtype):
         rest[[2, 5, 7]] = False
         assert torch.equal(y[rest], clean[rest])
         assert y[2].isnan().all() and (y[7] == float("inf")).all() and torch.equal(y[5], r[5])
-        z = B.linear_forward(x, w, b, "silu", training=True)
-        assert z[0][2].isnan().all() and (z[1][2] == -32768).all()
-        dx = B.linear_backward(dy, x, w, z[1], "silu", needs=(True, False))[0]
-        assert dx[2].isnan().all() and not dx[rest].isnan().any()
+        for save8 in (False, True):
+            z, kept = B.linear_forward(x, w, b, "silu", training=True, save8=save8)
+            assert z[2].isnan().all() and (not save8 or (kept[2] == 255).all())
+            dx = B.linear_backward(dy, x, w, kept, "silu", needs=(True, False))[0]
+            assert dx[2].isnan().all() and not dx[rest].isnan().any()
+        _, kept = B.linear_forward(x, w, b, "relu", training=True)
+        dx = B.linear_backward(dy, x, w, kept, "relu", needs=(True, False))[0]
+        assert dx[7].isfinite().all() and not dx[5].any()   # slopes 1 and 0
 
 
 def test_linear_repeats_bit_for_bit_and_autograd(B):

@@ -29,8 +29,9 @@ def test_linear_refusals_and_sizes(L):
         assert sizes(L, layer(L, **kw))[0] == bad, kw
     for kw in (dict(dtype=5), dict(activation=9), dict(activation=-2), dict(rows=(1 << 31) - 1, in_features=1 << 20, out_features=1 << 20)):
         assert sizes(L, layer(L, **kw))[0] == unsup, kw
-    kept = lambda **kw: sizes(L, layer(L, **kw))[1][0]
-    n = 1000 * 128
+    n = 1000 * 200
+    assert sizes(L, layer(L))[1][0] == 0 and sizes(L, layer(L, save8=1))[1][0] == 1000 * 128   # narrow rows make them again
+    kept = lambda **kw: sizes(L, layer(L, out_features=200, **kw))[1][0]
     assert kept() == 2 * n and kept(save8=1) == n and kept(dtype=L.DTYPE_F32) == 4 * n and kept(dtype=L.DTYPE_F32, save8=1) == 2 * n
     assert kept(activation=L.ACT_RELU) == kept(activation=L.ACT_RELU, save8=1) == n and kept(activation=L.ACT_NONE) == 0
     big = layer(L, rows=4096, in_features=1024, out_features=1001)
@@ -46,6 +47,11 @@ def test_linear_refusals_and_sizes(L):
         ct.byref(f), dy, kept, codes, steps, dx, dw, db, ws, n, None)
     assert bw(big, n=bwd - 1) == L.NEST_ERR_WORKSPACE and bw(big, codes=16, steps=16, n=packed - 1) == L.NEST_ERR_WORKSPACE
     assert bw(big, dy=None) == bad and bw(big, kept=None) == bad and bw(big, codes=16) == bad and bw(big, steps=16) == bad
+    assert bw(layer(L), codes=16, steps=16, kept=None) == bad and bw(layer(L, x=None), dw=None) == bad
+    from nest_splat import residual as B
+    for dtype, code in ((torch.float32, L.DTYPE_F32), (torch.float16, L.DTYPE_F16), (torch.bfloat16, L.DTYPE_BF16)):
+        for i, o in ((128, 128), (129, 1), (1, 129), (1, 1)):
+            assert B._narrow(dtype, i, o) == (sizes(L, layer(L, dtype=code, in_features=i, out_features=o))[1][0] == 0)
     assert bw(layer(L, x=None)) == bad and bw(layer(L, weight=None)) == bad and bw(big, dx=20) == bad
     assert bw(big, dx=None, dw=None, db=None, dy=None) == L.NEST_OK
 
