@@ -41,7 +41,7 @@ hipError_t linear_forward(const LinearParams& p, hipStream_t s) {
   const Epilogue<T> ep{static_cast<const T*>(p.bias), static_cast<const T*>(p.residual), static_cast<T*>(p.y), p.kept, p.slope_bytes,
                        p.activation, p.out};
   if constexpr (sizeof(T) == 2)
-    if (l.narrow) return launch_narrow_layer<T>(p, ep, s);
+    if (l.narrow) return launch_narrow_layer<T>(p, s);
   if (l.few) {
     const Few<T> few{x, w, nullptr, p.in, (int)p.rows, p.out, p.in, static_cast<T*>(p.y), p.out, nullptr, 0};
     return launch_few<T, false>(few, s, FinishSum<T>{ep});

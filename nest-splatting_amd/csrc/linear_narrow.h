@@ -23,7 +23,9 @@
 namespace nest {
 namespace {
 
-constexpr int kForwardRows = 128;   // of a workgroup's turn: four waves of 32
+// Groups of 16 rows that a wave takes in a turn: two share a read of the
+// weights.
+constexpr int forward_groups(int ki, int ko) { return ki + ko <= 5 ? 2 : 1; }
 
 template <typename T>
 struct NarrowLayer {
@@ -32,7 +34,9 @@ struct NarrowLayer {
   const uint8_t* steps;
   int64_t rows;
   int in, out, act;
-  Epilogue<T> ep;            // forward
+  const T* residual;         // forward; or null
+  T* y;
+  uint8_t* kept;
   const T* dy;               // backward
   const uint8_t* slopes;     // or null: none, or made again
   T* dx;
@@ -57,6 +61,15 @@ __device__ __forceinline__ uint2 row_bytes(const void* p, int n) {
   }
   return v;
 }
+__device__ __forceinline__ void store_bytes(uint8_t* p, uint2 v, int n) {
+  if (n >= 8) {
+    store_whole(p, v);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; i++)
+      if (i < n) p[i] = (uint8_t)((i < 4 ? v.x : v.y) >> (i % 4 * 8));
+  }
+}
 __device__ __forceinline__ float byte_of(uint2 v, int i) { return (float)(((i < 4 ? v.x : v.y) >> (i % 4 * 8)) & 0xffu); }
 
 // Feature of the first operand's row m in half jj of 32: lane quarter q's sums
@@ -74,15 +87,16 @@ __device__ __forceinline__ void stage_weights(T* lds, const T* w, int rows, int 
   }
 }
 
-// acc[jj][g] over K / 32 steps: features 32 J + 8 (lane / 16) + 4 jj + 0..3 of
-// row lane % 16 of group g.
+// acc[jj][g] over K / 32 steps, from init on: features 32 J + 8 (lane / 16) +
+// 4 jj + 0..3 of row lane % 16 of group g.
 template <typename T, int K, int G>
-__device__ __forceinline__ void narrow_product(const T* lds, int J, const typename Mma<T>::Frag (&rows)[G][K / 32], f32x4 (&acc)[2][G]) {
+__device__ __forceinline__ void narrow_product(const T* lds, int J, const typename Mma<T>::Frag (&rows)[G][K / 32], const f32x4 (&init)[2],
+                                               f32x4 (&acc)[2][G]) {
   const int lane = threadIdx.x & 63, r = lane & 15, q = lane >> 4;
 #pragma unroll
   for (int jj = 0; jj < 2; jj++)
 #pragma unroll
-    for (int g = 0; g < G; g++) acc[jj][g] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int g = 0; g < G; g++) acc[jj][g] = init[jj];
 #pragma unroll
   for (int k = 0; k < K / 32; k++)
 #pragma unroll
@@ -93,49 +107,79 @@ __device__ __forceinline__ void narrow_product(const T* lds, int J, const typena
     }
 }
 
-template <typename T, int KI, int KO>
+// The bias to LDS, zeros after it: float32, four to an element.
+template <typename T>
+__device__ __forceinline__ void stage_bias(f32x4* lds, const T* bias, int out, int padded) {
+  for (int i = threadIdx.x; i < padded; i += 256) reinterpret_cast<float*>(lds)[i] = bias && i < out ? to_f32(bias[i]) : 0.0f;
+}
+
+// kKept: the slopes' codes are written too.
+template <typename T, int KI, int KO, bool kKept>
 __global__ __launch_bounds__(256) void narrow_layer_kernel(NarrowLayer<T> p) {
   typedef typename Mma<T>::Frag Frag;
   __shared__ __attribute__((aligned(16))) T w[KO * 32 * (KI * 32 + 8)];
+  __shared__ f32x4 bias[KO * 8];
   stage_weights<T, KO * 32, KI * 32, false>(w, p.w, p.out, p.in);
+  stage_bias(bias, p.bias, p.out, KO * 32);
   __syncthreads();
   const int lane = threadIdx.x & 63, r = lane & 15, q = lane >> 4;
-  const int64_t step = (int64_t)gridDim.x * kForwardRows;
-  int64_t row = (int64_t)blockIdx.x * kForwardRows + wave_id() * 32 + r;
-  Frag x[2][KI];
+  constexpr int G = forward_groups(KI, KO);
+  const int64_t step = (int64_t)gridDim.x * 64 * G;
+  Frag x[G][KI], res[G][KO];
   auto load = [&](int64_t at) {
 #pragma unroll
-    for (int g = 0; g < 2; g++)
+    for (int g = 0; g < G; g++) {
+      const bool in = at + g * 16 < p.rows;
 #pragma unroll
-      for (int k = 0; k < KI; k++) {
-        const int c = k * 32 + q * 8;
-        x[g][k] = row_frag(p.x + (at + g * 16) * p.in + c, at + g * 16 < p.rows ? p.in - c : 0);
-      }
-  };
-  load(row);
-  with_activation(p.act, [&](auto act) {
-    for (; row - r < p.rows; row += step) {
-      Frag now[2][KI];
+      for (int k = 0; k < KI; k++) x[g][k] = row_frag(p.x + (at + g * 16) * p.in + k * 32 + q * 8, in ? p.in - k * 32 - q * 8 : 0);
+      if (p.residual) {
 #pragma unroll
-      for (int g = 0; g < 2; g++)
-#pragma unroll
-        for (int k = 0; k < KI; k++) now[g][k] = x[g][k];
-      load(row + step);   // on its way while this turn is worked on
-#pragma unroll
-      for (int J = 0; J < KO; J++) {
-        f32x4 acc[2][2];
-        narrow_product<T, KI * 32, 2>(w, J, now, acc);
-        const int c = J * 32 + q * 8;
-#pragma unroll
-        for (int g = 0; g < 2; g++) {
-          float z[8];
-#pragma unroll
-          for (int e = 0; e < 8; e++) z[e] = acc[e >> 2][g][e & 3];
-          if (row + g * 16 < p.rows && c < p.out) p.ep.template finish<8, act.value>(row + g * 16, c, p.out - c, z);
-        }
+        for (int k = 0; k < KO; k++) res[g][k] = row_frag(p.residual + (at + g * 16) * p.out + k * 32 + q * 8, in ? p.out - k * 32 - q * 8 : 0);
       }
     }
-  });
+  };
+  int64_t row = ((int64_t)blockIdx.x * 4 + wave_id()) * 16 * G + r;
+  load(row);
+  for (; row - r < p.rows; row += step) {
+    Frag now[G][KI], add[G][KO];
+#pragma unroll
+    for (int g = 0; g < G; g++) {
+#pragma unroll
+      for (int k = 0; k < KI; k++) now[g][k] = x[g][k];
+#pragma unroll
+      for (int k = 0; k < KO; k++) add[g][k] = res[g][k];
+    }
+    load(row + step);   // on its way while this turn is worked on
+#pragma unroll
+    for (int J = 0; J < KO; J++) {
+      const f32x4 init[2] = {bias[J * 8 + q * 2], bias[J * 8 + q * 2 + 1]};
+      f32x4 acc[2][G];
+      narrow_product<T, KI * 32, G>(w, J, now, init, acc);
+      const int c = J * 32 + q * 8;
+#pragma unroll
+      for (int g = 0; g < G; g++) {
+        const int64_t at = (row + g * 16) * p.out + c;
+        const int n = row + g * 16 < p.rows ? p.out - c : 0;
+        float v[8];
+        uint2 codes = make_uint2(0, 0);
+        with_activation(p.act, [&](auto act) {
+#pragma unroll
+          for (int e = 0; e < 8; e++) {
+            float slope;
+            v[e] = activate<T, act.value, kKept>(acc[e >> 2][g][e & 3], slope);
+            if constexpr (kKept) (e < 4 ? codes.x : codes.y) |= (uint32_t)coarse_code(slope) << (e % 4 * 8);
+          }
+        });
+        if constexpr (kKept) store_bytes(p.kept + at, codes, n);
+        if (p.residual) {
+#pragma unroll
+          for (int e = 0; e < 8; e++) v[e] += to_f32((T)add[g][J][e]);
+        }
+        store_vec<T>(p.y + at, v, n);
+      }
+      __builtin_amdgcn_sched_barrier(0);   // one 32 features at a time: their registers are the next one's
+    }
+  }
 }
 
 constexpr int pow2_of(int k) { return k == 3 ? 4 : k; }   // 32s of a tile's row
@@ -167,6 +211,8 @@ __global__ __launch_bounds__(256) void narrow_layer_backward_kernel(NarrowLayer<
   constexpr int G = narrow_groups(KI, KO), kRows = L::rows, NO = 2 * KO, NI = 2 * KI;
   constexpr int WO = NO % 4 == 0 ? 4 : 2, WI = 4 / WO, FO = NO / WO, FI = NI / WI;   // waves and fragments of dW
   __shared__ __attribute__((aligned(16))) T lds[L::total];
+  __shared__ f32x4 bias[kSaved ? 1 : KO * 8];
+  if constexpr (!kSaved) stage_bias(bias, p.bias, p.out, KO * 32);
   if constexpr (!kSaved) stage_weights<T, KO * 32, KI * 32, false>(lds, p.w, p.out, p.in);
   if (p.dx) stage_weights<T, KI * 32, KO * 32, true>(lds + L::wt, p.w, p.in, p.out);
   __syncthreads();
@@ -224,15 +270,15 @@ __global__ __launch_bounds__(256) void narrow_layer_backward_kernel(NarrowLayer<
     }
 #pragma unroll
     for (int J = 0; J < KO; J++) {
-      float z[G][8], bias[8];
+      float z[G][8];
       if (again) {
+        const f32x4 init[2] = {bias[J * 8 + q * 2], bias[J * 8 + q * 2 + 1]};
         f32x4 acc[2][G];
-        narrow_product<T, KI * 32, G>(lds, J, x, acc);
-        load_param(bias, p.bias + J * 32 + q * 8, p.bias ? p.out - J * 32 - q * 8 : 0);
+        narrow_product<T, KI * 32, G>(lds, J, x, init, acc);
 #pragma unroll
         for (int g = 0; g < G; g++)
 #pragma unroll
-          for (int e = 0; e < 8; e++) z[g][e] = acc[e >> 2][g][e & 3] + bias[e];
+          for (int e = 0; e < 8; e++) z[g][e] = acc[e >> 2][g][e & 3];
         with_act(p.act, [&](auto act) {
 #pragma unroll
           for (int g = 0; g < G; g++)
@@ -265,7 +311,8 @@ __global__ __launch_bounds__(256) void narrow_layer_backward_kernel(NarrowLayer<
 #pragma unroll
       for (int J = 0; J < KI; J++) {
         f32x4 acc[2][G];
-        narrow_product<T, KO * 32, G>(lds + L::wt, J, dz, acc);
+        const f32x4 zero[2] = {};
+        narrow_product<T, KO * 32, G>(lds + L::wt, J, dz, zero, acc);
         const int c = J * 32 + q * 8;
 #pragma unroll
         for (int g = 0; g < G; g++) {
@@ -339,7 +386,7 @@ void with_widths(int in, int out, F f) {
 }
 
 template <typename T>
-hipError_t launch_narrow_layer(const LinearParams& p, const Epilogue<T>& ep, hipStream_t s) {
+hipError_t launch_narrow_layer(const LinearParams& p, hipStream_t s) {
   NarrowLayer<T> n{};
   n.x = static_cast<const T*>(p.x);
   n.w = static_cast<const T*>(p.w);
@@ -347,11 +394,16 @@ hipError_t launch_narrow_layer(const LinearParams& p, const Epilogue<T>& ep, hip
   n.in = p.in;
   n.out = p.out;
   n.act = p.activation;
-  n.ep = ep;
-  const int64_t turns = (p.rows + kForwardRows - 1) / kForwardRows;
-  const unsigned grid = (unsigned)(turns < 1024 ? turns : 1024);
+  n.bias = static_cast<const T*>(p.bias);
+  n.residual = static_cast<const T*>(p.residual);
+  n.y = static_cast<T*>(p.y);
+  n.kept = p.slope_bytes ? static_cast<uint8_t*>(p.kept) : nullptr;
   with_widths(p.in, p.out, [&](auto ki, auto ko) {
-    narrow_layer_kernel<T, ki.value, ko.value><<<grid, 256, 0, s>>>(n);
+    constexpr int kRows = 64 * forward_groups(ki.value, ko.value);
+    const int64_t turns = (p.rows + kRows - 1) / kRows;
+    const unsigned grid = (unsigned)(turns < 256 * 3 ? turns : 256 * 3);   // as many as run at once
+    if (n.kept) narrow_layer_kernel<T, ki.value, ko.value, true><<<grid, 256, 0, s>>>(n);
+    else narrow_layer_kernel<T, ki.value, ko.value, false><<<grid, 256, 0, s>>>(n);
   });
   return hipGetLastError();
 }

@@ -35,13 +35,13 @@ __device__ __forceinline__ void with_activation(int act, F f) {
   else with_act(act, f);
 }
 
-template <typename T, int kAct>
+template <typename T, int kAct, bool kSlope = true>
 __device__ __forceinline__ float activate(float z, float& slope) {
   if constexpr (kAct == NEST_ACT_NONE) {
     slope = 1.0f;
     return z;
   } else {
-    return act_value<T, kAct, true>(z, slope);
+    return act_value<T, kAct, kSlope>(z, slope);
   }
 }
 
@@ -64,7 +64,7 @@ struct Pack {
   E v[K];
   __device__ __forceinline__ void store(E* p, int n) const {
     if (n >= K) {
-      __builtin_memcpy(p, v, sizeof(v));
+      store_whole(p, *this);
     } else {
 #pragma unroll
       for (int i = 0; i < K; i++)
@@ -114,7 +114,7 @@ struct Epilogue {
 #pragma unroll
         for (int i = 0; i < K; i++) s.v[i] = fine_code(slope[i]);
         s.store(static_cast<int16_t*>(kept) + at, n);
-      } else {
+      } else if constexpr (sizeof(T) == 4) {
         Pack<float, K> s;
 #pragma unroll
         for (int i = 0; i < K; i++) s.v[i] = slope[i];
@@ -245,7 +245,7 @@ struct FinishSum {
       v = activate<T, act.value>(ep.bias ? v + to_f32(ep.bias[c]) : v, slope);
       if (act.value != NEST_ACT_NONE && ep.kept) {
         if (ep.slope_bytes == 1) static_cast<uint8_t*>(ep.kept)[at] = coarse_code(slope);
-        else if (ep.slope_bytes == 2) static_cast<int16_t*>(ep.kept)[at] = fine_code(slope);
+        else if (sizeof(T) == 2 || ep.slope_bytes == 2) static_cast<int16_t*>(ep.kept)[at] = fine_code(slope);
         else static_cast<float*>(ep.kept)[at] = slope;
       }
       ep.y[at] = from_f32<T>(ep.residual ? v + to_f32(ep.residual[at]) : v);
@@ -319,8 +319,8 @@ hipError_t launch_slopes(const SlopeRows<T>& p, int groups, hipStream_t s) {
   while (lanes < vecs && lanes < 64) lanes *= 2;
   const dim3 grid((unsigned)((vecs + lanes - 1) / lanes), (unsigned)groups);
   if (p.slope_bytes <= 1) linear_slope_kernel<T, uint8_t><<<grid, 256, 0, s>>>(p, lanes);
-  else if (p.slope_bytes == 2) linear_slope_kernel<T, int16_t><<<grid, 256, 0, s>>>(p, lanes);
-  else linear_slope_kernel<T, float><<<grid, 256, 0, s>>>(p, lanes);
+  else if (sizeof(T) == 2 || p.slope_bytes == 2) linear_slope_kernel<T, int16_t><<<grid, 256, 0, s>>>(p, lanes);
+  else if constexpr (sizeof(T) == 4) linear_slope_kernel<T, float><<<grid, 256, 0, s>>>(p, lanes);
   return hipGetLastError();
 }
 

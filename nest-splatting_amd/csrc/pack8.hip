@@ -75,7 +75,7 @@ __global__ __launch_bounds__(kThreads) void pack8_kernel(int64_t rows, int cols,
     }
     int8_t* to = codes + at.row * cols + at.col;
     if (left >= kValues) {
-      __builtin_memcpy(to, &c, kValues);
+      store_whole(to, c);
     } else {
 #pragma unroll
       for (int k = 0; k < kValues; k++)

@@ -41,6 +41,19 @@ __device__ __forceinline__ Vec16<T> load_raw(const T* p, int n) {
   return t;
 }
 
+// 4, 8 or 16 bytes at any alignment, as one store: of elements the compiler
+// would share the last ones with the code of a shorter row's end, and split the
+// rest (three requests a store instead of one).
+typedef uint32_t u32x4_any __attribute__((ext_vector_type(4), aligned(1)));
+typedef uint32_t u32x2_any __attribute__((ext_vector_type(2), aligned(1)));
+typedef uint32_t u32_any __attribute__((aligned(1)));
+template <typename V>
+__device__ __forceinline__ void store_whole(void* p, const V& v) {
+  if constexpr (sizeof(V) == 16) *static_cast<u32x4_any*>(p) = __builtin_bit_cast(u32x4_any, v);
+  else if constexpr (sizeof(V) == 8) *static_cast<u32x2_any*>(p) = __builtin_bit_cast(u32x2_any, v);
+  else *static_cast<u32_any*>(p) = __builtin_bit_cast(uint32_t, v);
+}
+
 template <typename T>
 __device__ __forceinline__ void load_vec(float (&f)[Vec16<T>::kN], const T* p, int n) {
   const Vec16<T> t = load_raw(p, n);
@@ -55,7 +68,7 @@ __device__ __forceinline__ void store_vec(T* p, const float (&f)[Vec16<T>::kN], 
     Vec16<T> t;
 #pragma unroll
     for (int i = 0; i < N; i++) t.v[i] = from_f32<T>(f[i]);
-    __builtin_memcpy(p, &t, 16);
+    store_whole(p, t);
   } else {
 #pragma unroll
     for (int i = 0; i < N; i++)
@@ -68,7 +81,7 @@ template <typename T>
 __device__ __forceinline__ void store_raw(T* p, const Vec16<T>& t, int n) {
   constexpr int N = Vec16<T>::kN;
   if (n >= N) {
-    __builtin_memcpy(p, &t, 16);
+    store_whole(p, t);
   } else {
 #pragma unroll
     for (int i = 0; i < N; i++)
