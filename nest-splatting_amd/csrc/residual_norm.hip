@@ -207,7 +207,7 @@ struct Items {
 };
 
 template <typename T, typename P, int NV, bool kBlock, bool kEach>
-__global__ __launch_bounds__((kBlock ? most_threads<T, NV>() : kThreads)) void residual_norm_backward_kernel(ResidualNormParams p, int lanes,
+__global__ __launch_bounds__((kBlock ? most_threads<T, NV>() : kThreads), (NV == 1 && !kEach ? 4 : 1)) void residual_norm_backward_kernel(ResidualNormParams p, int lanes,
                                                                                                      Items items) {
   constexpr int N = Vec16<T>::kN;
   constexpr bool kAhead = NV * N < 16;   // a row's gate loaded with the row before; past the registers else
@@ -218,8 +218,8 @@ __global__ __launch_bounds__((kBlock ? most_threads<T, NV>() : kThreads)) void r
   const int lane = kBlock ? threadIdx.x : threadIdx.x & (lanes - 1);
   const int D = p.cols;
   const float inv = 1.0f / (float)D;
-  float post[NV][N], pre[NV][N], gate[NV][N], acc[NV][N], dpre[NV][N];
-  load_columns<P>(post, p.post, lane, lanes, D, 1.0f);
+  float w[NV][N], pre[NV][N], gate[NV][N], acc[NV][N], dpre[NV][N];   // w: post, times the item's gate unless every row has its own
+  if constexpr (kEach) load_columns<P>(w, p.post, lane, lanes, D, 1.0f);
   load_columns<P>(pre, p.pre, lane, lanes, D, 0.0f);
 #pragma unroll
   for (int k = 0; k < NV; k++)
@@ -230,11 +230,17 @@ __global__ __launch_bounds__((kBlock ? most_threads<T, NV>() : kThreads)) void r
     const int64_t first = group * items.rows, last = first + items.rows;
     const int64_t step = (int64_t)items.parts * rows_wg;
     int64_t row = first + (item - group * items.parts) * rows_wg + (kBlock ? 0 : threadIdx.x / lanes);
-    if constexpr (!kEach) load_columns<P>(gate, p.gate ? static_cast<const P*>(p.gate) + group * D : nullptr, lane, lanes, D, 1.0f);
+    if constexpr (!kEach) {
+      load_columns<P>(w, p.post, lane, lanes, D, 1.0f);
+      load_columns<P>(gate, p.gate ? static_cast<const P*>(p.gate) + group * D : nullptr, lane, lanes, D, 1.0f);
+    }
 #pragma unroll
     for (int k = 0; k < NV; k++)
 #pragma unroll
-      for (int i = 0; i < N; i++) acc[k][i] = 0.0f;
+      for (int i = 0; i < N; i++) {
+        if constexpr (!kEach) w[k][i] *= gate[k][i];
+        acc[k][i] = 0.0f;
+      }
     Vec16<T> nr[NV], nh[NV], ndr[NV], ndy[NV];
     ParamVec<P, N> ng[NV];
     float na = 1.0f, nc = 0.0f;
@@ -306,14 +312,14 @@ __global__ __launch_bounds__((kBlock ? most_threads<T, NV>() : kThreads)) void r
         if constexpr (kEach) {
           float dg[N];
 #pragma unroll
-          for (int i = 0; i < N; i++) dg[i] = e[k][i] * (hat[k][i] * post[k][i]);
+          for (int i = 0; i < N; i++) dg[i] = e[k][i] * (hat[k][i] * w[k][i]);
           store_param<P>(static_cast<P*>(p.dgate) + row * D + c, dg, D - c);
         }
 #pragma unroll
         for (int i = 0; i < N; i++) {
-          const float dt = e[k][i] * gate[k][i];
-          acc[k][i] = fmaf(kEach ? dt : e[k][i], hat[k][i], acc[k][i]);
-          e[k][i] = dt * post[k][i];
+          if constexpr (kEach) e[k][i] *= gate[k][i];
+          acc[k][i] = fmaf(e[k][i], hat[k][i], acc[k][i]);
+          e[k][i] *= w[k][i];
           s = fmaf(e[k][i], hat[k][i], s);
         }
       }
@@ -378,12 +384,12 @@ struct Plan {
 };
 Plan plan_of(int64_t rows, int cols, int dtype, int64_t gates) {
   Plan l{};
+  l.each = gates == rows && rows > 1;
   const Shape h = shape_of(cols, dtype);
   const int waves = h.block ? h.lanes / 64 : kThreads / 64;
   const int values = h.nv * (dtype == NEST_DTYPE_F32 ? 4 : 8);   // a lane's
-  const int a_cu = values == 4 ? 20 : values == 8 ? 12 : 8;      // waves, by the registers
+  const int a_cu = values == 4 ? 20 : values == 8 ? (h.nv == 1 && !l.each ? 16 : 12) : 8;   // waves, by the registers
   const int64_t most = 256 * (a_cu > waves ? a_cu / waves : 1);
-  l.each = gates == rows && rows > 1;
   const int64_t n = l.each || gates == 0 ? 1 : gates;
   l.items.rows = rows / n;
   const int64_t turns = cdiv(l.items.rows, rows_of_group(h)), share = most / n > 1 ? most / n : 1;

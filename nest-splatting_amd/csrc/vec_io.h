@@ -54,6 +54,21 @@ __device__ __forceinline__ void store_whole(void* p, const V& v) {
   else *static_cast<u32_any*>(p) = __builtin_bit_cast(uint32_t, v);
 }
 
+// kWhole: rows are whole vectors, so n is <= 0 or kN at least; that leaves out
+// the code of a row's end, for every load.
+template <bool kWhole, typename T>
+__device__ __forceinline__ Vec16<T> load_piece(const T* p, int n) {
+  if constexpr (!kWhole) return load_raw(p, n);
+  Vec16<T> t;
+  if (n > 0) {
+    __builtin_memcpy(&t, p, 16);
+  } else {
+#pragma unroll
+    for (int i = 0; i < Vec16<T>::kN; i++) t.v[i] = (T)0.0f;
+  }
+  return t;
+}
+
 template <typename T>
 __device__ __forceinline__ void load_vec(float (&f)[Vec16<T>::kN], const T* p, int n) {
   const Vec16<T> t = load_raw(p, n);
@@ -87,6 +102,12 @@ __device__ __forceinline__ void store_raw(T* p, const Vec16<T>& t, int n) {
     for (int i = 0; i < N; i++)
       if (i < n) p[i] = t.v[i];
   }
+}
+
+template <bool kWhole, typename T>
+__device__ __forceinline__ void store_piece(T* p, const Vec16<T>& t, int n) {
+  if constexpr (!kWhole) store_raw(p, t, n);
+  else if (n > 0) store_whole(p, t);
 }
 
 // N parameters (weights, biases) of a type of their own as float32.

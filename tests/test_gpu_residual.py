@@ -407,15 +407,18 @@ def some_ids(n, rows, seed, skew=1, outside=True, dtype=torch.int64):
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("n,rows,cols,skew", [(1, 1, 1, 1), (1, 5, 64, 1), (15, 3, 7, 1), (16, 1, 64, 1), (17, 300, 33, 1), (33, 2, 8, 1), (100, 255, 130, 1),
                                               (1000, 256, 64, 1), (1000, 257, 20, 4), (5000, 70000, 24, 3), (5000, 1, 16, 1), (4096, 40, 515, 2),
-                                              (300, 50, 2048, 1), (20000, 3, 64, 6), (65, 9, 1100, 1), (70000, 300, 32, 1)])
+                                              (300, 50, 2048, 1), (20000, 3, 64, 6), (65, 9, 1100, 1), (70000, 300, 32, 1), (8192, 5000, 40, 2),
+                                              (8193, 5000, 40, 2), (70001, 1024, 64, 1), (3001, 1025, 64, 1), (9000, 384, 128, 1), (9000, 385, 128, 1),
+                                              (600, 4096, 9, 1), (130000, 200, 96, 1), (12000, 7, 4096, 3)])
 def test_embedding_values_and_gradients(B, n, rows, cols, skew, dtype):
     ids = some_ids(n, rows, seed=n, skew=skew)
     embed_check(B, ids, rand(rows, cols, dtype=dtype, seed=1), 1.25, rand(n, cols, dtype=dtype, seed=2), rand(n, cols, dtype=dtype, seed=3))
 
 
 def test_embedding_runs_that_end_at_chunks(B):
-    """Sorted ids whose runs begin and end at, before and after multiples of the chunks that the gradient sums."""
-    for lengths in ([16] * 40, [32, 16, 48, 64, 1, 15], [17, 15, 31, 33, 1, 1, 1, 13], [1] * 200, [640], [5, 2000, 5], [1024, 1024, 1023, 1025], [16, 5000, 16]):
+    """Sorted ids whose runs begin and end at, before and after multiples of the chunks that the gradient sums, past the sizes
+    whose positions are sorted at once too."""
+    for lengths in ([16] * 40, [32, 16, 48, 64, 1, 15], [17, 15, 31, 33, 1, 1, 1, 13], [1] * 200, [640], [5, 2000, 5], [1024, 1024, 1023, 1025], [16, 5000, 16], [9000], [1, 20000, 1, 300, 5], [2048] * 9):
         ids = torch.cat([torch.full((k,), 3 * i + 1, device=DEV) for i, k in enumerate(lengths)])
         rows = 3 * len(lengths) + 2
         embed_check(B, ids, rand(rows, 72, dtype=torch.float32, seed=4), 1.0, None, rand(len(ids), 72, dtype=torch.float32, seed=5))
@@ -448,6 +451,28 @@ def test_embedding_no_rows_strides_and_alignment(B, dtype):
     ids = some_ids(14, 9, seed=2, outside=False)
     embed_check(B, ids[::2], rand(24, 9, dtype=dtype, seed=3).t(), 1.0, rand(7, 30, dtype=dtype, seed=4)[:, 2:26], rand(7, 30, dtype=dtype, seed=5)[:, 1:25])
     embed_check(B, ids, rand(1 + 9 * 24, dtype=dtype, seed=6)[1:].view(9, 24), -1.0, None, rand(1 + 14 * 24, dtype=dtype, seed=7)[1:].view(14, 24))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows", [20, 3000])
+def test_embedding_infinities_and_nan_of_dy_stay_with_their_ids(B, rows, dtype):
+    n, inf, nan = 700, float("inf"), float("nan")
+    ids = some_ids(n, rows, seed=1, outside=False)
+    ids[:12] = torch.arange(12, device=DEV)
+    dy = rand(n, 48, dtype=dtype, seed=4)
+    dy[0, 3], dy[1, 4], dy[2, 5] = inf, -inf, nan
+    dy[3, 6], dy[4, 7] = inf, torch.finfo(dtype).max
+    ids[600] = 3
+    dy[600, 6] = -inf   # with the infinity above: NaN
+    ids[601], dy[601, 8] = -1, nan   # of no id
+    clean = R.embedding_back(dy, ids, rows, -2.0)[0]
+    got = B.embedding_backward(dy, ids, rows, -2.0)
+    assert torch.equal(got.isnan(), clean.isnan()) and torch.equal(got.isinf(), clean.to(dtype).isinf())
+    assert got[0, 3] == -inf and got[1, 4] == inf and got[2, 5].isnan() and got[3, 6].isnan()
+    finite = clean.to(dtype).isfinite()
+    value, bound = R.embedding_back(torch.where(dy.isfinite(), dy, torch.zeros_like(dy)), ids, rows, -2.0)
+    assert ((got.double() - value).abs() <= bound)[finite].all()
+    assert torch.equal(got, B.embedding_backward(dy, ids, rows, -2.0)) or got.isnan().any()
 
 
 def test_embedding_nan_stays_in_its_row_and_autograd(B):
