@@ -68,12 +68,12 @@ __global__ __launch_bounds__(kThreads) void embedding_kernel(EmbeddingParams p, 
     for (int u = 0; u < U; u++) at[u] = next[u];
     load_ids(first + step * U);   // on their way while these rows are
     for (int c = lane * N; c < D; c += lanes * N) {
-      Vec16<T> t[U], r[U];
+      Words16<T> t[U], r[U];
 #pragma unroll
       for (int u = 0; u < U; u++) {
         const int64_t row = first + u * step;
-        if (p.residual) r[u] = load_piece<kWhole>(static_cast<const T*>(p.residual) + row * D + c, row < p.rows ? D - c : 0);
-        t[u] = load_piece<kWhole>(static_cast<const T*>(p.table) + (int64_t)at[u] * D + c, at[u] != kNoRun ? D - c : 0);
+        if (p.residual) r[u] = load_words<kWhole>(static_cast<const T*>(p.residual) + row * D + c, row < p.rows ? D - c : 0);
+        t[u] = load_words<kWhole>(static_cast<const T*>(p.table) + (int64_t)at[u] * D + c, at[u] != kNoRun ? D - c : 0);
       }
 #pragma unroll
       for (int u = 0; u < U; u++) {
@@ -81,8 +81,8 @@ __global__ __launch_bounds__(kThreads) void embedding_kernel(EmbeddingParams p, 
         Vec16<T> out;
 #pragma unroll
         for (int i = 0; i < N; i++) {
-          const float v = p.residual ? fmaf(p.scale, to_f32(t[u].v[i]), to_f32(r[u].v[i])) : p.scale * to_f32(t[u].v[i]);
-          out.v[i] = at[u] != kNoRun ? from_f32<T>(v) : p.residual ? r[u].v[i] : (T)0.0f;
+          const float v = p.residual ? fmaf(p.scale, to_f32(t[u][i]), to_f32(r[u][i])) : p.scale * to_f32(t[u][i]);
+          out.v[i] = at[u] != kNoRun ? from_f32<T>(v) : p.residual ? r[u][i] : (T)0.0f;
         }
         store_piece<kWhole>(static_cast<T*>(p.y) + row * D + c, out, row < p.rows ? D - c : 0);
       }
@@ -94,46 +94,41 @@ __global__ __launch_bounds__(kThreads) void embedding_kernel(EmbeddingParams p, 
 
 __device__ __forceinline__ uint32_t key_of(int64_t id, int64_t table_rows) { return (uint32_t)(id >= 0 && id < table_rows ? id : table_rows); }
 
-// A table of zeros, by workgroup `at` of n.
-__device__ __forceinline__ void fill_zero(uint8_t* zero, int64_t bytes, int64_t at, int64_t n) {
-  const int64_t step = n * kThreads, first = at * kThreads + threadIdx.x, whole = bytes / 16;
-  for (int64_t i = first; i < whole; i += step) store_whole(zero + i * 16, make_uint4(0, 0, 0, 0));
-  for (int64_t i = whole * 16 + first; i < bytes; i += step) zero[i] = 0;
-}
-
 // The keys to sort, ids outside the table last, and a table of zeros.
 template <typename I>
 __global__ __launch_bounds__(kThreads) void embedding_keys_kernel(const I* ids, int64_t rows, int64_t table_rows, uint32_t* keys,
                                                                   uint8_t* zero, int64_t zero_bytes) {
-  for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < rows; i += (int64_t)gridDim.x * kThreads) keys[i] = key_of(ids[i], table_rows);
-  fill_zero(zero, zero_bytes, blockIdx.x, gridDim.x);
+  const int64_t step = (int64_t)gridDim.x * kThreads, first = (int64_t)blockIdx.x * kThreads + threadIdx.x, whole = zero_bytes / 16;
+  for (int64_t i = first; i < rows; i += step) keys[i] = key_of(ids[i], table_rows);
+  for (int64_t i = first; i < whole; i += step) store_whole(zero + i * 16, make_uint4(0, 0, 0, 0));
+  for (int64_t i = whole * 16 + first; i < zero_bytes; i += step) zero[i] = 0;
 }
 
 // Sorted at once: a position's place is the number of keys before its own.  A
 // workgroup takes kRanked positions and compares each with all keys, kThreads /
-// kRanked threads a position; the workgroups behind fill the table.  N^2
-// comparisons, spread over the chip: 8192 positions 7 us, where two passes of
-// the radix sort take 28 in six launches.
+// kRanked threads a position.  N^2 comparisons, spread over the chip.
 constexpr int64_t kMostRanked = 8192;
-constexpr int kRanked = 32;
+constexpr int kRanked = 16;
 template <typename I>
-__global__ __launch_bounds__(kThreads) void embedding_rank_kernel(const I* ids, int rows, int64_t table_rows, uint32_t* sorted,
-                                                                  uint32_t* index, uint8_t* zero, int64_t zero_bytes) {
+__global__ __launch_bounds__(kThreads) void embedding_rank_kernel(const I* ids, int rows, int64_t table_rows, uint32_t* sorted, uint32_t* index) {
   constexpr int kSlices = kThreads / kRanked;
   __shared__ __attribute__((aligned(16))) uint32_t keys[kMostRanked];
   __shared__ int counts[kSlices][kRanked];
-  const int groups = (rows + kRanked - 1) / kRanked;
-  if ((int)blockIdx.x >= groups) {
-    fill_zero(zero, zero_bytes, blockIdx.x - groups, gridDim.x - groups);
-    return;
-  }
   const int padded = (rows + 4 * kSlices - 1) / (4 * kSlices) * (4 * kSlices);
-  for (int i = threadIdx.x; i < padded; i += kThreads) keys[i] = i < rows ? key_of(ids[i], table_rows) : kNoRun;
+  for (int i = threadIdx.x; i < padded; i += kThreads * 8) {   // eight loads in flight
+    I id[8];
+#pragma unroll
+    for (int u = 0; u < 8; u++) id[u] = i + u * kThreads < rows ? ids[i + u * kThreads] : 0;
+#pragma unroll
+    for (int u = 0; u < 8; u++)
+      if (i + u * kThreads < padded) keys[i + u * kThreads] = i + u * kThreads < rows ? key_of(id[u], table_rows) : kNoRun;
+  }
   __syncthreads();
   const int t = threadIdx.x % kRanked, slice = threadIdx.x / kRanked, mine = blockIdx.x * kRanked + t;
   const int per = padded / kSlices;
   const uint32_t key = mine < rows ? keys[mine] : 0;
   int count = 0;
+#pragma unroll 4
   for (int j = slice * per; j < (slice + 1) * per; j += 4) {
     const uint4 k = *reinterpret_cast<const uint4*>(&keys[j]);
     count += (k.x < key + (j < mine)) + (k.y < key + (j + 1 < mine)) + (k.z < key + (j + 2 < mine)) + (k.w < key + (j + 3 < mine));
@@ -202,11 +197,11 @@ __global__ __launch_bounds__(kThreads) void embedding_runs_kernel(Runs<T> p, int
     uint32_t key[kBatch], row[kBatch];
     __builtin_memcpy(key, p.keys + k, sizeof(key));
     __builtin_memcpy(row, p.index + k, sizeof(row));
-    Vec16<T> v[kBatch];
+    Words16<T> v[kBatch];
 #pragma unroll
     for (int u = 0; u < kBatch; u++) {
       const bool has = k + u < end && key[u] < p.table_rows;
-      v[u] = load_piece<kWhole>(p.dy + (int64_t)(has ? row[u] : 0) * p.cols + c, has ? left : 0);
+      v[u] = load_words<kWhole>(p.dy + (int64_t)(has ? row[u] : 0) * p.cols + c, has ? left : 0);
     }
 #pragma unroll
     for (int u = 0; u < kBatch; u++) {
@@ -218,7 +213,7 @@ __global__ __launch_bounds__(kThreads) void embedding_runs_kernel(Runs<T> p, int
         for (int i = 0; i < N; i++) acc[i] = 0.0f;
       }
 #pragma unroll
-      for (int i = 0; i < N; i++) acc[i] += to_f32(v[u].v[i]);
+      for (int i = 0; i < N; i++) acc[i] += to_f32(v[u][i]);
     }
   }
   flush(true);
@@ -299,6 +294,11 @@ int chunk_of(int64_t n, int cols, int values) {
 // ---- gradient: a small table in the accumulators ----
 
 constexpr int kCountThreads = 512, kCountRows = 256;   // of a workgroup's turn
+// Accumulators of 16 x 16 that a wave holds, by its 16s of columns: 128
+// registers at most, 96 where the next turn's rows take 32; up to 48 leave room
+// for two workgroups a CU, whose loads overlap.
+constexpr int most_counted(int fd) { return fd == 8 ? 24 : 32; }
+constexpr int kTwiceCounted = 12;
 
 template <typename T>
 struct Counted {
@@ -334,20 +334,20 @@ __global__ __launch_bounds__(kThreads) void embedding_clear_kernel(uint32_t* p, 
 // FD: 16s of columns, a power of two; FV: 16s of ids a wave, every eighth.
 // Sums of ids 16 (8 i + wave) + lane % 16 and columns 16 j + 4 (lane / 16) + 0..3.
 template <typename T, int FV, int FD>
-__global__ __launch_bounds__(kCountThreads) void embedding_count_kernel(Counted<T> p) {
+__global__ __launch_bounds__(kCountThreads, (FD < 8 && FV * FD <= kTwiceCounted ? 4 : 2)) void embedding_count_kernel(Counted<T> p) {
   typedef typename Mma<T>::Frag Frag;
   constexpr int R = FD * 16, kVecs = R / 8, kLoads = kCountRows * kVecs / kCountThreads;   // pieces of 16 bytes
   __shared__ __attribute__((aligned(16))) uint8_t tile[2][kCountRows * R * 2];
   __shared__ __attribute__((aligned(16))) uint16_t keys[2][kCountRows];
   const int lane = threadIdx.x & 63, r = lane & 15, q = lane >> 4, wave = wave_id();
   const int64_t step = (int64_t)gridDim.x * kCountRows;
-  Vec16<T> next[kLoads > 0 ? kLoads : 1];
+  Words16<T> next[kLoads];
   int next_key = 0;
   auto load = [&](int64_t turn) {
 #pragma unroll
     for (int i = 0; i < kLoads; i++) {
       const int at = i * kCountThreads + threadIdx.x, row = at / kVecs, c = (at % kVecs) * 8;
-      next[i] = load_raw(p.dy + (turn + row) * p.cols + c, turn + row < p.rows ? p.cols - c : 0);
+      next[i] = load_words<false>(p.dy + (turn + row) * p.cols + c, turn + row < p.rows ? p.cols - c : 0);
     }
     if (threadIdx.x < kCountRows) {
       const int64_t row = turn + threadIdx.x;
@@ -361,25 +361,22 @@ __global__ __launch_bounds__(kCountThreads) void embedding_count_kernel(Counted<
     for (int i = 0; i < kLoads; i++) {
       const int at = i * kCountThreads + threadIdx.x, row = at / kVecs, v = at % kVecs;
       u16x2 most = {0, 0};
-      uint4 w = __builtin_bit_cast(uint4, next[i]);
-      const uint32_t words[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-      for (int k = 0; k < 4; k++) most = __builtin_elementwise_max(most, __builtin_bit_cast(u16x2, words[k] & 0x7fff7fffu));
+      for (int k = 0; k < 4; k++) most = __builtin_elementwise_max(most, __builtin_bit_cast(u16x2, next[i].w[k] & 0x7fff7fffu));
       if (most[0] >= kInfinity<T> || most[1] >= kInfinity<T>) {   // taken out, and remembered for its id
         int64_t id = -1;
         if (turn + row < p.rows) id = p.wide_ids ? static_cast<const int64_t*>(p.ids)[turn + row] : static_cast<const int32_t*>(p.ids)[turn + row];
         const bool has = id >= 0 && id < p.table_rows;
 #pragma unroll
         for (int e = 0; e < 8; e++) {
-          const uint16_t b = __builtin_bit_cast(uint16_t, next[i].v[e]);
+          const uint16_t b = (uint16_t)(next[i].w[e / 2] >> (e % 2 * 16));
           if ((b & 0x7fff) < kInfinity<T>) continue;
           if (has) atomicOr(&p.flags[id * p.cols + v * 8 + e], (b & 0x7fff) > kInfinity<T> ? 4u : b >> 15 ? 2u : 1u);
-          next[i].v[e] = (T)0.0f;
+          next[i].w[e / 2] &= e % 2 ? 0xffffu : 0xffff0000u;
         }
-        w = __builtin_bit_cast(uint4, next[i]);
       }
       const int unit = (v >> 1) ^ unit_swizzle<T, R>(row);
-      *reinterpret_cast<uint4*>(&tile[buf][row * R * 2 + (unit << 5) + (v & 1) * 16]) = w;
+      *reinterpret_cast<uint4*>(&tile[buf][row * R * 2 + (unit << 5) + (v & 1) * 16]) = __builtin_bit_cast(uint4, next[i]);
     }
     if (threadIdx.x < kCountRows) keys[buf][threadIdx.x] = (uint16_t)next_key;
   };
@@ -465,9 +462,6 @@ __global__ __launch_bounds__(1024) void embedding_sum_kernel(const float* part, 
   }
 }
 
-// Accumulators of 16 x 16 that a wave holds, by its 16s of columns: 128
-// registers at most, 96 where the next turn's rows take 32.
-constexpr int most_counted(int fd) { return fd == 8 ? 24 : 32; }
 int column_frags(int cols) { return pow2_at_least(cdiv(cols, 16)); }
 
 // Whether the table's sums fit a workgroup of eight waves.
@@ -498,7 +492,8 @@ Plan plan_of(int64_t rows, int cols, int64_t table_rows, int dtype) {
   l.counted = counted(rows, cols, table_rows, dtype);
   if (l.counted) {
     const int64_t turns = cdiv(rows, kCountRows);
-    l.groups = turns < 256 ? turns : 256;
+    const int64_t at_once = cols <= 64 && cdiv(table_rows, 16 * 8) * column_frags(cols) <= kTwiceCounted ? 512 : 256;
+    l.groups = turns < at_once ? turns : at_once;
     l.flags = take((size_t)table_rows * cols * 4);
     l.part = take((size_t)l.groups * table_rows * cols * 4);
     l.bytes = at;
@@ -546,9 +541,20 @@ hipError_t count_gradient(const EmbeddingParams& p, const Plan& l, hipStream_t s
                      reinterpret_cast<uint32_t*>(ws + l.flags), size};
   embedding_clear_kernel<<<(unsigned)cdiv(size, kThreads), kThreads, 0, s>>>(q.flags, size);
   auto launch = [&](auto fd) {
-    constexpr int FD = fd.value, kMost = most_counted(FD) / FD, kFew = kMost < 4 ? 1 : kMost / 4;
-    if (cdiv(p.table_rows, 16 * 8) <= kFew) embedding_count_kernel<T, kFew, FD><<<(unsigned)l.groups, kCountThreads, 0, s>>>(q);
-    else embedding_count_kernel<T, kMost, FD><<<(unsigned)l.groups, kCountThreads, 0, s>>>(q);
+    constexpr int FD = fd.value, kMost = most_counted(FD) / FD;
+    const int need = (int)cdiv(p.table_rows, 16 * 8);
+    auto with = [&](auto fv) { embedding_count_kernel<T, fv.value, FD><<<(unsigned)l.groups, kCountThreads, 0, s>>>(q); };
+    if constexpr (FD == 8) {
+      if (need == 1) with(Number<1>());
+      else if (need == 2) with(Number<2>());
+      else with(Number<3>());
+    } else {
+      if (need * 8 <= kMost) with(Number<kMost / 8>());
+      else if (need * 4 <= kMost) with(Number<kMost / 4>());
+      else if (need * 8 <= kMost * 3) with(Number<kMost * 3 / 8>());
+      else if (need * 2 <= kMost) with(Number<kMost / 2>());
+      else with(Number<kMost>());
+    }
   };
   const int fd = column_frags(p.cols);
   if (fd == 1) launch(Number<1>());
@@ -565,15 +571,12 @@ hipError_t sort_ids(const EmbeddingParams& p, const Plan& l, uint32_t* sorted, u
   uint8_t *ws = static_cast<uint8_t*>(p.ws), *table = static_cast<uint8_t*>(p.dtable);
   const I* ids = static_cast<const I*>(p.ids);
   const int64_t bytes = p.table_rows * p.cols * (int64_t)sizeof(T), pieces = cdiv(bytes, 16 * kThreads);
-  if (l.ranked) {
-    const unsigned fill = (unsigned)(pieces < 4096 ? pieces : 4096);
-    embedding_rank_kernel<I><<<(unsigned)cdiv(p.rows, kRanked) + fill, kThreads, 0, s>>>(ids, (int)p.rows, p.table_rows, sorted, index, table, bytes);
-    return hipGetLastError();
-  }
   uint32_t* keys = reinterpret_cast<uint32_t*>(ws + l.keys);
-  const int64_t need = cdiv(p.rows, kThreads) > pieces ? cdiv(p.rows, kThreads) : pieces;
-  embedding_keys_kernel<I><<<(unsigned)(need < 8192 ? need : 8192), kThreads, 0, s>>>(ids, p.rows, p.table_rows, keys, table, bytes);
+  const int64_t need = !l.ranked && cdiv(p.rows, kThreads) > pieces ? cdiv(p.rows, kThreads) : pieces;
+  embedding_keys_kernel<I><<<(unsigned)(need < 8192 ? need : 8192), kThreads, 0, s>>>(ids, l.ranked ? 0 : p.rows, p.table_rows, keys, table, bytes);
+  if (l.ranked) embedding_rank_kernel<I><<<(unsigned)cdiv(p.rows, kRanked), kThreads, 0, s>>>(ids, (int)p.rows, p.table_rows, sorted, index);
   if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
+  if (l.ranked) return hipSuccess;
   int bits = 1;
   while (((int64_t)1 << bits) <= p.table_rows) bits++;
   return launch_sort_indices(keys, sorted, index, p.rows, bits, ws + l.sort, s);

@@ -43,10 +43,11 @@ struct NarrowLayer {
   float *dw, *db;            // [groups][out][in], [groups][out]; each may be null
 };
 
-// 8 elements of a row with n left at p as a fragment.
+// 16 bytes of a row as a fragment.  What a loop carries stays words: the
+// compiler would take a register for each element of a fragment.
 template <typename T>
-__device__ __forceinline__ typename Mma<T>::Frag row_frag(const T* p, int n) {
-  return __builtin_bit_cast(typename Mma<T>::Frag, load_raw(p, n));
+__device__ __forceinline__ typename Mma<T>::Frag frag_of(const Words16<T>& w) {
+  return __builtin_bit_cast(typename Mma<T>::Frag, w);
 }
 
 // 8 bytes of a row with n left at p, zeros past its end.
@@ -125,27 +126,28 @@ __global__ __launch_bounds__(256) void narrow_layer_kernel(NarrowLayer<T> p) {
   const int lane = threadIdx.x & 63, r = lane & 15, q = lane >> 4;
   constexpr int G = forward_groups(KI, KO);
   const int64_t step = (int64_t)gridDim.x * 64 * G;
-  Frag x[G][KI], res[G][KO];
+  Words16<T> x[G][KI], res[G][KO];
   auto load = [&](int64_t at) {
 #pragma unroll
     for (int g = 0; g < G; g++) {
       const bool in = at + g * 16 < p.rows;
 #pragma unroll
-      for (int k = 0; k < KI; k++) x[g][k] = row_frag(p.x + (at + g * 16) * p.in + k * 32 + q * 8, in ? p.in - k * 32 - q * 8 : 0);
+      for (int k = 0; k < KI; k++) x[g][k] = load_words<false>(p.x + (at + g * 16) * p.in + k * 32 + q * 8, in ? p.in - k * 32 - q * 8 : 0);
       if (p.residual) {
 #pragma unroll
-        for (int k = 0; k < KO; k++) res[g][k] = row_frag(p.residual + (at + g * 16) * p.out + k * 32 + q * 8, in ? p.out - k * 32 - q * 8 : 0);
+        for (int k = 0; k < KO; k++) res[g][k] = load_words<false>(p.residual + (at + g * 16) * p.out + k * 32 + q * 8, in ? p.out - k * 32 - q * 8 : 0);
       }
     }
   };
   int64_t row = ((int64_t)blockIdx.x * 4 + wave_id()) * 16 * G + r;
   load(row);
   for (; row - r < p.rows; row += step) {
-    Frag now[G][KI], add[G][KO];
+    Frag now[G][KI];
+    Words16<T> add[G][KO];
 #pragma unroll
     for (int g = 0; g < G; g++) {
 #pragma unroll
-      for (int k = 0; k < KI; k++) now[g][k] = x[g][k];
+      for (int k = 0; k < KI; k++) now[g][k] = frag_of(x[g][k]);
 #pragma unroll
       for (int k = 0; k < KO; k++) add[g][k] = res[g][k];
     }
@@ -173,7 +175,7 @@ __global__ __launch_bounds__(256) void narrow_layer_kernel(NarrowLayer<T> p) {
         if constexpr (kKept) store_bytes(p.kept + at, codes, n);
         if (p.residual) {
 #pragma unroll
-          for (int e = 0; e < 8; e++) v[e] += to_f32((T)add[g][J][e]);
+          for (int e = 0; e < 8; e++) v[e] += to_f32(add[g][J][e]);
         }
         store_vec<T>(p.y + at, v, n);
       }
@@ -205,7 +207,7 @@ __device__ __forceinline__ int tile_place(int row, int J, int q) {
 // kSaved: what the backward needs may lie in 8 bits, x (codes) as well as the
 // slopes, and no slopes are made again.
 template <typename T, int KI, int KO, bool kSaved>
-__global__ __launch_bounds__(256) void narrow_layer_backward_kernel(NarrowLayer<T> p) {
+__global__ __launch_bounds__(256, narrow_groups_cu(KI, KO)) void narrow_layer_backward_kernel(NarrowLayer<T> p) {
   typedef typename Mma<T>::Frag Frag;
   typedef NarrowLayerLds<KI, KO, kSaved> L;
   constexpr int G = narrow_groups(KI, KO), kRows = L::rows, NO = 2 * KO, NI = 2 * KI;
@@ -219,7 +221,7 @@ __global__ __launch_bounds__(256) void narrow_layer_backward_kernel(NarrowLayer<
   const int lane = threadIdx.x & 63, r = lane & 15, q = lane >> 4, wave = wave_id();
   const int64_t step = (int64_t)gridDim.x * kRows;
   const int64_t first = (int64_t)blockIdx.x * kRows;
-  Frag x[G][KI], dy[G][KO];
+  Words16<T> xw[G][KI], dy[G][KO];
   uint2 slopes[G][KO], codes[G][KI];
   int steps[G][KI];
   const int groups_in = (p.in + 31) / 32;
@@ -236,13 +238,13 @@ __global__ __launch_bounds__(256) void narrow_layer_backward_kernel(NarrowLayer<
           codes[g][k] = row_bytes(p.codes + at * p.in + c, n);
           steps[g][k] = n > 0 ? p.steps[at * groups_in + k] : 0;
         } else {
-          x[g][k] = row_frag(p.x + at * p.in + c, p.x ? n : 0);
+          xw[g][k] = load_words<false>(p.x + at * p.in + c, p.x ? n : 0);
         }
       }
 #pragma unroll
       for (int k = 0; k < KO; k++) {
         const int c = k * 32 + q * 8, n = in ? p.out - c : 0;
-        dy[g][k] = row_frag(p.dy + at * p.out + c, n);
+        dy[g][k] = load_words<false>(p.dy + at * p.out + c, n);
         if constexpr (kSaved) slopes[g][k] = row_bytes(p.slopes + at * p.out + c, p.slopes ? n : 0);
       }
     }
@@ -253,7 +255,11 @@ __global__ __launch_bounds__(256) void narrow_layer_backward_kernel(NarrowLayer<
   const int wo = wave % WO, wi = wave / WO;
   const int base_o = fragment_base<T, false, L::RO>(0), base_i = fragment_base<T, false, L::RI>(0);
   for (int64_t turn = first; turn < p.rows; turn += step) {
-    Frag dz[G][KO];
+    Frag x[G][KI], dz[G][KO];
+#pragma unroll
+    for (int g = 0; g < G; g++)
+#pragma unroll
+      for (int k = 0; k < KI; k++) x[g][k] = frag_of(xw[g][k]);
     if constexpr (kSaved) {
       if (p.codes) {
 #pragma unroll
@@ -290,13 +296,14 @@ __global__ __launch_bounds__(256) void narrow_layer_backward_kernel(NarrowLayer<
       for (int g = 0; g < G; g++)
 #pragma unroll
         for (int e = 0; e < 8; e++) {
-          float d = to_f32((T)dy[g][J][e]);   // zero past the ends
+          float d = to_f32(dy[g][J][e]);   // zero past the ends
           if (kSaved && p.slopes) d *= coarse_slope(byte_of(slopes[g][J], e));
           else if (again) d *= z[g][e];
           if (J == KO - 1 && J * 32 + q * 8 + e >= p.out) d = 0.0f;   // of no feature: an infinity in x makes its z NaN
           dz[g][J][e] = from_f32<T>(d);
           db[J][e] += d;
         }
+      __builtin_amdgcn_sched_barrier(0);   // phases one after another: their registers are the next one's
     }
 #pragma unroll
     for (int g = 0; g < G; g++) {
@@ -322,6 +329,7 @@ __global__ __launch_bounds__(256) void narrow_layer_backward_kernel(NarrowLayer<
           for (int e = 0; e < 8; e++) v[e] = acc[e >> 2][g][e & 3];
           store_vec<T>(p.dx + at * p.in + c, v, at < p.rows ? p.in - c : 0);
         }
+        __builtin_amdgcn_sched_barrier(0);
       }
     }
     __syncthreads();   // all rows of the turn are in LDS
@@ -338,6 +346,7 @@ __global__ __launch_bounds__(256) void narrow_layer_backward_kernel(NarrowLayer<
 #pragma unroll
           for (int i = 0; i < FO; i++) dw[i][j] = Mma<T>::run(b, a[i], dw[i][j]);
         }
+        if (kb % 2) __builtin_amdgcn_sched_barrier(0);
       }
     }
     __syncthreads();   // and read

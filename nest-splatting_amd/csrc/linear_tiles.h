@@ -277,12 +277,12 @@ __global__ __launch_bounds__(256) void linear_slope_kernel(SlopeRows<T> p, int l
   float sum[K] = {};
   const int64_t step = (int64_t)gridDim.y * rows_wg;
   for (int64_t row = (int64_t)blockIdx.y * rows_wg + sub; row < p.rows; row += step * U) {
-    Vec16<T> d[U];
+    Words16<T> d[U];
     Pack<E, K> s[U];
 #pragma unroll
     for (int u = 0; u < U; u++) {
       const int64_t r = row + u * step;
-      d[u] = load_raw(p.dy + r * p.N + c, r < p.rows ? n : 0);
+      d[u] = load_words<false>(p.dy + r * p.N + c, r < p.rows ? n : 0);
       if (p.kept) s[u].load(static_cast<const E*>(p.kept) + r * p.N + c, r < p.rows ? n : 0);
     }
 #pragma unroll
@@ -291,7 +291,7 @@ __global__ __launch_bounds__(256) void linear_slope_kernel(SlopeRows<T> p, int l
       float v[K];
 #pragma unroll
       for (int i = 0; i < K; i++) {
-        v[i] = to_f32(d[u].v[i]);
+        v[i] = to_f32(d[u][i]);
         if (p.kept) v[i] *= slope_of(s[u].v[i]);
         if (i >= n || r >= p.rows) v[i] = 0.0f;
         sum[i] += v[i];

@@ -31,9 +31,9 @@ __device__ __forceinline__ void load16(float (&f)[kValues], const T* p, int n) {
   constexpr int N = Vec16<T>::kN;
 #pragma unroll
   for (int k = 0; k < kValues / N; k++) {
-    const Vec16<T> t = load_raw(p + k * N, n - k * N);
+    const Words16<T> t = load_words<false>(p + k * N, n - k * N);
 #pragma unroll
-    for (int i = 0; i < N; i++) f[k * N + i] = to_f32(t.v[i]);
+    for (int i = 0; i < N; i++) f[k * N + i] = to_f32(t[i]);
   }
 }
 

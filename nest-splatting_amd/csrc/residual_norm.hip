@@ -31,11 +31,8 @@ namespace nest {
 namespace {
 
 constexpr int kThreads = 256;        // of rows that stay with a wave
-// Most threads that share a row: a lane of four float32 values does with the
-// 128 registers that 1024 threads leave it, one of 8 or 16 values with 256.
-template <typename T, int NV>
-constexpr int most_threads() { return sizeof(T) == 4 && NV == 1 ? 1024 : 512; }
-constexpr int kMostWaves = 16;
+constexpr int kMostThreads = 512;    // that share a row: 16 values a lane at most
+constexpr int kMostWaves = kMostThreads / 64;
 constexpr int64_t kForwardGrid = 2048;   // workgroups
 
 // Sums over the lanes of a row; every lane gets the result.  Two LDS buffers
@@ -65,12 +62,12 @@ template <typename P, int N>
 struct ParamVec {
   static constexpr int K = Vec16<P>::kN;
   static_assert(N % K == 0, "");
-  Vec16<P> v[N / K];
+  Words16<P> v[N / K];
   __device__ __forceinline__ void load(const P* p, int n) {
 #pragma unroll
-    for (int k = 0; k < N / K; k++) v[k] = load_raw(p + k * K, n - k * K);
+    for (int k = 0; k < N / K; k++) v[k] = load_words<false>(p + k * K, n - k * K);
   }
-  __device__ __forceinline__ float operator[](int i) const { return to_f32(v[i / K].v[i % K]); }
+  __device__ __forceinline__ float operator[](int i) const { return to_f32(v[i / K][i % K]); }
 };
 
 // Parameters of this lane's columns, `other` where there are none.
@@ -89,7 +86,7 @@ __device__ __forceinline__ void load_columns(float (&w)[NV][N], const void* p, i
 }
 
 template <typename T, typename P, int NV, bool kBlock>
-__global__ __launch_bounds__((kBlock ? most_threads<T, NV>() : kThreads)) void residual_norm_kernel(ResidualNormParams p, int lanes,
+__global__ __launch_bounds__((kBlock ? kMostThreads : kThreads)) void residual_norm_kernel(ResidualNormParams p, int lanes,
                                                                                             uint32_t rows_gate) {
   constexpr int N = Vec16<T>::kN;
   __shared__ float lds[2][kMostWaves];
@@ -101,15 +98,15 @@ __global__ __launch_bounds__((kBlock ? most_threads<T, NV>() : kThreads)) void r
   const int64_t step = (int64_t)gridDim.x * rows_wg;
   int64_t row = (int64_t)blockIdx.x * rows_wg + (kBlock ? 0 : threadIdx.x / lanes);
   const bool row_gates = p.gate && p.gates > 1;
-  Vec16<T> nx[NV], nh[NV];
+  Words16<T> nx[NV], nh[NV];
   ParamVec<P, N> ng[NV];
   auto load = [&](int64_t at) {
     const bool in = at < p.rows;
 #pragma unroll
     for (int k = 0; k < NV; k++) {
       const int c = (k * lanes + lane) * N, n = in ? D - c : 0;
-      nx[k] = load_raw(static_cast<const T*>(p.x) + at * D + c, n);
-      if (p.h) nh[k] = load_raw(static_cast<const T*>(p.h) + at * D + c, n);
+      nx[k] = load_words<false>(static_cast<const T*>(p.x) + at * D + c, n);
+      if (p.h) nh[k] = load_words<false>(static_cast<const T*>(p.h) + at * D + c, n);
       if (row_gates) ng[k].load(static_cast<const P*>(p.gate) + (int64_t)((uint32_t)at / rows_gate) * D + c, n);
     }
   };
@@ -125,9 +122,9 @@ __global__ __launch_bounds__((kBlock ? most_threads<T, NV>() : kThreads)) void r
     for (int k = 0; k < NV; k++)
 #pragma unroll
       for (int i = 0; i < N; i++) {
-        r[k][i] = to_f32(nx[k].v[i]);
+        r[k][i] = to_f32(nx[k][i]);
         if (p.h) {
-          t[k][i] = to_f32(nh[k].v[i]);
+          t[k][i] = to_f32(nh[k][i]);
           s = fmaf(t[k][i], t[k][i], s);
           if (row_gates) gate[k][i] = ng[k][i];
         }
@@ -207,7 +204,7 @@ struct Items {
 };
 
 template <typename T, typename P, int NV, bool kBlock, bool kEach>
-__global__ __launch_bounds__((kBlock ? most_threads<T, NV>() : kThreads), (NV == 1 && !kEach ? 4 : 1)) void residual_norm_backward_kernel(ResidualNormParams p, int lanes,
+__global__ __launch_bounds__((kBlock ? kMostThreads : kThreads), (NV * Vec16<T>::kN <= 8 && (NV == 1 || kBlock) && !kEach ? 4 : 1)) void residual_norm_backward_kernel(ResidualNormParams p, int lanes,
                                                                                                      Items items) {
   constexpr int N = Vec16<T>::kN;
   constexpr bool kAhead = NV * N < 16;   // a row's gate loaded with the row before; past the registers else
@@ -241,7 +238,7 @@ __global__ __launch_bounds__((kBlock ? most_threads<T, NV>() : kThreads), (NV ==
         if constexpr (!kEach) w[k][i] *= gate[k][i];
         acc[k][i] = 0.0f;
       }
-    Vec16<T> nr[NV], nh[NV], ndr[NV], ndy[NV];
+    Words16<T> nr[NV], nh[NV], ndr[NV], ndy[NV];
     ParamVec<P, N> ng[NV];
     float na = 1.0f, nc = 0.0f;
     auto load = [&](int64_t at) {
@@ -249,10 +246,10 @@ __global__ __launch_bounds__((kBlock ? most_threads<T, NV>() : kThreads), (NV ==
 #pragma unroll
       for (int k = 0; k < NV; k++) {
         const int c = (k * lanes + lane) * N, n = in ? D - c : 0;
-        if (p.pre) nr[k] = load_raw(static_cast<const T*>(p.r) + at * D + c, n);
-        if (p.h) nh[k] = load_raw(static_cast<const T*>(p.h) + at * D + c, n);
-        ndr[k] = load_raw(static_cast<const T*>(p.dr) + at * D + c, p.dr ? n : 0);
-        if (p.pre) ndy[k] = load_raw(static_cast<const T*>(p.dy) + at * D + c, p.dy ? n : 0);
+        if (p.pre) nr[k] = load_words<false>(static_cast<const T*>(p.r) + at * D + c, n);
+        if (p.h) nh[k] = load_words<false>(static_cast<const T*>(p.h) + at * D + c, n);
+        ndr[k] = load_words<false>(static_cast<const T*>(p.dr) + at * D + c, p.dr ? n : 0);
+        if (p.pre) ndy[k] = load_words<false>(static_cast<const T*>(p.dy) + at * D + c, p.dy ? n : 0);
         if constexpr (kEach && kAhead) ng[k].load(static_cast<const P*>(p.gate) + at * D + c, n);
       }
       if (in && p.post) na = p.rstd_post[at];
@@ -268,8 +265,8 @@ __global__ __launch_bounds__((kBlock ? most_threads<T, NV>() : kThreads), (NV ==
         for (int k = 0; k < NV; k++)
 #pragma unroll
           for (int i = 0; i < N; i++) {
-            const float g = to_f32(ndy[k].v[i]);
-            hat[k][i] = to_f32(nr[k].v[i]) * c0;
+            const float g = to_f32(ndy[k][i]);
+            hat[k][i] = to_f32(nr[k][i]) * c0;
             dpre[k][i] = fmaf(g, hat[k][i], dpre[k][i]);
             e[k][i] = g * pre[k][i];   // past the row's end zero
             s = fmaf(e[k][i], hat[k][i], s);
@@ -278,19 +275,19 @@ __global__ __launch_bounds__((kBlock ? most_threads<T, NV>() : kThreads), (NV ==
 #pragma unroll
         for (int k = 0; k < NV; k++)
 #pragma unroll
-          for (int i = 0; i < N; i++) e[k][i] = fmaf(c0, e[k][i] - hat[k][i] * s, to_f32(ndr[k].v[i]));
+          for (int i = 0; i < N; i++) e[k][i] = fmaf(c0, e[k][i] - hat[k][i] * s, to_f32(ndr[k][i]));
       } else {
 #pragma unroll
         for (int k = 0; k < NV; k++)
 #pragma unroll
-          for (int i = 0; i < N; i++) e[k][i] = to_f32(ndr[k].v[i]);
+          for (int i = 0; i < N; i++) e[k][i] = to_f32(ndr[k][i]);
       }
       if (p.h) {
 #pragma unroll
         for (int k = 0; k < NV; k++)
 #pragma unroll
           for (int i = 0; i < N; i++) {
-            hat[k][i] = to_f32(nh[k].v[i]) * a;
+            hat[k][i] = to_f32(nh[k][i]) * a;
             if constexpr (kEach && kAhead) gate[k][i] = ng[k][i];
           }
       }
@@ -354,9 +351,9 @@ struct Shape {
   bool block;
 };
 Shape shape_of(int cols, int dtype) {
-  const int n = dtype == NEST_DTYPE_F32 ? 4 : 8, vecs = (cols + n - 1) / n, most = dtype == NEST_DTYPE_F32 ? 1024 : 512;
+  const int n = dtype == NEST_DTYPE_F32 ? 4 : 8, vecs = (cols + n - 1) / n;
   if (vecs <= 128) return {vecs <= 64 ? pow2_at_least(vecs) : 64, (vecs + 63) / 64, false};
-  const int nv = vecs <= most ? 1 : dtype == NEST_DTYPE_F32 ? 4 : 2;
+  const int nv = vecs <= kMostThreads ? 1 : vecs <= 2 * kMostThreads ? 2 : 4;   // 4: float32 alone
   return {(vecs + 64 * nv - 1) / (64 * nv) * 64, nv, true};
 }
 
@@ -367,7 +364,8 @@ void with_shape(const Shape& h, F f) {
     if (h.nv == 1) f(integral_constant<int, 1>(), integral_constant<bool, false>());
     else f(integral_constant<int, 2>(), integral_constant<bool, false>());
   } else if (h.nv == 1) f(integral_constant<int, 1>(), integral_constant<bool, true>());
-  else f(integral_constant<int, sizeof(T) == 4 ? 4 : 2>(), integral_constant<bool, true>());
+  else if (sizeof(T) == 2 || h.nv == 2) f(integral_constant<int, 2>(), integral_constant<bool, true>());
+  else if constexpr (sizeof(T) == 4) f(integral_constant<int, 4>(), integral_constant<bool, true>());
 }
 
 int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
@@ -388,7 +386,7 @@ Plan plan_of(int64_t rows, int cols, int dtype, int64_t gates) {
   const Shape h = shape_of(cols, dtype);
   const int waves = h.block ? h.lanes / 64 : kThreads / 64;
   const int values = h.nv * (dtype == NEST_DTYPE_F32 ? 4 : 8);   // a lane's
-  const int a_cu = values == 4 ? 20 : values == 8 ? (h.nv == 1 && !l.each ? 16 : 12) : 8;   // waves, by the registers
+  const int a_cu = values == 4 ? 20 : values == 8 ? ((h.nv == 1 || h.block) && !l.each ? 16 : 12) : 8;   // waves, by the registers
   const int64_t most = 256 * (a_cu > waves ? a_cu / waves : 1);
   const int64_t n = l.each || gates == 0 ? 1 : gates;
   l.items.rows = rows / n;

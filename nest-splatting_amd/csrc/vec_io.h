@@ -54,17 +54,32 @@ __device__ __forceinline__ void store_whole(void* p, const V& v) {
   else *static_cast<u32_any*>(p) = __builtin_bit_cast(uint32_t, v);
 }
 
-// kWhole: rows are whole vectors, so n is <= 0 or kN at least; that leaves out
-// the code of a row's end, for every load.
+// The same 16 bytes as words: where a load may be skipped, an array of 16-bit
+// elements takes a register each from there to its use, twice as many.
+template <typename T>
+struct Words16 {
+  static constexpr int kN = 16 / (int)sizeof(T);
+  uint32_t w[4];
+  __device__ __forceinline__ T operator[](int i) const {
+    if constexpr (sizeof(T) == 4) return __builtin_bit_cast(T, w[i]);
+    else return __builtin_bit_cast(T, (uint16_t)(w[i / 2] >> (i % 2 * 16)));
+  }
+};
+
+// kWhole: rows are whole vectors, so n is <= 0 or kN at least.
 template <bool kWhole, typename T>
-__device__ __forceinline__ Vec16<T> load_piece(const T* p, int n) {
-  if constexpr (!kWhole) return load_raw(p, n);
-  Vec16<T> t;
-  if (n > 0) {
+__device__ __forceinline__ Words16<T> load_words(const T* p, int n) {
+  constexpr int N = Words16<T>::kN;
+  Words16<T> t = {{0, 0, 0, 0}};
+  if (kWhole ? n > 0 : n >= N) {
     __builtin_memcpy(&t, p, 16);
-  } else {
+  } else if (!kWhole) {
 #pragma unroll
-    for (int i = 0; i < Vec16<T>::kN; i++) t.v[i] = (T)0.0f;
+    for (int i = 0; i < N; i++)
+      if (i < n) {
+        if constexpr (sizeof(T) == 4) t.w[i] = __builtin_bit_cast(uint32_t, p[i]);
+        else t.w[i / 2] |= (uint32_t)__builtin_bit_cast(uint16_t, p[i]) << (i % 2 * 16);
+      }
   }
   return t;
 }
