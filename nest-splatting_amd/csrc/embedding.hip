@@ -106,32 +106,41 @@ __global__ __launch_bounds__(kThreads) void embedding_keys_kernel(const I* ids, 
 
 // Sorted at once: a position's place is the number of keys before its own.  A
 // workgroup takes kRanked positions and compares each with all keys, kThreads /
-// kRanked threads a position.  N^2 comparisons, spread over the chip.
+// kRanked threads a position.  N^2 comparisons, spread over the chip: 8192
+// positions take less time than the six launches of a radix sort.
 constexpr int64_t kMostRanked = 8192;
 constexpr int kRanked = 16;
-template <typename I>
-__global__ __launch_bounds__(kThreads) void embedding_rank_kernel(const I* ids, int rows, int64_t table_rows, uint32_t* sorted, uint32_t* index) {
+__global__ __launch_bounds__(kThreads) void embedding_rank_kernel(const uint32_t* from, int rows, uint32_t* sorted, uint32_t* index) {
   constexpr int kSlices = kThreads / kRanked;
-  __shared__ __attribute__((aligned(16))) uint32_t keys[kMostRanked];
+  __shared__ uint4 keys[kMostRanked / 4];
   __shared__ int counts[kSlices][kRanked];
-  const int padded = (rows + 4 * kSlices - 1) / (4 * kSlices) * (4 * kSlices);
-  for (int i = threadIdx.x; i < padded; i += kThreads * 8) {   // eight loads in flight
-    I id[8];
+  constexpr int kLoads = kMostRanked / 4 / kThreads;
+  uint4 v[kLoads];
+  const int pieces = (rows + 3) / 4;   // the keys' array ends after whole pieces
 #pragma unroll
-    for (int u = 0; u < 8; u++) id[u] = i + u * kThreads < rows ? ids[i + u * kThreads] : 0;
-#pragma unroll
-    for (int u = 0; u < 8; u++)
-      if (i + u * kThreads < padded) keys[i + u * kThreads] = i + u * kThreads < rows ? key_of(id[u], table_rows) : kNoRun;
+  for (int u = 0; u < kLoads; u++) {
+    const int i = u * kThreads + threadIdx.x;
+    v[u] = i < pieces ? reinterpret_cast<const uint4*>(from)[i] : make_uint4(kNoRun, kNoRun, kNoRun, kNoRun);
+    if (i * 4 + 1 >= rows) v[u].y = kNoRun;
+    if (i * 4 + 2 >= rows) v[u].z = kNoRun;
+    if (i * 4 + 3 >= rows) v[u].w = kNoRun;
   }
+#pragma unroll
+  for (int u = 0; u < kLoads; u++) keys[u * kThreads + threadIdx.x] = v[u];
   __syncthreads();
-  const int t = threadIdx.x % kRanked, slice = threadIdx.x / kRanked, mine = blockIdx.x * kRanked + t;
-  const int per = padded / kSlices;
-  const uint32_t key = mine < rows ? keys[mine] : 0;
+  const int t = threadIdx.x % kRanked, slice = threadIdx.x / kRanked, first = blockIdx.x * kRanked, mine = first + t;
+  const int per = (pieces + kSlices - 1) / kSlices | 1;   // pieces of 4 keys; odd, so the slices of a wave fall on different banks
+  const int begin = slice * per, end = begin + per < pieces ? begin + per : pieces;
+  const uint32_t key = mine < rows ? reinterpret_cast<const uint32_t*>(keys)[mine] : 0;
   int count = 0;
-#pragma unroll 4
-  for (int j = slice * per; j < (slice + 1) * per; j += 4) {
-    const uint4 k = *reinterpret_cast<const uint4*>(&keys[j]);
-    count += (k.x < key + (j < mine)) + (k.y < key + (j + 1 < mine)) + (k.z < key + (j + 2 < mine)) + (k.w < key + (j + 3 < mine));
+  if (end * 4 <= first || begin * 4 >= first + kRanked) {   // all before, or all after these positions
+    const uint32_t least = end * 4 <= first ? key + 1 : key;
+#pragma unroll 8
+    for (int j = begin; j < end; j++) count += (keys[j].x < least) + (keys[j].y < least) + (keys[j].z < least) + (keys[j].w < least);
+  } else {
+    for (int j = begin; j < end; j++)
+      count += (keys[j].x < key + (j * 4 < mine)) + (keys[j].y < key + (j * 4 + 1 < mine)) + (keys[j].z < key + (j * 4 + 2 < mine)) +
+               (keys[j].w < key + (j * 4 + 3 < mine));
   }
   counts[slice][t] = count;
   __syncthreads();
@@ -402,7 +411,7 @@ __global__ __launch_bounds__(kCountThreads, (FD < 8 && FV * FD <= kTwiceCounted 
       for (int j = 0; j < FD; j++) b[j] = fragment<T, false, R>(tile[buf], base, j, kb);
 #pragma unroll
       for (int i = 0; i < FV; i++) {
-        if (i * 8 + wave >= frags) break;
+        if (i == FV - 1 && i * 8 + wave >= frags) break;   // no branch before the last: it would part the products
         uint32_t ones[4];
 #pragma unroll
         for (int e = 0; e < 4; e++) {
@@ -502,10 +511,8 @@ Plan plan_of(int64_t rows, int cols, int64_t table_rows, int dtype) {
   l.ranked = rows <= kMostRanked;
   l.chunk = chunk_of(rows, cols, dtype == NEST_DTYPE_F32 ? 4 : 8);
   l.chunks = cdiv(rows, l.chunk);
-  if (!l.ranked) {
-    l.keys = take((size_t)rows * 4);
-    l.sort = take(index_sort_ws_bytes(rows));
-  }
+  l.keys = take((size_t)(rows + 3) / 4 * 16);
+  if (!l.ranked) l.sort = take(index_sort_ws_bytes(rows));
   l.sorted = take((size_t)(rows + kBatch) * 4);
   l.index = take((size_t)(rows + kBatch) * 4);
   l.part = take((size_t)l.chunks * 2 * cols * 4);
@@ -572,9 +579,9 @@ hipError_t sort_ids(const EmbeddingParams& p, const Plan& l, uint32_t* sorted, u
   const I* ids = static_cast<const I*>(p.ids);
   const int64_t bytes = p.table_rows * p.cols * (int64_t)sizeof(T), pieces = cdiv(bytes, 16 * kThreads);
   uint32_t* keys = reinterpret_cast<uint32_t*>(ws + l.keys);
-  const int64_t need = !l.ranked && cdiv(p.rows, kThreads) > pieces ? cdiv(p.rows, kThreads) : pieces;
-  embedding_keys_kernel<I><<<(unsigned)(need < 8192 ? need : 8192), kThreads, 0, s>>>(ids, l.ranked ? 0 : p.rows, p.table_rows, keys, table, bytes);
-  if (l.ranked) embedding_rank_kernel<I><<<(unsigned)cdiv(p.rows, kRanked), kThreads, 0, s>>>(ids, (int)p.rows, p.table_rows, sorted, index);
+  const int64_t need = cdiv(p.rows, kThreads) > pieces ? cdiv(p.rows, kThreads) : pieces;
+  embedding_keys_kernel<I><<<(unsigned)(need < 8192 ? need : 8192), kThreads, 0, s>>>(ids, p.rows, p.table_rows, keys, table, bytes);
+  if (l.ranked) embedding_rank_kernel<<<(unsigned)cdiv(p.rows, kRanked), kThreads, 0, s>>>(keys, (int)p.rows, sorted, index);
   if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
   if (l.ranked) return hipSuccess;
   int bits = 1;

@@ -25,7 +25,7 @@ namespace {
 
 // Groups of 16 rows that a wave takes in a turn: two share a read of the
 // weights.
-constexpr int forward_groups(int ki, int ko) { return ki + ko <= 5 ? 2 : 1; }
+constexpr int forward_groups(int ki, int ko) { return ki + ko <= 4 ? 2 : 1; }
 
 template <typename T>
 struct NarrowLayer {
@@ -73,23 +73,22 @@ __device__ __forceinline__ void store_bytes(uint8_t* p, uint2 v, int n) {
 }
 __device__ __forceinline__ float byte_of(uint2 v, int i) { return (float)(((i < 4 ? v.x : v.y) >> (i % 4 * 8)) & 0xffu); }
 
-// Feature of the first operand's row m in half jj of 32: lane quarter q's sums
-// of the two halves are features 8 q .. 8 q + 7.
-__device__ __forceinline__ int feature_of(int m, int jj) { return 8 * (m >> 2) + (m & 3) + 4 * jj; }
-
 // A [rows][cols] matrix of the weights (transposed: [cols][rows] in memory) to
-// LDS, zeros around it.
+// LDS, zeros around it, its rows in the order that the products read them:
+// pitches of an odd number of 16 bytes, so 16 rows one after another fall on
+// different banks.
 template <typename T, int R, int C, bool kTransposed>
 __device__ __forceinline__ void stage_weights(T* lds, const T* w, int rows, int cols) {
   constexpr int kPitch = C + 8;
   for (int i = threadIdx.x; i < R * C; i += 256) {
     const int r = kTransposed ? i % R : i / C, c = kTransposed ? i / R : i % C;
-    lds[r * kPitch + c] = r < rows && c < cols ? w[kTransposed ? c * rows + r : r * cols + c] : (T)0.0f;
+    lds[((r & ~31) | (r >> 2 & 1) << 4 | (r >> 3 & 3) << 2 | (r & 3)) * kPitch + c] = r < rows && c < cols ? w[kTransposed ? c * rows + r : r * cols + c] : (T)0.0f;
   }
 }
 
 // acc[jj][g] over K / 32 steps, from init on: features 32 J + 8 (lane / 16) +
-// 4 jj + 0..3 of row lane % 16 of group g.
+// 4 jj + 0..3 of row lane % 16 of group g.  Row m of the first operand in half
+// jj of 32 is feature 8 (m / 4) + m % 4 + 4 jj.
 template <typename T, int K, int G>
 __device__ __forceinline__ void narrow_product(const T* lds, int J, const typename Mma<T>::Frag (&rows)[G][K / 32], const f32x4 (&init)[2],
                                                f32x4 (&acc)[2][G]) {
@@ -102,7 +101,7 @@ __device__ __forceinline__ void narrow_product(const T* lds, int J, const typena
   for (int k = 0; k < K / 32; k++)
 #pragma unroll
     for (int jj = 0; jj < 2; jj++) {
-      const auto a = *reinterpret_cast<const typename Mma<T>::Frag*>(lds + (32 * J + feature_of(r, jj)) * (K + 8) + k * 32 + q * 8);
+      const auto a = *reinterpret_cast<const typename Mma<T>::Frag*>(lds + (32 * J + 16 * jj + r) * (K + 8) + k * 32 + q * 8);
 #pragma unroll
       for (int g = 0; g < G; g++) acc[jj][g] = Mma<T>::run(a, rows[g][k], acc[jj][g]);
     }
@@ -114,12 +113,19 @@ __device__ __forceinline__ void stage_bias(f32x4* lds, const T* bias, int out, i
   for (int i = threadIdx.x; i < padded; i += 256) reinterpret_cast<float*>(lds)[i] = bias && i < out ? to_f32(bias[i]) : 0.0f;
 }
 
-// kKept: the slopes' codes are written too.
+// Row of 16 in LDS, in 8 bytes.
+template <int KO>
+constexpr int kCodePitch = KO * 4 + 2;
+
+// kKept: the slopes' codes are written too, a row's side by side through LDS: a
+// wave's own, eight bytes a lane, are 32 bytes of each of 16 rows, and memory
+// took 46% more requests for them than their bytes need.
 template <typename T, int KI, int KO, bool kKept>
-__global__ __launch_bounds__(256) void narrow_layer_kernel(NarrowLayer<T> p) {
+__global__ __launch_bounds__(256, 3) void narrow_layer_kernel(NarrowLayer<T> p) {
   typedef typename Mma<T>::Frag Frag;
   __shared__ __attribute__((aligned(16))) T w[KO * 32 * (KI * 32 + 8)];
   __shared__ f32x4 bias[KO * 8];
+  __shared__ __attribute__((aligned(16))) uint2 codes[kKept ? 4 : 1][kKept ? 16 * kCodePitch<KO> : 1];   // of a wave's 16 rows
   stage_weights<T, KO * 32, KI * 32, false>(w, p.w, p.out, p.in);
   stage_bias(bias, p.bias, p.out, KO * 32);
   __syncthreads();
@@ -152,6 +158,7 @@ __global__ __launch_bounds__(256) void narrow_layer_kernel(NarrowLayer<T> p) {
       for (int k = 0; k < KO; k++) add[g][k] = res[g][k];
     }
     load(row + step);   // on its way while this turn is worked on
+    uint2 mine[G][kKept ? KO : 1];
 #pragma unroll
     for (int J = 0; J < KO; J++) {
       const f32x4 init[2] = {bias[J * 8 + q * 2], bias[J * 8 + q * 2 + 1]};
@@ -160,26 +167,47 @@ __global__ __launch_bounds__(256) void narrow_layer_kernel(NarrowLayer<T> p) {
       const int c = J * 32 + q * 8;
 #pragma unroll
       for (int g = 0; g < G; g++) {
-        const int64_t at = (row + g * 16) * p.out + c;
-        const int n = row + g * 16 < p.rows ? p.out - c : 0;
         float v[8];
-        uint2 codes = make_uint2(0, 0);
+        uint2 code = make_uint2(0, 0);
         with_activation(p.act, [&](auto act) {
 #pragma unroll
           for (int e = 0; e < 8; e++) {
             float slope;
             v[e] = activate<T, act.value, kKept>(acc[e >> 2][g][e & 3], slope);
-            if constexpr (kKept) (e < 4 ? codes.x : codes.y) |= (uint32_t)coarse_code(slope) << (e % 4 * 8);
+            if constexpr (kKept) (e < 4 ? code.x : code.y) |= (uint32_t)coarse_code(slope) << (e % 4 * 8);
           }
         });
-        if constexpr (kKept) store_bytes(p.kept + at, codes, n);
+        if constexpr (kKept) mine[g][J] = code;
         if (p.residual) {
 #pragma unroll
           for (int e = 0; e < 8; e++) v[e] += to_f32(add[g][J][e]);
         }
-        store_vec<T>(p.y + at, v, n);
+        store_vec<T>(p.y + (row + g * 16) * p.out + c, v, row + g * 16 < p.rows ? p.out - c : 0);
       }
       __builtin_amdgcn_sched_barrier(0);   // one 32 features at a time: their registers are the next one's
+    }
+    if constexpr (kKept) {
+      uint2* const stage = codes[wave_id()];
+#pragma unroll
+      for (int g = 0; g < G; g++) {
+#pragma unroll
+        for (int J = 0; J < KO; J++) stage[r * kCodePitch<KO> + J * 4 + q] = mine[g][J];
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int u = 0; u < (KO + 1) / 2; u++) {   // 16 bytes: KO * 2 to a row
+          const int t = u * 64 + lane, at = t / (KO * 2), c = t % (KO * 2) * 16;
+          const int64_t to = row - r + g * 16 + at;
+          if (at < 16 && to < p.rows) {
+            const uint4 v = *reinterpret_cast<const uint4*>(&stage[at * kCodePitch<KO> + c / 8]);
+            uint8_t* const y = p.kept + to * p.out + c;
+            store_bytes(y, make_uint2(v.x, v.y), p.out - c);
+            store_bytes(y + 8, make_uint2(v.z, v.w), p.out - c - 8);
+          }
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+      }
     }
   }
 }
@@ -291,6 +319,12 @@ __global__ __launch_bounds__(256, narrow_groups_cu(KI, KO)) void narrow_layer_ba
 #pragma unroll
             for (int e = 0; e < 8; e++) activate<T, act.value>(z[g][e], z[g][e]);   // the slope in its place
         });
+        if (J == KO - 1 && p.out % 32) {   // of no feature: an infinity in x makes its z NaN
+#pragma unroll
+          for (int g = 0; g < G; g++)
+#pragma unroll
+            for (int e = 0; e < 8; e++) z[g][e] = J * 32 + q * 8 + e < p.out ? z[g][e] : 0.0f;
+        }
       }
 #pragma unroll
       for (int g = 0; g < G; g++)
@@ -299,7 +333,6 @@ __global__ __launch_bounds__(256, narrow_groups_cu(KI, KO)) void narrow_layer_ba
           float d = to_f32(dy[g][J][e]);   // zero past the ends
           if (kSaved && p.slopes) d *= coarse_slope(byte_of(slopes[g][J], e));
           else if (again) d *= z[g][e];
-          if (J == KO - 1 && J * 32 + q * 8 + e >= p.out) d = 0.0f;   // of no feature: an infinity in x makes its z NaN
           dz[g][J][e] = from_f32<T>(d);
           db[J][e] += d;
         }
