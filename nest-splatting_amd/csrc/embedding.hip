@@ -133,15 +133,13 @@ __global__ __launch_bounds__(kThreads) void embedding_rank_kernel(const uint32_t
   const int begin = slice * per, end = begin + per < pieces ? begin + per : pieces;
   const uint32_t key = mine < rows ? reinterpret_cast<const uint32_t*>(keys)[mine] : 0;
   int count = 0;
-  if (end * 4 <= first || begin * 4 >= first + kRanked) {   // all before, or all after these positions
-    const uint32_t least = end * 4 <= first ? key + 1 : key;
 #pragma unroll 8
-    for (int j = begin; j < end; j++) count += (keys[j].x < least) + (keys[j].y < least) + (keys[j].z < least) + (keys[j].w < least);
-  } else {
-    for (int j = begin; j < end; j++)
-      count += (keys[j].x < key + (j * 4 < mine)) + (keys[j].y < key + (j * 4 + 1 < mine)) + (keys[j].z < key + (j * 4 + 2 < mine)) +
-               (keys[j].w < key + (j * 4 + 3 < mine));
+  for (int j = begin; j < end; j++) {
+    const uint32_t least = j * 4 < first ? key + 1 : key;   // equal keys before these positions count too
+    count += (keys[j].x < least) + (keys[j].y < least) + (keys[j].z < least) + (keys[j].w < least);
   }
+  if (slice == 0)
+    for (int j = first; j < mine; j++) count += reinterpret_cast<const uint32_t*>(keys)[j] == key;
   counts[slice][t] = count;
   __syncthreads();
   if (slice == 0 && mine < rows) {
@@ -303,11 +301,9 @@ int chunk_of(int64_t n, int cols, int values) {
 // ---- gradient: a small table in the accumulators ----
 
 constexpr int kCountThreads = 512, kCountRows = 256;   // of a workgroup's turn
-// Accumulators of 16 x 16 that a wave holds, by its 16s of columns: 128
-// registers at most, 96 where the next turn's rows take 32; up to 48 leave room
-// for two workgroups a CU, whose loads overlap.
-constexpr int most_counted(int fd) { return fd == 8 ? 24 : 32; }
-constexpr int kTwiceCounted = 12;
+// Accumulators of 16 x 16 that a wave holds: up to 12 leave room for two
+// workgroups a CU, whose loads overlap.
+constexpr int kMostCounted = 16, kTwiceCounted = 12;
 
 template <typename T>
 struct Counted {
@@ -473,13 +469,14 @@ __global__ __launch_bounds__(1024) void embedding_sum_kernel(const float* part, 
 
 int column_frags(int cols) { return pow2_at_least(cdiv(cols, 16)); }
 
-// Whether the table's sums fit a workgroup of eight waves.
-//
-// TODO-RULE
+// Whether the table's sums are made in accumulators.  us, so and sorted, for
+// bf16 rows: 1,702,400 x 64 of 16 ids 50 and 97, of 300 (12 accumulators) 95
+// and 124, of 1000 (32) 214 and 126; 1,702,400 x 128 of 100 (8) 124 and 143, of
+// 380 (24) 180 and 181; 65,536 x 64 of 300 29 and 42; 2000 x 64 of 300 19 and 23,
+// of 1000 43 and 23.
 bool counted(int64_t rows, int cols, int64_t table_rows, int dtype) {
   if (dtype == NEST_DTYPE_F32 || cols > 128) return false;
-  const int fd = column_frags(cols);
-  return cdiv(table_rows, 16 * 8) * fd <= most_counted(fd);
+  return cdiv(table_rows, 16 * 8) * column_frags(cols) <= kMostCounted;
 }
 
 struct Plan {
@@ -548,18 +545,16 @@ hipError_t count_gradient(const EmbeddingParams& p, const Plan& l, hipStream_t s
                      reinterpret_cast<uint32_t*>(ws + l.flags), size};
   embedding_clear_kernel<<<(unsigned)cdiv(size, kThreads), kThreads, 0, s>>>(q.flags, size);
   auto launch = [&](auto fd) {
-    constexpr int FD = fd.value, kMost = most_counted(FD) / FD;
+    constexpr int FD = fd.value, kMost = kMostCounted / FD;
     const int need = (int)cdiv(p.table_rows, 16 * 8);
     auto with = [&](auto fv) { embedding_count_kernel<T, fv.value, FD><<<(unsigned)l.groups, kCountThreads, 0, s>>>(q); };
     if constexpr (FD == 8) {
       if (need == 1) with(Number<1>());
-      else if (need == 2) with(Number<2>());
-      else with(Number<3>());
+      else with(Number<2>());
     } else {
-      if (need * 8 <= kMost) with(Number<kMost / 8>());
-      else if (need * 4 <= kMost) with(Number<kMost / 4>());
-      else if (need * 8 <= kMost * 3) with(Number<kMost * 3 / 8>());
+      if (need * 4 <= kMost) with(Number<kMost / 4>());
       else if (need * 2 <= kMost) with(Number<kMost / 2>());
+      else if (need * 4 <= kMost * 3) with(Number<kMost * 3 / 4>());
       else with(Number<kMost>());
     }
   };

@@ -377,8 +377,7 @@ struct Plan {
   Items items;
   int groups;                // workgroups
   bool each;
-  size_t s, dpre, sums;      // floats into the workspace
-  size_t floats;
+  size_t s, dpre, floats;    // into the workspace
 };
 Plan plan_of(int64_t rows, int cols, int dtype, int64_t gates) {
   Plan l{};
@@ -396,8 +395,7 @@ Plan plan_of(int64_t rows, int cols, int dtype, int64_t gates) {
   l.groups = (int)(l.items.n < most ? l.items.n : most);
   l.s = 0;
   l.dpre = (size_t)l.items.n * cols;
-  l.sums = l.dpre + (size_t)l.groups * cols;
-  l.floats = l.sums + (n > 1 ? (size_t)n * cols : 0);
+  l.floats = l.dpre + (size_t)l.groups * cols;
   return l;
 }
 
@@ -430,18 +428,18 @@ hipError_t backward(const ResidualNormParams& p, hipStream_t s) {
   }
   SumTasks tasks{};
   int n = 0;
-  if (p.pre) tasks.t[n++] = {l.items.dpre, l.groups, 1, p.cols, nullptr, nullptr, nullptr, p.dpre, nullptr, nullptr};
+  if (p.pre) tasks.t[n++] = {l.items.dpre, l.groups, 1, p.cols, nullptr, nullptr, nullptr, p.dpre, nullptr, 1};
   if (l.items.s) {
-    if (l.each) tasks.t[n++] = {l.items.s, l.items.n, 1, p.cols, nullptr, nullptr, nullptr, p.dpost, nullptr, nullptr};
-    else if (many) tasks.t[n++] = {l.items.s, l.items.parts, p.gates, p.cols, nullptr, p.post, nullptr, p.dgate, nullptr, p.ws + l.sums};
-    else tasks.t[n++] = {l.items.s, l.items.n, 1, p.cols, nullptr, p.post, p.gate, gate ? p.dgate : nullptr, post ? p.dpost : nullptr, nullptr};
+    if (l.each) {
+      tasks.t[n++] = {l.items.s, l.items.n, 1, p.cols, nullptr, nullptr, nullptr, p.dpost, nullptr, 1};
+    } else if (many) {
+      tasks.t[n++] = {l.items.s, l.items.parts, p.gates, p.cols, nullptr, p.post, nullptr, p.dgate, nullptr, 1};
+      if (post) tasks.t[n++] = {l.items.s, l.items.n, 1, p.cols, p.gate, nullptr, nullptr, p.dpost, nullptr, (uint32_t)l.items.parts};
+    } else {
+      tasks.t[n++] = {l.items.s, l.items.n, 1, p.cols, nullptr, p.post, p.gate, gate ? p.dgate : nullptr, post ? p.dpost : nullptr, 1};
+    }
   }
-  if (n == 0) return hipSuccess;
-  if (hipError_t e = launch_column_sums<P>(tasks, n, s); e != hipSuccess) return e;
-  if (!many || !post) return hipSuccess;
-  SumTasks last{};   // dpost, from every gate's S
-  last.t[0] = {p.ws + l.sums, p.gates, 1, p.cols, p.gate, nullptr, nullptr, p.dpost, nullptr, nullptr};
-  return launch_column_sums<P>(last, 1, s);
+  return n ? launch_column_sums<P>(tasks, n, s) : hipSuccess;
 }
 
 }  // namespace

@@ -269,30 +269,39 @@ def linear(x, weight, bias=None, activation: Optional[str] = None, residual=None
 
 # ---- the residual stream between two norms ----
 
+def _gates(x, gate):
+    """How many rows of gates there are, for a gate whose shape is not a row's."""
+    D = x.shape[-1]
+    if gate.dim() < 1 or gate.shape[-1] != D:
+        raise ValueError(f"gate of shape {tuple(gate.shape)} does not end in {D} values")
+    lead = list(gate.shape[:-1])
+    while lead and lead[-1] == 1:
+        lead.pop()
+    parts = x.dim() == 2 and len(lead) == 1 and lead[0] > 0 and x.shape[0] % lead[0] == 0
+    if not parts and lead != list(x.shape[:-1][:len(lead)]):
+        raise ValueError(f"gate of shape {tuple(gate.shape)} does not fit x of {tuple(x.shape)}: its leading dimensions are the first of x's")
+    return gate.numel() // D
+
+
 def _norm_params(x, gate, post, pre):
     """(code, parameters' code, gates, gate, post, pre): checked, contiguous, gate as [gates, cols]."""
     code = _code(x, "x")
     if x.dim() < 1 or not 1 <= x.shape[-1] <= MAX_NORM_COLS:
         raise ValueError(f"rows of 1 to {MAX_NORM_COLS} values are supported, x has shape {tuple(x.shape)}")
-    D = x.shape[-1]
-    pdt = next((t.dtype for t in (post, pre, gate) if t is not None), x.dtype)
-    if pdt not in (torch.float32, x.dtype):
-        raise TypeError(f"gate, post and pre are {pdt}: float32 or the type of x ({x.dtype}) is expected")
-    post = post if post is None else _like(post, x, (D,), "post", pdt)
-    pre = pre if pre is None else _like(pre, x, (D,), "pre", pdt)
+    row = x.shape[-1:]
+    some = post if post is not None else pre if pre is not None else gate
+    dtype = x.dtype if some is None else some.dtype
+    if dtype is not x.dtype and dtype is not torch.float32:
+        raise TypeError(f"gate, post and pre are {dtype}: float32 or the type of x ({x.dtype}) is expected")
+    if post is not None:
+        post = _like(post, x, row, "post", dtype)
+    if pre is not None:
+        pre = _like(pre, x, row, "pre", dtype)
     gates = 0
     if gate is not None:
-        if gate.dim() < 1 or gate.shape[-1] != D:
-            raise ValueError(f"gate of shape {tuple(gate.shape)} does not end in {D} values")
-        lead = list(gate.shape[:-1])
-        while lead and lead[-1] == 1:
-            lead.pop()
-        parts = x.dim() == 2 and len(lead) == 1 and lead[0] > 0 and x.shape[0] % lead[0] == 0
-        if not parts and lead != list(x.shape[:-1][:len(lead)]):
-            raise ValueError(f"gate of shape {tuple(gate.shape)} does not fit x of {tuple(x.shape)}: its leading dimensions are the first of x's")
-        gate = _like(gate, x, gate.shape, "gate", pdt)
-        gates = gate.numel() // D
-    return code, _CODE[pdt], gates, gate, post, pre
+        gates = 1 if gate.shape == row else _gates(x, gate)
+        gate = _like(gate, x, gate.shape, "gate", dtype)
+    return code, _CODE[dtype], gates, gate, post, pre
 
 
 def residual_norm_forward(x: torch.Tensor, h: Optional[torch.Tensor] = None, gate: Optional[torch.Tensor] = None,
