@@ -43,8 +43,8 @@ LinearLayout linear_layout(const LinearParams& p, bool back) {
   if (l.narrow) {
     if (!back) return l;
     // as many workgroups as run at once, by LDS and registers
-    const int ki = (p.in + 31) / 32, ko = (p.out + 31) / 32, a_cu = narrow_groups_cu(ki, ko);
-    const int64_t turns = cdiv(p.rows, 64 * narrow_groups(ki, ko));
+    const int ki = (p.in + 31) / 32, ko = (p.out + 31) / 32, a_cu = narrow_groups_cu(ki, ko, p.slope_bytes || p.codes);
+    const int64_t turns = cdiv(p.rows, kNarrowBackRows);
     l.sum_rows = (int)(turns < 256 * a_cu ? turns : 256 * a_cu);
     l.sums = take(l.sum_rows * (int64_t)p.out * 4);
     l.part = take(l.sum_rows * (int64_t)p.out * p.in * 4);

@@ -217,7 +217,7 @@ constexpr int pow2_of(int k) { return k == 3 ? 4 : k; }   // 32s of a tile's row
 // LDS of the backward, in elements.
 template <int KI, int KO, bool kSaved>
 struct NarrowLayerLds {
-  static constexpr int rows = 64 * narrow_groups(KI, KO);   // of a workgroup's turn
+  static constexpr int rows = kNarrowBackRows;
   static constexpr int RO = pow2_of(KO) * 32, RI = pow2_of(KI) * 32;
   static constexpr int wt = kSaved ? 0 : KO * 32 * (KI * 32 + 8);
   static constexpr int dz = wt + KI * 32 * (KO * 32 + 8);
@@ -235,10 +235,10 @@ __device__ __forceinline__ int tile_place(int row, int J, int q) {
 // kSaved: what the backward needs may lie in 8 bits, x (codes) as well as the
 // slopes, and no slopes are made again.
 template <typename T, int KI, int KO, bool kSaved>
-__global__ __launch_bounds__(256, narrow_groups_cu(KI, KO)) void narrow_layer_backward_kernel(NarrowLayer<T> p) {
+__global__ __launch_bounds__(256, narrow_groups_cu(KI, KO, kSaved)) void narrow_layer_backward_kernel(NarrowLayer<T> p) {
   typedef typename Mma<T>::Frag Frag;
   typedef NarrowLayerLds<KI, KO, kSaved> L;
-  constexpr int G = narrow_groups(KI, KO), kRows = L::rows, NO = 2 * KO, NI = 2 * KI;
+  constexpr int G = 1, kRows = L::rows, NO = 2 * KO, NI = 2 * KI;
   constexpr int WO = NO % 4 == 0 ? 4 : 2, WI = 4 / WO, FO = NO / WO, FI = NI / WI;   // waves and fragments of dW
   __shared__ __attribute__((aligned(16))) T lds[L::total];
   __shared__ f32x4 bias[kSaved ? 1 : KO * 8];

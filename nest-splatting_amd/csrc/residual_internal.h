@@ -110,11 +110,12 @@ LinearLayout linear_layout(const LinearParams& p, bool backward);
 // Rows that stay on the chip; a backward makes their slopes again from x and
 // the bias unless they are kept in 8 bits.
 inline bool linear_narrow(int in, int out, int dtype) { return dtype != NEST_DTYPE_F32 && in <= 128 && out <= 128; }
-// Groups of 16 rows that a wave of the backward takes, by 32s of features in
-// and out (two share a read of the weights, where their registers leave three
-// waves a SIMD), and its workgroups that run on a CU at once.
-constexpr int narrow_groups(int ki, int ko) { return ki + 2 * ko <= 4 ? 2 : 1; }
-constexpr int narrow_groups_cu(int ki, int ko) { return ki + ko <= 4 ? 3 : ki + ko <= 6 ? 2 : 1; }
+// Workgroups of their backward that run on a CU at once, by 32s of features in
+// and out and whether anything is kept in 8 bits: as the registers allow.
+constexpr int kNarrowBackRows = 64;   // of a workgroup's turn
+constexpr int narrow_groups_cu(int ki, int ko, bool saved) {
+  return ki + ko <= 3 || (ki + ko == 4 && ko <= 2 && !saved) ? 4 : ki + ko <= 4 ? 3 : ki + ko <= 6 ? 2 : 1;
+}
 int linear_slope_bytes(int in, int out, int dtype, int activation, bool save8);
 hipError_t launch_linear(const LinearParams& p, hipStream_t s, bool backward);
 hipError_t linear_f32(const LinearParams& p, hipStream_t s, bool backward);
