@@ -18,7 +18,9 @@ struct SumTask {
   void *out0, *out1;
   uint32_t shared;
 };
-constexpr int64_t kGroupsAtOnce = 16384;   // of a task; a workgroup takes every 16384th
+// Of a task; a workgroup takes every 4096th. 3 tasks of 256 workgroups across
+// stay under 2^32 threads a launch.
+constexpr int64_t kGroupsAtOnce = 4096;
 struct SumTasks {
   SumTask t[3];
   unsigned first[3];   // workgroup of each task
