@@ -1633,15 +1633,23 @@ int check_embedding(int64_t rows, int32_t cols, int64_t table_rows, int32_t dtyp
 int nest_linear_sizes(const nest_linear* f, size_t* kept, size_t* forward_ws, size_t* backward_ws, size_t* backward_ws_packed) {
   if (int rc = check_linear(f); rc != NEST_OK) return rc;
   LinearParams p = linear_params(f);
-  const LinearLayout fwd = linear_layout(p, false), bwd = linear_layout(p, true);
-  if (!fwd.fits || !bwd.fits) return too_many_tiles();
   if (kept) *kept = (size_t)p.rows * p.out * p.slope_bytes;
-  if (forward_ws) *forward_ws = fwd.bytes;
-  if (backward_ws) *backward_ws = bwd.bytes;
+  if (forward_ws) {
+    const LinearLayout l = linear_layout(p, false);
+    if (!l.fits) return too_many_tiles();
+    *forward_ws = l.bytes;
+  }
+  if (backward_ws) {
+    const LinearLayout l = linear_layout(p, true);
+    if (!l.fits) return too_many_tiles();
+    *backward_ws = l.bytes;
+  }
   if (backward_ws_packed) {
     const int8_t some = 0;
     p.codes = &some;
-    *backward_ws_packed = linear_layout(p, true).bytes;
+    const LinearLayout l = linear_layout(p, true);
+    if (!l.fits) return too_many_tiles();
+    *backward_ws_packed = l.bytes;
   }
   return NEST_OK;
 }

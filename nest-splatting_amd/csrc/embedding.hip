@@ -94,39 +94,54 @@ __global__ __launch_bounds__(kThreads) void embedding_kernel(EmbeddingParams p, 
 
 __device__ __forceinline__ uint32_t key_of(int64_t id, int64_t table_rows) { return (uint32_t)(id >= 0 && id < table_rows ? id : table_rows); }
 
+// Zeros, by thread `first` of `step`.
+__device__ __forceinline__ void fill_zero(uint8_t* to, int64_t bytes, int64_t first, int64_t step) {
+  const int64_t whole = bytes / 16;
+  for (int64_t i = first; i < whole; i += step) store_whole(to + i * 16, make_uint4(0, 0, 0, 0));
+  for (int64_t i = whole * 16 + first; i < bytes; i += step) to[i] = 0;
+}
+
 // The keys to sort, ids outside the table last, and a table of zeros.
 template <typename I>
 __global__ __launch_bounds__(kThreads) void embedding_keys_kernel(const I* ids, int64_t rows, int64_t table_rows, uint32_t* keys,
                                                                   uint8_t* zero, int64_t zero_bytes) {
-  const int64_t step = (int64_t)gridDim.x * kThreads, first = (int64_t)blockIdx.x * kThreads + threadIdx.x, whole = zero_bytes / 16;
+  const int64_t step = (int64_t)gridDim.x * kThreads, first = (int64_t)blockIdx.x * kThreads + threadIdx.x;
   for (int64_t i = first; i < rows; i += step) keys[i] = key_of(ids[i], table_rows);
-  for (int64_t i = first; i < whole; i += step) store_whole(zero + i * 16, make_uint4(0, 0, 0, 0));
-  for (int64_t i = whole * 16 + first; i < zero_bytes; i += step) zero[i] = 0;
+  fill_zero(zero, zero_bytes, first, step);
 }
 
 // Sorted at once: a position's place is the number of keys before its own.  A
 // workgroup takes kRanked positions and compares each with all keys, kThreads /
 // kRanked threads a position.  N^2 comparisons, spread over the chip: 8192
-// positions take less time than the six launches of a radix sort.
+// positions take less time than the launches of a radix sort, and the
+// workgroups behind the last position's clear the table meanwhile.
 constexpr int64_t kMostRanked = 8192;
 constexpr int kRanked = 16;
-__global__ __launch_bounds__(kThreads) void embedding_rank_kernel(const uint32_t* from, int rows, uint32_t* sorted, uint32_t* index) {
+template <typename I>
+__global__ __launch_bounds__(kThreads) void embedding_rank_kernel(const I* ids, int rows, int64_t table_rows, uint32_t* sorted, uint32_t* index,
+                                                                  uint8_t* zero, int64_t zero_bytes) {
   constexpr int kSlices = kThreads / kRanked;
   __shared__ uint4 keys[kMostRanked / 4];
   __shared__ int counts[kSlices][kRanked];
-  constexpr int kLoads = kMostRanked / 4 / kThreads;
-  uint4 v[kLoads];
-  const int pieces = (rows + 3) / 4;   // the keys' array ends after whole pieces
-#pragma unroll
-  for (int u = 0; u < kLoads; u++) {
-    const int i = u * kThreads + threadIdx.x;
-    v[u] = i < pieces ? reinterpret_cast<const uint4*>(from)[i] : make_uint4(kNoRun, kNoRun, kNoRun, kNoRun);
-    if (i * 4 + 1 >= rows) v[u].y = kNoRun;
-    if (i * 4 + 2 >= rows) v[u].z = kNoRun;
-    if (i * 4 + 3 >= rows) v[u].w = kNoRun;
+  const int ranking = (rows + kRanked - 1) / kRanked;
+  if ((int)blockIdx.x >= ranking) {
+    fill_zero(zero, zero_bytes, (int64_t)(blockIdx.x - ranking) * kThreads + threadIdx.x, (int64_t)(gridDim.x - ranking) * kThreads);
+    return;
   }
+  const int pieces = (rows + 3) / 4;
+  for (int first = 0; first < pieces * 4; first += 8 * kThreads) {   // to LDS, eight loads in flight
+    uint32_t v[8];
 #pragma unroll
-  for (int u = 0; u < kLoads; u++) keys[u * kThreads + threadIdx.x] = v[u];
+    for (int u = 0; u < 8; u++) {
+      const int i = first + u * kThreads + threadIdx.x;
+      v[u] = i < rows ? key_of(ids[i], table_rows) : kNoRun;
+    }
+#pragma unroll
+    for (int u = 0; u < 8; u++) {
+      const int i = first + u * kThreads + threadIdx.x;
+      if (i < pieces * 4) reinterpret_cast<uint32_t*>(keys)[i] = v[u];
+    }
+  }
   __syncthreads();
   const int t = threadIdx.x % kRanked, slice = threadIdx.x / kRanked, first = blockIdx.x * kRanked, mine = first + t;
   const int per = (pieces + kSlices - 1) / kSlices | 1;   // pieces of 4 keys; odd, so the slices of a wave fall on different banks
@@ -314,15 +329,13 @@ struct Counted {
   int cols, table_rows;
   float* part;         // [groups][table_rows][cols]
   uint32_t* flags;     // [table_rows][cols] bits: 1 an infinity, 2 a negative one, 4 a NaN
-  int64_t n_flags;
 };
 
+// A one is made as float16 for either type, and its bits are 2^-7 as bfloat16.
 template <typename T>
-constexpr uint16_t kOne = 0;
+constexpr float kOneInverse = 1.0f;
 template <>
-constexpr uint16_t kOne<f16_t> = 0x3c00;
-template <>
-constexpr uint16_t kOne<bf16_t> = 0x3f80;
+constexpr float kOneInverse<bf16_t> = 128.0f;
 template <typename T>
 constexpr uint16_t kInfinity = 0;
 template <>
@@ -331,6 +344,7 @@ template <>
 constexpr uint16_t kInfinity<bf16_t> = 0x7f80;
 
 typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 
 __global__ __launch_bounds__(kThreads) void embedding_clear_kernel(uint32_t* p, int64_t n) {
   for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < n; i += (int64_t)gridDim.x * kThreads) p[i] = 0;
@@ -343,11 +357,11 @@ __global__ __launch_bounds__(kCountThreads, (FD < 8 && FV * FD <= kTwiceCounted 
   typedef typename Mma<T>::Frag Frag;
   constexpr int R = FD * 16, kVecs = R / 8, kLoads = kCountRows * kVecs / kCountThreads;   // pieces of 16 bytes
   __shared__ __attribute__((aligned(16))) uint8_t tile[2][kCountRows * R * 2];
-  __shared__ __attribute__((aligned(16))) uint16_t keys[2][kCountRows];
+  __shared__ __attribute__((aligned(16))) _Float16 keys[2][kCountRows];
   const int lane = threadIdx.x & 63, r = lane & 15, q = lane >> 4, wave = wave_id();
   const int64_t step = (int64_t)gridDim.x * kCountRows;
   Words16<T> next[kLoads];
-  int next_key = 0;
+  _Float16 next_key = 0;   // at most 2048 ids: exact
   auto load = [&](int64_t turn) {
 #pragma unroll
     for (int i = 0; i < kLoads; i++) {
@@ -358,7 +372,7 @@ __global__ __launch_bounds__(kCountThreads, (FD < 8 && FV * FD <= kTwiceCounted 
       const int64_t row = turn + threadIdx.x;
       int64_t id = -1;
       if (row < p.rows) id = p.wide_ids ? static_cast<const int64_t*>(p.ids)[row] : static_cast<const int32_t*>(p.ids)[row];
-      next_key = id >= 0 && id < p.table_rows ? (int)id : 0xffff;
+      next_key = id >= 0 && id < p.table_rows ? (_Float16)(int)id : (_Float16)-1;
     }
   };
   auto stage = [&](int buf, int64_t turn) {
@@ -383,7 +397,7 @@ __global__ __launch_bounds__(kCountThreads, (FD < 8 && FV * FD <= kTwiceCounted 
       const int unit = (v >> 1) ^ unit_swizzle<T, R>(row);
       *reinterpret_cast<uint4*>(&tile[buf][row * R * 2 + (unit << 5) + (v & 1) * 16]) = __builtin_bit_cast(uint4, next[i]);
     }
-    if (threadIdx.x < kCountRows) keys[buf][threadIdx.x] = (uint16_t)next_key;
+    if (threadIdx.x < kCountRows) keys[buf][threadIdx.x] = next_key;
   };
   f32x4 acc[FV][FD] = {};
   const int base = fragment_base<T, false, R>(0);
@@ -399,9 +413,9 @@ __global__ __launch_bounds__(kCountThreads, (FD < 8 && FV * FD <= kTwiceCounted 
     for (int kb = 0; kb < kCountRows / 32; kb++) {
       const uint4 k = *reinterpret_cast<const uint4*>(&keys[buf][kb * 32 + q * 8]);
       const uint32_t words[4] = {k.x, k.y, k.z, k.w};
-      u16x2 mine[4];   // an id's distance from this lane's first
+      f16x2 mine[4];   // an id's distance from this lane's first
 #pragma unroll
-      for (int e = 0; e < 4; e++) mine[e] = __builtin_bit_cast(u16x2, words[e]) - (uint16_t)(wave * 16 + r);
+      for (int e = 0; e < 4; e++) mine[e] = __builtin_bit_cast(f16x2, words[e]) - (_Float16)(wave * 16 + r);
       Frag b[FD];
 #pragma unroll
       for (int j = 0; j < FD; j++) b[j] = fragment<T, false, R>(tile[buf], base, j, kb);
@@ -411,8 +425,9 @@ __global__ __launch_bounds__(kCountThreads, (FD < 8 && FV * FD <= kTwiceCounted 
         uint32_t ones[4];
 #pragma unroll
         for (int e = 0; e < 4; e++) {
-          const u16x2 off = mine[e] ^ (uint16_t)(i * 128);
-          ones[e] = __builtin_bit_cast(uint32_t, __builtin_elementwise_sub_sat(u16x2{1, 1}, off) * kOne<T>);
+          const f16x2 off = mine[e] - (_Float16)(i * 128);   // a whole number: 1 - off^2 is 1 or not above 0
+          const f16x2 one = __builtin_elementwise_fma(off, -off, f16x2{1, 1});
+          ones[e] = __builtin_bit_cast(uint32_t, __builtin_elementwise_min(__builtin_elementwise_max(one, f16x2{0, 0}), f16x2{1, 1}));
         }
         const Frag a = __builtin_bit_cast(Frag, make_uint4(ones[0], ones[1], ones[2], ones[3]));
 #pragma unroll
@@ -431,7 +446,7 @@ __global__ __launch_bounds__(kCountThreads, (FD < 8 && FV * FD <= kTwiceCounted 
       const int c = j * 16 + q * 4;
 #pragma unroll
       for (int e = 0; e < 4; e++)
-        if (c + e < p.cols) part[(int64_t)id * p.cols + c + e] = acc[i][j][e];
+        if (c + e < p.cols) part[(int64_t)id * p.cols + c + e] = acc[i][j][e] * kOneInverse<T>;
     }
   }
 }
@@ -508,8 +523,10 @@ Plan plan_of(int64_t rows, int cols, int64_t table_rows, int dtype) {
   l.ranked = rows <= kMostRanked;
   l.chunk = chunk_of(rows, cols, dtype == NEST_DTYPE_F32 ? 4 : 8);
   l.chunks = cdiv(rows, l.chunk);
-  l.keys = take((size_t)(rows + 3) / 4 * 16);
-  if (!l.ranked) l.sort = take(index_sort_ws_bytes(rows));
+  if (!l.ranked) {
+    l.keys = take((size_t)rows * 4);
+    l.sort = take(index_sort_ws_bytes(rows));
+  }
   l.sorted = take((size_t)(rows + kBatch) * 4);
   l.index = take((size_t)(rows + kBatch) * 4);
   l.part = take((size_t)l.chunks * 2 * cols * 4);
@@ -542,7 +559,7 @@ hipError_t count_gradient(const EmbeddingParams& p, const Plan& l, hipStream_t s
   uint8_t* ws = static_cast<uint8_t*>(p.ws);
   const int64_t size = p.table_rows * p.cols;
   const Counted<T> q{static_cast<const T*>(p.dy), p.ids, p.wide_ids, p.rows, p.cols, (int)p.table_rows, reinterpret_cast<float*>(ws + l.part),
-                     reinterpret_cast<uint32_t*>(ws + l.flags), size};
+                     reinterpret_cast<uint32_t*>(ws + l.flags)};
   embedding_clear_kernel<<<(unsigned)cdiv(size, kThreads), kThreads, 0, s>>>(q.flags, size);
   auto launch = [&](auto fd) {
     constexpr int FD = fd.value, kMost = kMostCounted / FD;
@@ -573,12 +590,15 @@ hipError_t sort_ids(const EmbeddingParams& p, const Plan& l, uint32_t* sorted, u
   uint8_t *ws = static_cast<uint8_t*>(p.ws), *table = static_cast<uint8_t*>(p.dtable);
   const I* ids = static_cast<const I*>(p.ids);
   const int64_t bytes = p.table_rows * p.cols * (int64_t)sizeof(T), pieces = cdiv(bytes, 16 * kThreads);
+  if (l.ranked) {
+    const int64_t clearing = pieces < 512 ? pieces : 512;   // two a CU, beside as many that rank
+    embedding_rank_kernel<I><<<(unsigned)(cdiv(p.rows, kRanked) + clearing), kThreads, 0, s>>>(ids, (int)p.rows, p.table_rows, sorted, index, table, bytes);
+    return hipGetLastError();
+  }
   uint32_t* keys = reinterpret_cast<uint32_t*>(ws + l.keys);
   const int64_t need = cdiv(p.rows, kThreads) > pieces ? cdiv(p.rows, kThreads) : pieces;
   embedding_keys_kernel<I><<<(unsigned)(need < 8192 ? need : 8192), kThreads, 0, s>>>(ids, p.rows, p.table_rows, keys, table, bytes);
-  if (l.ranked) embedding_rank_kernel<<<(unsigned)cdiv(p.rows, kRanked), kThreads, 0, s>>>(keys, (int)p.rows, sorted, index);
   if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
-  if (l.ranked) return hipSuccess;
   int bits = 1;
   while (((int64_t)1 << bits) <= p.table_rows) bits++;
   return launch_sort_indices(keys, sorted, index, p.rows, bits, ws + l.sort, s);

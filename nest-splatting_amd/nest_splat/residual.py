@@ -123,13 +123,13 @@ def _narrow(dtype, features, out_features):
     return dtype is not torch.float32 and features <= 128 and out_features <= 128
 
 
-def _linear_sizes(f):
-    """Bytes of (kept slopes, a forward's workspace, a backward's, a backward's with x in 8 bits)."""
-    kept, fwd, bwd, packed = ct.c_size_t(), ct.c_size_t(), ct.c_size_t(), ct.c_size_t()
-    rc = L.lib().nest_linear_sizes(f, kept, fwd, bwd, packed)
+def _linear_ws(f, forward=False, packed=False):
+    """Bytes of a forward's workspace, or of a backward's, without or with x in 8 bits."""
+    n = ct.c_size_t()
+    rc = L.lib().nest_linear_sizes(f, None, n if forward else None, None if forward or packed else n, n if packed else None)
     if rc != L.NEST_OK:
         L.check(rc, "nest_linear_sizes")
-    return kept.value, fwd.value, bwd.value, packed.value
+    return n.value
 
 
 def _matrix(weight):
@@ -163,16 +163,18 @@ def linear_forward(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.T
     if residual is not None:
         residual = _aligned(_like(residual, x, out_shape, "residual"))
         f.residual = residual.data_ptr()
-    _, fwd_bytes, _, _ = _linear_sizes(f)
-    y = torch.empty(out_shape, dtype=x.dtype, device=x.device)
+    nbytes = _linear_ws(f, forward=True)
+    if training:
+        _linear_ws(f)   # a backward that is refused is refused here
+    y = x.new_empty(out_shape)
     kept = slopes = None
     if training and activation is not None:
         if not save8 and _narrow(x.dtype, I, O):
             kept = x.new_empty(0) if bias is None else bias
         else:
             kept = slopes = torch.empty(out_shape, dtype=_slope_type(x.dtype, activation, save8), device=x.device)
-    work = _workspace(fwd_bytes, x.device)
-    _call("nest_linear_forward", x.device, f, y.data_ptr(), _at(slopes), _at(work), fwd_bytes)
+    work = _workspace(nbytes, x.device)
+    _call("nest_linear_forward", x.device, f, y.data_ptr(), _at(slopes), _at(work), nbytes)
     return y, kept
 
 
@@ -220,12 +222,11 @@ def linear_backward(dy: torch.Tensor, x: Union[torch.Tensor, Packed8, None], wei
             slopes = kept = _aligned(kept)
         else:
             raise ValueError("kept is not what linear_forward(training=True) returned for these arguments")
-    _, _, bwd_bytes, packed_bytes = _linear_sizes(f)
+    use_packed = packed and needs[1]
+    nbytes = _linear_ws(f, packed=use_packed)
     dx = torch.empty(in_shape, dtype=dy.dtype, device=dy.device) if needs[0] else None
     dw = torch.empty_like(weight) if needs[1] else None
     db = torch.empty(O, dtype=dy.dtype, device=dy.device) if with_bias else None
-    use_packed = packed and needs[1]
-    nbytes = packed_bytes if use_packed else bwd_bytes
     work = _workspace(nbytes, dy.device)
     _call("nest_linear_backward", dy.device, f, dy.data_ptr(), _at(slopes),
           x.codes.data_ptr() if use_packed else None, x.steps.data_ptr() if use_packed else None, _at(dx), _at(dw), _at(db), _at(work), nbytes)
@@ -293,14 +294,17 @@ def _norm_params(x, gate, post, pre):
     dtype = x.dtype if some is None else some.dtype
     if dtype is not x.dtype and dtype is not torch.float32:
         raise TypeError(f"gate, post and pre are {dtype}: float32 or the type of x ({x.dtype}) is expected")
-    if post is not None:
+    device = x.get_device()
+    fits = lambda t: t.dtype is dtype and t.get_device() == device and t.is_contiguous()   # what _like would return as it is
+    if post is not None and not (post.shape == row and fits(post)):
         post = _like(post, x, row, "post", dtype)
-    if pre is not None:
+    if pre is not None and not (pre.shape == row and fits(pre)):
         pre = _like(pre, x, row, "pre", dtype)
     gates = 0
     if gate is not None:
         gates = 1 if gate.shape == row else _gates(x, gate)
-        gate = _like(gate, x, gate.shape, "gate", dtype)
+        if not fits(gate):
+            gate = _like(gate, x, gate.shape, "gate", dtype)
     return code, _CODE[dtype], gates, gate, post, pre
 
 
@@ -326,7 +330,7 @@ def residual_norm_forward(x: torch.Tensor, h: Optional[torch.Tensor] = None, gat
     h = h if h is None else _like(h, x, x.shape, "h")
     r = x if h is None else torch.empty_like(x)
     y = None if pre is None else torch.empty_like(x)
-    stats = torch.empty((2, rows), dtype=torch.float32, device=x.device)
+    stats = x.new_empty((2, rows), dtype=torch.float32)
     if rows == 0:   # whose tensors have no addresses to tell them from those left out
         return r, y, stats
     at = stats.data_ptr()
