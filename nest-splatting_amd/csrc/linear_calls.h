@@ -77,7 +77,7 @@ hipError_t linear_backward(const LinearParams& p, hipStream_t s) {
     if (hipError_t e = launch_slopes(q, l.sum_rows, s); e != hipSuccess) return e;
     if (p.db) {
       SumTasks t{};
-      t.t[0] = {q.part, l.sum_rows, 1, p.out, nullptr, nullptr, nullptr, p.db, nullptr, 1};
+      t.t[0] = {q.part, l.sum_rows, 1, p.out, nullptr, nullptr, p.db, nullptr};
       if (hipError_t e = launch_column_sums<T>(t, 1, s); e != hipSuccess) return e;
     }
     if (made) dz = made;

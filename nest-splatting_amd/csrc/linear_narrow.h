@@ -475,8 +475,8 @@ hipError_t launch_narrow_layer_backward(const LinearParams& p, const LinearLayou
   if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
   SumTasks t{};
   int k = 0;
-  if (p.dw) t.t[k++] = {n.dw, l.sum_rows, 1, p.in * p.out, nullptr, nullptr, nullptr, p.dw, nullptr, 1};
-  if (p.db) t.t[k++] = {n.db, l.sum_rows, 1, p.out, nullptr, nullptr, nullptr, p.db, nullptr, 1};
+  if (p.dw) t.t[k++] = {n.dw, l.sum_rows, 1, p.in * p.out, nullptr, nullptr, p.dw, nullptr};
+  if (p.db) t.t[k++] = {n.db, l.sum_rows, 1, p.out, nullptr, nullptr, p.db, nullptr};
   return k ? launch_column_sums<T>(t, k, s) : hipSuccess;
 }
 

@@ -19,7 +19,8 @@
 // a longer one to a workgroup.  A gate is shared by consecutive rows; in the
 // backward pass an item is a part of the rows of one gate, and what its lanes
 // gather, S = sum e t^, gives both dgate = post S and its share gate S of
-// dpost.  Where every row has a gate of its own, dgate is written row by row
+// dpost, which gathers on over the items of a workgroup where there are several
+// gates.  Where every row has a gate of its own, dgate is written row by row
 // and dpost is gathered.  Sums over rows are joined in an order that the
 // sizes fix.
 #include "column_sums.h"
@@ -194,19 +195,24 @@ __device__ __forceinline__ void write_sums(const float (&v)[NV][N], float* out, 
 }
 
 // Items: `parts` parts of the rows of each gate (one gate for all rows where
-// there is none, or one a row: kEach).  A workgroup takes every gridDim.x-th;
-// it writes a row of S an item and one row of dpre.
+// there is none, or one a row: kEachRow).  A workgroup takes every
+// gridDim.x-th; it writes a row of S an item, one row of dpre and, with
+// several gates (kSeveral), one of dpost.
 struct Items {
   int64_t rows;       // of a gate
   int64_t n;          // items
   int parts;          // of a gate
-  float *s, *dpre;
+  float *s, *dpre, *dpost;
 };
+enum Gates { kOneGate, kSeveral, kEachRow };
+// Waves a SIMD that the registers leave room for: four where asked to.
+constexpr bool four_waves(int nv, int values, bool block, Gates gates) { return nv * values <= 8 && (nv == 1 || block) && gates != kEachRow; }
 
-template <typename T, typename P, int NV, bool kBlock, bool kEach>
-__global__ __launch_bounds__((kBlock ? kMostThreads : kThreads), (NV * Vec16<T>::kN <= 8 && (NV == 1 || kBlock) && !kEach ? 4 : 1)) void residual_norm_backward_kernel(ResidualNormParams p, int lanes,
-                                                                                                     Items items) {
+template <typename T, typename P, int NV, bool kBlock, Gates kGates>
+__global__ __launch_bounds__((kBlock ? kMostThreads : kThreads), (four_waves(NV, Vec16<T>::kN, kBlock, kGates) ? 4 : 1)) void
+residual_norm_backward_kernel(ResidualNormParams p, int lanes, Items items) {
   constexpr int N = Vec16<T>::kN;
+  constexpr bool kEach = kGates == kEachRow;
   constexpr bool kAhead = NV * N < 16;   // a row's gate loaded with the row before; past the registers else
   __shared__ float lds[2][kMostWaves];
   __shared__ float gather[kBlock ? 1 : kThreads][N + 1];
@@ -216,6 +222,11 @@ __global__ __launch_bounds__((kBlock ? kMostThreads : kThreads), (NV * Vec16<T>:
   const int D = p.cols;
   const float inv = 1.0f / (float)D;
   float w[NV][N], pre[NV][N], gate[NV][N], acc[NV][N], dpre[NV][N];   // w: post, times the item's gate unless every row has its own
+  __shared__ float dpost[kGates == kSeveral ? NV * N : 1][kBlock ? kMostThreads : kThreads];   // each thread's own: registers would cost a wave a SIMD
+  if constexpr (kGates == kSeveral) {
+#pragma unroll
+    for (int i = 0; i < NV * N; i++) dpost[i][threadIdx.x] = 0.0f;
+  }
   if constexpr (kEach) load_columns<P>(w, p.post, lane, lanes, D, 1.0f);
   load_columns<P>(pre, p.pre, lane, lanes, D, 0.0f);
 #pragma unroll
@@ -334,6 +345,22 @@ __global__ __launch_bounds__((kBlock ? kMostThreads : kThreads), (NV * Vec16<T>:
       }
     }
     if (items.s) write_sums<NV, N, kBlock>(acc, items.s + item * D, lane, lanes, D, gather);
+    if constexpr (kGates == kSeveral) {
+      load_columns<P>(gate, static_cast<const P*>(p.gate) + group * D, lane, lanes, D, 1.0f);   // again: not held over the rows
+#pragma unroll
+      for (int k = 0; k < NV; k++)
+#pragma unroll
+        for (int i = 0; i < N; i++) dpost[k * N + i][threadIdx.x] += gate[k][i] * acc[k][i];
+    }
+  }
+  if constexpr (kGates == kSeveral) {
+    if (items.dpost) {
+#pragma unroll
+      for (int k = 0; k < NV; k++)
+#pragma unroll
+        for (int i = 0; i < N; i++) acc[k][i] = dpost[k * N + i][threadIdx.x];
+      write_sums<NV, N, kBlock>(acc, items.dpost + (int64_t)blockIdx.x * D, lane, lanes, D, gather);
+    }
   }
   if (p.pre) write_sums<NV, N, kBlock>(dpre, items.dpre + (int64_t)blockIdx.x * D, lane, lanes, D, gather);
 }
@@ -375,27 +402,28 @@ int rows_of_group(const Shape& h) { return h.block ? 1 : kThreads / h.lanes; }
 // waits for a turn of its own and few partial sums are left to join.
 struct Plan {
   Items items;
-  int groups;                // workgroups
-  bool each;
-  size_t s, dpre, floats;    // into the workspace
+  int groups;                       // workgroups
+  Gates gates;
+  size_t s, dpre, dpost, floats;    // into the workspace
 };
 Plan plan_of(int64_t rows, int cols, int dtype, int64_t gates) {
   Plan l{};
-  l.each = gates == rows && rows > 1;
+  l.gates = gates <= 1 ? kOneGate : gates == rows ? kEachRow : kSeveral;
   const Shape h = shape_of(cols, dtype);
-  const int waves = h.block ? h.lanes / 64 : kThreads / 64;
-  const int values = h.nv * (dtype == NEST_DTYPE_F32 ? 4 : 8);   // a lane's
-  const int a_cu = values == 4 ? 20 : values == 8 ? ((h.nv == 1 || h.block) && !l.each ? 16 : 12) : 8;   // waves, by the registers
+  const int waves = h.block ? h.lanes / 64 : kThreads / 64, n = dtype == NEST_DTYPE_F32 ? 4 : 8;
+  const int values = h.nv * n;   // a lane's
+  const int a_cu = values == 4 ? 20 : values == 8 ? (four_waves(h.nv, n, h.block, l.gates) ? 16 : 12) : 8;   // waves, by the registers
   const int64_t most = 256 * (a_cu > waves ? a_cu / waves : 1);
-  const int64_t n = l.each || gates == 0 ? 1 : gates;
-  l.items.rows = rows / n;
-  const int64_t turns = cdiv(l.items.rows, rows_of_group(h)), share = most / n > 1 ? most / n : 1;
+  const int64_t shared = l.gates == kSeveral ? gates : 1;
+  l.items.rows = rows / shared;
+  const int64_t turns = cdiv(l.items.rows, rows_of_group(h)), share = most / shared > 1 ? most / shared : 1;
   l.items.parts = (int)(turns < share ? turns : share);
-  l.items.n = n * l.items.parts;
+  l.items.n = shared * l.items.parts;
   l.groups = (int)(l.items.n < most ? l.items.n : most);
   l.s = 0;
   l.dpre = (size_t)l.items.n * cols;
-  l.floats = l.dpre + (size_t)l.groups * cols;
+  l.dpost = l.dpre + (size_t)l.groups * cols;
+  l.floats = l.dpost + (l.gates == kSeveral ? (size_t)l.groups * cols : 0);
   return l;
 }
 
@@ -414,30 +442,30 @@ hipError_t forward(const ResidualNormParams& p, hipStream_t s) {
 template <typename T, typename P>
 hipError_t backward(const ResidualNormParams& p, hipStream_t s) {
   Plan l = plan_of(p.rows, p.cols, p.dtype, p.gates);
-  const bool gate = p.h && p.gate, post = p.h && p.post, many = gate && !l.each && p.gates > 1;
-  l.items.s = post || (gate && !l.each) ? p.ws + l.s : nullptr;
+  const bool gate = p.h && p.gate, post = p.h && p.post;
+  l.items.s = post || (gate && l.gates != kEachRow) ? p.ws + l.s : nullptr;
   l.items.dpre = p.ws + l.dpre;
+  l.items.dpost = post && l.gates == kSeveral ? p.ws + l.dpost : nullptr;
   if (l.groups > 0) {
     const Shape h = shape_of(p.cols, p.dtype);
     with_shape<T>(h, [&](auto nv, auto block) {
       const int threads = block ? h.lanes : kThreads;
-      if (l.each) residual_norm_backward_kernel<T, P, nv, block, true><<<l.groups, threads, 0, s>>>(p, h.lanes, l.items);
-      else residual_norm_backward_kernel<T, P, nv, block, false><<<l.groups, threads, 0, s>>>(p, h.lanes, l.items);
+      if (l.gates == kEachRow) residual_norm_backward_kernel<T, P, nv, block, kEachRow><<<l.groups, threads, 0, s>>>(p, h.lanes, l.items);
+      else if (l.gates == kSeveral) residual_norm_backward_kernel<T, P, nv, block, kSeveral><<<l.groups, threads, 0, s>>>(p, h.lanes, l.items);
+      else residual_norm_backward_kernel<T, P, nv, block, kOneGate><<<l.groups, threads, 0, s>>>(p, h.lanes, l.items);
     });
     if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
   }
   SumTasks tasks{};
   int n = 0;
-  if (p.pre) tasks.t[n++] = {l.items.dpre, l.groups, 1, p.cols, nullptr, nullptr, nullptr, p.dpre, nullptr, 1};
-  if (l.items.s) {
-    if (l.each) {
-      tasks.t[n++] = {l.items.s, l.items.n, 1, p.cols, nullptr, nullptr, nullptr, p.dpost, nullptr, 1};
-    } else if (many) {
-      tasks.t[n++] = {l.items.s, l.items.parts, p.gates, p.cols, nullptr, p.post, nullptr, p.dgate, nullptr, 1};
-      if (post) tasks.t[n++] = {l.items.s, l.items.n, 1, p.cols, p.gate, nullptr, nullptr, p.dpost, nullptr, (uint32_t)l.items.parts};
-    } else {
-      tasks.t[n++] = {l.items.s, l.items.n, 1, p.cols, nullptr, p.post, p.gate, gate ? p.dgate : nullptr, post ? p.dpost : nullptr, 1};
-    }
+  if (p.pre) tasks.t[n++] = {l.items.dpre, l.groups, 1, p.cols, nullptr, nullptr, p.dpre, nullptr};
+  if (l.items.s && l.gates == kEachRow) {
+    tasks.t[n++] = {l.items.s, l.items.n, 1, p.cols, nullptr, nullptr, p.dpost, nullptr};
+  } else if (l.items.s && l.gates == kSeveral) {
+    tasks.t[n++] = {l.items.s, l.items.parts, p.gates, p.cols, p.post, nullptr, p.dgate, nullptr};
+    if (post) tasks.t[n++] = {l.items.dpost, l.groups, 1, p.cols, nullptr, nullptr, p.dpost, nullptr};
+  } else if (l.items.s) {
+    tasks.t[n++] = {l.items.s, l.items.n, 1, p.cols, p.post, p.gate, gate ? p.dgate : nullptr, post ? p.dpost : nullptr};
   }
   return n ? launch_column_sums<P>(tasks, n, s) : hipSuccess;
 }

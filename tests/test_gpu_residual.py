@@ -290,6 +290,12 @@ def test_residual_norm_gates(B, rows, cols, gates, dtype):
     norm_check(B, norm_case(rows, cols, dtype, gates=gates))
 
 
+@pytest.mark.parametrize("rows,cols,gates", [(9000, 24, 3000), (6000, 1500, 3000), (5000, 4100, 2500)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_residual_norm_more_gates_than_workgroups(B, rows, cols, gates, dtype):
+    norm_check(B, norm_case(rows, cols, dtype, gates=gates))
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("rows,cols", [(41, 200), (6, 1300)])
 def test_residual_norm_parts_that_are_left_out(B, rows, cols, dtype):
