@@ -79,10 +79,26 @@ __device__ __forceinline__ float byte_of(uint2 v, int i) { return (float)(((i < 
 // different banks.
 template <typename T, int R, int C, bool kTransposed>
 __device__ __forceinline__ void stage_weights(T* lds, const T* w, int rows, int cols) {
-  constexpr int kPitch = C + 8;
-  for (int i = threadIdx.x; i < R * C; i += 256) {
-    const int r = kTransposed ? i % R : i / C, c = kTransposed ? i / R : i % C;
-    lds[((r & ~31) | (r >> 2 & 1) << 4 | (r >> 3 & 3) << 2 | (r & 3)) * kPitch + c] = r < rows && c < cols ? w[kTransposed ? c * rows + r : r * cols + c] : (T)0.0f;
+  constexpr int kPitch = C + 8, kLong = kTransposed ? R : C;   // of a row in memory
+  constexpr int kPieces = (R * C + 8 * 256 - 1) / (8 * 256);   // of 16 bytes, a thread's
+  const int length = kTransposed ? rows : cols, lines = kTransposed ? cols : rows;
+  Words16<T> v[kPieces];   // all on their way at once: one after another takes 20 us
+#pragma unroll
+  for (int u = 0; u < kPieces; u++) {
+    const int i = (u * 256 + threadIdx.x) * 8, line = i / kLong, at = i % kLong;
+    v[u] = load_words<false>(w + line * length + at, line < lines ? length - at : 0);
+  }
+#pragma unroll
+  for (int u = 0; u < kPieces; u++) {
+    const int i = (u * 256 + threadIdx.x) * 8, line = i / kLong, at = i % kLong;
+    if (i >= R * C) break;
+    auto row_at = [](int r) { return ((r & ~31) | (r >> 2 & 1) << 4 | (r >> 3 & 3) << 2 | (r & 3)) * kPitch; };
+    if constexpr (kTransposed) {
+#pragma unroll
+      for (int e = 0; e < 8; e++) lds[row_at(at + e) + line] = v[u][e];
+    } else {
+      *reinterpret_cast<uint4*>(lds + row_at(line) + at) = __builtin_bit_cast(uint4, v[u]);
+    }
   }
 }
 

@@ -15,8 +15,8 @@
 // type: what follows reads that r too, and the backward pass makes the same r^
 // from it.  All sums are float32; every result is rounded once.
 //
-// A row of up to 128 vectors of 16 bytes belongs to 1 to 64 lanes of a wave,
-// a longer one to a workgroup.  A gate is shared by consecutive rows; in the
+// A row of up to 64 vectors of 16 bytes (backward 128) belongs to 1 to 64 lanes
+// of a wave, a longer one to a workgroup.  A gate is shared by consecutive rows; in the
 // backward pass an item is a part of the rows of one gate, and what its lanes
 // gather, S = sum e t^, gives both dgate = post S and its share gate S of
 // dpost, which gathers on over the items of a workgroup where there are several
@@ -371,25 +371,28 @@ int pow2_at_least(int v) {
   return p;
 }
 
-// A row's lanes, and vectors a lane: up to 128 vectors stay with one wave (no
-// barrier), more with a workgroup of as many waves as they need.
+// A row's lanes, and vectors a lane.  Up to 64 vectors stay with one wave, in
+// the backward pass up to 128 (no barrier), more with a workgroup of as many
+// waves as they need.  us of 65,536 x 768 bf16 with a wave and with a workgroup
+// a row: forward 120 and 106, backward 123 and 179; 16,384 x 1024 33 and 28, 40
+// and 45.
 struct Shape {
   int lanes, nv;
   bool block;
 };
-Shape shape_of(int cols, int dtype) {
+Shape shape_of(int cols, int dtype, bool back) {
   const int n = dtype == NEST_DTYPE_F32 ? 4 : 8, vecs = (cols + n - 1) / n;
-  if (vecs <= 128) return {vecs <= 64 ? pow2_at_least(vecs) : 64, (vecs + 63) / 64, false};
+  if (vecs <= (back ? 128 : 64)) return {vecs <= 64 ? pow2_at_least(vecs) : 64, (vecs + 63) / 64, false};
   const int nv = vecs <= kMostThreads ? 1 : vecs <= 2 * kMostThreads ? 2 : 4;   // 4: float32 alone
   return {(vecs + 64 * nv - 1) / (64 * nv) * 64, nv, true};
 }
 
-template <typename T, typename F>
+template <typename T, bool kBack, typename F>
 void with_shape(const Shape& h, F f) {
   using std::integral_constant;
   if (!h.block) {
-    if (h.nv == 1) f(integral_constant<int, 1>(), integral_constant<bool, false>());
-    else f(integral_constant<int, 2>(), integral_constant<bool, false>());
+    if (!kBack || h.nv == 1) f(integral_constant<int, 1>(), integral_constant<bool, false>());
+    else if constexpr (kBack) f(integral_constant<int, 2>(), integral_constant<bool, false>());
   } else if (h.nv == 1) f(integral_constant<int, 1>(), integral_constant<bool, true>());
   else if (sizeof(T) == 2 || h.nv == 2) f(integral_constant<int, 2>(), integral_constant<bool, true>());
   else if constexpr (sizeof(T) == 4) f(integral_constant<int, 4>(), integral_constant<bool, true>());
@@ -409,7 +412,7 @@ struct Plan {
 Plan plan_of(int64_t rows, int cols, int dtype, int64_t gates) {
   Plan l{};
   l.gates = gates <= 1 ? kOneGate : gates == rows ? kEachRow : kSeveral;
-  const Shape h = shape_of(cols, dtype);
+  const Shape h = shape_of(cols, dtype, true);
   const int waves = h.block ? h.lanes / 64 : kThreads / 64, n = dtype == NEST_DTYPE_F32 ? 4 : 8;
   const int values = h.nv * n;   // a lane's
   const int a_cu = values == 4 ? 20 : values == 8 ? (four_waves(h.nv, n, h.block, l.gates) ? 16 : 12) : 8;   // waves, by the registers
@@ -429,11 +432,11 @@ Plan plan_of(int64_t rows, int cols, int dtype, int64_t gates) {
 
 template <typename T, typename P>
 hipError_t forward(const ResidualNormParams& p, hipStream_t s) {
-  const Shape h = shape_of(p.cols, p.dtype);
+  const Shape h = shape_of(p.cols, p.dtype, false);
   const int64_t need = cdiv(p.rows, rows_of_group(h));
   const unsigned grid = (unsigned)(need < kForwardGrid ? need : kForwardGrid);
   const uint32_t rows_gate = p.gates > 1 ? (uint32_t)(p.rows / p.gates) : 1;
-  with_shape<T>(h, [&](auto nv, auto block) {
+  with_shape<T, false>(h, [&](auto nv, auto block) {
     residual_norm_kernel<T, P, nv, block><<<grid, block ? h.lanes : kThreads, 0, s>>>(p, h.lanes, rows_gate);
   });
   return hipGetLastError();
@@ -447,8 +450,8 @@ hipError_t backward(const ResidualNormParams& p, hipStream_t s) {
   l.items.dpre = p.ws + l.dpre;
   l.items.dpost = post && l.gates == kSeveral ? p.ws + l.dpost : nullptr;
   if (l.groups > 0) {
-    const Shape h = shape_of(p.cols, p.dtype);
-    with_shape<T>(h, [&](auto nv, auto block) {
+    const Shape h = shape_of(p.cols, p.dtype, true);
+    with_shape<T, true>(h, [&](auto nv, auto block) {
       const int threads = block ? h.lanes : kThreads;
       if (l.gates == kEachRow) residual_norm_backward_kernel<T, P, nv, block, kEachRow><<<l.groups, threads, 0, s>>>(p, h.lanes, l.items);
       else if (l.gates == kSeveral) residual_norm_backward_kernel<T, P, nv, block, kSeveral><<<l.groups, threads, 0, s>>>(p, h.lanes, l.items);
