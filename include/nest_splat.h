@@ -664,7 +664,9 @@ int nest_gated_ffn_backward(const nest_gated_ffn *f, const void *dy, const void 
  * in_features], bias [out_features] or NULL, residual [rows, out_features] or
  * NULL, all of dtype.  A training step keeps act'(x W^T + b): one byte an
  * element for relu, else two (four for F32), and with save8 one (two for F32),
- * in steps of 1/200 (1/26000).  The backward rounds dz = dy act' to dtype as
+ * in steps of 1/200 (1/26000).  16-bit rows of at most 128 features in and out
+ * keep nothing without save8: their backward makes the slopes again from x,
+ * weight and bias.  The backward rounds dz = dy act' to dtype as
  * operand of its products: in 16 bits dx and dweight are off by about 1.4
  * times what one rounding makes.  Float32 products leave out at most 2^-24 of
  * each, as nest_gated_ffn_* do, and give NaN where an infinity enters.  Sizes
@@ -683,10 +685,10 @@ typedef struct nest_linear {
   const void *residual;
 } nest_linear;
 
-/* Bytes the calls below need, each may be 0 and each pointer may be NULL: the
- * slopes a training forward leaves for the backward; the workspaces of a
- * forward, of a backward, and of a backward whose x is given in 8 bits.  Host
- * only. */
+/* Bytes the calls below need, each may be 0 and each pointer may be NULL (what
+ * is not asked for is not looked at): the slopes a training forward leaves for
+ * the backward; the workspaces of a forward, of a backward, and of a backward
+ * whose x is given in 8 bits.  Host only. */
 int nest_linear_sizes(const nest_linear *f, size_t *kept, size_t *forward_ws, size_t *backward_ws,
                       size_t *backward_ws_packed);
 
@@ -695,8 +697,10 @@ int nest_linear_forward(const nest_linear *f, void *y, void *kept, void *ws, siz
 
 /* dx [rows, in_features], dweight and dbias (each NULL where it is not wanted)
  * are overwritten; with no rows dweight and dbias are zero.  kept: what the
- * forward left (NULL only without an activation).  codes and steps: x as
- * nest_pack8 left it, in place of f->x; or both NULL.  The residual's gradient
+ * forward left (NULL only where nest_linear_sizes gives it no bytes; with an
+ * activation f->x, f->weight and f->bias are then those of the forward).  codes
+ * and steps: x as nest_pack8 left it, in place of f->x; or both NULL.  f->x is
+ * read for dweight and for slopes that are made again.  The residual's gradient
  * is dy. */
 int nest_linear_backward(const nest_linear *f, const void *dy, const void *kept, const int8_t *codes,
                          const uint8_t *steps, void *dx, void *dweight, void *dbias, void *ws, size_t ws_bytes,
@@ -743,8 +747,8 @@ int nest_residual_norm_backward(int64_t rows, int32_t cols, int32_t dtype, int32
 int nest_embedding(int64_t rows, int32_t cols, int64_t table_rows, int32_t dtype, const void *ids, int32_t wide_ids,
                    const void *table, float scale, const void *residual, void *y, void *stream);
 
-/* dtable[v] = scale * sum of dy[i] over ids[i] == v, in the order of a stable
- * sort; every row is written.  The residual's gradient is dy. */
+/* dtable[v] = scale * sum of dy[i] over ids[i] == v, in an order that the sizes
+ * and ids fix; every row is written.  The residual's gradient is dy. */
 size_t nest_embedding_backward_workspace_size(int64_t rows, int32_t cols, int64_t table_rows, int32_t dtype);
 int nest_embedding_backward(int64_t rows, int32_t cols, int64_t table_rows, int32_t dtype, const void *ids,
                             int32_t wide_ids, const void *dy, float scale, void *dtable, void *ws, size_t ws_bytes,

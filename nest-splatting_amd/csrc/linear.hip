@@ -4,7 +4,11 @@
 namespace nest {
 namespace {
 
-constexpr int64_t kFewRows = 16;   // rows up to which the forward streams the weights through registers, as gated_ffn does
+// Rows up to which the forward streams the weights through registers, as
+// gated_ffn does.  us of a call so and in tiles: 2 rows of 8192 -> 2048 11 and
+// 16, 8 of 2048 -> 2048 11 and 14, 16 of 2048 -> 8192 12 and 12.  One row of 2048
+// -> 8192 takes 8.8 us on the GPU: 33.6 MB of weights at 3.8 TB/s.
+constexpr int64_t kFewRows = 16;
 
 int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
 

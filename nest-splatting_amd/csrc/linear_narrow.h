@@ -8,7 +8,7 @@
 // write and read two bytes of slope an element (a third of the traffic).  Only
 // what is kept in 8 bits on request is read instead.
 //
-// A wave takes 32 rows.  It computes transposed products, weights as the first
+// A wave takes 16 or 32 rows.  It computes transposed products, weights as the first
 // operand and rows as the second, with the first operand's rows in an order by
 // which a lane's accumulators of two fragments are 8 consecutive features of
 // one row: 16 bytes of y, of dy, or of the second operand of the next product,
@@ -16,6 +16,15 @@
 // gradient sums over rows: the four waves of a workgroup put dz and x into LDS
 // and each takes a part of the gradient over all 128 rows with transposing
 // reads; it gathers in registers over the workgroup's turns.
+//
+// 1,702,400 x 64 -> 64 of bf16 with GELU and a residual: forward 136 us (654 MB:
+// 4.8 TB/s, the vector ALU 0.57 busy with the exponential and reciprocal of
+// every result), backward 166 (654 MB: 3.9 TB/s; vector ALU 0.64, LDS 0.42, of
+// which conflicts 0.19).  us of a forward and a backward here and in tiles:
+// 640,000 x 64 -> 64 37 + 61 and 56 + 129, 32 -> 128 63 + 97 and 130 + 194, 128
+// -> 128 89 + 224 and 161 + 262, with 8 bits 89 + 228 and 149 + 248; 16,384 rows
+// of 128 -> 128 11 + 27 and 13 + 30, 64 rows 12 + 21 and 15 + 28.  float32, three
+// parts a value, would not fit: it runs in tiles.
 #pragma once
 
 #include "linear_tiles.h"
@@ -459,7 +468,11 @@ hipError_t launch_narrow_layer(const LinearParams& p, hipStream_t s) {
   with_widths(p.in, p.out, [&](auto ki, auto ko) {
     constexpr int kRows = 64 * forward_groups(ki.value, ko.value);
     const int64_t turns = (p.rows + kRows - 1) / kRows;
-    const unsigned grid = (unsigned)(turns < 256 * 3 ? turns : 256 * 3);   // as many as run at once
+    // Workgroups a CU: three with slopes to keep, else four.  us of both: kept,
+    // 640,000 x 32 -> 128 69 and 75, 1,702,400 x 64 119 and 130; not kept,
+    // 640,000 x 32 -> 128 63 and 60, x 128 -> 128 88 and 86, 1,702,400 x 64 99 and 100.
+    const int64_t most = 256 * (n.kept ? 3 : 4);
+    const unsigned grid = (unsigned)(turns < most ? turns : most);
     if (n.kept) narrow_layer_kernel<T, ki.value, ko.value, true><<<grid, 256, 0, s>>>(n);
     else narrow_layer_kernel<T, ki.value, ko.value, false><<<grid, 256, 0, s>>>(n);
   });

@@ -428,8 +428,8 @@ def embedding_forward(ids: torch.Tensor, table: torch.Tensor, scale: float = 1.0
 
 
 def embedding_backward(dy: torch.Tensor, ids: torch.Tensor, rows: int, scale: float = 1.0) -> torch.Tensor:
-    """dtable [rows, D]: scale times the sum of dy [*ids.shape, D] over the places of each id, in dy's type; the sums run in the
-    order of the places, so results repeat bit for bit. The residual's gradient is dy itself."""
+    """dtable [rows, D]: scale times the sum of dy [*ids.shape, D] over the places of each id, in dy's type; the sums run in an
+    order that the sizes and ids fix, so results repeat bit for bit. The residual's gradient is dy itself."""
     code = _code(dy, "dy")
     ids, wide = _id_args(ids)
     if ids.get_device() != dy.get_device():
