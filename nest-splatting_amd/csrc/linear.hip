@@ -43,11 +43,14 @@ LinearLayout linear_layout(const LinearParams& p, bool back) {
     at = (at + (size_t)bytes + 255) / 256 * 256;
     return o;
   };
-  l.narrow = linear_narrow(p.in, p.out, p.dtype);
+  const bool narrow_f32 = linear_narrow_f32(p.in, p.out, p.dtype);
+  l.narrow = narrow_f32 || linear_narrow(p.in, p.out, p.dtype);
   if (l.narrow) {
     if (!back) return l;
     // as many workgroups as run at once, by LDS and registers
-    const int ki = (p.in + 31) / 32, ko = (p.out + 31) / 32, a_cu = narrow_groups_cu(ki, ko, p.slope_bytes || p.codes);
+    auto blocks = [](int v, int of) { return (v + of - 1) / of; };
+    const int a_cu = narrow_f32 ? narrow_f32_groups(blocks(p.in, 16), blocks(p.out, 16))
+                                : narrow_groups_cu(blocks(p.in, 32), blocks(p.out, 32), p.slope_bytes || p.codes);
     const int64_t turns = cdiv(p.rows, kNarrowBackRows);
     l.sum_rows = (int)(turns < 256 * a_cu ? turns : 256 * a_cu);
     l.sums = take(l.sum_rows * (int64_t)p.out * 4);

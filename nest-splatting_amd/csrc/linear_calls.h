@@ -3,6 +3,7 @@
 #pragma once
 
 #include "linear_narrow.h"
+#include "linear_narrow_f32.h"
 #include "linear_tiles.h"
 
 namespace nest {
@@ -40,8 +41,11 @@ hipError_t linear_forward(const LinearParams& p, hipStream_t s) {
   const T *x = static_cast<const T*>(p.x), *w = static_cast<const T*>(p.w);
   const Epilogue<T> ep{static_cast<const T*>(p.bias), static_cast<const T*>(p.residual), static_cast<T*>(p.y), p.kept, p.slope_bytes,
                        p.activation, p.out};
-  if constexpr (sizeof(T) == 2)
+  if constexpr (sizeof(T) == 2) {
     if (l.narrow) return launch_narrow_layer<T>(p, s);
+  } else {
+    if (l.narrow) return launch_narrow_f32(p, ep, s);
+  }
   if (l.few) {
     const Few<T> few{x, w, nullptr, p.in, (int)p.rows, p.out, p.in, static_cast<T*>(p.y), p.out, nullptr, 0};
     return launch_few<T, false>(few, s, FinishSum<T>{ep});
@@ -66,8 +70,11 @@ hipError_t linear_forward(const LinearParams& p, hipStream_t s) {
 template <typename T>
 hipError_t linear_backward(const LinearParams& p, hipStream_t s) {
   const LinearLayout l = linear_layout(p, true);
-  if constexpr (sizeof(T) == 2)
+  if constexpr (sizeof(T) == 2) {
     if (l.narrow) return launch_narrow_layer_backward<T>(p, l, s);
+  } else {
+    if (l.narrow) return launch_narrow_f32_backward(p, l, s);
+  }
   uint8_t* ws = static_cast<uint8_t*>(p.ws);
   const bool products = p.dx || p.dw;
   const T *x = static_cast<const T*>(p.x), *w = static_cast<const T*>(p.w), *dz = static_cast<const T*>(p.dy);

@@ -279,26 +279,30 @@ __global__ __launch_bounds__(256, narrow_groups_cu(KI, KO, kSaved)) void narrow_
   int steps[G][KI];
   const int groups_in = (p.in + 31) / 32;
   const bool again = !kSaved && p.act != NEST_ACT_NONE;
-  auto load = [&](int64_t turn) {
+  auto load = [&](int64_t turn) {   // branches around the loops: inside, each load would wait for the last
 #pragma unroll
     for (int g = 0; g < G; g++) {
       const int64_t at = turn + wave * 16 * G + g * 16 + r;
       const bool in = at < p.rows;
+      auto left = [&](int k, int cols) { return in ? cols - k * 32 - q * 8 : 0; };
+      auto place = [&](int k, int cols) { return at * cols + k * 32 + q * 8; };
 #pragma unroll
-      for (int k = 0; k < KI; k++) {
-        const int c = k * 32 + q * 8, n = in ? p.in - c : 0;
-        if (kSaved && p.codes) {
-          codes[g][k] = row_bytes(p.codes + at * p.in + c, n);
-          steps[g][k] = n > 0 ? p.steps[at * groups_in + k] : 0;
-        } else {
-          xw[g][k] = load_words<false>(p.x + at * p.in + c, p.x ? n : 0);
+      for (int k = 0; k < KO; k++) dy[g][k] = load_words<false>(p.dy + place(k, p.out), left(k, p.out));
+      if (kSaved && p.codes) {
+#pragma unroll
+        for (int k = 0; k < KI; k++) {
+          codes[g][k] = row_bytes(p.codes + place(k, p.in), left(k, p.in));
+          steps[g][k] = left(k, p.in) > 0 ? p.steps[at * groups_in + k] : 0;
         }
-      }
+      } else {
 #pragma unroll
-      for (int k = 0; k < KO; k++) {
-        const int c = k * 32 + q * 8, n = in ? p.out - c : 0;
-        dy[g][k] = load_words<false>(p.dy + at * p.out + c, n);
-        if constexpr (kSaved) slopes[g][k] = row_bytes(p.slopes + at * p.out + c, p.slopes ? n : 0);
+        for (int k = 0; k < KI; k++) xw[g][k] = load_words<false>(p.x + place(k, p.in), p.x ? left(k, p.in) : 0);
+      }
+      if constexpr (kSaved) {
+        if (p.slopes) {
+#pragma unroll
+          for (int k = 0; k < KO; k++) slopes[g][k] = row_bytes(p.slopes + place(k, p.out), left(k, p.out));
+        }
       }
     }
   };
@@ -351,16 +355,19 @@ __global__ __launch_bounds__(256, narrow_groups_cu(KI, KO, kSaved)) void narrow_
             for (int e = 0; e < 8; e++) z[g][e] = J * 32 + q * 8 + e < p.out ? z[g][e] : 0.0f;
         }
       }
+      auto make_dz = [&](auto slope) {
 #pragma unroll
-      for (int g = 0; g < G; g++)
+        for (int g = 0; g < G; g++)
 #pragma unroll
-        for (int e = 0; e < 8; e++) {
-          float d = to_f32(dy[g][J][e]);   // zero past the ends
-          if (kSaved && p.slopes) d *= coarse_slope(byte_of(slopes[g][J], e));
-          else if (again) d *= z[g][e];
-          dz[g][J][e] = from_f32<T>(d);
-          db[J][e] += d;
-        }
+          for (int e = 0; e < 8; e++) {
+            const float d = to_f32(dy[g][J][e]) * slope(g, e);   // zero past the ends
+            dz[g][J][e] = from_f32<T>(d);
+            db[J][e] += d;
+          }
+      };
+      if (kSaved && p.slopes) make_dz([&](int g, int e) { return coarse_slope(byte_of(slopes[g][J], e)); });
+      else if (again) make_dz([&](int g, int e) { return z[g][e]; });
+      else make_dz([&](int, int) { return 1.0f; });
       __builtin_amdgcn_sched_barrier(0);   // phases one after another: their registers are the next one's
     }
 #pragma unroll

@@ -100,7 +100,7 @@ struct LinearLayout {
   int64_t ldx, ldz;
   size_t x, w, dz, sums, part, bytes;
   TileChoice y, dx, dw;
-  bool narrow;             // linear_narrow.h
+  bool narrow;             // linear_narrow.h, linear_narrow_f32.h
   bool few;                // gated_few.h (forward)
   bool fits;               // in launches
   bool copy_dz;            // the backward makes dz; it is dy itself otherwise
@@ -116,6 +116,12 @@ constexpr int kNarrowBackRows = 64;   // of a workgroup's turn
 constexpr int narrow_groups_cu(int ki, int ko, bool saved) {
   return ki + ko <= 3 || (ki + ko == 4 && ko <= 2 && !saved) ? 4 : ki + ko <= 4 ? 3 : ki + ko <= 6 ? 2 : 1;
 }
+// float32 rows that stay on the chip (linear_narrow_f32.h); their slopes are
+// kept.
+inline bool linear_narrow_f32(int in, int out, int dtype) { return dtype == NEST_DTYPE_F32 && in <= 64 && out <= 64; }
+// Workgroups of their backward on a CU, by 16s of features in and out: as the
+// registers allow.
+constexpr int narrow_f32_groups(int ki, int ko) { return ki * ko <= 4 && ko < 4 ? 4 : ki * ko <= 9 ? 3 : 2; }
 int linear_slope_bytes(int in, int out, int dtype, int activation, bool save8);
 hipError_t launch_linear(const LinearParams& p, hipStream_t s, bool backward);
 hipError_t linear_f32(const LinearParams& p, hipStream_t s, bool backward);

@@ -110,6 +110,12 @@ def test_linear_from_8_bits(B, rows, cols, out, act, dtype):
     linear_check(B, *linear_case(rows, cols, out, dtype), act, save8=True)
 
 
+@pytest.mark.parametrize("cols,out", [(1, 1), (16, 16), (1, 64), (64, 1), (17, 33), (33, 50), (50, 33), (64, 64), (20, 40), (48, 17), (47, 48), (30, 63)])
+@pytest.mark.parametrize("rows,act,save8", [(1, "silu", False), (70, "gelu", True), (70, "relu", False), (4111, "silu", True), (4111, None, False)])
+def test_linear_narrow_float32(B, rows, cols, out, act, save8):
+    linear_check(B, *linear_case(rows, cols, out, torch.float32, residual=rows != 1), act=act, save8=save8)
+
+
 @pytest.mark.parametrize("save8", [False, True])
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("act", ["relu", "silu", "gelu"])
