@@ -22,9 +22,9 @@
 // every result), backward 166 (654 MB: 3.9 TB/s; vector ALU 0.64, LDS 0.42, of
 // which conflicts 0.19).  us of a forward and a backward here and in tiles:
 // 640,000 x 64 -> 64 37 + 61 and 56 + 129, 32 -> 128 63 + 97 and 130 + 194, 128
-// -> 128 89 + 224 and 161 + 262, with 8 bits 89 + 228 and 149 + 248; 16,384 rows
-// of 128 -> 128 11 + 27 and 13 + 30, 64 rows 12 + 21 and 15 + 28.  float32, three
-// parts a value, would not fit: it runs in tiles.
+// -> 128 89 + 224 and 161 + 262, with 8 bits 89 + 180 and 149 + 248; 16,384 rows
+// of 128 -> 128 11 + 27 and 13 + 30, 64 rows 12 + 21 and 15 + 28.  float32 has
+// kernels of its own (linear_narrow_f32.h).
 #pragma once
 
 #include "linear_tiles.h"

@@ -114,7 +114,8 @@ inline bool linear_narrow(int in, int out, int dtype) { return dtype != NEST_DTY
 // and out and whether anything is kept in 8 bits: as the registers allow.
 constexpr int kNarrowBackRows = 64;   // of a workgroup's turn
 constexpr int narrow_groups_cu(int ki, int ko, bool saved) {
-  return ki + ko <= 3 || (ki + ko == 4 && ko <= 2 && !saved) ? 4 : ki + ko <= 4 ? 3 : ki + ko <= 6 ? 2 : 1;
+  const int size = ki + ko + (saved ? 1 : 0);
+  return size <= 4 ? 4 : size <= 5 ? 3 : ki + ko <= 6 ? 2 : 1;
 }
 // float32 rows that stay on the chip (linear_narrow_f32.h); their slopes are
 // kept.
