@@ -669,7 +669,7 @@ int nest_gated_ffn_backward(const nest_gated_ffn *f, const void *dy, const void 
  * weight and bias.  The backward rounds dz = dy act' to dtype as
  * operand of its products: in 16 bits dx and dweight are off by about 1.4
  * times what one rounding makes.  Float32 products leave out at most 2^-24 of
- * each, as nest_gated_ffn_* do, and give NaN where an infinity enters.  Sizes
+ * each, as nest_gated_ffn_* do, and may give NaN where an infinity enters.  Sizes
  * that would take 2^32 threads are refused as unsupported. */
 typedef struct nest_linear {
   uint32_t struct_size;
