@@ -267,8 +267,13 @@ __global__ __launch_bounds__(256, narrow_groups_cu(KI, KO, kSaved)) void narrow_
   constexpr int WO = NO % 4 == 0 ? 4 : 2, WI = 4 / WO, FO = NO / WO, FI = NI / WI;   // waves and fragments of dW
   __shared__ __attribute__((aligned(16))) T lds[L::total];
   __shared__ f32x4 bias[kSaved ? 1 : KO * 8];
-  if constexpr (!kSaved) stage_bias(bias, p.bias, p.out, KO * 32);
-  if constexpr (!kSaved) stage_weights<T, KO * 32, KI * 32, false>(lds, p.w, p.out, p.in);
+  const bool again = !kSaved && p.act != NEST_ACT_NONE;   // w may be null without it and dx
+  if constexpr (!kSaved) {
+    if (again) {
+      stage_bias(bias, p.bias, p.out, KO * 32);
+      stage_weights<T, KO * 32, KI * 32, false>(lds, p.w, p.out, p.in);
+    }
+  }
   if (p.dx) stage_weights<T, KI * 32, KO * 32, true>(lds + L::wt, p.w, p.in, p.out);
   __syncthreads();
   const int lane = threadIdx.x & 63, r = lane & 15, q = lane >> 4, wave = wave_id();
@@ -278,7 +283,6 @@ __global__ __launch_bounds__(256, narrow_groups_cu(KI, KO, kSaved)) void narrow_
   uint2 slopes[G][KO], codes[G][KI];
   int steps[G][KI];
   const int groups_in = (p.in + 31) / 32;
-  const bool again = !kSaved && p.act != NEST_ACT_NONE;
   auto load = [&](int64_t turn) {   // branches around the loops: inside, each load would wait for the last
 #pragma unroll
     for (int g = 0; g < G; g++) {
