@@ -697,11 +697,11 @@ int nest_linear_forward(const nest_linear *f, void *y, void *kept, void *ws, siz
 
 /* dx [rows, in_features], dweight and dbias (each NULL where it is not wanted)
  * are overwritten; with no rows dweight and dbias are zero.  kept: what the
- * forward left (NULL only where nest_linear_sizes gives it no bytes; with an
+ * forward left, or anything where nest_linear_sizes gives it no bytes (with an
  * activation f->x, f->weight and f->bias are then those of the forward).  codes
  * and steps: x as nest_pack8 left it, in place of f->x; or both NULL.  f->x is
- * read for dweight and for slopes that are made again.  The residual's gradient
- * is dy. */
+ * read for dweight and for slopes that are made again, f->weight for dx and for
+ * those.  The residual's gradient is dy. */
 int nest_linear_backward(const nest_linear *f, const void *dy, const void *kept, const int8_t *codes,
                          const uint8_t *steps, void *dx, void *dweight, void *dbias, void *ws, size_t ws_bytes,
                          void *stream);

@@ -1659,6 +1659,7 @@ int nest_linear_forward(const nest_linear* f, void* y, void* kept, void* ws, siz
   if (f->rows == 0) return NEST_OK;
   if (!f->x || !f->weight || !y) return fail(NEST_ERR_INVALID_ARGUMENT, "NULL tensor pointer");
   LinearParams p = linear_params(f);
+  if (!p.slope_bytes) kept = nullptr;
   const LinearLayout l = linear_layout(p, false);
   if (!l.fits) return too_many_tiles();
   if (ws_bytes < l.bytes || (l.bytes && !ws)) return fail(NEST_ERR_WORKSPACE, "linear workspace too small: %zu < %zu bytes", ws_bytes, l.bytes);
@@ -1675,6 +1676,7 @@ int nest_linear_backward(const nest_linear* f, const void* dy, const void* kept,
   if (int rc = check_linear(f); rc != NEST_OK) return rc;
   if (!dx && !dweight && !dbias) return NEST_OK;
   LinearParams p = linear_params(f);
+  if (!p.slope_bytes) kept = nullptr;   // of no bytes, wherever it points
   p.codes = codes;
   p.steps = steps;
   if ((codes == nullptr) != (steps == nullptr)) return fail(NEST_ERR_INVALID_ARGUMENT, "codes and steps come together");

@@ -57,3 +57,20 @@ def test_linear_backward_without_the_weight(L, B, dtype, cols, out, from8):
         _, dw2, db2 = backward(L, B, dy, x, None, packed=packed, wants=wants, shape=(out, cols))
         assert dw2 is None or torch.equal(dw2, dw)
         assert db2 is None or torch.equal(db2, db)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("cols,out", [(24, 40), (128, 70), (24, 140), (24, 139), (70, 200)])
+@pytest.mark.parametrize("from8", [False, True])
+def test_linear_backward_with_kept_of_no_bytes(L, B, dtype, cols, out, from8):
+    """Where nest_linear_sizes gives kept no bytes its pointer is not looked at: here it leads to bytes that are no slopes."""
+    x, w, dy = rand(300, cols, dtype=dtype, seed=1), rand(out, cols, dtype=dtype, seed=2), rand(300, out, dtype=dtype, seed=3)
+    packed = B.pack8(x) if from8 else None
+    x = None if from8 else x
+    want = backward(L, B, dy, x, w, packed=packed)
+    got = backward(L, B, dy, x, w, packed=packed, kept=torch.full((300 * out * 4,), 77, dtype=torch.uint8, device=DEV))
+    assert all(torch.equal(p, q) for p, q in zip(want, got))
+    if not from8 and B._narrow(dtype, cols, out):   # slopes that are made again
+        want = backward(L, B, dy, x, w, "silu")
+        got = backward(L, B, dy, x, w, "silu", kept=torch.full((300 * out * 4,), 77, dtype=torch.uint8, device=DEV))
+        assert all(torch.equal(p, q) for p, q in zip(want, got))
