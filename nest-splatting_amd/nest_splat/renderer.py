@@ -121,8 +121,9 @@ class HashINGP:
     residual.ViewRefiner that features pass through before the MLP, the
     composited ones of render() as well as rgb_decode's, as in evaluation (no
     dropout, no gradient: neither trains it).  render() hands a ViewRefiner the
-    camera's ``view`` (None: of none), rgb_decode none.  The modes that decode
-    no features do not use it."""
+    camera's ``view`` in every mode that decodes features (None: of none),
+    rgb_decode the ``view`` it is given, an int or one for each row.  The modes
+    that decode no features do not use it."""
 
     def __init__(self, encoding, mlp: NestMLP, gridrange, contract: bool = False, active_levels: Optional[int] = None,
                  refiner=None):
@@ -136,10 +137,12 @@ class HashINGP:
         self.level_dim = encoding.level_dim
         self.active_levels = self.levels if active_levels is None else active_levels
 
-    def rgb_decode(self, features, ray_unit):
+    def rgb_decode(self, features, ray_unit, view=None):
+        if view is not None and not hasattr(self.refiner, "views"):
+            raise ValueError("a view needs a refiner that is conditioned on it (residual.ViewRefiner)")
         if self.refiner is not None:
             with _evaluating(self.refiner):
-                features = self.refiner(features)
+                features = self.refiner(features, *(() if view is None else (view,)))
         return self.mlp_rgb.rgb_decode(features, ray_unit)
 
     def __call__(self, points_3D: torch.Tensor, with_xyz: bool = False) -> torch.Tensor:
@@ -185,6 +188,12 @@ def _evaluating(module: torch.nn.Module):
     finally:
         for m in training:
             m.training = True
+
+
+def _view_of(camera, refiner) -> tuple:
+    """What a refiner takes after the features: the camera's view if it has one and the refiner is conditioned on it."""
+    view = getattr(camera, "view", None) if hasattr(refiner, "views") else None
+    return () if view is None else (view,)
 
 
 @dataclass
@@ -329,9 +338,8 @@ def render(viewpoint_camera, pc, pipe, bg_color: torch.Tensor, scaling_modifier=
         if refiner is None:
             decoded = rendered_image
         else:
-            view = getattr(viewpoint_camera, "view", None) if hasattr(refiner, "views") else None
             with _evaluating(refiner):
-                decoded = refiner.refine_image(rendered_image.detach(), *(() if view is None else (view,)))
+                decoded = refiner.refine_image(rendered_image.detach(), *_view_of(viewpoint_camera, refiner))
         rgb = ingp.mlp_rgb.decode_image(decoded, view_ray_matrix(viewpoint_camera), alpha=render_alpha, bg=bg)
     rets["render"] = rgb
 
@@ -389,7 +397,7 @@ def _render_sh(cam, pc, pipe, bg_color, scaling_modifier, ingp, beta, max_inters
                 p0, rays_d, _ = depths_to_points(cam, median.detach())
                 points = p0.detach() + offset
         feats = ingp(points, with_xyz=False)
-        ngp = ingp.rgb_decode(feats, torch_F.normalize(rays_d, dim=-1).float())
+        ngp = ingp.rgb_decode(feats, torch_F.normalize(rays_d, dim=-1).float(), *_view_of(cam, getattr(ingp, "refiner", None)))
         ngp = ngp.view(H, W, 3).permute(2, 0, 1) * mask
         rets["ngp_rgb"] = ngp.clone()
         image = image + ngp if mode == "diffuse_ngp" else ngp
