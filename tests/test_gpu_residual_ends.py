@@ -10,6 +10,26 @@ pytestmark = pytest.mark.gpu
 
 # ---- dense layer ----
 
+@pytest.mark.parametrize("dtype", TYPES[1:])
+@pytest.mark.parametrize("rows,out", [(4096, 1), (4096, 130), (16, 130)])
+def test_gelu_far_below_zero_is_rounded_once(B, dtype, rows, out):
+    """y of z = x alone, against half a step and what the activation's arithmetic may add: its polynomial is off by at most
+    2^-16.2, two roundings of the exponent z^2 log2(e) / 2 <= 130 add 2 ln(2) 130 2^-24 = 2^-16.5, and a dozen operations 2^-20,
+    together below 2^-15.  Below its type's normal numbers y may be off by half of their step, or, for bfloat16, vanish with the
+    exponential."""
+    x = torch.zeros(rows, 8, dtype=dtype, device=DEV)
+    x[:, 0] = torch.linspace(-14.0, 4.0, rows, device=DEV).to(dtype)
+    w = torch.zeros(out, 8, dtype=dtype, device=DEV)
+    w[:, 0] = 1.0
+    z = x[:, :1].double()
+    want = (z * 0.5 * torch.special.erfc(-z * 0.5 ** 0.5)).expand(rows, out)
+    bound = (torch.finfo(dtype).eps / 2 + 2.0 ** -15) * want.abs() + (2.0 ** -25 if dtype is torch.float16 else 2.0 ** -126)
+    for save8 in (False, True):
+        y = B.linear_forward(x, w, None, "gelu", training=True, save8=save8)[0].double()
+        off = (y - want).abs()
+        assert (off <= bound).all(), (z.squeeze(1)[(off > bound).any(1)][:5], float((off / bound).max()))
+
+
 @pytest.mark.parametrize("rows,cols,out", [(2 * 131072 + 77, 16, 32), (2 * 131072 + 129, 64, 64), (2 * 65536 + 31, 128, 128), (2 * 65536 + 65, 40, 128)])
 @pytest.mark.parametrize("act", ["gelu", None])
 def test_linear_narrow_past_two_turns(B, rows, cols, out, act):
