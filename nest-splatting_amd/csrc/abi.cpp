@@ -21,7 +21,6 @@
 
 #include "../../include/nest_splat.h"
 #include "blocks_internal.h"
-#include "residual_internal.h"
 #include "nest_internal.h"
 #include "residual_internal.h"
 

@@ -44,7 +44,7 @@ hipError_t linear_forward(const LinearParams& p, hipStream_t s) {
   if constexpr (sizeof(T) == 2) {
     if (l.narrow) return launch_narrow_layer<T>(p, s);
   } else {
-    if (l.narrow) return launch_narrow_f32(p, ep, s);
+    if (l.narrow) return launch_narrow_f32<T>(p, ep, s);
   }
   if (l.few) {
     const Few<T> few{x, w, nullptr, p.in, (int)p.rows, p.out, p.in, static_cast<T*>(p.y), p.out, nullptr, 0};
@@ -73,7 +73,7 @@ hipError_t linear_backward(const LinearParams& p, hipStream_t s) {
   if constexpr (sizeof(T) == 2) {
     if (l.narrow) return launch_narrow_layer_backward<T>(p, l, s);
   } else {
-    if (l.narrow) return launch_narrow_f32_backward(p, l, s);
+    if (l.narrow) return launch_narrow_f32_backward<T>(p, l, s);
   }
   uint8_t* ws = static_cast<uint8_t*>(p.ws);
   const bool products = p.dx || p.dw;

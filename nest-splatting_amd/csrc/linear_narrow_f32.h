@@ -300,7 +300,10 @@ void with_widths_f32(int in, int out, F f) {
   else second(Number<4>());
 }
 
-hipError_t launch_narrow_f32(const LinearParams& p, const Epilogue<float>& ep, hipStream_t s) {
+// Templates, so that a unit of another type makes none of these kernels.
+template <typename T>
+hipError_t launch_narrow_f32(const LinearParams& p, const Epilogue<T>& ep, hipStream_t s) {
+  static_assert(sizeof(T) == 4, "");
   NarrowF32 n{};
   n.x = static_cast<const float*>(p.x);
   n.w = static_cast<const float*>(p.w);
@@ -314,7 +317,9 @@ hipError_t launch_narrow_f32(const LinearParams& p, const Epilogue<float>& ep, h
   return hipGetLastError();
 }
 
+template <typename T>
 hipError_t launch_narrow_f32_backward(const LinearParams& p, const LinearLayout& l, hipStream_t s) {
+  static_assert(sizeof(T) == 4, "");
   uint8_t* ws = static_cast<uint8_t*>(p.ws);
   NarrowF32 n{};
   n.x = p.dw ? static_cast<const float*>(p.x) : nullptr;
