@@ -140,7 +140,7 @@ __global__ __launch_bounds__(64 * kFewWaves) void few_kernel(Few<T> p, F finish)
         }
       }
   __syncthreads();
-  with_act(p.act, [&](auto act) {
+  auto join = [&](auto act) {
     for (int o = threadIdx.x; o < kOut; o += blockDim.x) {
       const int64_t c = n0 + o / C::columns;
       const int row = o % C::columns;
@@ -162,7 +162,9 @@ __global__ __launch_bounds__(64 * kFewWaves) void few_kernel(Few<T> p, F finish)
         finish(p, row, c, v[0]);
       }
     }
-  });
+  };
+  if constexpr (kGate) with_act(p.act, join);
+  else join(ActConstant<NEST_ACT_NONE>());   // whatever becomes of the sum is the functor's
 }
 
 template <typename T, typename C, bool kGate, typename F>
