@@ -723,7 +723,8 @@ int nest_unpack8(int64_t rows, int32_t cols, int32_t dtype, const int8_t *codes,
  *   r = scale x + gate t                   (gate NULL: 1; h NULL: r is x, is not
  *                                           written, and scale is 1)
  *   y = r / sqrt(mean(r^2) + eps) * pre    (pre NULL: no y)
- * y is the norm of r as it is stored.  gate is [gates, cols]; rows / gates
+ * y is the norm of r as it is stored.  Squares are summed in float32: from about
+ * 1e19 on they pass its range and a row's norm is zero.  gate is [gates, cols]; rows / gates
  * consecutive rows share one (gates divides rows).  gate, post and pre are of
  * param_dtype: F32 or dtype.  rstd_post and rstd_pre [rows] float32 receive
  * what the backward needs (either may be NULL). */

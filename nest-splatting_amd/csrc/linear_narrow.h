@@ -14,13 +14,13 @@
 // one row: 16 bytes of y, of dy, or of the second operand of the next product,
 // so no value changes lanes between loads, products and stores.  The weights'
 // gradient sums over rows: the four waves of a workgroup put dz and x into LDS
-// and each takes a part of the gradient over all 128 rows with transposing
-// reads; it gathers in registers over the workgroup's turns.
+// and each takes a part of the gradient over a turn's 64 rows with transposing
+// reads; it gathers in registers over the turns.
 //
-// 1,702,400 x 64 -> 64 of bf16 with GELU and a residual: forward 136 us (654 MB:
-// 4.8 TB/s, the vector ALU 0.57 busy with the exponential and reciprocal of
-// every result), backward 166 (654 MB: 3.9 TB/s; vector ALU 0.64, LDS 0.42, of
-// which conflicts 0.19).  us of a forward and a backward here and in tiles:
+// 1,702,400 x 64 -> 64 of bf16 with GELU and a residual: forward 139 us (654 MB:
+// 4.7 TB/s, the vector ALU 0.61 busy with the exponential and reciprocal of
+// every result), backward 167 (654 MB: 3.9 TB/s; vector ALU 0.62, LDS 0.43, of
+// which conflicts 0.20).  us of a forward and a backward here and in tiles:
 // 640,000 x 64 -> 64 37 + 61 and 56 + 129, 32 -> 128 63 + 97 and 130 + 194, 128
 // -> 128 89 + 224 and 161 + 262, with 8 bits 89 + 180 and 149 + 248; 16,384 rows
 // of 128 -> 128 11 + 27 and 13 + 30, 64 rows 12 + 21 and 15 + 28.  float32 has

@@ -21,7 +21,8 @@
 // 8192 rows of 2048 -> 8192 bf16 with GELU: forward 318 us (865 TFLOP/s; the
 // epilogue's exponentials and 268 MB of y and slopes stand behind the matrix
 // cores, 0.45 busy), dx 237 and dW 232 (1160 and 1185 TFLOP/s, 0.65 busy; the
-// library's 8192^3 product reaches 1126), dz 77 (402 MB: 5.2 TB/s).
+// library's 8192^3 product reaches 1380, its second operand transposed 1577), dz
+// 77 (402 MB: 5.2 TB/s).
 #pragma once
 
 #include "column_sums.h"

@@ -27,8 +27,8 @@
 // padding), so nothing an operand does not hold is multiplied.
 //
 // Measured: 8192 x 2048 x 8192 bf16 1170 TFLOP/s, 8192 x 2048 x 16384 1260,
-// where the library's 8192^3 product reaches 1395 on this card; the matrix
-// cores are busy 54 to 67% of the cycles, at a clock of 1.7 to 1.9 GHz, without
+// where the library's 8192^3 product reaches 1380 on this card, its second
+// operand transposed 1577; the matrix cores are busy 54 to 67% of the cycles, at a clock of 1.7 to 1.9 GHz, without
 // LDS bank conflicts; the rest is the barrier and the wait for loads that two
 // buffers leave.  float32 4096 x 2048, 4096: 202 TFLOP/s, 155 the library's
 // product; that is 1210 of the parts' products, and in 64 x 64 tiles, whose

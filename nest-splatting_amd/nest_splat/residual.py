@@ -311,7 +311,8 @@ def _norm_params(x, gate, post, pre):
 def residual_norm_forward(x: torch.Tensor, h: Optional[torch.Tensor] = None, gate: Optional[torch.Tensor] = None,
                           post: Optional[torch.Tensor] = None, pre: Optional[torch.Tensor] = None, scale: float = 1.0, eps: float = 1e-6):
     """(r, y, stats): r = scale x + gate t with t = h / rms(h) post, and y = r / rms(r) pre, over the last dimension (at most 8192
-    values); rms(v) = sqrt(mean(v^2) + eps). y is the norm of r as it is stored, in x's type.
+    values); rms(v) = sqrt(mean(v^2) + eps), whose squares are summed in float32: from about 1e19 on they pass its range and the
+    row's norm is zero. y is the norm of r as it is stored, in x's type.
 
     x is the residual stream and h a branch's output, of one shape. post [D]: the norm after the branch, None for none. pre [D]:
     the norm before the next one, None for none (y is None). gate: None, [D], or with leading dimensions that are the first of
