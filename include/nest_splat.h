@@ -655,8 +655,9 @@ int nest_gated_ffn_backward(const nest_gated_ffn *f, const void *dy, const void 
  * held in 8 bits for its backward, the residual stream between two norms, and
  * an embedding of each row's view.  As above: dtype is that of the rows and
  * their gradients, rows are contiguous, sums are float32 and run in a fixed
- * order (results repeat bit for bit), and each result is rounded once.  The
- * pointers of nest_linear_* are multiples of 16 bytes. */
+ * order (results repeat bit for bit), and each result is rounded once.  Silu and
+ * gelu are off by at most 2^-15 of their value in 16 bits, in float32 by 2^-19 of
+ * it and 2^-22 |z|.  The pointers of nest_linear_* are multiples of 16 bytes. */
 
 #define NEST_ACT_NONE (-1)
 

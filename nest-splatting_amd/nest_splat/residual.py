@@ -16,7 +16,9 @@ Three levels, as in ``blocks``:
 
 Tensors are on the GPU, of float32, float16 or bfloat16, with any leading
 dimensions; sums are float32, run in an order that the sizes (and ids) fix, and
-each result is rounded once.  linear also rounds dz = dy act'(z) to the type, as
+each result is rounded once; before that silu and gelu are off by at most 2^-15
+of their value in 16 bits, and in float32 by 2^-19 of it and 2^-22 |z| (its gelu
+is by erf).  linear also rounds dz = dy act'(z) to the type, as
 the operand of its backward products: in 16 bits dx and dw are off by about 1.4
 times what one rounding makes, and in float16 a dz past 65504 is infinite.  Its
 float32 products leave out at most 2^-24 of each, and a float32 result that an

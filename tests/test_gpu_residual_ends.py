@@ -30,6 +30,22 @@ def test_gelu_far_below_zero_is_rounded_once(B, dtype, rows, out):
         assert (off <= bound).all(), (z.squeeze(1)[(off > bound).any(1)][:5], float((off / bound).max()))
 
 
+@pytest.mark.parametrize("dtype", TYPES[1:])
+@pytest.mark.parametrize("rows,out", [(4096, 1), (4096, 130), (16, 130)])
+def test_silu_far_below_zero_is_rounded_once(B, dtype, rows, out):
+    """The same of silu: the exponent z log2(e) <= 116 is rounded once and so is its factor, 2 ln(2) 116 2^-24 = 2^-16.7, and a few
+    operations 2^-21, together below 2^-15."""
+    x = torch.zeros(rows, 8, dtype=dtype, device=DEV)
+    x[:, 0] = torch.linspace(-80.0, 4.0, rows, device=DEV).to(dtype)
+    w = torch.zeros(out, 8, dtype=dtype, device=DEV)
+    w[:, 0] = 1.0
+    z = x[:, :1].double()
+    want = (z / (1 + torch.exp(-z))).expand(rows, out)
+    bound = (torch.finfo(dtype).eps / 2 + 2.0 ** -15) * want.abs() + (2.0 ** -25 if dtype is torch.float16 else 2.0 ** -126)
+    off = (B.linear_forward(x, w, None, "silu")[0].double() - want).abs()
+    assert (off <= bound).all(), (z.squeeze(1)[(off > bound).any(1)][:5], float((off / bound).max()))
+
+
 @pytest.mark.parametrize("rows,cols,out", [(2 * 131072 + 77, 16, 32), (2 * 131072 + 129, 64, 64), (2 * 65536 + 31, 128, 128), (2 * 65536 + 65, 40, 128)])
 @pytest.mark.parametrize("act", ["gelu", None])
 def test_linear_narrow_past_two_turns(B, rows, cols, out, act):
